@@ -45,7 +45,7 @@ _LAZY = {
     "samples_last": ("layout", "samples_last"),
 }
 _SUBMODULES = ("math", "diff", "runtime", "artifact", "compile", "ir", "emit_hip", "trace", "chaining", "policy",
-               "layout")
+               "layout", "stages")
 
 __all__ = ["Grid", "HawkError", "Index", "Matrix", "Mutable", "Param", "Scalar", "Table", "TensorType", "Terminated",
            "Vector",

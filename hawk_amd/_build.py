@@ -1,8 +1,9 @@
 """Build step of hawk's gfx950 target: compile ``libhawk_core.so`` in-tree.
 
 The library is the C-ABI launcher (``csrc/hawk_core.cpp``) plus the
-hand-written team-stage kernels (``csrc/hawk_team.hip``, ``csrc/hawk_linalg.hip``), built by ``hipcc``
-for gfx950 only.  Its build digest is the sha256 of its own sources (each
+hand-written team-stage kernels (``csrc/hawk_team.hip``, ``csrc/hawk_linalg.hip``) and training stages
+(``csrc/hawk_recurrence.hip``, ``csrc/hawk_rows.hip``, ``csrc/hawk_dropout.hip``), built by ``hipcc``
+for gfx950 only, each file by a compiler of its own.  Its build digest is the sha256 of its own sources (each
 file's name and sha256, in sorted order), stamped into the library and
 recomputed by :mod:`hawk_amd._core` at load, the same self-check the
 reference runs at import (reference ``hawk/__init__.py:146-212``).
@@ -14,6 +15,8 @@ import hashlib
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -22,6 +25,10 @@ CSRC = PACKAGE / "csrc"
 INCLUDE = ROOT / "include"
 LIBRARY = PACKAGE / "libhawk_core.so"
 HIPCC = os.environ.get("HAWK_HIPCC", "/opt/rocm/bin/hipcc")
+
+#: The library's translation units.
+UNITS = ("hawk_core.cpp", "hawk_team.hip", "hawk_linalg.hip", "hawk_recurrence.hip", "hawk_rows.hip",
+         "hawk_dropout.hip")
 
 #: Flags every HIP translation unit of this target is built with: gfx950
 #: only, no floating-point contraction (the host oracle's ``native`` profile
@@ -50,16 +57,21 @@ def build_library(verbose: bool = False) -> Path:
     digest = source_digest()
     info = "compiler=" + HIPCC + "\\nflags=" + " ".join(HIP_FLAGS) + "\\noffload_arch=gfx950"
     tmp = LIBRARY.with_suffix(".so.tmp")
-    cmd = [HIPCC, *HIP_FLAGS, "-fPIC", "-shared", "-std=c++17",
-           f"-I{INCLUDE}", f"-I{CSRC}",
-           f'-DHAWK_BUILD_DIGEST="{digest}"', f'-DHAWK_BUILD_INFO="{info}"',
-           str(CSRC / "hawk_core.cpp"), str(CSRC / "hawk_team.hip"), str(CSRC / "hawk_linalg.hip"),
-           "-o", str(tmp), "-lhiprtc", "-lamdhip64"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed building {LIBRARY.name}:\n{proc.stdout}\n{proc.stderr}")
+    flags = [*HIP_FLAGS, "-fPIC", "-std=c++17", f"-I{INCLUDE}", f"-I{CSRC}",
+             f'-DHAWK_BUILD_DIGEST="{digest}"', f'-DHAWK_BUILD_INFO="{info}"']
+
+    def call(cmd: list) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"hipcc failed building {LIBRARY.name}:\n{proc.stdout}\n{proc.stderr}")
+
+    with tempfile.TemporaryDirectory() as made, ThreadPoolExecutor(len(UNITS)) as pool:
+        objects = [str(Path(made) / f"{name}.o") for name in UNITS]
+        list(pool.map(lambda pair: call([HIPCC, *flags, "-c", str(CSRC / pair[0]), "-o", pair[1]]),
+                      zip(UNITS, objects)))
+        call([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared", *objects, "-o", str(tmp), "-lhiprtc", "-lamdhip64"])
     os.replace(tmp, LIBRARY)
     return LIBRARY
 

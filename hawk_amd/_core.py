@@ -84,6 +84,17 @@ def _declare(lib) -> None:
         "hk_keyed_sample_sum_f32": (I, [V, I64, I64, V, V]),
         "hk_keyed_log_fold_f64": (I, [V, I64, V, I64, I64, ctypes.c_int32, V, I64, V, V, V]),
         "hk_keyed_log_fold_f32": (I, [V, I64, V, I64, I64, ctypes.c_int32, V, I64, V, V, V]),
+        "hk_recurrence_scratch_bytes": (SZ, [V, ctypes.c_int32]),
+        "hk_recurrence": (I, [V, V, V]),
+        "hk_recurrence_vjp": (I, [V, V, V]),
+        "hk_row_loss_scratch_bytes": (SZ, [V]),
+        "hk_token_logp": (I, [V, V, V]),
+        "hk_token_logp_vjp": (I, [V, V, V]),
+        "hk_policy_loss": (I, [V, V, V]),
+        "hk_policy_loss_vjp": (I, [V, V, V]),
+        "hk_preference_loss": (I, [V, V, V]),
+        "hk_preference_loss_vjp": (I, [V, V, V]),
+        "hk_dropout": (I, [V, V]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -506,3 +517,38 @@ def band_ordered_sum_scratch_bytes() -> int:
 def band_ordered_sum(u: int, n: int, out: int, scratch: int, stream: int = 0) -> None:
     check(lib().hk_band_ordered_sum_f64(u or None, int(n), out,
                                         scratch, stream or None))
+
+
+class SeqPlane(ctypes.Structure):
+    """A (sequence, step, channel) plane (``hk_plane``): strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("seq", ctypes.c_int64), ("step", ctypes.c_int64), ("chan", ctypes.c_int64)]
+
+
+class RecurrenceJob(ctypes.Structure):
+    """The arguments of ``hk_recurrence`` and its derivative (``hk_recurrence_job``)."""
+
+    _fields_ = ([(n, SeqPlane) for n in ("gate", "x", "h", "bar_h", "bar_gate", "bar_x")]
+                + [(n, ctypes.c_void_p) for n in ("h0", "bar_last", "last", "bar_h0", "offsets")]
+                + [(n, ctypes.c_int64) for n in ("seqs", "steps", "chans")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "sigmoid", "reverse", "offsets64")])
+
+
+class RowLossJob(ctypes.Structure):
+    """The arguments of the losses over rows of logits (``hk_row_loss_job``)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "bar_logits", "target", "logp", "lse", "loss", "margin",
+                                                "bar_logp", "bar_loss", "old_logp", "ref_logp", "advantage", "weight",
+                                                "offsets")]
+                + [(n, ctypes.c_int64) for n in ("rows", "vocab", "row_stride", "bar_stride", "pairs")]
+                + [(n, ctypes.c_float) for n in ("scale", "clip_low", "clip_high", "kl", "beta", "smoothing")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "target64", "offsets64")])
+
+
+class DropoutJob(ctypes.Structure):
+    """The arguments of ``hk_dropout`` (``hk_dropout_job``)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "residual", "y", "offset_cell")]
+                + [(n, ctypes.c_int64) for n in ("rows", "cols", "x_stride", "residual_stride", "y_stride")]
+                + [(n, ctypes.c_uint64) for n in ("seed", "offset")]
+                + [(n, ctypes.c_int32) for n in ("cut", "dtype")])

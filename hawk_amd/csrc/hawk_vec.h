@@ -1,0 +1,109 @@
+// hawk_vec.h — element types, vector loads and stores and small numerics the
+// sequence, row and dropout kernels share (not part of the C-ABI).
+#ifndef HAWK_VEC_H
+#define HAWK_VEC_H
+
+#include "hawk_core.h"
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+namespace hawk_vec {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// The type an element's arithmetic and states are held in: 32 bits for every
+// type of 32 bits or fewer, 64 for double.
+template <class T> struct AccOf { typedef float type; };
+template <> struct AccOf<double> { typedef double type; };
+template <class T> using Acc = typename AccOf<T>::type;
+
+// N elements in one register group.  Loads and stores assume no more than an
+// element's own alignment: gfx950 takes a 16-byte access at any 2-byte address,
+// so a row that starts anywhere is read as wide as an aligned one.
+template <class T, int N> struct VecOf {
+    typedef T type __attribute__((ext_vector_type(N)));
+    typedef type loose __attribute__((aligned(sizeof(T))));
+};
+template <class T> struct VecOf<T, 1> { typedef T type; typedef T loose; };
+
+// Stream: data that this pass touches once, so it is not kept in the caches.
+template <class T, int N, bool Stream = false>
+__device__ __forceinline__ void load(const T* p, Acc<T> (&out)[N]) {
+    if constexpr (N == 1) {
+        T x;
+        if constexpr (Stream) x = __builtin_nontemporal_load(p);
+        else x = *p;
+        out[0] = static_cast<Acc<T>>(x);
+    } else {
+        typename VecOf<T, N>::type v;
+        if constexpr (Stream) v = __builtin_nontemporal_load(reinterpret_cast<const typename VecOf<T, N>::loose*>(p));
+        else v = *reinterpret_cast<const typename VecOf<T, N>::loose*>(p);
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = static_cast<Acc<T>>(v[j]);
+    }
+}
+
+// Rounds to nearest even, once, to the plane's type.
+template <class T, int N, bool Stream = false>
+__device__ __forceinline__ void store(T* p, const Acc<T> (&x)[N]) {
+    if constexpr (N == 1) {
+        if constexpr (Stream) __builtin_nontemporal_store(static_cast<T>(x[0]), p);
+        else *p = static_cast<T>(x[0]);
+    } else {
+        typename VecOf<T, N>::type v;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = static_cast<T>(x[j]);
+        if constexpr (Stream) __builtin_nontemporal_store(v, reinterpret_cast<typename VecOf<T, N>::loose*>(p));
+        else *reinterpret_cast<typename VecOf<T, N>::loose*>(p) = v;
+    }
+}
+
+// a * b, and 0 where either is 0 whatever the other is.
+__device__ __forceinline__ float cutmul(float a, float b) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double cutmul(double a, double b) { return a == 0.0 || b == 0.0 ? 0.0 : a * b; }
+
+// The product of two gates' products.  It is 0 only where one of them is (a
+// cut): a product too small for the type stays the least normal number, so an
+// infinity or a NaN that enters a long run of small gates also leaves it.
+__device__ __forceinline__ float chain(float a, float b) {
+    const float p = cutmul(a, b);
+    return p == 0.0f && a != 0.0f && b != 0.0f ? 1.17549435e-38f : p;
+}
+__device__ __forceinline__ double chain(double a, double b) {
+    const double p = cutmul(a, b);
+    return p == 0.0 && a != 0.0 && b != 0.0 ? 2.2250738585072014e-308 : p;
+}
+
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// sigma(z) and 1 - sigma(z), each to its own relative accuracy: e = exp(-|z|)
+// never overflows and neither value is formed by a subtraction.
+__device__ __forceinline__ void sigmoid(float z, float& a, float& rest) {
+    const float e = __builtin_amdgcn_exp2f(-kLog2e * __builtin_fabsf(z));
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    const float small = e * r;
+    a = z >= 0.0f ? r : small;
+    rest = z >= 0.0f ? small : r;
+    if (!(z == z)) a = rest = z;
+}
+__device__ __forceinline__ void sigmoid(double z, double& a, double& rest) {
+    const double e = exp(-fabs(z));
+    const double r = 1.0 / (1.0 + e), small = e * r;
+    a = z >= 0.0 ? r : small;
+    rest = z >= 0.0 ? small : r;
+    if (!(z == z)) a = rest = z;
+}
+
+}  // namespace hawk_vec
+
+#endif

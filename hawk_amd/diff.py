@@ -425,7 +425,19 @@ def vjp(kernel, wrt=None) -> Program:
     ``bar_<x>`` for each input ``x`` of ``wrt`` (default: every real input
     plane).  A ``Param`` named in ``wrt`` gets a cell ``bar_<param>``: the
     sum over samples of each sample's contribution, by ``hawk.sum``'s default
-    policy."""
+    policy.
+
+    Of a stage (:mod:`hawk_amd.stages`): the stage that is its derivative; it
+    writes the ``bar_`` planes a call gives, so ``wrt`` is not taken."""
+    from .runtime import Stage
+    if isinstance(kernel, Stage):
+        derivative = getattr(kernel, "vjp", None)
+        if derivative is None:
+            raise HawkError(f"{kernel.name} has no derivative")
+        if wrt is not None:
+            raise HawkError(f"{kernel.name}: wrt= is for traced kernels; a stage's derivative writes the bar_ planes "
+                            "that a call gives")
+        return derivative
     program = _program_of(kernel)
     _refuse_prior_reads(program, "vjp")
     _refuse_extremes(program, "vjp")

@@ -167,6 +167,16 @@ class _Workspace(dict):
         return self.take(key, (max(1, nbytes),), _torch().uint8, zero)
 
 
+class Stage:
+    """What :func:`run` takes beside a loaded kernel: a hand-written stage of
+    :mod:`hawk_amd.stages`."""
+
+    name = "stage"
+
+    def run(self, arrays: dict, stream=None) -> None:
+        raise NotImplementedError
+
+
 class DeviceKernel:
     """One kernel of a built unit, loaded for the gfx950 target."""
 
@@ -1007,11 +1017,20 @@ def run(kernel: DeviceKernel, *, base: int = 0, count: int | None = None, n_samp
 
     ``layout`` (``"samples_first"`` / ``"samples_last"``) and the markers
     :func:`hawk_amd.samples_first` / :func:`~hawk_amd.samples_last` say which
-    axis of a per-sample plane holds the samples (:mod:`hawk_amd.layout`)."""
+    axis of a per-sample plane holds the samples (:mod:`hawk_amd.layout`).
+
+    A stage of :mod:`hawk_amd.stages` takes its planes and ``stream`` alone."""
     if steps is None and entry == "plain" and type(kernel) is DeviceKernel and kernel._direct_held is not None:
         if kernel.run_direct(arrays, base, count, n_samples, layout,
                              _current_stream() if stream is None else _stream_of(stream)):
             return
+    if isinstance(kernel, Stage):
+        if base != 0 or count is not None or n_samples is not None or layout is not None or steps is not None \
+                or entry != "plain":
+            raise HawkError(f"{kernel.name}: a stage takes its planes and stream= (no base=, count=, n_samples=, "
+                            "layout=, steps= or entry=)")
+        kernel.run(arrays, stream)
+        return
     from . import layout as _layout
     torch = _torch()
     if isinstance(kernel, ChainedKernel):
@@ -1033,7 +1052,7 @@ def run(kernel: DeviceKernel, *, base: int = 0, count: int | None = None, n_samp
                         dst.copy_(copy.movedim(-1, 0))
         return
     if not isinstance(kernel, DeviceKernel):
-        raise HawkError("hawk.run takes a kernel loaded with hawk.load")
+        raise HawkError("hawk.run takes a kernel loaded with hawk.load, or a stage of hawk.stages")
     stream = _stream_of(stream)
     arrays, major = _layout.classify(kernel, arrays, layout, _PER_SAMPLE)
     rows, write_back = bool(major) and kernel.takes_rows(arrays, major, entry), []

@@ -361,6 +361,128 @@ int hk_mm16_f32(const float* const* in, int n_in, float* const* out, int n_out,
 int hk_mm16_f64(const double* const* in, int n_in, double* const* out, int n_out,
                 const int32_t* products, int64_t n, void* stream);
 
+/* ---- training stages: recurrences, row losses, dropout ------------------- */
+
+/* The element type of a stage's planes. */
+enum { HK_F32 = 0, HK_F64 = 1, HK_BF16 = 2, HK_F16 = 3 };
+
+/* A (sequence, step, channel) plane: element (s, t, c) at
+ * data + s*seq + t*step + c*chan elements.  A packed plane has no sequence
+ * axis (seq unused): its steps are the rows of all sequences in turn. */
+typedef struct hk_plane {
+    void* data;
+    int64_t seq, step, chan;
+} hk_plane;
+
+/* A gated linear recurrence over the step axis, h_t = a_t h_(t-1) + b_t:
+ *   sigmoid == 0:  a = gate, b = x;
+ *   sigmoid != 0:  a = 1 / (1 + exp(-gate)), b = (1 - a) x;
+ * from h0 (0 if NULL) and, with reverse, from the last step down.  A gate that
+ * is exactly 0 cuts: nothing before it reaches the state, not even an infinity
+ * or a NaN.  States (h0, last, bar_last, bar_h0) are [seqs, chans] row-major,
+ * in 64 bits for HK_F64 and 32 bits for every other type, each may be NULL.
+ * offsets (NULL for dense planes): seqs + 1 ascending row numbers from 0 to
+ * steps, on the device, 64-bit words if offsets64 != 0 else 32-bit; sequence s
+ * is rows [offsets[s], offsets[s+1]) and may be empty (its last is its h0).
+ *
+ * hk_recurrence reads gate, x, h0 and writes h, last.  h may be x or gate
+ * itself (same strides), last may be h0.
+ * hk_recurrence_vjp reads gate, h (the forward's), x (sigmoid only), h0,
+ * bar_h, bar_last and writes bar_gate, bar_x (either may be NULL data) and
+ * bar_h0:  G_t = bar_h_t + C_(t+1), C_t = a_t G_t, C past the end = bar_last;
+ *   bar_gate = G h_(t-1), bar_x = G;  sigmoid: bar_gate = G (h_(t-1) - x)
+ *   a (1 - a), bar_x = (1 - a) G;  bar_h0 = C_0.
+ * bar_x may be bar_h itself and bar_gate may be gate or x itself (h is read
+ * a step away, so nothing may overwrite it).
+ * Scratch: hk_recurrence_scratch_bytes(job, vjp) bytes, no contents needed.
+ * HK_EVALUE for sizes below 0, a missing plane or another type. */
+typedef struct hk_recurrence_job {
+    hk_plane gate, x, h, bar_h, bar_gate, bar_x;
+    const void *h0, *bar_last;
+    void *last, *bar_h0;
+    const void* offsets;
+    int64_t seqs, steps, chans;
+    int32_t dtype, sigmoid, reverse, offsets64;
+} hk_recurrence_job;
+size_t hk_recurrence_scratch_bytes(const hk_recurrence_job* job, int32_t vjp);
+int hk_recurrence(const hk_recurrence_job* job, void* scratch, void* stream);
+int hk_recurrence_vjp(const hk_recurrence_job* job, void* scratch, void* stream);
+
+/* Losses over rows of logits.  logits is [rows, vocab], element (n, v) at
+ * logits + n*row_stride + v; dtype HK_F32, HK_BF16 or HK_F16; targets are 64-bit
+ * if target64 != 0 else 32-bit.  With l = scale * logits:
+ *   lse_n = log sum_v exp(l[n, v]),  logp_n = l[n, target_n] - lse_n.
+ * A row whose target is below 0 is left out: its logits are not read, its logp,
+ * lse and loss are 0 and its gradient is 0.  A target of vocab or more gives a
+ * NaN.  Every other plane is float.  bar_logits is [rows, vocab] of dtype,
+ * bar_stride elements a row, and may be logits itself.
+ *
+ * hk_token_logp writes logp and lse (either may be NULL).
+ * hk_token_logp_vjp reads logits, target, lse, bar_logp and writes
+ *   bar_logits[n, v] = scale bar_logp_n (1[v = target_n] - exp(l[n, v] - lse_n)).
+ *
+ * hk_policy_loss: r = exp(logp - old_logp),
+ *   L_n = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *         + kl (exp(ref_logp - logp) - (ref_logp - logp) - 1),
+ *   *loss = sum_n weight_n L_n in a fixed order,
+ * A = advantage, weight 1/rows if NULL (a weight of 0 leaves the row out of
+ * the loss and the gradient whatever its values), ref_logp read only if kl != 0.
+ * It writes loss, logp, lse (each may be NULL) and, if bar_logits is not NULL,
+ * the gradient of *bar_loss * loss (bar_loss NULL: 1): the derivative of -min
+ * is -r A where r A <= clamp(r) A and 0 elsewhere.
+ * hk_policy_loss_vjp reads logp and lse instead and writes bar_logits.
+ *
+ * hk_preference_loss: 2*pairs sequences of rows cut by offsets (2*pairs + 1
+ * ascending row numbers from 0 to rows; 64-bit if offsets64 != 0); pair p
+ * prefers sequence 2p to 2p + 1.  With s_k = sum over sequence k's kept rows of
+ * (logp - ref_logp) (ref_logp NULL: 0): margin_p = s_2p - s_2p+1, z = beta margin,
+ *   *loss = sum_p weight_p (-(1 - smoothing) log sigma(z) - smoothing log sigma(-z)),
+ * weight 1/pairs if NULL (a weight of 0 leaves the pair out).  It writes loss,
+ * margin, logp, lse (each may be NULL).
+ * hk_preference_loss_vjp reads logits, target, offsets, margin, lse and writes
+ * bar_logits.
+ *
+ * Scratch: hk_row_loss_scratch_bytes(job) bytes, no contents needed.  The
+ * sums over rows and pairs are taken in 64 bits in a fixed order. */
+typedef struct hk_row_loss_job {
+    const void* logits;
+    void* bar_logits;
+    const void* target;
+    float *logp, *lse, *loss, *margin;
+    const float *bar_logp, *bar_loss, *old_logp, *ref_logp, *advantage, *weight;
+    const void* offsets;
+    int64_t rows, vocab, row_stride, bar_stride, pairs;
+    float scale, clip_low, clip_high, kl, beta, smoothing;
+    int32_t dtype, target64, offsets64;
+} hk_row_loss_job;
+size_t hk_row_loss_scratch_bytes(const hk_row_loss_job* job);
+int hk_token_logp(const hk_row_loss_job* job, void* scratch, void* stream);
+int hk_token_logp_vjp(const hk_row_loss_job* job, void* scratch, void* stream);
+int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream);
+int hk_policy_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stream);
+int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream);
+int hk_preference_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stream);
+
+/* Dropout from a counter-based generator, no mask stored: element i of the
+ * row-major [rows, cols] array (x, residual and y may have row strides of their
+ * own) is kept where its 16-bit number is >= cut,
+ *   y_i = kept ? x_i * 65536 / (65536 - cut) : 0, + residual_i (NULL: none).
+ * The numbers are Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random
+ * numbers: as easy as 1, 2, 3, SC 2011) of the key seed and the counter
+ * (i / 8, offset), 64 bits each: half i % 8 of the four words, low half first.
+ * offset_cell (a 64-bit word on the device) is added to offset if not NULL, so
+ * a captured launch takes a new mask a replay.  cut in [0, 65536]; 65536
+ * drops everything.  y may be x or residual itself.  dtype any. */
+typedef struct hk_dropout_job {
+    const void *x, *residual;
+    void* y;
+    const int64_t* offset_cell;
+    int64_t rows, cols, x_stride, residual_stride, y_stride;
+    uint64_t seed, offset;
+    int32_t cut, dtype;
+} hk_dropout_job;
+int hk_dropout(const hk_dropout_job* job, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

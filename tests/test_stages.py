@@ -1,0 +1,929 @@
+"""The training stages (``hawk.stages``) against plain loops in 64 bits.
+
+Tolerances.  ``u`` is half an ulp of 1 in the arithmetic's type (2^-24, 2^-53
+for float64), ``r`` half an ulp of 1 in the output's type (2^-8 for bfloat16, 2^-11
+for float16).  A recurrence of T steps joins each step's term through at most T
+products and sums, each with a relative error of at most u (a sigmoid gate's
+own error is below 24 u for |z| <= 8), so its error is at most ``(c T + 16) u``
+times the same recurrence of absolute values, c = 4 or 28; the output rounds
+once, by r.  A row's log-sum-exp errs by 8 u (1 + |lse|) (its terms are joined in
+a tree), and a gradient element by the exponent's absolute error, 16 u (1 + |l|),
+times itself.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+import hawk_amd as hawk
+from hawk_amd import HawkError, _core, diff
+
+TYPES = ("float32", "bfloat16", "float16", "float64")
+U = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -24, "float16": 2.0 ** -24, "float64": 2.0 ** -53}
+R = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11, "float64": 2.0 ** -53}
+TINY = {"float32": 1e-37, "bfloat16": 1e-37, "float16": 2.0 ** -25, "float64": 1e-300}
+
+
+def torch_type(name):
+    import torch
+    return getattr(torch, name)
+
+
+def plane(x, dtype, device):
+    """``x`` in ``dtype`` on the device, and the values it holds, in 64 bits."""
+    import torch
+    held = torch.from_numpy(np.asarray(x, dtype=np.float64)).to(torch_type(dtype)).to(device)
+    return held, held.double().cpu().numpy()
+
+
+def back(x):
+    return x.double().cpu().numpy()
+
+
+# -- the plain forms, in 64 bits -------------------------------------------------------------
+
+def gates(gate, x, form):
+    if form == "value":
+        return gate, x
+    a = np.where(gate >= 0, 1 / (1 + np.exp(-np.abs(gate))), np.exp(-np.abs(gate)) / (1 + np.exp(-np.abs(gate))))
+    return a, (1 - a) * x
+
+
+def loop(a, b, state):
+    """``h_t = a_t h_{t-1} + b_t``, a gate of 0 cutting, over axis 0."""
+    out = np.empty_like(b)
+    for t in range(len(b)):
+        state = np.where(a[t] == 0, b[t], a[t] * state + b[t])
+        out[t] = state
+    return out, state
+
+
+def spans(S, T, offsets):
+    if offsets is None:
+        return [(s, slice(0, T)) for s in range(S)]
+    return [(s, slice(int(offsets[s]), int(offsets[s + 1]))) for s in range(len(offsets) - 1)]
+
+
+def take(x, s, rows, packed):
+    return x[rows] if packed else x[s][rows]
+
+
+def oracle_forward(gate, x, h0, offsets, form, reverse):
+    packed = offsets is not None
+    S = len(offsets) - 1 if packed else gate.shape[0]
+    C = gate.shape[-1]
+    h, scale = np.zeros_like(x), np.zeros_like(x)
+    last = np.zeros((S, C))
+    for s, rows in spans(S, gate.shape[-2], offsets):
+        a, b = gates(take(gate, s, rows, packed), take(x, s, rows, packed), form)
+        if reverse:
+            a, b = a[::-1], b[::-1]
+        start = np.zeros(C) if h0 is None else h0[s]
+        out, last[s] = loop(a, b, start)
+        size, _ = loop(np.abs(a), np.abs(b), np.abs(start))
+        if reverse:
+            out, size = out[::-1], size[::-1]
+        take(h, s, rows, packed)[:] = out
+        take(scale, s, rows, packed)[:] = size
+    return h, last, scale
+
+
+def oracle_vjp(gate, x, h, h0, bar_h, bar_last, offsets, form, reverse):
+    packed = offsets is not None
+    S = len(offsets) - 1 if packed else gate.shape[0]
+    C = gate.shape[-1]
+    bar_gate, bar_x = np.zeros_like(gate), np.zeros_like(gate)
+    size_gate, size_x = np.zeros_like(gate), np.zeros_like(gate)
+    bar_h0, size_0 = np.zeros((S, C)), np.zeros((S, C))
+    for s, rows in spans(S, gate.shape[-2], offsets):
+        g, xs = take(gate, s, rows, packed), take(x, s, rows, packed) if x is not None else None
+        hs, bs = take(h, s, rows, packed), take(bar_h, s, rows, packed)
+        a, _ = gates(g, xs if xs is not None else g, form)
+        order = range(len(g))
+        order = list(order) if reverse else list(reversed(order))
+        carry = np.zeros(C) if bar_last is None else bar_last[s]
+        mass = np.abs(carry)
+        for i, t in enumerate(order):
+            before = order[i + 1] if i + 1 < len(order) else None
+            prior = hs[before] if before is not None else (np.zeros(C) if h0 is None else h0[s])
+            G, m = bs[t] + carry, np.abs(bs[t]) + mass
+            if form == "sigmoid":
+                bg, bx = G * (prior - xs[t]) * a[t] * (1 - a[t]), (1 - a[t]) * G
+                mg, mx = m * (np.abs(prior) + np.abs(xs[t])) * a[t] * (1 - a[t]), (1 - a[t]) * m
+            else:
+                bg, bx, mg, mx = G * prior, G, m * np.abs(prior), m
+            take(bar_gate, s, rows, packed)[t], take(bar_x, s, rows, packed)[t] = bg, bx
+            take(size_gate, s, rows, packed)[t], take(size_x, s, rows, packed)[t] = mg, mx
+            carry, mass = np.where(a[t] == 0, 0, a[t] * G), np.abs(a[t]) * m
+        bar_h0[s], size_0[s] = carry, mass
+    return (bar_gate, bar_x, bar_h0), (size_gate, size_x, size_0)
+
+
+def close(got, want, size, T, form, dtype, state=False):
+    c = 28 if form == "sigmoid" else 4
+    r = U[dtype] if state else R[dtype]
+    bound = ((c * T + 16) * U[dtype] + r) * size * (1 + 2 * r) + TINY["float64" if state else dtype]
+    assert np.isfinite(got).all()
+    worst = np.abs(got - want) - bound
+    assert (worst <= 0).all(), f"off by {np.abs(got - want).max()} where {bound[np.unravel_index(worst.argmax(), worst.shape)]} is allowed"
+
+
+def recurrence_case(S, T, C, dtype, form, reverse, layout, state, packed, device, seed=0):
+    g = np.random.default_rng([seed, S, T, C])
+    shape = (T, C) if packed else (S, T, C)
+    gate = g.normal(size=shape) + 1.0 if form == "sigmoid" else 1 / (1 + np.exp(-g.normal(size=shape) - 2))
+    if form == "value":
+        gate *= g.random(shape) > 0.03
+        gate = np.where(g.random(shape) < 0.1, -gate, gate)
+    offsets = None
+    if packed:
+        cut = np.sort(g.integers(0, T + 1, S - 1)) if S > 1 else np.array([], int)
+        if S >= 4:
+            cut[1] = cut[0]
+            cut[-1] = T
+        offsets = np.concatenate([[0], cut, [T]])
+    got, held = {}, {}
+
+    def put(name, x):
+        t, held[name] = plane(x, dtype, device)
+        if layout == "steps":
+            t = t.transpose(-1, -2).contiguous().transpose(-1, -2)
+        elif layout == "sliced":                                # odd strides, odd alignment
+            import torch
+            wide = torch.zeros((*t.shape[:-1], t.shape[-1] + 3), dtype=t.dtype, device=device)
+            wide[..., 1:1 + t.shape[-1]] = t
+            t = wide[..., 1:1 + t.shape[-1]]
+        elif layout == "scattered":                             # neither axis contiguous
+            import torch
+            wide = torch.zeros((*t.shape[:-2], 2 * t.shape[-2], 2 * t.shape[-1]), dtype=t.dtype, device=device)
+            wide[..., ::2, ::2] = t
+            t = wide[..., ::2, ::2]
+        got[name] = t
+    for n in ("gate", "x", "bar_h"):
+        put(n, gate if n == "gate" else g.normal(size=shape))
+    sd = "float64" if dtype == "float64" else "float32"
+    if state:
+        for n in ("h0", "bar_last"):
+            got[n], held[n] = plane(g.normal(size=(S, C)), sd, device)
+    return got, held, offsets
+
+
+SHAPES = [(1, 1, 1), (3, 1, 5), (2, 2, 8), (1, 7, 64), (5, 33, 9), (2, 129, 24), (3, 300, 1), (1, 1025, 40),
+          (1, 2500, 3), (70, 5, 2), (2, 640, 513)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["value", "sigmoid"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_recurrence_and_its_derivative_are_the_loop(gpu, shape, dtype, form):
+    import torch
+    S, T, C = shape
+    for k, (layout, reverse, state, packed) in enumerate([
+            ("channels", False, True, False), ("steps", True, True, False), ("sliced", True, False, False),
+            ("steps", False, False, False), ("channels", False, True, True), ("sliced", True, True, True),
+            ("scattered", False, True, False)]):
+        print(shape, dtype, form, layout, reverse, state, packed, flush=True)
+        got, held, offsets = recurrence_case(S, T, C, dtype, form, reverse, layout, state, packed, gpu, seed=k)
+        stage = hawk.stages.recurrence(gate=form, reverse=reverse)
+        planes = {n: got[n] for n in ("gate", "x", "h0") if n in got}
+        if packed:
+            planes["offsets"] = torch.from_numpy(offsets).to(gpu, torch.int64 if k % 2 else torch.int32)
+        h = torch.empty_like(got["x"])
+        last = torch.empty_like(got["h0"]) if state else None
+        hawk.run(stage, h=h, last=last, **planes)
+        want, want_last, size = oracle_forward(held["gate"], held["x"], held.get("h0"), offsets, form, reverse)
+        close(back(h), want, size, T, form, dtype)
+        if state:
+            mass = np.abs(want_last) + (np.abs(size).max() if size.size else 0) + np.abs(held["h0"])
+            close(back(last), want_last, mass, T, form, dtype, state=True)
+        # the derivative, of the h the forward wrote
+        bars = {n: torch.empty_like(got["x"]) for n in ("bar_gate", "bar_x")}
+        if state:
+            bars["bar_h0"] = torch.empty_like(got["h0"])
+            planes["bar_last"] = got["bar_last"]
+        hawk.run(stage.vjp, h=h, bar_h=got["bar_h"], **planes, **bars)
+        wants, sizes = oracle_vjp(held["gate"], held["x"], back(h), held.get("h0"), held["bar_h"],
+                                  held.get("bar_last"), offsets, form, reverse)
+        for n, w, z in zip(("bar_gate", "bar_x", "bar_h0"), wants, sizes):
+            if n in bars:
+                close(back(bars[n]), w, z, T, form, dtype, state=n == "bar_h0")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["value", "sigmoid"])
+def test_the_recurrences_derivative_is_its_difference_quotient(gpu, form):
+    """Central differences of sum(w h) + sum(v last) in float64: an error of e^2 / 6 times the third
+    derivative and of 1e-16 / e from rounding, so 1e-8 at e = 1e-5 for sums of order 1."""
+    import torch
+    g = np.random.default_rng(7)
+    S, T, C = 2, 19, 3
+    base = {"gate": g.uniform(0.2, 0.9, (S, T, C)) if form == "value" else g.normal(size=(S, T, C)),
+            "x": g.normal(size=(S, T, C)), "h0": g.normal(size=(S, C))}
+    w, v = g.normal(size=(S, T, C)), g.normal(size=(S, C))
+    stage = hawk.stages.recurrence(gate=form)
+
+    def forward(values):
+        t = {n: torch.from_numpy(x).to(gpu) for n, x in values.items()}
+        h, last = torch.empty_like(t["x"]), torch.empty_like(t["h0"])
+        hawk.run(stage, h=h, last=last, **t)
+        return h, last
+    h, _ = forward(base)
+    bars = {"bar_" + n: torch.empty_like(torch.from_numpy(x)).to(gpu) for n, x in base.items()}
+    hawk.run(diff.vjp(stage), **{n: torch.from_numpy(x).to(gpu) for n, x in base.items()}, h=h,
+             bar_h=torch.from_numpy(w).to(gpu), bar_last=torch.from_numpy(v).to(gpu), **bars)
+    e = 1e-5
+    for n in base:
+        for index in [tuple(g.integers(0, d) for d in base[n].shape) for _ in range(8)]:
+            ends = []
+            for sign in (1, -1):
+                moved = {m: x.copy() for m, x in base.items()}
+                moved[n][index] += sign * e
+                hh, ll = forward(moved)
+                ends.append((back(hh) * w).sum() + (back(ll) * v).sum())
+            slope = (ends[0] - ends[1]) / (2 * e)
+            assert abs(slope - back(bars["bar_" + n])[index]) < 1e-7 * (1 + abs(slope)), (n, index)
+
+
+@pytest.mark.gpu
+def test_a_gate_of_zero_and_a_sequences_start_cut_infinities_and_nan(gpu):
+    import torch
+    T = 700
+    for C, layout in ((1, "steps"), (16, "channels")):
+        x = torch.randn(1, T, C, device=gpu)
+        gate = torch.full_like(x, 0.5)
+        x[0, 100] = math.nan
+        x[0, 300] = math.inf
+        gate[0, 200] = 0.0
+        gate[0, 301] = 0.0
+        h = torch.empty_like(x)
+        hawk.run(hawk.stages.recurrence(), gate=gate, x=x, h=h)
+        assert torch.isnan(h[0, 100:200]).all() and torch.isfinite(h[0, :100]).all()
+        assert torch.isfinite(h[0, 200:300]).all() and torch.isinf(h[0, 300]).all() and torch.isfinite(h[0, 301:]).all()
+        want, _, _ = oracle_forward(back(gate[:, 200:300]), back(x[:, 200:300]), None, None, "value", False)
+        assert np.abs(back(h[:, 200:300]) - want).max() < 1e-5
+        # the same through packed sequences: nothing crosses a bound
+        gate.fill_(0.5)
+        offsets = torch.tensor([0, 200, 200, 301, T], device=gpu)
+        for reverse in (False, True):
+            hp = torch.empty(T, C, device=gpu)
+            hawk.run(hawk.stages.recurrence(reverse=reverse), gate=gate[0].contiguous(), x=x[0].contiguous(), h=hp,
+                     offsets=offsets)
+            assert torch.isfinite(hp[301:]).all() and torch.isfinite(hp[200:300] if not reverse else hp[101:200]).all()
+            assert torch.isnan(hp[100]).all()
+        # a NaN gate is not lost where the state is 0
+        z = torch.zeros_like(x)
+        gate[0, 5] = math.nan
+        hawk.run(hawk.stages.recurrence(), gate=gate, x=z, h=h)
+        assert torch.isnan(h[0, 5:]).all() and (h[0, :5] == 0).all()
+
+
+@pytest.mark.gpu
+def test_one_token_at_a_time_is_the_whole_sequence(gpu):
+    import torch
+    S, T, C = 5, 37, 130
+    g = torch.Generator(device=gpu).manual_seed(3)
+    z, x = (torch.randn(S, T, C, generator=g, device=gpu) for _ in range(2))
+    stage = hawk.stages.recurrence(gate="sigmoid")
+    whole = torch.empty_like(x)
+    hawk.run(stage, gate=z, x=x, h=whole)
+    state = torch.zeros(S, C, device=gpu)
+    one = torch.empty(S, 1, C, device=gpu)
+    for t in range(T):
+        hawk.run(stage, gate=z[:, t:t + 1], x=x[:, t:t + 1], h=one, h0=state, last=state)      # in place
+        assert (one[:, 0] - whole[:, t]).abs().max() <= 64 * 2.0 ** -24 * (1 + whole[:, t].abs().max())
+        assert torch.equal(one[:, 0], state)
+
+
+@pytest.mark.gpu
+def test_recurrences_in_place_replayed_and_on_two_streams(gpu):
+    import torch
+    S, T, C = 3, 1500, 72
+    g = torch.Generator(device=gpu).manual_seed(4)
+    gate = torch.rand(S, T, C, generator=g, device=gpu).bfloat16()
+    x = torch.randn(S, T, C, generator=g, device=gpu).bfloat16()
+    stage = hawk.stages.recurrence()
+    want = torch.empty_like(x)
+    hawk.run(stage, gate=gate, x=x, h=want)
+    held = x.clone()
+    hawk.run(stage, gate=gate, x=held, h=held)
+    assert torch.equal(held, want)
+    # the same bits whatever stream, and however many run at once
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(x) for _ in range(8)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for k, out in enumerate(outs):
+        hawk.run(stage, gate=gate, x=x, h=out, stream=streams[k % 2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+    # a captured call
+    h = torch.empty_like(x)
+    launch = stage.prepare(gate=gate, x=x, h=h)
+    launch()
+    torch.cuda.synchronize()
+    assert torch.equal(h, want)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        captured = stage.prepare(gate=gate, x=x, h=h, stream=side)
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        captured()
+    other = torch.randn_like(x)
+    for k in range(4):
+        x.copy_(other * (k + 1))
+        h.zero_()
+        graph.replay()
+        eager = torch.empty_like(x)
+        hawk.run(stage, gate=gate, x=x, h=eager)
+        torch.cuda.synchronize()
+        assert torch.equal(h, eager)
+
+
+@pytest.mark.gpu
+def test_recurrence_without_steps_sequences_or_channels(gpu):
+    import torch
+    stage = hawk.stages.recurrence()
+    h0 = torch.randn(3, 5, device=gpu)
+    last = torch.empty_like(h0)
+    e = torch.empty(3, 0, 5, device=gpu)
+    hawk.run(stage, gate=e, x=e.clone(), h=e.clone(), h0=h0, last=last)
+    assert torch.equal(last, h0)
+    bar = torch.empty_like(h0)
+    hawk.run(stage.vjp, gate=e, h=e.clone(), bar_h=e.clone(), bar_last=h0, bar_h0=bar)
+    assert torch.equal(bar, h0)
+    p = torch.empty(0, 5, device=gpu)
+    last.zero_()
+    hawk.run(stage, gate=p, x=p.clone(), h=p.clone(), h0=h0, last=last,
+             offsets=torch.zeros(4, dtype=torch.int32, device=gpu))
+    assert torch.equal(last, h0)
+    for shape in ((0, 4, 5), (3, 4, 0)):
+        e = torch.empty(shape, device=gpu)
+        hawk.run(stage, gate=e, x=e.clone(), h=e.clone())
+
+
+# -- rows of logits --------------------------------------------------------------------------
+
+ROW_TYPES = ("float32", "bfloat16", "float16")
+ROWS = [(1, 1), (3, 2), (7, 33), (64, 48), (5, 257), (2, 1000), (9, 1024), (3, 4097), (2, 32768), (3, 50001), (1, 140001)]
+
+
+def rows_case(N, V, dtype, device, seed=0, masked=True, strided=False):
+    import torch
+    g = np.random.default_rng([seed, N, V])
+    logits, held = plane(g.normal(size=(N, V)) * 3, dtype, device)
+    if strided:
+        wide = torch.zeros((N, V + 5), dtype=logits.dtype, device=device)
+        wide[:, 3:3 + V] = logits
+        logits = wide[:, 3:3 + V]
+    target = g.integers(0, V, N)
+    if masked and N >= 3:
+        target[1] = -1
+        target[N - 1] = -100
+    return logits, held, target
+
+
+def oracle_rows(held, target, scale):
+    l = held * scale
+    top = l.max(1)
+    lse = top + np.log(np.exp(l - top[:, None]).sum(1))
+    kept = target >= 0
+    logp = l[np.arange(len(l)), np.maximum(target, 0)] - lse
+    return np.where(kept, logp, 0), np.where(kept, lse, 0), l
+
+
+def oracle_gradient(l, target, lse, c, scale):
+    kept = target >= 0
+    p = np.exp(l - lse[:, None])
+    grad = -c[:, None] * p
+    grad[np.arange(len(l)), np.maximum(target, 0)] += c
+    size = np.abs(c)[:, None] * p
+    size[np.arange(len(l)), np.maximum(target, 0)] += np.abs(c)
+    return np.where(kept[:, None], grad * scale, 0), size * scale
+
+
+def close_row(got, want, lse):
+    assert (np.abs(got - want) <= 8 * 2.0 ** -24 * (2 + np.abs(lse) + np.abs(want))).all(), np.abs(got - want).max()
+
+
+def close_gradient(got, want, size, l, lse, dtype, slack=0.0):
+    reach = 16 * 2.0 ** -24 * (1 + np.abs(l) + np.abs(lse[:, None])) + slack
+    bound = size * (reach + R[dtype] * (1 + reach)) + TINY[dtype]
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) - bound).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ROW_TYPES)
+@pytest.mark.parametrize("shape", ROWS, ids=str)
+def test_token_logp_and_its_derivative(gpu, shape, dtype):
+    import torch
+    N, V = shape
+    for k, (scale, strided, wide) in enumerate([(1.0, False, True), (0.7, True, False)]):
+        print(shape, dtype, scale, strided, flush=True)
+        logits, held, target = rows_case(N, V, dtype, gpu, k, strided=strided)
+        y = torch.from_numpy(target).to(gpu, torch.int64 if wide else torch.int32)
+        logp, lse = torch.empty(N, device=gpu), torch.empty(N, device=gpu)
+        stage = hawk.stages.token_logp(scale=scale)
+        hawk.run(stage, logits=logits, target=y, logp=logp, lse=lse)
+        want, want_lse, l = oracle_rows(held, target, scale)
+        close_row(back(logp), want, want_lse)
+        close_row(back(lse), want_lse, want_lse)
+        c = np.random.default_rng(k).normal(size=N).astype(np.float32)
+        bar = torch.empty_like(logits)
+        hawk.run(stage.vjp, logits=logits, target=y, lse=lse, bar_logp=torch.from_numpy(c).to(gpu), bar_logits=bar)
+        grad, size = oracle_gradient(l, target, back(lse), c.astype(np.float64), scale)
+        close_gradient(back(bar), grad, size, l, back(lse), dtype)
+        # in place, and only logp
+        again = torch.empty(N, device=gpu)
+        hawk.run(stage, logits=logits, target=y, logp=again)
+        assert torch.equal(again, logp)
+        hawk.run(stage.vjp, logits=logits, target=y, lse=lse, bar_logp=torch.from_numpy(c).to(gpu), bar_logits=logits)
+        assert torch.equal(logits, bar)
+
+
+def oracle_policy(logp, target, old, A, ref, weight, clip, kl, bar):
+    kept = target >= 0
+    r = np.exp(logp - old)
+    plain, clipped = r * A, np.clip(r, 1 - clip[0], 1 + clip[1]) * A
+    loss, slope = -np.minimum(plain, clipped), np.where(plain <= clipped, -plain, 0.0)
+    if kl:
+        d = ref - logp
+        loss, slope = loss + kl * (np.expm1(d) - d), slope - kl * np.expm1(d)
+    return np.where(kept, loss * weight, 0), np.where(kept, slope * weight * bar, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+@pytest.mark.parametrize("dtype", ROW_TYPES)
+@pytest.mark.parametrize("shape", ROWS, ids=str)
+def test_policy_loss_and_its_gradient_in_one_pass_and_two(gpu, shape, dtype, kl):
+    import torch
+    N, V = shape
+    print(shape, dtype, kl, flush=True)
+    clip, scale = (0.2, 0.3), 0.9
+    logits, held, target = rows_case(N, V, dtype, gpu, 5, strided=True)
+    logp64, lse64, l = oracle_rows(held, target, scale)
+    g = np.random.default_rng([11, N, V])
+    f32 = lambda x: np.asarray(x, dtype=np.float32)  # noqa: E731
+    old, ref = f32(logp64 + 0.3 * g.normal(size=N)), f32(logp64 + 0.3 * g.normal(size=N))
+    A, weight = f32(g.normal(size=N)), f32(g.uniform(0.5, 1.5, N) / N)
+    y = torch.from_numpy(target).to(gpu)
+    dev = {n: torch.from_numpy(v).to(gpu) for n, v in (("old_logp", old), ("ref_logp", ref), ("advantage", A),
+                                                       ("weight", weight))}
+    out = {n: torch.empty(k, device=gpu) for n, k in (("loss", 1), ("logp", N), ("lse", N))}
+    stage = hawk.stages.policy_loss(clip=clip, kl=kl, scale=scale)
+    bar, cell = torch.empty_like(logits), torch.tensor([1.5], device=gpu)
+    hawk.run(stage, logits=logits, target=y, bar_logits=bar, bar_loss=cell, **dev, **out)
+    close_row(back(out["logp"]), logp64, lse64)
+    close_row(back(out["lse"]), lse64, lse64)
+    # the loss and slope of the log-probability that was written: a row near a bound of the ratio
+    # may fall on either side of it by an ulp of logp, so the slopes are the written logp's
+    logp = back(out["logp"])
+    loss, slope = oracle_policy(logp, target, *(v.astype(np.float64) for v in (old, A, ref, weight)), clip, kl, 1.5)
+    mass = np.abs(loss).sum() + np.abs(weight).sum() * (1 + np.abs(A).max())
+    assert abs(back(out["loss"])[0] - loss.sum()) <= 32 * 2.0 ** -24 * mass
+    edge = np.isclose(np.exp(logp - old), 1 - clip[0], atol=1e-6) | np.isclose(np.exp(logp - old), 1 + clip[1], atol=1e-6)
+    assert not edge.any()
+    grad, size = oracle_gradient(l, target, back(out["lse"]), slope, scale)
+    big = oracle_gradient(l, target, back(out["lse"]), 1.5 * weight * (np.abs(A) * 2 + 4 * kl), scale)[1]
+    close_gradient(back(bar), grad, np.maximum(size, big), l, back(out["lse"]), dtype)
+    two = torch.empty_like(logits)
+    saved = {n: out[n] for n in ("logp", "lse")}
+    hawk.run(stage.vjp, logits=logits, target=y, bar_logits=two, bar_loss=cell, **dev, **saved)
+    close_gradient(back(two), grad, np.maximum(size, big), l, back(out["lse"]), dtype)
+    # the loss alone, and the mean where no weight is given
+    alone = torch.empty(1, device=gpu)
+    hawk.run(stage, logits=logits, target=y, loss=alone, **dev)
+    assert torch.equal(alone, out["loss"])
+    del dev["weight"]
+    hawk.run(stage, logits=logits, target=y, loss=alone, **dev)
+    loss, _ = oracle_policy(logp, target, old.astype(np.float64), A.astype(np.float64), ref.astype(np.float64),
+                            np.full(N, 1.0 / N), clip, kl, 1.0)
+    assert abs(back(alone)[0] - loss.sum()) <= 32 * 2.0 ** -24 * (np.abs(loss).sum() + 1 + np.abs(A).max())
+    # in place
+    held_bar = bar.clone()
+    dev["weight"] = torch.from_numpy(weight).to(gpu)
+    hawk.run(stage, logits=logits, target=y, bar_logits=logits, bar_loss=cell, **dev, **out)
+    assert torch.equal(logits, held_bar)
+
+
+@pytest.mark.gpu
+def test_rows_that_are_masked_hold_anything(gpu):
+    """A left-out row, and one of weight 0, reach neither loss nor gradient whatever they hold; a target
+    past the vocabulary and a row with no finite logit are loud."""
+    import torch
+    for V in (40, 3000, 70000):
+        for dtype in (torch.float32, torch.bfloat16):
+            N = 6
+            logits = torch.randn(N, V, device=gpu).to(dtype)
+            logits[1] = math.nan
+            logits[2] = -math.inf
+            logits[4, 3:] = torch.finfo(dtype).min           # masked vocabulary
+            logits[4, 1] = -math.inf
+            target = torch.tensor([1, -1, 2, 3, 0, 1], device=gpu)
+            old = torch.zeros(N, device=gpu)
+            old[1], old[2] = math.nan, math.inf
+            A = torch.ones(N, device=gpu)
+            A[1] = A[2] = math.nan
+            weight = torch.full((N,), 0.25, device=gpu)
+            weight[1] = math.nan
+            weight[2] = 0.0
+            loss, logp, lse = (torch.empty(k, device=gpu) for k in (1, N, N))
+            bar = torch.empty_like(logits)
+            stage = hawk.stages.policy_loss(kl=0.1)
+            planes = dict(logits=logits, target=target, old_logp=old, advantage=A, ref_logp=old, weight=weight)
+            hawk.run(stage, loss=loss, logp=logp, lse=lse, bar_logits=bar, **planes)
+            assert torch.isfinite(loss).all() and torch.isfinite(bar).all()
+            assert (bar[1] == 0).all() and (bar[2] == 0).all() and logp[1] == 0 and lse[1] == 0
+            assert (bar[4, 3:] == 0).all() and bar[4, 0] != 0
+            want = torch.log_softmax(logits[4].double()[:3], 0)[0]
+            assert abs(logp[4].double() - want) < 1e-5
+            two = torch.empty_like(bar)
+            hawk.run(stage.vjp, logp=logp, lse=lse, bar_logits=two, **planes)
+            assert torch.isfinite(two).all() and (two[2] == 0).all()
+            target[3] = V
+            hawk.run(stage, loss=loss, logp=logp, bar_logits=bar, **planes)
+            assert torch.isnan(loss).all() and torch.isnan(logp[3]) and torch.isnan(bar[3]).all()
+            assert torch.isfinite(bar[0]).all()
+            # a row with no finite logit has no distribution
+            hawk.run(hawk.stages.token_logp(), logits=logits, target=target.clamp(max=V - 1), logp=logp, lse=lse)
+            assert torch.isnan(logp[2]) and lse[2] == -math.inf and torch.isfinite(logp[0])
+            # a row of the lowest value throughout is a row of equal logits
+            logits[0] = torch.finfo(dtype).min
+            hawk.run(hawk.stages.token_logp(), logits=logits, target=target.clamp(max=V - 1), logp=logp)
+            assert abs(float(logp[0]) + math.log(V)) < 1e-5
+
+
+@pytest.mark.gpu
+def test_the_policy_gradient_is_the_losss_difference_quotient(gpu):
+    """float32: a step of 2^-6 gives a truncation of about e^2 and a rounding of 2^-24 / e relative to
+    the loss, both below 1e-3."""
+    import torch
+    N, V = 5, 12
+    g = torch.Generator(device=gpu).manual_seed(9)
+    logits = torch.randn(N, V, generator=g, device=gpu)
+    target = torch.tensor([3, 0, 11, -1, 5], device=gpu)
+    base = torch.log_softmax(logits, 1)[torch.arange(N), target.clamp(min=0)]
+    planes = dict(target=target, old_logp=base + torch.tensor([0.05, -0.4, 0.4, 0.0, 0.1], device=gpu),
+                  ref_logp=base + 0.2, advantage=torch.tensor([1.0, 0.7, -0.8, 1.0, -0.5], device=gpu))
+    stage = hawk.stages.policy_loss(kl=0.2)
+    bar, loss = torch.empty_like(logits), torch.empty(1, device=gpu)
+    hawk.run(stage, logits=logits, loss=loss, bar_logits=bar, **planes)
+    e = 2.0 ** -6
+    for n, v in [(0, 3), (0, 1), (1, 0), (1, 7), (2, 11), (2, 2), (3, 4), (4, 5)]:
+        ends = []
+        for sign in (1, -1):
+            moved = logits.clone()
+            moved[n, v] += sign * e
+            hawk.run(stage, logits=moved, loss=loss, **planes)
+            ends.append(float(loss))
+        assert abs((ends[0] - ends[1]) / (2 * e) - float(bar[n, v])) < 1e-3, (n, v)
+
+
+def oracle_pairs(logp, target, ref, offsets, weight, beta, eps):
+    ratio = np.where(target >= 0, logp - ref, 0)
+    sums = np.array([ratio[offsets[k]:offsets[k + 1]].sum() for k in range(len(offsets) - 1)])
+    margin = sums[0::2] - sums[1::2]
+    z = beta * margin
+    soft = np.log1p(np.exp(-np.abs(z)))
+    loss = (1 - eps) * (soft + np.maximum(-z, 0)) + eps * (soft + np.maximum(z, 0))
+    up = 1 / (1 + np.exp(-z))
+    return margin, (weight * loss).sum(), beta * weight * (eps * up - (1 - eps) * (1 - up))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ROW_TYPES)
+@pytest.mark.parametrize("lengths,V", [((1, 1), 5), ((3, 0, 0, 2), 17), ((30, 41, 7, 64, 129, 2), 300),
+                                       ((5, 4, 3, 9, 0, 0, 8, 1, 2, 6), 5003)], ids=str)
+def test_preference_loss_and_its_gradient(gpu, lengths, V, dtype):
+    import torch
+    N, P = sum(lengths), len(lengths) // 2
+    print(lengths, V, dtype, flush=True)
+    beta, eps, scale = 0.3, 0.1, 1.2
+    logits, held, target = rows_case(N, V, dtype, gpu, 3)
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    g = np.random.default_rng([13, N, V])
+    logp64, lse64, l = oracle_rows(held, target, scale)
+    ref = (logp64 + 0.2 * g.normal(size=N)).astype(np.float32)
+    weight = g.uniform(0.5, 1.5, P).astype(np.float32)
+    stage = hawk.stages.preference_loss(beta=beta, smoothing=eps, scale=scale)
+    planes = dict(logits=logits, target=torch.from_numpy(target).to(gpu),
+                  offsets=torch.from_numpy(offsets).to(gpu, torch.int32 if P % 2 else torch.int64))
+    out = {n: torch.empty(k, device=gpu) for n, k in (("loss", 1), ("margin", P), ("logp", N), ("lse", N))}
+    w = torch.from_numpy(weight).to(gpu)
+    hawk.run(stage, ref_logp=torch.from_numpy(ref).to(gpu), weight=w, **planes, **out)
+    margin, loss, slope = oracle_pairs(back(out["logp"]), target, ref.astype(np.float64), offsets,
+                                       weight.astype(np.float64), beta, eps)
+    close_row(back(out["logp"]), logp64, lse64)
+    # the sums are in 64 bits over the written log-probabilities: only the cells round
+    assert (np.abs(back(out["margin"]) - margin) <= 4 * 2.0 ** -24 * (np.abs(margin) + 1e-6)).all()
+    assert abs(back(out["loss"])[0] - loss) <= 16 * 2.0 ** -24 * (abs(loss) + weight.sum())
+    seq = np.searchsorted(offsets, np.arange(N), side="right") - 1
+    c = 1.5 * np.where(seq % 2 == 0, slope[seq // 2], -slope[seq // 2])
+    grad, size = oracle_gradient(l, target, back(out["lse"]), c, scale)
+    bar = torch.empty_like(logits)
+    hawk.run(stage.vjp, margin=out["margin"], lse=out["lse"], weight=w, bar_loss=torch.tensor(1.5, device=gpu),
+             bar_logits=bar, **planes)
+    # sigma's own error: 32 u relative
+    close_gradient(back(bar), grad, size, l, back(out["lse"]), dtype, slack=64 * 2.0 ** -24)
+    # the loss alone, no reference: 1 / pairs each
+    hawk.run(stage, loss=out["loss"], **planes)
+    _, mean, _ = oracle_pairs(logp64, target, np.zeros(N), offsets, np.full(P, 1.0 / P), beta, eps)
+    assert abs(back(out["loss"])[0] - mean) <= 1e-5 * (1 + abs(mean) + np.abs(logp64).sum())
+
+
+@pytest.mark.gpu
+def test_a_pair_of_weight_zero_and_an_extreme_margin(gpu):
+    import torch
+    logits = torch.randn(4, 50, device=gpu)
+    target = torch.tensor([0, 1, 2, 3], device=gpu)
+    planes = dict(logits=logits, target=target, offsets=torch.tensor([0, 1, 2, 3, 4], device=gpu))
+    ref = torch.tensor([0.0, 0.0, -2000.0, 3000.0], device=gpu)
+    out = {n: torch.empty(k, device=gpu) for n, k in (("loss", 1), ("margin", 2), ("lse", 4))}
+    stage = hawk.stages.preference_loss(beta=1.0)
+    hawk.run(stage, ref_logp=ref, **planes, **out)
+    assert torch.isfinite(out["loss"]).all()
+    hawk.run(stage, ref_logp=-ref, **planes, **out)
+    assert abs(float(out["loss"]) - 2500) < 10            # half of about 5000: the losing pair's -log sigma(z) = -z
+    ref[2] = math.nan
+    weight = torch.tensor([1.0, 0.0], device=gpu)
+    hawk.run(stage, ref_logp=ref, weight=weight, **planes, **out)
+    assert torch.isfinite(out["loss"]).all() and torch.isnan(out["margin"][1])
+    bar = torch.empty_like(logits)
+    hawk.run(stage.vjp, weight=weight, margin=out["margin"], lse=out["lse"], bar_logits=bar, **planes)
+    assert torch.isfinite(bar).all() and (bar[2:] == 0).all() and (bar[:2] != 0).any()
+
+
+@pytest.mark.gpu
+def test_row_losses_replayed_from_a_graph_and_repeated(gpu):
+    import torch
+    N, V = 40, 9001
+    logits = torch.randn(N, V, device=gpu).bfloat16()
+    target = torch.randint(0, V, (N,), device=gpu)
+    old, A = -9.0 + torch.randn(N, device=gpu), torch.randn(N, device=gpu)
+    stage = hawk.stages.policy_loss()
+    planes = dict(logits=logits, target=target, old_logp=old, advantage=A)
+    loss, bar = torch.empty(1, device=gpu), torch.empty_like(logits)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    launch = stage.prepare(loss=loss, bar_logits=bar, stream=side, **planes)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        launch()
+    for k in range(4):
+        logits.copy_(torch.randn(N, V, device=gpu))
+        want, wbar = torch.empty(1, device=gpu), torch.empty_like(logits)
+        hawk.run(stage, loss=want, bar_logits=wbar, **planes)
+        loss.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want) and torch.equal(bar, wbar)
+
+
+# -- dropout ---------------------------------------------------------------------------------
+
+def philox(group, offset, seed):
+    """Philox4x32-10 in Python integers."""
+    low = 0xFFFFFFFF
+    c = [group & low, group >> 32, offset & low, offset >> 32]
+    k = [seed & low, seed >> 32]
+    for _ in range(10):
+        p, q = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(q >> 32) ^ c[1] ^ k[0], q & low, (p >> 32) ^ c[3] ^ k[1], p & low]
+        k = [(k[0] + 0x9E3779B9) & low, (k[1] + 0xBB67AE85) & low]
+    return c
+
+
+def kept(n, cut, offset, seed):
+    out = np.empty(n, bool)
+    for g in range((n + 7) // 8):
+        w = philox(g, offset, seed)
+        for j in range(min(8, n - 8 * g)):
+            out[8 * g + j] = (w[j // 2] >> (16 * (j % 2)) & 0xFFFF) >= cut
+    return out
+
+
+def test_the_generator_is_philox_4x32_10():
+    """The published known answers (Random123's kat_vectors)."""
+    assert philox(0, 0, 0) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = (1 << 64) - 1
+    assert philox(ones, ones, ones) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert philox(0x85A308D3243F6A88, 0x0370734413198A2E, 0x299F31D0A4093822) == [
+        0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1,), (7,), (8,), (3, 5), (65, 129), (2, 3, 40), (1000, 17), (31, 512)], ids=str)
+def test_dropout_and_its_derivative_are_the_generators_mask(gpu, shape, dtype):
+    import torch
+    print(shape, dtype, flush=True)
+    g = np.random.default_rng(21)
+    n = int(np.prod(shape))
+    for p, seed, offset in ((0.25, 5, 0), (0.1, (1 << 64) - 3, (1 << 40) + 7), (0.0, 1, 2), (1.0, 1, 2)):
+        x, xv = plane(g.normal(size=shape), dtype, gpu)
+        res, rv = plane(g.normal(size=shape), dtype, gpu)
+        cut = round(p * 65536)
+        mask = kept(n, cut, offset, seed).reshape(shape)
+        stage = hawk.stages.dropout(p)
+        y = torch.empty_like(x)
+        hawk.run(stage, x=x, y=y, seed=seed, offset=offset)
+        # two roundings: the factor and the product in the arithmetic's type, then the output's
+        want = np.where(mask, xv * (65536.0 / (65536 - cut) if cut < 65536 else 0), 0)
+        assert (np.abs(back(y) - want) <= (4 * U[dtype] + R[dtype]) * 1.01 * np.abs(want) + TINY[dtype]).all()
+        assert ((back(y) == 0) == ~mask).all() or p == 0
+        hawk.run(stage, x=x, residual=res, y=y, seed=seed, offset=offset)
+        size = np.abs(want) + np.abs(rv)
+        assert (np.abs(back(y) - want - rv) <= (8 * U[dtype] + R[dtype]) * 1.01 * size + TINY[dtype]).all()
+        bar = torch.empty_like(x)
+        hawk.run(diff.vjp(stage), bar_y=x, bar_x=bar, seed=seed, offset=offset)
+        assert (np.abs(back(bar) - want) <= (4 * U[dtype] + R[dtype]) * 1.01 * np.abs(want) + TINY[dtype]).all()
+        # the offset from a cell, in place, and through rows apart: the same mask
+        hawk.run(stage, x=x.clone(), y=bar, seed=seed, offset=torch.tensor([offset], device=gpu))
+        hawk.run(stage, x=x, y=y, seed=seed, offset=offset)
+        assert torch.equal(bar, y)
+        if len(shape) > 1:
+            wide = torch.zeros((*shape[:-1], shape[-1] + 3), dtype=x.dtype, device=gpu)
+            apart = wide[..., 1:1 + shape[-1]]
+            apart.copy_(x)
+            hawk.run(stage, x=apart, y=apart, seed=seed, offset=offset)
+            assert torch.equal(apart, y) and (wide[..., 0] == 0).all() and (wide[..., -2:] == 0).all()
+        hawk.run(stage, x=x, y=x, seed=seed, offset=offset)
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_dropout_drops_infinities_and_keeps_its_rate(gpu):
+    import torch
+    n = 1 << 20
+    x = torch.full((n,), math.inf, device=gpu)
+    y = torch.empty_like(x)
+    hawk.run(hawk.stages.dropout(0.5), x=x, y=y, seed=3)
+    assert ((y == 0) | torch.isinf(y)).all()
+    hawk.run(hawk.stages.dropout(0.1), x=torch.ones_like(x), y=y, seed=4, offset=9)
+    rate = float((y == 0).double().mean())
+    cut = 6554 / 65536                                    # round(0.1 * 2^16) / 2^16
+    assert abs(rate - cut) < 6 * math.sqrt(cut * (1 - cut) / n)
+    other = torch.empty_like(y)
+    hawk.run(hawk.stages.dropout(0.1), x=torch.ones_like(x), y=other, seed=4, offset=10)
+    assert abs(float(((y == 0) & (other == 0)).double().mean()) - cut ** 2) < 6 * cut / math.sqrt(n)
+
+
+@pytest.mark.gpu
+def test_dropout_draws_a_new_mask_a_replay(gpu):
+    import torch
+    x = torch.ones(5000, device=gpu)
+    y, cell = torch.empty_like(x), torch.zeros(1, dtype=torch.int64, device=gpu)
+    stage = hawk.stages.dropout(0.5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    launch = stage.prepare(x=x, y=y, seed=8, offset=cell, stream=side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        launch()
+        cell.add_(1)
+    for k in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.empty_like(x)
+        hawk.run(stage, x=x, y=want, seed=8, offset=k)
+        assert torch.equal(y, want)
+
+
+# -- refusals --------------------------------------------------------------------------------
+
+def test_options_out_of_range_are_refused():
+    s = hawk.stages
+    for call, text in ((lambda: s.recurrence(gate="tanh"), "gate="), (lambda: s.dropout(1.5), "p="),
+                       (lambda: s.dropout(1e-7), "resolution"), (lambda: s.dropout(True), "p="),
+                       (lambda: s.policy_loss(clip=-0.1), "clip="), (lambda: s.policy_loss(kl=math.nan), "kl="),
+                       (lambda: s.token_logp(scale=0.0), "scale="), (lambda: s.token_logp(scale=math.inf), "scale="),
+                       (lambda: s.preference_loss(smoothing=1.5), "smoothing="),
+                       (lambda: s.preference_loss(beta=math.inf), "beta=")):
+        with pytest.raises(HawkError, match=text):
+            call()
+
+
+def test_names_missing_planes_and_launch_options_are_refused():
+    import torch
+    x = torch.zeros(1, 2, 3)
+    scan = hawk.stages.recurrence()
+    with pytest.raises(HawkError, match="no plane is named 'y'"):
+        hawk.run(scan, gate=x, x=x, y=x)
+    with pytest.raises(HawkError, match="'x' is not given"):
+        hawk.run(scan, gate=x, h=x)
+    with pytest.raises(HawkError, match="no output"):
+        hawk.run(scan.vjp, gate=x, h=x, bar_h=x)
+    with pytest.raises(HawkError, match="not on a ROCm device"):
+        hawk.run(scan, gate=x, x=x, h=x)
+    with pytest.raises(HawkError, match="torch tensor"):
+        hawk.run(scan, gate=x.numpy(), x=x, h=x)
+    with pytest.raises(HawkError, match="no base="):
+        hawk.run(scan, base=1, gate=x, x=x, h=x)
+    with pytest.raises(HawkError, match="seed"):
+        hawk.run(hawk.stages.dropout(0.5), x=x, y=x)
+    with pytest.raises(HawkError, match="wrt="):
+        diff.vjp(scan, wrt=("x",))
+    with pytest.raises(HawkError, match="no derivative"):
+        diff.vjp(scan.vjp)
+
+
+@pytest.mark.gpu
+def test_planes_that_do_not_fit_are_refused(gpu):
+    import torch
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device=gpu)  # noqa: E731
+    scan, x = hawk.stages.recurrence(), z(2, 5, 3)
+    bad = [
+        (scan, dict(gate=x, x=z(2, 5, 4), h=x.clone()), "x.*is"),
+        (scan, dict(gate=x, x=x.half(), h=x.clone()), "float16"),
+        (scan, dict(gate=x.int(), x=x.int(), h=x.int()), "planes are"),
+        (scan, dict(gate=x[0], x=x[0], h=x[0].clone()), "offsets"),
+        (scan, dict(gate=x, x=x, h=z(2, 1, 3).expand(2, 5, 3)), "repeats memory"),
+        (scan, dict(gate=x, x=x, h=x.clone(), h0=z(2, 4)), "state"),
+        (scan, dict(gate=x, x=x, h=x.clone(), h0=z(2, 3, dtype=torch.float64)), "state"),
+        (scan, dict(gate=x[0], x=x[0], h=x[0].clone(), offsets=z(3)), "int32 or int64"),
+        (scan, dict(gate=x, x=x, h=x.clone(), offsets=z(3, dtype=torch.int32)), "packed planes"),
+        (scan.vjp, dict(gate=x, h=x, bar_h=x, bar_x=x), "one tensor"),
+        (hawk.stages.recurrence("sigmoid").vjp, dict(gate=x, h=x, bar_h=x, bar_gate=x.clone()), "'x' is not given"),
+    ]
+    t = torch.zeros(4, dtype=torch.int64, device=gpu)
+    logp, pol, pref = hawk.stages.token_logp(), hawk.stages.policy_loss(kl=0.1), hawk.stages.preference_loss()
+    l = z(4, 9)
+    bad += [
+        (logp, dict(logits=l.double(), target=t, logp=z(4)), "float32"),
+        (logp, dict(logits=z(9, 4).t(), target=t, logp=z(4)), "contiguous"),
+        (logp, dict(logits=l, target=t[:3], logp=z(4)), "rows"),
+        (logp, dict(logits=l, target=t.float(), logp=z(4)), "int32 or int64"),
+        (logp, dict(logits=l, target=t, logp=z(5)), "'logp'"),
+        (logp, dict(logits=l, target=t), "no output"),
+        (logp.vjp, dict(logits=l, target=t, lse=z(4), bar_logp=z(4), bar_logits=l.half()), "bar_logits"),
+        (logp.vjp, dict(logits=l, target=t, lse=z(4), bar_logp=z(4), bar_logits=z(40).as_strided((4, 9), (5, 1))),
+         "overlap"),
+        (pol, dict(logits=l, target=t, old_logp=z(4), advantage=z(4), loss=z(1)), "ref_logp"),
+        (pol, dict(logits=l, target=t, old_logp=z(4), advantage=z(4), ref_logp=z(4), loss=z(2)), "'loss'"),
+        (pref, dict(logits=l, target=t, offsets=t, loss=z(1)), "2 \\* pairs"),
+        (pref, dict(logits=l, target=t, offsets=t[:3], loss=z(1), margin=z(2)), "'margin'"),
+    ]
+    d = hawk.stages.dropout(0.5)
+    bad += [
+        (d, dict(x=l, y=z(4, 8), seed=0), "'y'"),
+        (d, dict(x=l, y=l.half(), seed=0), "float16"),
+        (d, dict(x=l, y=l.clone(), seed=-1), "seed="),
+        (d, dict(x=l, y=l.clone(), seed=0, offset=1 << 64), "offset="),
+        (d, dict(x=l, y=l.clone(), seed=0, offset=z(1)), "int64 cell"),
+        (d, dict(x=z(9, 4).t(), y=l.clone(), seed=0), "contiguous"),
+        (d, dict(x=z(4, 3, 2, 9)[:, :2], y=z(4, 2, 2, 9), seed=0), "evenly apart"),
+    ]
+    for stage, planes, text in bad:
+        with pytest.raises(HawkError, match=text):
+            hawk.run(stage, **planes)
+        with pytest.raises(HawkError, match=text):
+            stage.prepare(**planes)
+
+
+def test_the_entries_refuse_bad_jobs():
+    """The C entries check their jobs before any launch."""
+    L = _core.lib()
+    r = _core.RecurrenceJob()
+    r.seqs, r.steps, r.chans = 1, 4, 4
+    ref = ctypes.byref(r)
+    assert L.hk_recurrence(None, None, None) == 1
+    assert L.hk_recurrence(ref, None, None) == 1 and b"plane is missing" in L.hk_last_error()
+    r.steps = -1
+    assert L.hk_recurrence_vjp(ref, None, None) == 1 and b">= 0" in L.hk_last_error()
+    r.steps, r.dtype = 4, 9
+    assert L.hk_recurrence(ref, None, None) == 1 and b"element type" in L.hk_last_error()
+    assert L.hk_recurrence_scratch_bytes(None, 0) == 0
+    w = _core.RowLossJob()
+    w.rows, w.vocab, w.scale = 2, 5, 1.0
+    ref = ctypes.byref(w)
+    for fn in (L.hk_token_logp, L.hk_token_logp_vjp, L.hk_policy_loss, L.hk_policy_loss_vjp, L.hk_preference_loss,
+               L.hk_preference_loss_vjp):
+        assert fn(None, None, None) == 1
+        assert fn(ref, None, None) == 1 and b"required" in L.hk_last_error()
+    w.scale = 0.0
+    assert L.hk_token_logp(ref, None, None) == 1 and b"scale" in L.hk_last_error()
+    w.scale, w.dtype = 1.0, 1
+    assert L.hk_token_logp(ref, None, None) == 1 and b"16-bit" in L.hk_last_error()
+    d = _core.DropoutJob()
+    d.rows, d.cols, d.cut = 1, 4, 70000
+    assert L.hk_dropout(ctypes.byref(d), None) == 1 and b"cut" in L.hk_last_error()
+    d.cut = 5
+    assert L.hk_dropout(ctypes.byref(d), None) == 1 and b"required" in L.hk_last_error()
+    # nothing to do is not an error
+    r.dtype, r.seqs = 0, 0
+    assert L.hk_recurrence(ctypes.byref(r), None, None) == 0
+    w.dtype, w.rows = 0, 0
+    assert L.hk_token_logp(ctypes.byref(w), None, None) == 0
+
+
+def test_the_jobs_are_laid_out_as_the_header_has_them():
+    assert ctypes.sizeof(_core.SeqPlane) == 32
+    assert ctypes.sizeof(_core.RecurrenceJob) == 6 * 32 + 5 * 8 + 3 * 8 + 4 * 4
+    assert ctypes.sizeof(_core.RowLossJob) == 14 * 8 + 5 * 8 + 6 * 4 + 3 * 4 + 4
+    assert ctypes.sizeof(_core.DropoutJob) == 4 * 8 + 5 * 8 + 2 * 8 + 2 * 4
