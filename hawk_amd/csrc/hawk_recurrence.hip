@@ -35,6 +35,14 @@ struct Plane {
     int64_t seq, step, chan;
 };
 
+// What tiles tell each other goes through words that say themselves whether
+// they are written: all bits set is "not yet", and a NaN is published as the
+// one quiet NaN, which is not that.  So relaxed accesses at the GPU's scope are
+// enough, with no order among them.
+template <class A> struct Word;
+template <> struct Word<float> { typedef uint32_t type; static constexpr uint32_t kNan = 0x7fc00000u; };
+template <> struct Word<double> { typedef uint64_t type; static constexpr uint64_t kNan = 0x7ff8000000000000ull; };
+
 template <class T>
 struct RecArgs {
     Plane<T> gate, x, h, bar_h, bar_gate, bar_x;
@@ -42,15 +50,14 @@ struct RecArgs {
     const Acc<T>* h0;         // the derivative's h_(-1)
     Acc<T>* fin;              // the state that leaves it: last, or bar_h0
     const void* offsets;
-    Acc<T>*agg_p, *agg_h;     // [chunk][seqs * chans]: each tile's (P, H)
-    Acc<T>* carry;            // [chunk][seqs * chans]: the state that enters each tile
+    uint32_t* counter;        // hands the tiles out in order
+    typename Word<Acc<T>>::type* agg;      // [chunk][states][2]: each tile's (P, H)
+    typename Word<Acc<T>>::type* state;    // [chunk][states]: the state that leaves each tile
     int64_t seqs, chans, cols, states;   // states: those of one tile row, seqs * chans (packed: chans)
     int steps, groups;        // groups: threads across a row's channels
-    int lcol, lt, chunks;     // log2 of a tile's columns and of its time lanes
+    int lcol, nt, strips, chunks;   // a tile: 2^lcol columns by nt threads along the steps
     int rev, offsets64;       // rev: scan step i is row steps - 1 - i (packed planes)
 };
-
-enum Phase { kSingle, kAggregate, kApply };
 
 __device__ __forceinline__ int64_t cut_at(const void* offsets, int wide, int64_t s) {
     return wide ? static_cast<const int64_t*>(offsets)[s] : static_cast<const int32_t*>(offsets)[s];
@@ -67,30 +74,31 @@ __device__ __forceinline__ int64_t sequence_of(const void* offsets, int wide, in
     return low;
 }
 
-// One thread's K steps of V channels.  Chan: V consecutive channels a step,
-// each step a load of its own; otherwise one channel, K steps in one load where
-// the steps are contiguous (Dir 1, or -1 where the scan runs down the axis).
-// A step past the end repeats the last one's address, so every load is issued
-// without a branch; its value is replaced afterwards.
+// One thread's K steps of V channels, left in the plane's type.  Dir 0: V
+// consecutive channels a step, each step a load of its own; otherwise one
+// channel, K steps in one load where the steps are contiguous (Dir 1, or -1
+// where the scan runs down the axis).  A step past the end repeats the last
+// one's address, so every load is issued without a branch.
 template <class T, int V, int K, int Dir>
-__device__ __forceinline__ void tile_load(const Plane<T>& p, const T* base, int row0, int steps, Acc<T> (&out)[K][V]) {
+__device__ __forceinline__ void tile_load(const Plane<T>& p, int64_t s, int64_t c, int row0, int steps,
+                                          Raw<T, V> (&out)[K]) {
+    const T* base = p.data + s * p.seq + c * p.chan;
     if constexpr (Dir == 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int row = row0 + k < steps ? row0 + k : steps - 1;
-            load<T, V>(base + row * p.step, out[k]);
+            out[k] = load_raw<T, V>(base + row * p.step);
         }
     } else {
         if (row0 + K <= steps) {
-            Acc<T> flat[K];
-            load<T, K>(Dir > 0 ? base + row0 : base - (row0 + K - 1), flat);
+            const Raw<T, K> flat = load_raw<T, K>(Dir > 0 ? base + row0 : base - (row0 + K - 1));
 #pragma unroll
-            for (int k = 0; k < K; ++k) out[k][0] = flat[Dir > 0 ? k : K - 1 - k];
+            for (int k = 0; k < K; ++k) out[k] = flat[Dir > 0 ? k : K - 1 - k];
         } else {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int row = row0 + k < steps ? row0 + k : steps - 1;
-                load<T, 1>(Dir > 0 ? base + row : base - row, out[k]);
+                out[k] = Dir > 0 ? base[row] : base[-row];
             }
         }
     }
@@ -99,77 +107,126 @@ __device__ __forceinline__ void tile_load(const Plane<T>& p, const T* base, int 
 // Stores the tile's steps that exist; `skip` leading channels belong to the
 // neighbouring thread.
 template <class T, int V, int K, int Dir>
-__device__ __forceinline__ void tile_store(const Plane<T>& p, T* base, int row0, int rows, int skip,
-                                           const Acc<T> (&x)[K][V]) {
+__device__ __forceinline__ void tile_store(const Plane<T>& p, int64_t s, int64_t c, int row0, int rows, int skip,
+                                           const Raw<T, V> (&x)[K]) {
+    T* base = p.data + s * p.seq + c * p.chan;
     if constexpr (Dir == 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             T* to = base + (row0 + k) * p.step;
             if (k >= rows) continue;
             if (skip == 0) {
-                store<T, V>(to, x[k]);
-            } else {
+                *reinterpret_cast<typename VecOf<T, V>::loose*>(to) = x[k];
+            } else if constexpr (V > 1) {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (v >= skip) to[v] = static_cast<T>(x[k][v]);
+                    if (v >= skip) to[v] = x[k][v];
             }
         }
     } else {
         if (rows == K) {
-            Acc<T> flat[K];
+            Raw<T, K> flat;
 #pragma unroll
-            for (int k = 0; k < K; ++k) flat[Dir > 0 ? k : K - 1 - k] = x[k][0];
-            store<T, K>(Dir > 0 ? base + row0 : base - (row0 + K - 1), flat);
+            for (int k = 0; k < K; ++k) flat[Dir > 0 ? k : K - 1 - k] = x[k];
+            *reinterpret_cast<typename VecOf<T, K>::loose*>(Dir > 0 ? base + row0 : base - (row0 + K - 1)) = flat;
         } else {
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (k < rows) *(Dir > 0 ? base + row0 + k : base - row0 - k) = static_cast<T>(x[k][0]);
+                if (k < rows) *(Dir > 0 ? base + row0 + k : base - row0 - k) = x[k];
         }
     }
 }
 
+template <class A>
+__device__ __forceinline__ void publish(typename Word<A>::type* at, A x) {
+    typedef typename Word<A>::type W;
+    W w = __builtin_bit_cast(W, x);
+    if (!(x == x)) w = Word<A>::kNan;
+    __hip_atomic_store(at, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class A>
+__device__ __forceinline__ bool read(const typename Word<A>::type* at, A& x) {
+    typedef typename Word<A>::type W;
+    const W w = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = __builtin_bit_cast(A, w);
+    return w != ~W(0);
+}
+// A word that its tile has written, or is about to: that tile has begun (see
+// the order of tiles below), so the wait ends.
+template <class A>
+__device__ __forceinline__ A await(const typename Word<A>::type* at) {
+    A x;
+    while (!read<A>(at, x)) __builtin_amdgcn_s_sleep(1);
+    return x;
+}
+
+constexpr int kBatch = 8;        // aggregates read at once
+
 template <class T, int V, int K, int Dir, bool Sigmoid, bool Vjp, bool Packed>
-__global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T> a, const int phase) {
+__global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T> a) {
     typedef Acc<T> A;
-    __shared__ A lds_p[kThreads * V], lds_h[kThreads * V];
+    // A sigmoid gate is never 0, so only packed bounds and plain gates can cut.
+    constexpr bool Cut = !Sigmoid || Packed;
+    __shared__ A lds_p[kThreads * V], lds_h[kThreads * V], lds_c[kThreads * V];
+    __shared__ int lds_tile, lds_from;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int ncol = 1 << a.lcol, nt = 1 << a.lt;
-    const int chunk = blockIdx.x % a.chunks;
-    const int here = Dir == 0 ? tid & (ncol - 1) : tid >> a.lt;
-    const int tl = Dir == 0 ? tid >> a.lcol : tid & (nt - 1);
-    const int64_t col = static_cast<int64_t>(blockIdx.x / a.chunks) * ncol + here;
-    const bool live = col < a.cols;
-    const int64_t s = live ? col / a.groups : 0;
-    int64_t c0 = live ? (col % a.groups) * V : 0;
-    int skip = 0;
-    if (c0 + V > a.chans) {              // the row's last channels: a full vector that ends with them
-        skip = static_cast<int>(c0 + V - a.chans);
-        c0 = a.chans - V;
+    const int ncol = 1 << a.lcol, nt = a.nt;
+
+    // Tiles are taken in the order of a counter, all columns of a chunk of steps
+    // before the next chunk's: whatever a tile waits for has begun before it.
+    int tile = blockIdx.x;
+    if (a.chunks > 1) {
+        if (tid == 0) lds_tile = static_cast<int>(atomicAdd(a.counter, 1u));
+        __syncthreads();
+        tile = lds_tile;
     }
+    const int chunk = tile / a.strips;
+    const int64_t col0 = static_cast<int64_t>(tile - chunk * a.strips) << a.lcol;
+    const int here = Dir == 0 ? tid & (ncol - 1) : tid / nt;
+    const int tl = Dir == 0 ? tid >> a.lcol : tid - here * nt;
+    // a column's sequence and first channel; the row's last channels are a full
+    // vector that ends with them, whose first `skip` are the neighbour's
+    auto place = [&](int64_t col, int64_t& s, int64_t& c, int& skip) {
+        s = col / a.groups;
+        c = (col - s * a.groups) * V;
+        skip = 0;
+        if (c + V > a.chans) {
+            skip = static_cast<int>(c + V - a.chans);
+            c = a.chans - V;
+        }
+    };
+    const bool live = here < ncol && col0 + here < a.cols;
+    int64_t s = 0, c0 = 0;
+    int skip = 0;
+    if (live) place(col0 + here, s, c0, skip);
     const int row0 = chunk * (nt * K) + tl * K;
     const int left = a.steps - row0;
     const int rows = !live || left < 0 ? 0 : left < K ? left : K;
     const int64_t first_state = s * a.chans + c0;    // dense planes: this thread's states
 
-    // load everything the tile needs
     const int at = row0 < a.steps ? row0 : a.steps - 1;
-    A gate[K][V], in[K][V], x[K][V], prior[K][V];
-    tile_load<T, V, K, Dir>(a.gate, a.gate.data + s * a.gate.seq + c0 * a.gate.chan, at, a.steps, gate);
+    Raw<T, V> gate[K], in[K], x[K], prior[K];
+    tile_load<T, V, K, Dir>(a.gate, s, c0, at, a.steps, gate);
+    tile_load<T, V, K, Dir>(Vjp ? a.bar_h : a.x, s, c0, at, a.steps, in);
     if constexpr (Vjp) {
-        tile_load<T, V, K, Dir>(a.bar_h, a.bar_h.data + s * a.bar_h.seq + c0 * a.bar_h.chan, at, a.steps, in);
-        if (phase != kAggregate) {
-            if constexpr (Sigmoid)
-                tile_load<T, V, K, Dir>(a.x, a.x.data + s * a.x.seq + c0 * a.x.chan, at, a.steps, x);
-            // h a step earlier in the primal's direction, a step later in the scan's
-            tile_load<T, V, K, Dir>(a.h, a.h.data + s * a.h.seq + c0 * a.h.chan,
-                                    at + 1 < a.steps ? at + 1 : a.steps - 1, a.steps, prior);
+        // h a step earlier in the primal's direction, a step later in the scan's
+        tile_load<T, V, K, Dir>(a.h, s, c0, at + 1 < a.steps ? at + 1 : a.steps - 1, a.steps, prior);
+        if constexpr (Sigmoid) tile_load<T, V, K, Dir>(a.x, s, c0, at, a.steps, x);
+    }
+    if (rows < K) {                       // steps that do not exist leave the state as it is
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (k < rows) continue;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                put<T, V>(gate[k], v, static_cast<T>(Sigmoid ? INFINITY : 1.0f));
+                put<T, V>(in[k], v, static_cast<T>(0.0f));
+            }
         }
-    } else {
-        tile_load<T, V, K, Dir>(a.x, a.x.data + s * a.x.seq + c0 * a.x.chan, at, a.steps, in);
     }
 
     // packed rows: which of this thread's begin a sequence in the scan's
-    // direction, which end one, and the sequence each is in
+    // direction, which end one, and the sequence the first is in
     unsigned begins = 0, ends = 0;
     int64_t seq_at = 0;
     if constexpr (Packed) {
@@ -179,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
             int64_t q = seq_at, low = cut_at(a.offsets, a.offsets64, q), high = cut_at(a.offsets, a.offsets64, q + 1);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (k >= rows) break;
+                if (k >= rows) continue;
                 const int64_t r = a.rev ? row - k : row + k;
                 while (!a.rev && r >= high && q + 1 < a.seqs) {
                     ++q;
@@ -196,16 +253,32 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
             }
         }
     }
-    // The sequence of the k-th row, walking on from the k-1st's: begins bit k
-    // moves to the next sequence that is not empty.
+    // The sequence of the k-th row where it begins one.
     auto moved = [&](int k, int64_t q) -> int64_t {
-        if (k == 0) return q;
-        const int64_t r = a.rev ? a.steps - 1 - row0 - k : row0 + k;
-        return sequence_of(a.offsets, a.offsets64, a.seqs, r);
+        return k == 0 ? q : sequence_of(a.offsets, a.offsets64, a.seqs, a.rev ? a.steps - 1 - row0 - k : row0 + k);
     };
+    auto begin = [&](int64_t q, int v) -> A { return a.init ? a.init[q * a.chans + c0 + v] : A(0); };
+
+    // The forward's sigmoid is taken once and its (a, b) kept; other gates and
+    // inputs cost less to convert twice than to hold twice as wide.
+    constexpr bool Keep = Sigmoid && !Vjp;
+    A kept_a[Keep ? K : 1][V], kept_b[Keep ? K : 1][V];
+    auto coefficients = [&](int k, int v, A& g, A& rest, A& b) {
+        g = widen<T, V>(gate[k], v);
+        if constexpr (Sigmoid) sigmoid(g, g, rest);
+        b = widen<T, V>(in[k], v);
+        if constexpr (!Vjp && Sigmoid) b *= rest;
+    };
+    // one step: the state after it, of the state before it
+    auto step = [&](A g, A b, A h) -> A {
+        if constexpr (Vjp) return Cut && g == A(0) ? A(0) : g * (b + h);
+        else return Cut && g == A(0) ? b : fused(g, h, b);
+    };
+    auto join = [&](A p, A q) -> A { return Cut ? chain(p, q) : p * q; };
+    auto apply = [&](A p, A h, A add) -> A { return Cut ? add + cutmul(p, h) : fused(p, h, add); };
 
     // fold this thread's steps from a zero state
-    A local[K][V], product[K][V], P[V], H[V];
+    A P[V], H[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { P[v] = A(1); H[v] = A(0); }
     int64_t q = seq_at;
@@ -215,154 +288,231 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
             if (begins >> k & 1) {
                 q = moved(k, q);
 #pragma unroll
-                for (int v = 0; v < V; ++v) { P[v] = A(0); H[v] = a.init ? a.init[q * a.chans + c0 + v] : A(0); }
+                for (int v = 0; v < V; ++v) { P[v] = A(0); H[v] = begin(q, v); }
             }
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            A g = gate[k][v], rest = A(0), b;
-            if constexpr (Sigmoid) sigmoid(gate[k][v], g, rest);
-            if constexpr (Vjp) b = g == A(0) ? A(0) : g * in[k][v];
-            else b = Sigmoid ? rest * in[k][v] : in[k][v];
-            if (k >= rows) { g = A(1); b = A(0); }
-            if constexpr (Vjp) {           // what the gradient needs: the state before the step
-                local[k][v] = H[v];
-                product[k][v] = P[v];
-            }
-            H[v] = g == A(0) ? b : fused(g, H[v], b);
-            P[v] = chain(P[v], g);
-            if constexpr (!Vjp) {
-                local[k][v] = H[v];
-                product[k][v] = P[v];
-            }
+            A g, rest, b;
+            coefficients(k, v, g, rest, b);
+            if constexpr (Keep) { kept_a[k][v] = g; kept_b[k][v] = b; }
+            H[v] = step(g, b, H[v]);
+            P[v] = join(P[v], g);
         }
     }
 
-    // join the tile's threads: within a wave, then across its waves
-    const int wt = Dir == 0 ? (ncol < 64 ? 64 >> a.lcol : 1) : (nt < 64 ? nt : 64);
-    const int spacing = Dir == 0 ? ncol : 1;
-    const int in_wave = Dir == 0 ? (ncol < 64 ? lane >> a.lcol : 0) : tl & (wt - 1);
-    const int wave_group = tl / wt, wave_groups = nt / wt > 0 ? nt / wt : 1;
-    for (int d = 1; d < wt; d <<= 1) {
+    A enter[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const A p = __shfl_up(P[v], d * spacing), h = __shfl_up(H[v], d * spacing);
-            if (in_wave >= d) {
-                H[v] = H[v] + cutmul(P[v], h);
-                P[v] = chain(P[v], p);
-            }
-        }
-    }
-    A before_p[V], before_h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        before_p[v] = A(1);
-        before_h[v] = A(0);
-        if (wt > 1) {
-            const A p = __shfl_up(P[v], spacing), h = __shfl_up(H[v], spacing);
-            if (in_wave > 0) { before_p[v] = p; before_h[v] = h; }
-        }
-    }
-    if (wave_groups > 1) {
-        if (in_wave == wt - 1) {
+    for (int v = 0; v < V; ++v) enter[v] = !Packed && a.init && live ? a.init[first_state + v] : A(0);
+    if (nt > 1 || a.chunks > 1) {
+        // join the tile's threads: within a wave, then across its waves
+        const int wt = Dir == 0 ? (ncol < 64 ? 64 >> a.lcol : 1) : 64;    // a wave's threads along the steps
+        const int spacing = Dir == 0 ? ncol : 1;
+        const int in_wave = Dir == 0 ? (ncol < 64 ? lane >> a.lcol : 0) : lane < tl ? lane : tl;
+        for (int d = 1; d < wt; d <<= 1) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                lds_p[(wave_group * V + v) * ncol + here] = P[v];
-                lds_h[(wave_group * V + v) * ncol + here] = H[v];
+                const A p = __shfl_up(P[v], d * spacing), h = __shfl_up(H[v], d * spacing);
+                if (in_wave >= d) {
+                    H[v] = apply(P[v], h, H[v]);
+                    P[v] = join(P[v], p);
+                }
+            }
+        }
+        A before_p[V], before_h[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            before_p[v] = A(1);
+            before_h[v] = A(0);
+            if (wt > 1) {
+                const A p = __shfl_up(P[v], spacing), h = __shfl_up(H[v], spacing);
+                if (in_wave > 0) { before_p[v] = p; before_h[v] = h; }
+            }
+        }
+        // Runs of a wave, in order: Dir 0, run r of a column is its threads r wt
+        // to r wt + wt - 1; otherwise a column's run in a wave ends with the
+        // wave or with the column.
+        const int run = Dir == 0 ? tl / wt : tid >> 6;
+        const int first_run = Dir == 0 ? 0 : (tid - tl) >> 6;
+        auto slot = [&](int r, int column, int v) -> int {
+            return Dir == 0 ? (r * V + v) * ncol + column : r;
+        };
+        if (Dir == 0 ? tl % wt == wt - 1 || tl == nt - 1 : lane == 63) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                lds_p[slot(run, here, v)] = P[v];
+                lds_h[slot(run, here, v)] = H[v];
             }
         }
         __syncthreads();
-        A p[V], h[V];
+        A earlier_p[V], earlier_h[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) { p[v] = A(1); h[v] = A(0); }
-        for (int w = 0; w < wave_group; ++w) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const A wp = lds_p[(w * V + v) * ncol + here], wh = lds_h[(w * V + v) * ncol + here];
-                h[v] = wh + cutmul(wp, h[v]);
-                p[v] = chain(wp, p[v]);
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            H[v] = H[v] + cutmul(P[v], h[v]);
-            P[v] = chain(P[v], p[v]);
-            before_h[v] = before_h[v] + cutmul(before_p[v], h[v]);
-            before_p[v] = chain(before_p[v], p[v]);
-        }
-    }
-
-    const int64_t states = a.states;
-    if (phase == kAggregate) {
-        if (tl == nt - 1 && live) {
+        for (int v = 0; v < V; ++v) { earlier_p[v] = A(1); earlier_h[v] = A(0); }
+        for (int r = first_run; r < run; ++r) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                if (v < skip) continue;
-                a.agg_p[chunk * states + first_state + v] = P[v];
-                a.agg_h[chunk * states + first_state + v] = H[v];
+                const A p = lds_p[slot(r, here, v)], h = lds_h[slot(r, here, v)];
+                earlier_h[v] = apply(p, earlier_h[v], h);
+                earlier_p[v] = join(p, earlier_p[v]);
             }
         }
-        return;
-    }
-
-    // the state that enters this thread's steps
-    A enter[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        A c = A(0);
-        if (phase == kApply) c = a.carry[chunk * states + first_state + v];
-        else if (!Packed && a.init) c = a.init[first_state + v];
-        enter[v] = before_h[v] + cutmul(before_p[v], c);
-    }
-    if (rows > 0) {
-        if constexpr (Vjp) {
-            A bar_gate[K][V], bar_x[K][V];
-            q = seq_at;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if constexpr (Packed) {
-                    if (begins >> k & 1) q = moved(k, q);
-                }
-                const bool last = k < rows && (Packed ? (ends >> k & 1) : row0 + k == a.steps - 1);
-                const int64_t state = Packed ? q * a.chans + c0 : first_state;
+        if (a.chunks > 1) {
+            // the tile's own (P, H): its last time lanes hold them
+            __syncthreads();
+            if (tl == nt - 1 && here < ncol) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    A g = gate[k][v], rest = A(0);
-                    if constexpr (Sigmoid) sigmoid(gate[k][v], g, rest);
-                    const A G = in[k][v] + (local[k][v] + cutmul(product[k][v], enter[v]));
-                    const A h = last ? (a.h0 ? a.h0[state + v] : A(0)) : prior[k][v];
-                    if constexpr (Sigmoid) {
-                        bar_gate[k][v] = G * (h - x[k][v]) * g * rest;
-                        bar_x[k][v] = rest * G;
-                    } else {
-                        bar_gate[k][v] = G * h;
-                        bar_x[k][v] = G;
+                    lds_h[here * V + v] = apply(P[v], earlier_h[v], H[v]);
+                    lds_p[here * V + v] = join(P[v], earlier_p[v]);
+                }
+            }
+            __syncthreads();
+            typedef typename Word<A>::type W;
+            const bool more = chunk + 1 < a.chunks;
+            if (more) {
+                for (int i = tid; i < ncol * V; i += blockDim.x) {
+                    const int64_t col = col0 + i / V;
+                    int64_t cs, cc;
+                    int cskip;
+                    if (col >= a.cols) break;
+                    place(col, cs, cc, cskip);
+                    if (i % V < cskip) continue;
+                    W* word = a.agg + 2 * (chunk * a.states + cs * a.chans + cc + i % V);
+                    publish<A>(word, lds_p[i]);
+                    publish<A>(word + 1, lds_h[i]);
+                }
+            }
+            // How far back a state is known.  One wave looks at 64 chunks before
+            // this one, through a channel that the strip's tiles all write.
+            if (chunk > 0 && tid < 64) {
+                int64_t cs, cc;
+                int cskip;
+                place(col0, cs, cc, cskip);
+                const int64_t watch = cs * a.chans + cc + V - 1;
+                const int look = chunk - 1 - lane;
+                int from = 0;
+                for (;;) {
+                    A p, h, st;
+                    bool has_state = look < 0, has_agg = false;
+                    if (look >= 0) {
+                        const W* word = a.agg + 2 * (look * a.states + watch);
+                        has_agg = read<A>(word, p) & read<A>(word + 1, h);
+                        has_state = read<A>(a.state + look * a.states + watch, st);
                     }
-                    if (last && a.fin && v >= skip) a.fin[state + v] = g == A(0) ? A(0) : g * G;
+                    const uint64_t states = __ballot(has_state), aggs = __ballot(has_agg);
+                    if (states) {
+                        from = __builtin_ctzll(states);
+                        const uint64_t need = (uint64_t(1) << from) - 1;
+                        if ((aggs & need) == need) break;
+                    }
+                    __builtin_amdgcn_s_sleep(2);
+                }
+                if (lane == 0) lds_from = chunk - 1 - from;     // -1: the state before the first chunk
+            }
+            __syncthreads();
+            // The state that enters: the known one, then the chunks since in
+            // order, so the bits do not depend on how far back that was.
+            const int from = chunk > 0 ? lds_from : -1;
+            for (int i = tid; i < ncol * V; i += blockDim.x) {
+                const int64_t col = col0 + i / V;
+                int64_t cs, cc;
+                int cskip;
+                if (col >= a.cols) break;
+                place(col, cs, cc, cskip);
+                if (i % V < cskip) continue;
+                const int64_t state = cs * a.chans + cc + i % V;
+                A carry;
+                if (from >= 0) carry = await<A>(a.state + from * a.states + state);
+                else carry = !Packed && a.init ? a.init[state] : A(0);
+                for (int k = from + 1; k < chunk; k += kBatch) {
+                    A p[kBatch], h[kBatch];
+                    bool ok[kBatch];
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        const W* word = a.agg + 2 * ((k + b < chunk ? k + b : k) * a.states + state);
+                        ok[b] = read<A>(word, p[b]) & read<A>(word + 1, h[b]);
+                    }
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        if (k + b >= chunk) continue;
+                        if (!ok[b]) {
+                            const W* word = a.agg + 2 * ((k + b) * a.states + state);
+                            p[b] = await<A>(word);
+                            h[b] = await<A>(word + 1);
+                        }
+                        carry = apply(p[b], carry, h[b]);
+                    }
+                }
+                if (more) publish<A>(a.state + chunk * a.states + state, apply(lds_p[i], carry, lds_h[i]));
+                lds_c[i] = carry;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < V; ++v) enter[v] = lds_c[(here < ncol ? here : 0) * V + v];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            enter[v] = apply(before_p[v], apply(earlier_p[v], enter[v], earlier_h[v]), before_h[v]);
+    }
+
+    // the steps again, from the state that enters them
+    if (rows > 0) {
+        const bool has_end = Packed ? ends != 0 : row0 + rows == a.steps;
+        q = seq_at;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if constexpr (Packed) {
+                if (begins >> k & 1) {
+                    q = moved(k, q);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) enter[v] = begin(q, v);
                 }
             }
-            if (a.bar_gate.data)
-                tile_store<T, V, K, Dir>(a.bar_gate, a.bar_gate.data + s * a.bar_gate.seq + c0 * a.bar_gate.chan, row0,
-                                         rows, skip, bar_gate);
-            if (a.bar_x.data)
-                tile_store<T, V, K, Dir>(a.bar_x, a.bar_x.data + s * a.bar_x.seq + c0 * a.bar_x.chan, row0, rows, skip,
-                                         bar_x);
-        } else {
-            q = seq_at;
+            const bool last = has_end && k < rows && (Packed ? (ends >> k & 1) : row0 + k == a.steps - 1);
+            const int64_t state = Packed ? q * a.chans + c0 : first_state;
+            if constexpr (Vjp) {
+                A h[V];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if constexpr (Packed) {
-                    if (begins >> k & 1) q = moved(k, q);
+                for (int v = 0; v < V; ++v) h[v] = widen<T, V>(prior[k], v);
+                if (last) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) h[v] = a.h0 ? a.h0[state + v] : A(0);
                 }
-                const bool last = k < rows && (Packed ? (ends >> k & 1) : row0 + k == a.steps - 1);
-                const int64_t state = Packed ? q * a.chans + c0 : first_state;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    local[k][v] = local[k][v] + cutmul(product[k][v], enter[v]);
-                    if (last && a.fin && v >= skip) a.fin[state + v] = local[k][v];
+                    A g, rest, b;
+                    coefficients(k, v, g, rest, b);
+                    const A G = b + enter[v];
+                    A to_gate = G * h[v], to_x = G;
+                    if constexpr (Sigmoid) {
+                        to_x = rest * G;
+                        to_gate = to_x * ((h[v] - widen<T, V>(x[k], v)) * g);
+                    }
+                    put<T, V>(gate[k], v, static_cast<T>(to_gate));
+                    put<T, V>(in[k], v, static_cast<T>(to_x));
+                    enter[v] = Cut && g == A(0) ? A(0) : g * G;
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    A g, rest, b;
+                    if constexpr (Keep) { g = kept_a[k][v]; b = kept_b[k][v]; }
+                    else coefficients(k, v, g, rest, b);
+                    enter[v] = step(g, b, enter[v]);
+                    put<T, V>(in[k], v, static_cast<T>(enter[v]));
                 }
             }
-            tile_store<T, V, K, Dir>(a.h, a.h.data + s * a.h.seq + c0 * a.h.chan, row0, rows, skip, local);
+            if (last && a.fin) {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (v >= skip) a.fin[state + v] = enter[v];
+            }
+        }
+        if constexpr (Vjp) {
+            if (a.bar_gate.data) tile_store<T, V, K, Dir>(a.bar_gate, s, c0, row0, rows, skip, gate);
+            if (a.bar_x.data) tile_store<T, V, K, Dir>(a.bar_x, s, c0, row0, rows, skip, in);
+        } else {
+            tile_store<T, V, K, Dir>(a.h, s, c0, row0, rows, skip, in);
         }
     }
     if constexpr (Packed) {               // a sequence without rows: its state passes through
@@ -371,24 +521,17 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
                 if (cut_at(a.offsets, a.offsets64, e) < cut_at(a.offsets, a.offsets64, e + 1)) continue;
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (v >= skip) a.fin[e * a.chans + c0 + v] = a.init ? a.init[e * a.chans + c0 + v] : A(0);
+                    if (v >= skip) a.fin[e * a.chans + c0 + v] = begin(e, v);
             }
         }
     }
 }
 
-// The state that enters each tile: one thread a (sequence, channel) folds the
-// tiles' (P, H) in order.
-template <class A>
-__global__ void __launch_bounds__(256) hawk_recurrence_carry(const A* agg_p, const A* agg_h, A* carry, const A* init,
-                                                             int64_t states, int chunks) {
-    const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (j >= states) return;
-    A state = init ? init[j] : A(0);
-    for (int c = 0; c < chunks; ++c) {
-        carry[c * states + j] = state;
-        state = agg_h[c * states + j] + cutmul(agg_p[c * states + j], state);
-    }
+// Before tiles that tell each other states: no word written, the counter at 0.
+__global__ void __launch_bounds__(256) hawk_recurrence_clear(uint32_t* counter, uint4* words, int64_t count) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
+    const uint4 ones = make_uint4(~0u, ~0u, ~0u, ~0u);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += 256LL * gridDim.x) words[i] = ones;
 }
 
 // No steps at all: every state passes through.
@@ -407,12 +550,13 @@ int log2_up(int64_t n) {
 // How a call is cut.  Dir 0: a wave's lanes lie along the channels first, so
 // its loads are runs of a row; what is left of the workgroup lies along the
 // steps, and across sequences where the steps are few.  Otherwise lanes lie
-// along the steps.
+// along the steps, as many as a sequence needs, and what is left takes further
+// sequences.
 struct Shape {
     int v, k, dir;
-    int lcol, lt, chunks, threads;
+    int lcol, nt, chunks, threads;
     int groups;
-    int64_t cols, blocks, states;
+    int64_t cols, strips, states;
 };
 
 template <class T, bool Vjp> struct Tile {
@@ -421,6 +565,8 @@ template <class T, bool Vjp> struct Tile {
     static constexpr int kSteps = Vjp ? 4 : 8;
     static constexpr int kAlong = Vjp ? 4 : (kVec > 4 ? kVec : 4);   // steps a thread where they are contiguous
 };
+
+constexpr int kAcross = 4;       // log2 of the lanes across a row where it is long
 
 template <class T, bool Vjp>
 Shape shape_of(const hk_recurrence_job& j) {
@@ -432,38 +578,42 @@ Shape shape_of(const hk_recurrence_job& j) {
         chan &= p->chan == 1;
         along &= p->step == 1;
     }
-    const int64_t packed_seqs = j.offsets ? 1 : j.seqs;
+    const int64_t seqs = j.offsets ? 1 : j.seqs;
     if (along && (j.chans == 1 || !chan)) {
         s.dir = (j.reverse != 0) != Vjp ? -1 : 1;
         s.v = 1;
         s.k = Tile<T, Vjp>::kAlong;
         s.groups = static_cast<int>(j.chans);
-        s.cols = packed_seqs * s.groups;
-        s.lt = log2_up((j.steps + s.k - 1) / s.k);
-        if ((1 << s.lt) > kThreads) s.lt = log2_up(kThreads);
-        s.lcol = log2_up(kThreads) - s.lt;
+        s.cols = seqs * s.groups;
+        const int64_t need = (j.steps + s.k - 1) / s.k;
+        s.chunks = static_cast<int>((need + kThreads - 1) / kThreads);
+        s.nt = static_cast<int>((need + s.chunks - 1) / s.chunks);
+        s.lcol = 0;
+        while ((2 << s.lcol) * s.nt <= kThreads && (int64_t(1) << s.lcol) < s.cols) ++s.lcol;
     } else {
         s.dir = 0;
         s.v = chan && j.chans >= Tile<T, Vjp>::kVec ? Tile<T, Vjp>::kVec : 1;
         s.k = Tile<T, Vjp>::kSteps;
         s.groups = static_cast<int>((j.chans + s.v - 1) / s.v);
-        s.cols = packed_seqs * s.groups;
-        int across = log2_up(s.groups);
-        if (across > 6) across = 6;
-        s.lt = log2_up((j.steps + s.k - 1) / s.k);
-        if (s.lt + across > log2_up(kThreads)) s.lt = log2_up(kThreads) - across;
-        s.lcol = log2_up(kThreads) - s.lt;
+        s.cols = seqs * s.groups;
+        s.lcol = log2_up(s.groups);
+        if (s.lcol > kAcross) s.lcol = kAcross;
+        const int64_t need = (j.steps + s.k - 1) / s.k;
+        int most = kThreads >> s.lcol;
+        // few steps: the lanes they leave take more columns
+        while (need <= most / 2 && (int64_t(1) << s.lcol) < s.cols && s.lcol < 8) {
+            ++s.lcol;
+            most /= 2;
+        }
+        const int wt = s.lcol < 6 ? 64 >> s.lcol : 1;
+        s.chunks = static_cast<int>((need + most - 1) / most);
+        s.nt = static_cast<int>((need + s.chunks - 1) / s.chunks);
+        s.nt = (s.nt + wt - 1) / wt * wt;          // whole waves
+        s.chunks = static_cast<int>((need + s.nt - 1) / s.nt);
     }
-    if (s.lcol > log2_up(s.cols)) s.lcol = log2_up(s.cols);
-    s.threads = 1 << (s.lcol + s.lt);
-    if (s.threads < 64) {
-        s.lcol = 6 - s.lt;
-        s.threads = 64;
-    }
-    const int64_t rows = int64_t(s.k) << s.lt;
-    s.chunks = static_cast<int>((j.steps + rows - 1) / rows);
-    s.blocks = ((s.cols + (int64_t(1) << s.lcol) - 1) >> s.lcol) * s.chunks;
-    s.states = packed_seqs * j.chans;
+    s.threads = ((s.nt << s.lcol) + 63) / 64 * 64;
+    s.strips = (s.cols + (int64_t(1) << s.lcol) - 1) >> s.lcol;
+    s.states = seqs * j.chans;
     return s;
 }
 
@@ -495,11 +645,17 @@ Plane<T> plane_of(const hk_plane& p, int64_t steps, bool flip) {
     return q;
 }
 
+constexpr size_t kCounterBytes = 256;
+// (P, H) and the state of every (chunk, state), in whole 16-byte words
+size_t word_bytes(const Shape& s, size_t word) {
+    return (3 * word * static_cast<size_t>(s.states) * s.chunks + 15) / 16 * 16;
+}
+
 template <class T, bool Vjp>
 size_t scratch_of(const hk_recurrence_job& j) {
     if (j.seqs <= 0 || j.steps <= 0 || j.chans <= 0) return 0;
     const Shape s = shape_of<T, Vjp>(j);
-    return s.chunks > 1 ? 3 * sizeof(Acc<T>) * static_cast<size_t>(s.states) * s.chunks : 0;
+    return s.chunks > 1 ? kCounterBytes + word_bytes(s, sizeof(Acc<T>)) : 0;
 }
 
 int launched(const char* what) {
@@ -508,17 +664,17 @@ int launched(const char* what) {
 }
 
 template <class T, int V, int K, int Dir, bool Vjp>
-void launch_tile(const hk_recurrence_job& j, const RecArgs<T>& a, const Shape& s, int phase, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(s.blocks)), block(s.threads);
+void launch_tile(const hk_recurrence_job& j, const RecArgs<T>& a, const Shape& s, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(s.strips * s.chunks)), block(s.threads);
     if constexpr (Dir == 0) {
         if (j.offsets) {
-            if (j.sigmoid) hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, true, Vjp, true>), grid, block, 0, stream, a, phase);
-            else hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, false, Vjp, true>), grid, block, 0, stream, a, phase);
+            if (j.sigmoid) hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, true, Vjp, true>), grid, block, 0, stream, a);
+            else hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, false, Vjp, true>), grid, block, 0, stream, a);
             return;
         }
     }
-    if (j.sigmoid) hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, true, Vjp, false>), grid, block, 0, stream, a, phase);
-    else hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, false, Vjp, false>), grid, block, 0, stream, a, phase);
+    if (j.sigmoid) hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, true, Vjp, false>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((hawk_recurrence_tile<T, V, K, Dir, false, Vjp, false>), grid, block, 0, stream, a);
 }
 
 template <class T, bool Vjp>
@@ -535,7 +691,7 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
         return launched("hawk_recurrence_pass launch");
     }
     const Shape s = shape_of<T, Vjp>(j);
-    if (s.blocks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, who + ": the planes exceed the grid limit");
+    if (s.strips * s.chunks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, who + ": the planes exceed the grid limit");
     if (s.chunks > 1 && !scratch) return hawk_internal::set_error(HK_EVALUE, who + ": scratch is required");
     const bool flip = (j.reverse != 0) != Vjp;
     RecArgs<T> a{};
@@ -556,28 +712,29 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
     a.steps = static_cast<int>(j.steps);
     a.groups = s.groups;
     a.lcol = s.lcol;
-    a.lt = s.lt;
+    a.nt = s.nt;
+    a.strips = static_cast<int>(s.strips);
     a.chunks = s.chunks;
     a.states = s.states;
     a.rev = flip;
-    a.agg_p = static_cast<A*>(scratch);
-    a.agg_h = a.agg_p + s.states * s.chunks;
-    a.carry = a.agg_h + s.states * s.chunks;
+    if (s.chunks > 1) {
+        typedef typename Word<A>::type W;
+        a.counter = static_cast<uint32_t*>(scratch);
+        a.agg = reinterpret_cast<W*>(static_cast<unsigned char*>(scratch) + kCounterBytes);
+        a.state = a.agg + 2 * s.states * s.chunks;
+        const int64_t words = static_cast<int64_t>(word_bytes(s, sizeof(A)) / 16);
+        const int64_t blocks = (words + 1023) / 1024;
+        hipLaunchKernelGGL(hawk_recurrence_clear, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256),
+                           0, stream, a.counter, reinterpret_cast<uint4*>(a.agg), words);
+        const int rc = launched("hawk_recurrence_clear launch");
+        if (rc != HK_OK) return rc;
+    }
     constexpr int VV = Tile<T, Vjp>::kVec, KC = Tile<T, Vjp>::kSteps, KT = Tile<T, Vjp>::kAlong;
-    auto tiles = [&](int phase) {
-        if (s.dir > 0) launch_tile<T, 1, KT, 1, Vjp>(j, a, s, phase, stream);
-        else if (s.dir < 0) launch_tile<T, 1, KT, -1, Vjp>(j, a, s, phase, stream);
-        else if (s.v > 1) launch_tile<T, VV, KC, 0, Vjp>(j, a, s, phase, stream);
-        else launch_tile<T, 1, KC, 0, Vjp>(j, a, s, phase, stream);
-        return launched("hawk_recurrence_tile launch");
-    };
-    if (s.chunks == 1) return tiles(kSingle);
-    int rc = tiles(kAggregate);
-    if (rc != HK_OK) return rc;
-    hipLaunchKernelGGL(hawk_recurrence_carry<A>, dim3(static_cast<unsigned>((s.states + 255) / 256)), dim3(256), 0,
-                       stream, a.agg_p, a.agg_h, a.carry, j.offsets ? nullptr : init, s.states, s.chunks);
-    rc = launched("hawk_recurrence_carry launch");
-    return rc != HK_OK ? rc : tiles(kApply);
+    if (s.dir > 0) launch_tile<T, 1, KT, 1, Vjp>(j, a, s, stream);
+    else if (s.dir < 0) launch_tile<T, 1, KT, -1, Vjp>(j, a, s, stream);
+    else if (s.v > 1) launch_tile<T, VV, KC, 0, Vjp>(j, a, s, stream);
+    else launch_tile<T, 1, KC, 0, Vjp>(j, a, s, stream);
+    return launched("hawk_recurrence_tile launch");
 }
 
 }  // namespace

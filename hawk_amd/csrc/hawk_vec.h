@@ -45,6 +45,23 @@ __device__ __forceinline__ void load(const T* p, Acc<T> (&out)[N]) {
     }
 }
 
+// The same load left in the plane's type, for values that wait in registers.
+template <class T, int N> using Raw = typename VecOf<T, N>::type;
+template <class T, int N>
+__device__ __forceinline__ Raw<T, N> load_raw(const T* p) {
+    return *reinterpret_cast<const typename VecOf<T, N>::loose*>(p);
+}
+template <class T, int N>
+__device__ __forceinline__ Acc<T> widen(const Raw<T, N>& v, int j) {
+    if constexpr (N == 1) return static_cast<Acc<T>>(v);
+    else return static_cast<Acc<T>>(v[j]);
+}
+template <class T, int N>
+__device__ __forceinline__ void put(Raw<T, N>& v, int j, T x) {
+    if constexpr (N == 1) v = x;
+    else v[j] = x;
+}
+
 // Rounds to nearest even, once, to the plane's type.
 template <class T, int N, bool Stream = false>
 __device__ __forceinline__ void store(T* p, const Acc<T> (&x)[N]) {
@@ -92,16 +109,14 @@ __device__ __forceinline__ void sigmoid(float z, float& a, float& rest) {
     const float e = __builtin_amdgcn_exp2f(-kLog2e * __builtin_fabsf(z));
     const float r = __builtin_amdgcn_rcpf(1.0f + e);
     const float small = e * r;
-    a = z >= 0.0f ? r : small;
+    a = z >= 0.0f ? r : small;           // a NaN z makes both values NaN
     rest = z >= 0.0f ? small : r;
-    if (!(z == z)) a = rest = z;
 }
 __device__ __forceinline__ void sigmoid(double z, double& a, double& rest) {
     const double e = exp(-fabs(z));
     const double r = 1.0 / (1.0 + e), small = e * r;
     a = z >= 0.0 ? r : small;
     rest = z >= 0.0 ? small : r;
-    if (!(z == z)) a = rest = z;
 }
 
 }  // namespace hawk_vec
