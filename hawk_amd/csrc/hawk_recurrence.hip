@@ -104,36 +104,32 @@ __device__ __forceinline__ void tile_load(const Plane<T>& p, int64_t s, int64_t 
     }
 }
 
-// Stores the tile's steps that exist; `skip` leading channels belong to the
-// neighbouring thread.
-template <class T, int V, int K, int Dir>
-__device__ __forceinline__ void tile_store(const Plane<T>& p, int64_t s, int64_t c, int row0, int rows, int skip,
-                                           const Raw<T, V> (&x)[K]) {
-    T* base = p.data + s * p.seq + c * p.chan;
-    if constexpr (Dir == 0) {
+// Stores step k of a tile at p (the thread's first step) if it exists; `skip`
+// leading channels belong to the neighbouring thread.
+template <class T, int V>
+__device__ __forceinline__ void row_store(T* p, int64_t step, int k, int rows, int skip, const Raw<T, V>& x) {
+    if (k >= rows) return;
+    T* to = p + k * step;
+    if (skip == 0) {
+        *reinterpret_cast<typename VecOf<T, V>::loose*>(to) = x;
+    } else if constexpr (V > 1) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            T* to = base + (row0 + k) * p.step;
-            if (k >= rows) continue;
-            if (skip == 0) {
-                *reinterpret_cast<typename VecOf<T, V>::loose*>(to) = x[k];
-            } else if constexpr (V > 1) {
+        for (int v = 0; v < V; ++v)
+            if (v >= skip) to[v] = x[v];
+    }
+}
+// The same for all steps of a thread whose steps are contiguous.
+template <class T, int K, int Dir>
+__device__ __forceinline__ void run_store(T* p, int rows, const T (&x)[K]) {
+    if (rows == K) {
+        Raw<T, K> flat;
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (v >= skip) to[v] = x[k][v];
-            }
-        }
+        for (int k = 0; k < K; ++k) flat[Dir > 0 ? k : K - 1 - k] = x[k];
+        *reinterpret_cast<typename VecOf<T, K>::loose*>(Dir > 0 ? p : p - (K - 1)) = flat;
     } else {
-        if (rows == K) {
-            Raw<T, K> flat;
 #pragma unroll
-            for (int k = 0; k < K; ++k) flat[Dir > 0 ? k : K - 1 - k] = x[k];
-            *reinterpret_cast<typename VecOf<T, K>::loose*>(Dir > 0 ? base + row0 : base - (row0 + K - 1)) = flat;
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (k < rows) *(Dir > 0 ? base + row0 + k : base - row0 - k) = x[k];
-        }
+        for (int k = 0; k < K; ++k)
+            if (k < rows) *(Dir > 0 ? p + k : p - k) = x[k];
     }
 }
 
@@ -216,12 +212,8 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
     if (rows < K) {                       // steps that do not exist leave the state as it is
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if (k < rows) continue;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                put<T, V>(gate[k], v, static_cast<T>(Sigmoid ? INFINITY : 1.0f));
-                put<T, V>(in[k], v, static_cast<T>(0.0f));
-            }
+            gate[k] = choose(k < rows, gate[k], splat<T, V>(static_cast<T>(Sigmoid ? INFINITY : 1.0f)));
+            in[k] = choose(k < rows, in[k], splat<T, V>(static_cast<T>(0.0f)));
         }
     }
 
@@ -277,10 +269,11 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
     auto join = [&](A p, A q) -> A { return Cut ? chain(p, q) : p * q; };
     auto apply = [&](A p, A h, A add) -> A { return Cut ? add + cutmul(p, h) : fused(p, h, add); };
 
-    // fold this thread's steps from a zero state
-    A P[V], H[V];
+    // fold this thread's steps from a zero state; `least` tells a product that is
+    // 0 because a gate is from one too small for the type (see chain)
+    A P[V], H[V], least[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) { P[v] = A(1); H[v] = A(0); }
+    for (int v = 0; v < V; ++v) { P[v] = least[v] = A(1); H[v] = A(0); }
     int64_t q = seq_at;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -288,17 +281,26 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
             if (begins >> k & 1) {
                 q = moved(k, q);
 #pragma unroll
-                for (int v = 0; v < V; ++v) { P[v] = A(0); H[v] = begin(q, v); }
+                for (int v = 0; v < V; ++v) { P[v] = least[v] = A(0); H[v] = begin(q, v); }
             }
         }
+        forget(gate[k]);                  // values are widened a step at a time
+        forget(in[k]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             A g, rest, b;
             coefficients(k, v, g, rest, b);
             if constexpr (Keep) { kept_a[k][v] = g; kept_b[k][v] = b; }
             H[v] = step(g, b, H[v]);
-            P[v] = join(P[v], g);
+            P[v] = Cut ? cutmul(P[v], g) : P[v] * g;
+            if constexpr (Cut) least[v] = smaller(least[v], g);
         }
+#pragma unroll
+        for (int v = 0; v < V; ++v) asm volatile("" : "+v"(P[v]), "+v"(H[v]));
+    }
+    if constexpr (Cut) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) P[v] = P[v] == A(0) && least[v] != A(0) ? least_normal(A(0)) : P[v];
     }
 
     A enter[V];
@@ -313,10 +315,9 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const A p = __shfl_up(P[v], d * spacing), h = __shfl_up(H[v], d * spacing);
-                if (in_wave >= d) {
-                    H[v] = apply(P[v], h, H[v]);
-                    P[v] = join(P[v], p);
-                }
+                const A joined_h = apply(P[v], h, H[v]), joined_p = join(P[v], p);
+                H[v] = in_wave >= d ? joined_h : H[v];
+                P[v] = in_wave >= d ? joined_p : P[v];
             }
         }
         A before_p[V], before_h[V];
@@ -326,7 +327,8 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
             before_h[v] = A(0);
             if (wt > 1) {
                 const A p = __shfl_up(P[v], spacing), h = __shfl_up(H[v], spacing);
-                if (in_wave > 0) { before_p[v] = p; before_h[v] = h; }
+                before_p[v] = in_wave > 0 ? p : A(1);
+                before_h[v] = in_wave > 0 ? h : A(0);
             }
         }
         // Runs of a wave, in order: Dir 0, run r of a column is its threads r wt
@@ -457,6 +459,9 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
 
     // the steps again, from the state that enters them
     if (rows > 0) {
+        const Plane<T>& to = Vjp ? a.bar_x : a.h;
+        T* out = to.data + s * to.seq + c0 * to.chan + row0 * to.step;
+        T* out_gate = Vjp ? a.bar_gate.data + s * a.bar_gate.seq + c0 * a.bar_gate.chan + row0 * a.bar_gate.step : nullptr;
         const bool has_end = Packed ? ends != 0 : row0 + rows == a.steps;
         q = seq_at;
 #pragma unroll
@@ -468,9 +473,15 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
                     for (int v = 0; v < V; ++v) enter[v] = begin(q, v);
                 }
             }
-            const bool last = has_end && k < rows && (Packed ? (ends >> k & 1) : row0 + k == a.steps - 1);
+            const bool last = (Packed || Vjp) && has_end && k < rows && (Packed ? (ends >> k & 1) : k == rows - 1);
             const int64_t state = Packed ? q * a.chans + c0 : first_state;
+            if constexpr (!Keep) {
+                forget(gate[k]);
+                forget(in[k]);
+            }
             if constexpr (Vjp) {
+                forget(prior[k]);
+                if constexpr (Sigmoid) forget(x[k]);
                 A h[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = widen<T, V>(prior[k], v);
@@ -478,41 +489,55 @@ __global__ void __launch_bounds__(kThreads) hawk_recurrence_tile(const RecArgs<T
 #pragma unroll
                     for (int v = 0; v < V; ++v) h[v] = a.h0 ? a.h0[state + v] : A(0);
                 }
+                Raw<T, V> to_gate, to_x;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     A g, rest, b;
                     coefficients(k, v, g, rest, b);
                     const A G = b + enter[v];
-                    A to_gate = G * h[v], to_x = G;
+                    A bar_gate = G * h[v], bar_x = G;
                     if constexpr (Sigmoid) {
-                        to_x = rest * G;
-                        to_gate = to_x * ((h[v] - widen<T, V>(x[k], v)) * g);
+                        bar_x = rest * G;
+                        bar_gate = bar_x * ((h[v] - widen<T, V>(x[k], v)) * g);
                     }
-                    put<T, V>(gate[k], v, static_cast<T>(to_gate));
-                    put<T, V>(in[k], v, static_cast<T>(to_x));
+                    put<T, V>(to_gate, v, static_cast<T>(bar_gate));
+                    put<T, V>(to_x, v, static_cast<T>(bar_x));
                     enter[v] = Cut && g == A(0) ? A(0) : g * G;
                 }
+                if constexpr (Dir == 0) {
+                    if (a.bar_gate.data) row_store<T, V>(out_gate, a.bar_gate.step, k, rows, skip, to_gate);
+                    if (a.bar_x.data) row_store<T, V>(out, a.bar_x.step, k, rows, skip, to_x);
+                } else {
+                    gate[k] = to_gate;
+                    in[k] = to_x;
+                }
             } else {
+                Raw<T, V> h;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     A g, rest, b;
                     if constexpr (Keep) { g = kept_a[k][v]; b = kept_b[k][v]; }
                     else coefficients(k, v, g, rest, b);
                     enter[v] = step(g, b, enter[v]);
-                    put<T, V>(in[k], v, static_cast<T>(enter[v]));
+                    put<T, V>(h, v, static_cast<T>(enter[v]));
                 }
+                if constexpr (Dir == 0) row_store<T, V>(out, a.h.step, k, rows, skip, h);
+                else in[k] = h;
             }
-            if (last && a.fin) {
+            if (Packed && last && a.fin) {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
                     if (v >= skip) a.fin[state + v] = enter[v];
             }
         }
-        if constexpr (Vjp) {
-            if (a.bar_gate.data) tile_store<T, V, K, Dir>(a.bar_gate, s, c0, row0, rows, skip, gate);
-            if (a.bar_x.data) tile_store<T, V, K, Dir>(a.bar_x, s, c0, row0, rows, skip, in);
-        } else {
-            tile_store<T, V, K, Dir>(a.h, s, c0, row0, rows, skip, in);
+        if (!Packed && has_end && a.fin) {     // the steps past the end left the state as it was
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v >= skip) a.fin[first_state + v] = enter[v];
+        }
+        if constexpr (Dir != 0) {
+            if (Vjp && a.bar_gate.data) run_store<T, K, Dir>(out_gate, rows, gate);
+            if (!Vjp || a.bar_x.data) run_store<T, K, Dir>(out, rows, in);
         }
     }
     if constexpr (Packed) {               // a sequence without rows: its state passes through

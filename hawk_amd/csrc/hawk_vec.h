@@ -62,6 +62,44 @@ __device__ __forceinline__ void put(Raw<T, N>& v, int j, T x) {
     else v[j] = x;
 }
 
+template <class T, int N>
+__device__ __forceinline__ Raw<T, N> splat(T x) {
+    Raw<T, N> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) put<T, N>(v, j, x);
+    return v;
+}
+
+// Vectors of narrow elements stay whole registers: chosen between as words, and
+// (forget) what the compiler derived from one may not be carried past a point,
+// so values held in a narrow type are converted again instead of held wide.
+template <class R>
+__device__ __forceinline__ R choose(bool first, const R& x, const R& y) {
+    if constexpr (sizeof(R) % 4 == 0) {
+        typedef uint32_t W __attribute__((ext_vector_type(sizeof(R) / 4)));
+        if constexpr (sizeof(R) == 4) {
+            return __builtin_bit_cast(R, first ? __builtin_bit_cast(uint32_t, x) : __builtin_bit_cast(uint32_t, y));
+        } else {
+            const W u = __builtin_bit_cast(W, x), v = __builtin_bit_cast(W, y);
+            W w;
+#pragma unroll
+            for (unsigned j = 0; j < sizeof(R) / 4; ++j) w[j] = first ? u[j] : v[j];
+            return __builtin_bit_cast(R, w);
+        }
+    } else {
+        return first ? x : y;
+    }
+}
+template <class R>
+__device__ __forceinline__ void forget(R& v) {
+    if constexpr (sizeof(R) == 16) {
+        typedef uint32_t W __attribute__((ext_vector_type(4)));
+        W w = __builtin_bit_cast(W, v);
+        asm volatile("" : "+v"(w));
+        v = __builtin_bit_cast(R, w);
+    }
+}
+
 // Rounds to nearest even, once, to the plane's type.
 template <class T, int N, bool Stream = false>
 __device__ __forceinline__ void store(T* p, const Acc<T> (&x)[N]) {
@@ -88,14 +126,16 @@ __device__ __forceinline__ double cutmul(double a, double b) { return a == 0.0 |
 // The product of two gates' products.  It is 0 only where one of them is (a
 // cut): a product too small for the type stays the least normal number, so an
 // infinity or a NaN that enters a long run of small gates also leaves it.
-__device__ __forceinline__ float chain(float a, float b) {
-    const float p = cutmul(a, b);
-    return p == 0.0f && a != 0.0f && b != 0.0f ? 1.17549435e-38f : p;
+__device__ __forceinline__ float least_normal(float) { return 1.17549435e-38f; }
+__device__ __forceinline__ double least_normal(double) { return 2.2250738585072014e-308; }
+template <class A>
+__device__ __forceinline__ A chain(A a, A b) {
+    const A p = cutmul(a, b);
+    return p == A(0) && a != A(0) && b != A(0) ? least_normal(A(0)) : p;
 }
-__device__ __forceinline__ double chain(double a, double b) {
-    const double p = cutmul(a, b);
-    return p == 0.0 && a != 0.0 && b != 0.0 ? 2.2250738585072014e-308 : p;
-}
+// The smaller of m and |g|; a NaN g leaves m.
+__device__ __forceinline__ float smaller(float m, float g) { return __builtin_fminf(m, __builtin_fabsf(g)); }
+__device__ __forceinline__ double smaller(double m, double g) { return __builtin_fmin(m, __builtin_fabs(g)); }
 
 __device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
