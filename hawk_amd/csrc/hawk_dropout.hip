@@ -44,38 +44,112 @@ struct DropArgs {
     uint32_t cut;
 };
 
-// One thread takes the eight elements of one counter.
+__device__ __forceinline__ Words numbers(const DropArgs& a, uint64_t offset, int64_t g) {
+    return philox(static_cast<uint32_t>(g), static_cast<uint32_t>(g >> 32), static_cast<uint32_t>(offset),
+                  static_cast<uint32_t>(offset >> 32), static_cast<uint32_t>(a.seed),
+                  static_cast<uint32_t>(a.seed >> 32));
+}
+__device__ __forceinline__ uint64_t offset_of(const DropArgs& a) {
+    return a.offset + (a.offset_cell ? static_cast<uint64_t>(*a.offset_cell) : 0);
+}
+template <class A>
+__device__ __forceinline__ A dropped(const DropArgs& a, const Words& u, int j, A x, A factor) {
+    const uint32_t word = j < 4 ? (j < 2 ? u.w[0] : u.w[1]) : (j < 6 ? u.w[2] : u.w[3]);
+    const uint32_t number = j & 1 ? word >> 16 : word & 0xffffu;
+    return number >= a.cut ? x * factor : A(0);
+}
+
+// Eight elements of one counter as vectors: kSets counters a thread, whose loads
+// are issued together.  A row is whole counters (Rows), or the array one run.
+constexpr int kSets = 2;
+template <class T, bool Residual, bool Rows>
+__global__ void __launch_bounds__(kThreads) hawk_dropout(const DropArgs a, const T* x, const T* residual, T* y,
+                                                         const Acc<T> factor) {
+    typedef Acc<T> A;
+    constexpr int V = sizeof(T) == 8 ? 2 : sizeof(T) == 4 ? 4 : 8;
+    const int64_t groups = Rows ? a.rows * (a.cols / kNumbers) : a.cols / kNumbers;
+    const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kSets) + threadIdx.x;
+    const int64_t per_row = a.cols / kNumbers;
+    const uint64_t offset = offset_of(a);
+    Raw<T, V> in[kSets][kNumbers / V], add[kSets][kNumbers / V];
+    int64_t row[kSets], c[kSets];
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+        const int64_t g = g0 + s * kThreads;
+        row[s] = Rows ? g / per_row : 0;
+        c[s] = (Rows ? g - row[s] * per_row : g) * kNumbers;
+        if (g >= groups) continue;
+#pragma unroll
+        for (int j = 0; j < kNumbers / V; ++j) {
+            in[s][j] = load_raw<T, V, true>(x + row[s] * a.x_stride + c[s] + j * V);
+            if (Residual) add[s][j] = load_raw<T, V, true>(residual + row[s] * a.residual_stride + c[s] + j * V);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+        const int64_t g = g0 + s * kThreads;
+        if (g >= groups) continue;
+        const Words u = numbers(a, offset, g);
+#pragma unroll
+        for (int j = 0; j < kNumbers / V; ++j) {
+            A out[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                out[v] = dropped(a, u, j * V + v, widen<T, V>(in[s][j], v), factor);
+                if (Residual) out[v] += widen<T, V>(add[s][j], v);
+            }
+            store<T, V, true>(y + row[s] * a.y_stride + c[s] + j * V, out);
+        }
+    }
+    if constexpr (!Rows) {                // the last counter's elements, of an array that is no whole counters
+        const int64_t i = groups * kNumbers + threadIdx.x;
+        if (blockIdx.x == 0 && i < a.cols) {
+            A v = dropped(a, numbers(a, offset, groups), threadIdx.x, static_cast<A>(x[i]), factor);
+            if (Residual) v += static_cast<A>(residual[i]);
+            y[i] = static_cast<T>(v);
+        }
+    }
+}
+
+// Rows apart whose counters run on from one row into the next: an element at a time.
 template <class T>
-__global__ void __launch_bounds__(kThreads) hawk_dropout(const DropArgs a, const T* x, const T* residual, T* y) {
-    const int64_t n = a.rows * a.cols, groups = (n + kNumbers - 1) / kNumbers;
+__global__ void __launch_bounds__(kThreads) hawk_dropout_apart(const DropArgs a, const T* x, const T* residual, T* y,
+                                                               const Acc<T> factor) {
+    const int64_t n = a.rows * a.cols;
     const int64_t g = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (g >= groups) return;
-    const uint64_t offset = a.offset + (a.offset_cell ? static_cast<uint64_t>(*a.offset_cell) : 0);
-    const Words u = philox(static_cast<uint32_t>(g), static_cast<uint32_t>(g >> 32), static_cast<uint32_t>(offset),
-                           static_cast<uint32_t>(offset >> 32), static_cast<uint32_t>(a.seed),
-                           static_cast<uint32_t>(a.seed >> 32));
-    const Acc<T> factor = a.cut < 65536u ? Acc<T>(65536) / Acc<T>(65536u - a.cut) : Acc<T>(0);
+    if (g * kNumbers >= n) return;
+    const Words u = numbers(a, offset_of(a), g);
+    int64_t row = g * kNumbers / a.cols, c = g * kNumbers - row * a.cols;
+#pragma unroll
     for (int j = 0; j < kNumbers; ++j) {
-        const int64_t i = g * kNumbers + j;
-        if (i >= n) break;
-        const int64_t row = i / a.cols, c = i - row * a.cols;
-        const uint32_t number = j & 1 ? u.w[j / 2] >> 16 : u.w[j / 2] & 0xffffu;
-        Acc<T> v = number >= a.cut ? static_cast<Acc<T>>(x[row * a.x_stride + c]) * factor : Acc<T>(0);
-        if (residual) v += static_cast<Acc<T>>(residual[row * a.residual_stride + c]);
-        y[row * a.y_stride + c] = static_cast<T>(v);
+        if (row < a.rows) {
+            Acc<T> v = dropped(a, u, j, static_cast<Acc<T>>(x[row * a.x_stride + c]), factor);
+            if (residual) v += static_cast<Acc<T>>(residual[row * a.residual_stride + c]);
+            y[row * a.y_stride + c] = static_cast<T>(v);
+        }
+        if (++c == a.cols) { c = 0; ++row; }
     }
 }
 
 template <class T>
 int dropout(const hk_dropout_job& j, hipStream_t stream) {
-    const int64_t groups = (j.rows * j.cols + kNumbers - 1) / kNumbers;
-    if (groups == 0) return HK_OK;
-    const int64_t blocks = (groups + kThreads - 1) / kThreads;
+    const int64_t n = j.rows * j.cols;
+    if (n == 0) return HK_OK;
+    const bool whole = j.cols % kNumbers == 0, vectors = j.rows == 1 || whole;
+    const int64_t groups = (n + kNumbers - 1) / kNumbers, per = vectors ? kThreads * kSets : kThreads;
+    const int64_t blocks = (groups + per - 1) / per;
     if (blocks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, "hk_dropout: the planes exceed the grid limit");
     const DropArgs a{j.offset_cell, j.seed, j.offset, j.rows, j.cols, j.x_stride, j.residual_stride, j.y_stride,
                      static_cast<uint32_t>(j.cut)};
-    hipLaunchKernelGGL(hawk_dropout<T>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, a,
-                       static_cast<const T*>(j.x), static_cast<const T*>(j.residual), static_cast<T*>(j.y));
+    const Acc<T> factor = j.cut < 65536 ? Acc<T>(65536) / Acc<T>(65536 - j.cut) : Acc<T>(0);
+    const T *x = static_cast<const T*>(j.x), *residual = static_cast<const T*>(j.residual);
+    T* y = static_cast<T*>(j.y);
+    const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
+    if (!vectors) hipLaunchKernelGGL(hawk_dropout_apart<T>, grid, block, 0, stream, a, x, residual, y, factor);
+    else if (j.rows == 1 && residual) hipLaunchKernelGGL((hawk_dropout<T, true, false>), grid, block, 0, stream, a, x, residual, y, factor);
+    else if (j.rows == 1) hipLaunchKernelGGL((hawk_dropout<T, false, false>), grid, block, 0, stream, a, x, residual, y, factor);
+    else if (residual) hipLaunchKernelGGL((hawk_dropout<T, true, true>), grid, block, 0, stream, a, x, residual, y, factor);
+    else hipLaunchKernelGGL((hawk_dropout<T, false, true>), grid, block, 0, stream, a, x, residual, y, factor);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error("hawk_dropout launch", err);
 }

@@ -28,28 +28,20 @@ template <class T, int N> struct VecOf {
 };
 template <class T> struct VecOf<T, 1> { typedef T type; typedef T loose; };
 
-// Stream: data that this pass touches once, so it is not kept in the caches.
-template <class T, int N, bool Stream = false>
-__device__ __forceinline__ void load(const T* p, Acc<T> (&out)[N]) {
-    if constexpr (N == 1) {
-        T x;
-        if constexpr (Stream) x = __builtin_nontemporal_load(p);
-        else x = *p;
-        out[0] = static_cast<Acc<T>>(x);
-    } else {
-        typename VecOf<T, N>::type v;
-        if constexpr (Stream) v = __builtin_nontemporal_load(reinterpret_cast<const typename VecOf<T, N>::loose*>(p));
-        else v = *reinterpret_cast<const typename VecOf<T, N>::loose*>(p);
-#pragma unroll
-        for (int j = 0; j < N; ++j) out[j] = static_cast<Acc<T>>(v[j]);
-    }
-}
-
-// The same load left in the plane's type, for values that wait in registers.
+// A vector in the plane's type.  Stream: data that this pass touches once, so it
+// is not kept in the caches.
 template <class T, int N> using Raw = typename VecOf<T, N>::type;
-template <class T, int N>
+template <class T, int N, bool Stream = false>
 __device__ __forceinline__ Raw<T, N> load_raw(const T* p) {
-    return *reinterpret_cast<const typename VecOf<T, N>::loose*>(p);
+    const auto* at = reinterpret_cast<const typename VecOf<T, N>::loose*>(p);
+    if constexpr (Stream) return __builtin_nontemporal_load(at);
+    else return *at;
+}
+template <class T, int N, bool Stream = false>
+__device__ __forceinline__ void store_raw(T* p, const Raw<T, N>& x) {
+    auto* at = reinterpret_cast<typename VecOf<T, N>::loose*>(p);
+    if constexpr (Stream) __builtin_nontemporal_store(x, at);
+    else *at = x;
 }
 template <class T, int N>
 __device__ __forceinline__ Acc<T> widen(const Raw<T, N>& v, int j) {
@@ -100,19 +92,19 @@ __device__ __forceinline__ void forget(R& v) {
     }
 }
 
-// Rounds to nearest even, once, to the plane's type.
+// The same widened, and rounded to nearest even, once, to the plane's type.
+template <class T, int N, bool Stream = false>
+__device__ __forceinline__ void load(const T* p, Acc<T> (&out)[N]) {
+    const Raw<T, N> v = load_raw<T, N, Stream>(p);
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = widen<T, N>(v, j);
+}
 template <class T, int N, bool Stream = false>
 __device__ __forceinline__ void store(T* p, const Acc<T> (&x)[N]) {
-    if constexpr (N == 1) {
-        if constexpr (Stream) __builtin_nontemporal_store(static_cast<T>(x[0]), p);
-        else *p = static_cast<T>(x[0]);
-    } else {
-        typename VecOf<T, N>::type v;
+    Raw<T, N> v;
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = static_cast<T>(x[j]);
-        if constexpr (Stream) __builtin_nontemporal_store(v, reinterpret_cast<typename VecOf<T, N>::loose*>(p));
-        else *reinterpret_cast<typename VecOf<T, N>::loose*>(p) = v;
-    }
+    for (int j = 0; j < N; ++j) put<T, N>(v, j, static_cast<T>(x[j]));
+    store_raw<T, N, Stream>(p, v);
 }
 
 // a * b, and 0 where either is 0 whatever the other is.
