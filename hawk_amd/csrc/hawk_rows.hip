@@ -17,6 +17,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 namespace {
 
@@ -73,9 +74,9 @@ __device__ __forceinline__ void policy_row(const RowArgs<T>& a, int64_t n, float
     slope *= a.bar_loss ? w * *a.bar_loss : w;
 }
 
-// (m, s) of a run of a row: its largest logit x and the sum of 2^((x - m) k).
-// The difference is taken before the product, so a row of the type's lowest
-// value is a row of equal logits.  m = -inf with s = 0 for none above -inf.
+// A run of a row: its largest logit m and the sum s of 2^((x - m) k).  The
+// difference comes before the product, so a row of the type's lowest value is a
+// row of equal logits.  m = -inf with s = 0 where no logit is above -inf.
 __device__ __forceinline__ float floor_of(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, float k) {
     const float top = fmaxf(m, m2), base = floor_of(top);
@@ -83,93 +84,303 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, flo
     m = top;
 }
 
-template <class T, Work W, bool Grad>
-__global__ void __launch_bounds__(kThreads) hawk_row(const RowArgs<T> a) {
-    constexpr int V = 16 / static_cast<int>(sizeof(T));
+template <class T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+// Sixteen bytes of a row as words: what waits in registers stays packed.
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+template <class T> using Pack = Raw<T, kVec<T>>;
+template <class T>
+__device__ __forceinline__ float element(const Words& w, int j) {
+    return widen<T, kVec<T>>(__builtin_bit_cast(Pack<T>, w), j);
+}
+
+// Vector v of a row, -inf past its end; an out row (nothing of it is read) is -inf throughout.
+template <class T, bool Stream>
+__device__ __forceinline__ Words row_vector(const T* row, int64_t v, int64_t vocab, bool out) {
+    constexpr int V = kVec<T>;
+    Words x = __builtin_bit_cast(Words, (splat<T, V>(static_cast<T>(-INFINITY))));
+    if (!out) {
+        if (v + V <= vocab) {
+            x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(row + v)));
+        } else if (v < vocab) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (v + j >= vocab) continue;
+                if constexpr (sizeof(T) == 4) {
+                    x[j] = __builtin_bit_cast(uint32_t, row[v + j]);
+                } else {
+                    const uint32_t bits = __builtin_bit_cast(uint16_t, row[v + j]);
+                    x[j / 2] = j & 1 ? (x[j / 2] & 0xffffu) | bits << 16 : (x[j / 2] & 0xffff0000u) | bits;
+                }
+            }
+        }
+    }
+    return x;
+}
+template <class T, bool Stream>
+__device__ __forceinline__ void put_vector(T* row, int64_t v, int64_t vocab, const float (&x)[kVec<T>]) {
+    constexpr int V = kVec<T>;
+    if (v + V <= vocab) {
+        store<T, V, Stream>(row + v, x);
+    } else if (v < vocab) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (v + j < vocab) row[v + j] = static_cast<T>(x[j]);
+    }
+}
+
+// (m, s) of L lanes' runs joined in every lane: a fixed tree within a wave, the
+// waves in order.  `turn` alternates, so one barrier a row is enough.
+template <int L>
+__device__ __forceinline__ void join_lanes(float& m, float& s, float k, int turn) {
+#pragma unroll
+    for (int d = (L < 64 ? L : 64) / 2; d > 0; d >>= 1) {
+        const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+        join(m, s, m2, s2, k);
+    }
+    if constexpr (L > 64) {
+        constexpr int W = L / 64;
+        __shared__ float lds[2][2][W];
+        if ((threadIdx.x & 63) == 0) {
+            lds[turn][0][threadIdx.x >> 6] = m;
+            lds[turn][1][threadIdx.x >> 6] = s;
+        }
+        __syncthreads();
+        const int w = threadIdx.x & (W - 1);
+        m = lds[turn][0][w];
+        s = lds[turn][1][w];
+#pragma unroll
+        for (int d = W / 2; d > 0; d >>= 1) {
+            const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+            join(m, s, m2, s2, k);
+        }
+    }
+}
+
+// What a row's (m, s) and target give; lane 0 of the row writes it.
+template <Work W, class T>
+__device__ __forceinline__ void finish_row(const RowArgs<T>& a, int64_t n, bool out, bool writes, float top, float s,
+                                           float at, float& logs, float& c) {
+    logs = log2f(s);
+    float logp = 0.0f, lse = 0.0f, loss = 0.0f;
+    c = 0.0f;
+    if (!out) {
+        const float ln = logs * kLn2;
+        lse = fused(top, a.scale, ln);
+        logp = fused(at - top, a.scale, -ln);
+        if constexpr (W == kPolicy) policy_row(a, n, logp, loss, c);
+    }
+    if (writes) {
+        if (a.logp) a.logp[n] = logp;
+        if (a.lse) a.lse[n] = lse;
+        if (W == kPolicy && a.row_loss) a.row_loss[n] = loss;
+    }
+    c *= a.scale;
+}
+
+// A number that is one for the L lanes of a row, told to the compiler where they
+// are whole waves: rows are then addressed by a scalar and a lane's offset.
+template <int L>
+__device__ __forceinline__ int one_of(int x) {
+    if constexpr (L >= 64) return __builtin_amdgcn_readfirstlane(x);
+    else return x;
+}
+
+// Rows held whole in the registers of L lanes, NV vectors a lane: one read of the
+// logits for the loss and, where bar_logits is given, its gradient.  A workgroup
+// goes from row to row, and a vector's register takes the next row's as soon as
+// its gradient is stored, so loads run beside the second pass over the row.  The
+// row has more than half the vectors (NV > 1), so the first half needs no bounds.
+template <class T, int L, int NV, Work W, bool Grad, bool Stream>
+__global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(const RowArgs<T> a) {
+    constexpr int V = kVec<T>, R = (L > kThreads ? L : kThreads) / L;
+    const int lane = threadIdx.x % L, sub = one_of<L>(threadIdx.x / L), mine = lane * V;
+    const int vocab = static_cast<int>(a.vocab);
+    const float k = a.scale * kLog2e;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * R;
+    int64_t n = static_cast<int64_t>(blockIdx.x) * R + sub;
+    // -1: nothing of the row is read; vocab: a target past the vocabulary
+    auto target = [&](int64_t row) -> int {
+        if (row >= a.rows) return -1;
+        const int64_t y = target_of(a.target, a.target64, row);
+        return one_of<L>(y < 0 ? -1 : y < vocab ? static_cast<int>(y) : vocab);
+    };
+    // A row that is left out is not read: its lanes go on with what they hold, and
+    // nothing of it is used.
+    auto fetch = [&](Words& x, const T* row, int i) {
+        const int rest = vocab - i * L * V;     // what the row has from the lanes' first vector on
+        if (i < NV / 2) {
+            x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(row + i * L * V + static_cast<unsigned>(mine))));
+        } else {
+            x = __builtin_bit_cast(Words, (splat<T, V>(static_cast<T>(-INFINITY))));
+            if (mine + V <= rest) x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(row + i * L * V + static_cast<unsigned>(mine))));
+            else if (mine < rest) x = row_vector<T, Stream>(row + i * L * V, mine, rest, false);
+        }
+    };
+    int y = target(n);
+    Words x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        x[i] = Words{0, 0, 0, 0};
+        if (y >= 0) fetch(x[i], a.logits + n * a.row_stride, i);
+    }
+    int turn = 0;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * R; base < a.rows; base += step, turn ^= 1) {
+        const bool real = n < a.rows, out = y < 0;
+        float at = out ? 0.0f : y < vocab ? static_cast<float>(a.logits[n * a.row_stride + y]) : NAN;
+        const int64_t next = n + step;
+        const int next_y = target(next);
+        float m = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = fmaxf(m, element<T>(x[i], j));
+        const float own = floor_of(m);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            forget(x[i]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += exp2_fast((element<T>(x[i], j) - own) * k);
+            asm volatile("" : "+v"(s));
+        }
+        // read before any lane may store the gradient over it
+        asm volatile("" : "+v"(at));
+        join_lanes<L>(m, s, k, turn);
+        const float top = floor_of(m);
+        float logs, c;
+        finish_row<W>(a, n, out, real && lane == 0, top, s, at, logs, c);
+        const T* ahead = a.logits + next * a.row_stride;
+        if constexpr (Grad) {
+            T* bar = a.bar_logits + n * a.bar_stride;
+            const bool zero = out || c == 0.0f;
+            if (real) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int rest = vocab - i * L * V, hit = y - mine - i * L * V;
+                    float g[V];
+                    forget(x[i]);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) g[j] = -c * exp2_fast(fused(element<T>(x[i], j) - top, k, -logs));
+                    if (hit >= 0 && hit < V) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) g[j] = j == hit ? c + g[j] : g[j];
+                    }
+                    if (zero) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) g[j] = 0.0f;
+                    }
+                    if (i < NV / 2 || mine + V <= rest) store<T, V, Stream>(bar + i * L * V + static_cast<unsigned>(mine), g);
+                    else put_vector<T, Stream>(bar + i * L * V, mine, rest, g);
+                    if (next_y >= 0) fetch(x[i], ahead, i);
+                    asm volatile("" ::: "memory");     // a vector is stored before the next one is widened
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (next_y >= 0) fetch(x[i], ahead, i);
+        }
+        n = next;
+        y = next_y;
+    }
+}
+
+// Rows of any length, a workgroup of L lanes each, kAhead vectors a lane at a
+// time: the log-sum-exp as a running (m, s), then, for the gradient, the row
+// once more.
+constexpr int kAhead = 4;
+template <class T, int L, Work W, bool Stream>
+__global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
+    constexpr int V = kVec<T>;
     const int64_t n = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lane = threadIdx.x;
+    const float k = a.scale * kLog2e;
     const T* row = a.logits + n * a.row_stride;
     const int64_t y = target_of(a.target, a.target64, n);
     const bool out = y < 0;
-    const int64_t whole = a.vocab / V * V;
-    T* bar = Grad ? a.bar_logits + n * a.bar_stride : nullptr;
-    const float k = a.scale * kLog2e;
-    float c = 0.0f, lse = 0.0f;
+    float at = out ? 0.0f : y < a.vocab ? static_cast<float>(row[y]) : NAN;
+    float m = -INFINITY, s = 0.0f;
     if (!out) {
-        const float at = y < a.vocab ? static_cast<float>(row[y]) : NAN;
-        if constexpr (W == kLogp || W == kPolicy) {
-            float m = -INFINITY, s = 0.0f;
-            for (int64_t v = static_cast<int64_t>(tid) * V; v < whole; v += kThreads * V) {
-                float x[V], top = m;
-                load<T, V>(row + v, x);
+        for (int64_t v0 = static_cast<int64_t>(lane) * V; v0 < a.vocab; v0 += kAhead * L * V) {
+            Words x[kAhead];
 #pragma unroll
-                for (int j = 0; j < V; ++j) top = fmaxf(top, x[j]);
-                const float base = floor_of(top);
-                s *= exp2_fast((m - base) * k);
-                m = top;
+            for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row, v0 + i * L * V, a.vocab, false);
+            float top = m;
 #pragma unroll
-                for (int j = 0; j < V; ++j) s += exp2_fast((x[j] - base) * k);
-            }
-            for (int64_t v = whole + tid; v < a.vocab; v += kThreads) {
-                const float x = static_cast<float>(row[v]), top = fmaxf(m, x), base = floor_of(top);
-                s = s * exp2_fast((m - base) * k) + exp2_fast((x - base) * k);
-                m = top;
-            }
-            __shared__ float lds_m[kWaves], lds_s[kWaves];
-            for (int d = 32; d > 0; d >>= 1) {
-                const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
-                join(m, s, m2, s2, k);
-            }
-            if (lane == 0) { lds_m[wave] = m; lds_s[wave] = s; }
-            __syncthreads();
-            m = lds_m[0];
-            s = lds_s[0];
-            for (int w = 1; w < kWaves; ++w) join(m, s, lds_m[w], lds_s[w], k);
-            const float base = floor_of(m), logs = log2f(s);
-            lse = fused(base, a.scale, logs * kLn2);
-            const float logp = ((at - base) * k - logs) * kLn2;
-            float loss = 0.0f;
-            if constexpr (W == kPolicy) policy_row(a, n, logp, loss, c);
-            if (tid == 0) {
-                if (a.logp) a.logp[n] = logp;
-                if (a.lse) a.lse[n] = lse;
-                if (W == kPolicy && a.row_loss) a.row_loss[n] = loss;
-            }
-        } else {
-            lse = a.lse[n];
-            if constexpr (W == kGradient) c = a.bar_logp[n];
-            else {
-                float loss;
-                policy_row(a, n, a.logp[n], loss, c);
-            }
-            if (y >= a.vocab) c = NAN;
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) top = fmaxf(top, element<T>(x[i], j));
+            const float base = floor_of(top);
+            s *= exp2_fast((m - base) * k);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s += exp2_fast((element<T>(x[i], j) - base) * k);
+            m = top;
         }
-    } else if ((W == kLogp || W == kPolicy) && tid == 0) {
-        if (a.logp) a.logp[n] = 0.0f;
-        if (a.lse) a.lse[n] = 0.0f;
-        if (W == kPolicy && a.row_loss) a.row_loss[n] = 0.0f;
     }
-    if constexpr (Grad) {
-        c *= a.scale;
-        if (out || c == 0.0f) {
-            const float zero[V] = {};
-            for (int64_t v = static_cast<int64_t>(tid) * V; v < whole; v += kThreads * V) store<T, V>(bar + v, zero);
-            for (int64_t v = whole + tid; v < a.vocab; v += kThreads) bar[v] = static_cast<T>(0.0f);
-            return;
-        }
-        auto gradient = [&](float x, int64_t v) {
-            const float p = exp2_fast(fused(x, a.scale, -lse) * kLog2e);
-            return v == y ? c - c * p : -c * p;
-        };
-        for (int64_t v = static_cast<int64_t>(tid) * V; v < whole; v += kThreads * V) {
-            float x[V];
-            load<T, V>(row + v, x);
+    asm volatile("" : "+v"(at));
+    join_lanes<L>(m, s, k, 0);
+    const float top = floor_of(m);
+    float logs, c;
+    finish_row<W>(a, n, out, lane == 0, top, s, at, logs, c);
+    if (W != kPolicy || !a.bar_logits) return;
+    T* bar = a.bar_logits + n * a.bar_stride;
+    const bool zero = out || c == 0.0f;
+    for (int64_t v = static_cast<int64_t>(lane) * V; v < a.vocab; v += L * V) {
+        const Words x = row_vector<T, Stream>(row, v, a.vocab, zero);
+        float g[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = gradient(x[j], v + j);
-            store<T, V>(bar + v, x);
+        for (int j = 0; j < V; ++j) {
+            const float p = exp2_fast(fused(element<T>(x, j) - top, k, -logs));
+            g[j] = zero ? 0.0f : v + j == y ? c - c * p : -c * p;
         }
-        for (int64_t v = whole + tid; v < a.vocab; v += kThreads)
-            bar[v] = static_cast<T>(gradient(static_cast<float>(row[v]), v));
+        put_vector<T, Stream>(bar, v, a.vocab, g);
+    }
+}
+
+// The gradient from a saved lse: L lanes a row, kAhead vectors a lane at a time.
+template <class T, int L, Work W, bool Stream>
+__global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradient(const RowArgs<T> a) {
+    constexpr int V = kVec<T>, R = (L > kThreads ? L : kThreads) / L;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / L;
+    const int lane = threadIdx.x % L;
+    if (n >= a.rows) return;
+    const int64_t y = target_of(a.target, a.target64, n);
+    const T* row = a.logits + n * a.row_stride;
+    T* bar = a.bar_logits + n * a.bar_stride;
+    float c = 0.0f, lse = 0.0f;
+    if (y >= 0) {
+        lse = a.lse[n];
+        if constexpr (W == kGradient) {
+            c = a.bar_logp[n];
+        } else {
+            float loss;
+            policy_row(a, n, a.logp[n], loss, c);
+        }
+        c = (y < a.vocab ? c : NAN) * a.scale;
+    }
+    const bool zero = c == 0.0f;
+    for (int64_t v0 = static_cast<int64_t>(lane) * V; v0 < a.vocab; v0 += kAhead * L * V) {
+        Words x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row, v0 + i * L * V, a.vocab, zero);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t v = v0 + i * L * V;
+            float g[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                // l - lse is rounded once, from the saved lse, before it is taken to base 2
+                const float p = exp2_fast(fused(element<T>(x[i], j), a.scale, -lse) * kLog2e);
+                g[j] = zero ? 0.0f : -c * p;
+            }
+            if (y >= v && y < v + V) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[j] = v + j == y ? c + g[j] : g[j];
+            }
+            put_vector<T, Stream>(bar, v, a.vocab, g);
+        }
     }
 }
 
@@ -292,14 +503,89 @@ int launched(const char* what) {
     return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error(what, err);
 }
 
+// Rows that begin and end with 128-byte lines are passed as a stream.
+template <class T>
+bool whole_lines(const RowArgs<T>& a) {
+    auto whole = [&](const T* p, int64_t stride) {
+        return !p || (reinterpret_cast<uintptr_t>(p) % 128 == 0 && (stride * static_cast<int64_t>(sizeof(T))) % 128 == 0);
+    };
+    return whole(a.logits, a.row_stride) && whole(a.bar_logits, a.bar_stride);
+}
+
+constexpr int64_t kUnits = 256;  // compute units
+
+template <class T, int L, int NV, Work W, bool Grad, bool Stream>
+void launch_held(const RowArgs<T>& a, hipStream_t s) {
+    constexpr int threads = L > kThreads ? L : kThreads, R = threads / L;
+    const int64_t blocks = (a.rows + R - 1) / R;
+    // as many workgroups as the card holds at once, each taking row after row
+    const int64_t most = kUnits * (L > kThreads ? 1 : NV >= 16 ? 4 : 8);
+    hipLaunchKernelGGL((hawk_row_held<T, L, NV, W, Grad, Stream>), dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
+                       dim3(threads), 0, s, a);
+}
+
 template <class T, Work W>
 int rows_of(const RowArgs<T>& a, hipStream_t s) {
     if (a.rows == 0) return HK_OK;
-    const dim3 grid(static_cast<unsigned>(a.rows)), block(kThreads);
-    if constexpr (W == kGradient || W == kPolicyGradient) hipLaunchKernelGGL((hawk_row<T, W, true>), grid, block, 0, s, a);
-    else if (W == kPolicy && a.bar_logits) hipLaunchKernelGGL((hawk_row<T, W, W == kPolicy>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((hawk_row<T, W, false>), grid, block, 0, s, a);
-    return launched("hawk_row launch");
+    const int64_t vectors = (a.vocab + kVec<T> - 1) / kVec<T>;
+    const bool stream = whole_lines(a), few = a.rows < 2 * kUnits;
+    if constexpr (W == kGradient || W == kPolicyGradient) {
+        auto go = [&](auto lanes) {
+            constexpr int L = decltype(lanes)::value, R = (L > kThreads ? L : kThreads) / L;
+            const dim3 grid(static_cast<unsigned>((a.rows + R - 1) / R)), block(R * L);
+            if (stream) hipLaunchKernelGGL((hawk_row_gradient<T, L, W, true>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((hawk_row_gradient<T, L, W, false>), grid, block, 0, s, a);
+        };
+        if (vectors <= 32) go(std::integral_constant<int, 16>{});
+        else if (vectors <= 256) go(std::integral_constant<int, 64>{});
+        else if (few && vectors > 4096) go(std::integral_constant<int, 1024>{});
+        else go(std::integral_constant<int, 256>{});
+    } else {
+        const bool hold = W == kPolicy && a.bar_logits;
+        auto held = [&](auto lanes, auto count) {
+            constexpr int L = decltype(lanes)::value, NV = decltype(count)::value;
+            if constexpr (L >= 256) {         // taken for the gradient alone
+                if (stream) launch_held<T, L, NV, W, W == kPolicy, true>(a, s);
+                else launch_held<T, L, NV, W, W == kPolicy, false>(a, s);
+            } else {
+                if (hold) launch_held<T, L, NV, W, W == kPolicy, false>(a, s);
+                else launch_held<T, L, NV, W, false, false>(a, s);
+            }
+        };
+        std::integral_constant<int, 16> l16;
+        std::integral_constant<int, 64> l64;
+        std::integral_constant<int, 256> l256;
+        std::integral_constant<int, 1024> l1024;
+        std::integral_constant<int, 1> n1;
+        std::integral_constant<int, 2> n2;
+        std::integral_constant<int, 4> n4;
+        std::integral_constant<int, 8> n8;
+        std::integral_constant<int, 16> n16;
+        if (vectors <= 16) held(l16, n1);
+        else if (vectors <= 32) held(l16, n2);
+        else if (vectors <= 64) held(l16, n4);
+        else if (vectors <= 128) held(l64, n2);
+        else if (vectors <= 256) held(l64, n4);
+        else if (vectors <= 512) held(l64, n8);
+        else if (W == kPolicy && hold && vectors <= 16384) {
+            if constexpr (W == kPolicy) {
+                if (vectors <= 1024) held(l256, n4);
+                else if (vectors <= 2048) held(l256, n8);
+                else if (vectors <= 4096 && few) held(l1024, n4);
+                else if (vectors <= 4096) held(l256, n16);
+                else if (vectors <= 8192) held(l1024, n8);
+                else held(l1024, n16);
+            }
+        } else {
+            const dim3 grid(static_cast<unsigned>(a.rows));
+            const bool big = few || (W == kPolicy && a.bar_logits);
+            if (big && stream) hipLaunchKernelGGL((hawk_row_long<T, 1024, W, true>), grid, dim3(1024), 0, s, a);
+            else if (big) hipLaunchKernelGGL((hawk_row_long<T, 1024, W, false>), grid, dim3(1024), 0, s, a);
+            else if (stream) hipLaunchKernelGGL((hawk_row_long<T, 256, W, true>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((hawk_row_long<T, 256, W, false>), grid, dim3(256), 0, s, a);
+        }
+    }
+    return launched("row kernel launch");
 }
 
 // Calls f with the logits' type.
