@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(kThreads) hawk_dropout(const DropArgs a, const
                                                          const Acc<T> factor) {
     typedef Acc<T> A;
     constexpr int V = sizeof(T) == 8 ? 2 : sizeof(T) == 4 ? 4 : 8;
+    constexpr bool Stream = sizeof(T) == 2;
     const int64_t groups = Rows ? a.rows * (a.cols / kNumbers) : a.cols / kNumbers;
     const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kSets) + threadIdx.x;
     const int64_t per_row = a.cols / kNumbers;
@@ -81,8 +82,8 @@ __global__ void __launch_bounds__(kThreads) hawk_dropout(const DropArgs a, const
         if (g >= groups) continue;
 #pragma unroll
         for (int j = 0; j < kNumbers / V; ++j) {
-            in[s][j] = load_raw<T, V, true>(x + row[s] * a.x_stride + c[s] + j * V);
-            if (Residual) add[s][j] = load_raw<T, V, true>(residual + row[s] * a.residual_stride + c[s] + j * V);
+            in[s][j] = load_raw<T, V, Stream>(x + row[s] * a.x_stride + c[s] + j * V);
+            if (Residual) add[s][j] = load_raw<T, V, Stream>(residual + row[s] * a.residual_stride + c[s] + j * V);
         }
     }
 #pragma unroll
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) hawk_dropout(const DropArgs a, const
                 out[v] = dropped(a, u, j * V + v, widen<T, V>(in[s][j], v), factor);
                 if (Residual) out[v] += widen<T, V>(add[s][j], v);
             }
-            store<T, V, true>(y + row[s] * a.y_stride + c[s] + j * V, out);
+            store<T, V, Stream>(y + row[s] * a.y_stride + c[s] + j * V, out);
         }
     }
     if constexpr (!Rows) {                // the last counter's elements, of an array that is no whole counters

@@ -50,28 +50,42 @@ __device__ __forceinline__ int64_t target_of(const void* target, int wide, int64
     return wide ? static_cast<const int64_t*>(target)[n] : static_cast<const int32_t*>(target)[n];
 }
 
-// A row's loss by its log-probability (times its weight) and the loss's
+// What a row's loss reads beside its logits, asked for before they are reduced.
+struct PolicyRow {
+    float w, A, old, ref;
+};
+template <class T>
+__device__ __forceinline__ PolicyRow policy_planes(const RowArgs<T>& a, int64_t n, bool read) {
+    PolicyRow r{0.0f, 0.0f, 0.0f, 0.0f};
+    if (read) {
+        r.w = a.weight ? a.weight[n] : a.even;
+        r.A = a.advantage[n];
+        r.old = a.old_logp[n];
+        if (a.kl != 0.0f) r.ref = a.ref_logp[n];
+    }
+    return r;
+}
+
+// The row's loss by its log-probability (times its weight) and the loss's
 // derivative by it (times weight and bar_loss).  A weight of 0 gives 0.
 template <class T>
-__device__ __forceinline__ void policy_row(const RowArgs<T>& a, int64_t n, float logp, float& loss, float& slope) {
-    const float w = a.weight ? a.weight[n] : a.even;
+__device__ __forceinline__ void policy_row(const RowArgs<T>& a, const PolicyRow& p, float logp, float& loss, float& slope) {
     loss = slope = 0.0f;
-    if (w == 0.0f) return;
-    const float A = a.advantage[n];
-    const float r = expf(logp - a.old_logp[n]);
-    const float plain = r * A, clipped = fminf(fmaxf(r, a.low), a.high) * A;
+    if (p.w == 0.0f) return;
+    const float r = expf(logp - p.old);
+    const float plain = r * p.A, clipped = fminf(fmaxf(r, a.low), a.high) * p.A;
     // a NaN ratio stays one: fminf and fmaxf would drop it
     if (!(r == r)) { loss = slope = r; return; }
     loss = plain <= clipped ? -plain : -clipped;
     slope = plain <= clipped ? -plain : 0.0f;
-    if (!(A == A)) loss = slope = A;
+    if (!(p.A == p.A)) loss = slope = p.A;
     if (a.kl != 0.0f) {
-        const float d = a.ref_logp[n] - logp;
+        const float d = p.ref - logp;
         loss += a.kl * (expm1f(d) - d);
         slope -= a.kl * expm1f(d);
     }
-    loss *= w;
-    slope *= a.bar_loss ? w * *a.bar_loss : w;
+    loss *= p.w;
+    slope *= a.bar_loss ? p.w * *a.bar_loss : p.w;
 }
 
 // A run of a row: its largest logit m and the sum s of 2^((x - m) k).  The
@@ -94,39 +108,42 @@ __device__ __forceinline__ float element(const Words& w, int j) {
     return widen<T, kVec<T>>(__builtin_bit_cast(Pack<T>, w), j);
 }
 
-// Vector v of a row, -inf past its end; an out row (nothing of it is read) is -inf throughout.
+// A row is passed in vectors that start at 16-byte addresses, wherever the row
+// itself starts: position p of it is element p - lead, and what lies before the
+// row or past its end is -inf and neither read nor written.  (Vectors at the
+// row's own address, 2 bytes off: 4096 rows of 50001 bfloat16 logits 87 us.)
+template <class T>
+__device__ __forceinline__ int lead_of(const T* row) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+}
+// The vector at position p of [low, high): from (the row's address less its lead).
 template <class T, bool Stream>
-__device__ __forceinline__ Words row_vector(const T* row, int64_t v, int64_t vocab, bool out) {
+__device__ __forceinline__ Words row_vector(const T* from, int64_t p, int low, int64_t high) {
     constexpr int V = kVec<T>;
+    if (p >= low && p + V <= high) return __builtin_bit_cast(Words, (load_raw<T, V, Stream>(from + p)));
     Words x = __builtin_bit_cast(Words, (splat<T, V>(static_cast<T>(-INFINITY))));
-    if (!out) {
-        if (v + V <= vocab) {
-            x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(row + v)));
-        } else if (v < vocab) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (v + j >= vocab) continue;
-                if constexpr (sizeof(T) == 4) {
-                    x[j] = __builtin_bit_cast(uint32_t, row[v + j]);
-                } else {
-                    const uint32_t bits = __builtin_bit_cast(uint16_t, row[v + j]);
-                    x[j / 2] = j & 1 ? (x[j / 2] & 0xffffu) | bits << 16 : (x[j / 2] & 0xffff0000u) | bits;
-                }
-            }
+    for (int j = 0; j < V; ++j) {
+        if (p + j < low || p + j >= high) continue;
+        if constexpr (sizeof(T) == 4) {
+            x[j] = __builtin_bit_cast(uint32_t, from[p + j]);
+        } else {
+            const uint32_t bits = __builtin_bit_cast(uint16_t, from[p + j]);
+            x[j / 2] = j & 1 ? (x[j / 2] & 0xffffu) | bits << 16 : (x[j / 2] & 0xffff0000u) | bits;
         }
     }
     return x;
 }
 template <class T, bool Stream>
-__device__ __forceinline__ void put_vector(T* row, int64_t v, int64_t vocab, const float (&x)[kVec<T>]) {
+__device__ __forceinline__ void put_vector(T* to, int64_t p, int low, int64_t high, const float (&x)[kVec<T>]) {
     constexpr int V = kVec<T>;
-    if (v + V <= vocab) {
-        store<T, V, Stream>(row + v, x);
-    } else if (v < vocab) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (v + j < vocab) row[v + j] = static_cast<T>(x[j]);
+    if (p >= low && p + V <= high) {
+        store<T, V, Stream>(to + p, x);
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (p + j >= low && p + j < high) to[p + j] = static_cast<T>(x[j]);
 }
 
 // (m, s) of L lanes' runs joined in every lane: a fixed tree within a wave, the
@@ -159,7 +176,7 @@ __device__ __forceinline__ void join_lanes(float& m, float& s, float k, int turn
 
 // What a row's (m, s) and target give; lane 0 of the row writes it.
 template <Work W, class T>
-__device__ __forceinline__ void finish_row(const RowArgs<T>& a, int64_t n, bool out, bool writes, float top, float s,
+__device__ __forceinline__ void finish_row(const RowArgs<T>& a, const PolicyRow& planes, int64_t n, bool out, bool writes, float top, float s,
                                            float at, float& logs, float& c) {
     logs = log2f(s);
     float logp = 0.0f, lse = 0.0f, loss = 0.0f;
@@ -168,7 +185,7 @@ __device__ __forceinline__ void finish_row(const RowArgs<T>& a, int64_t n, bool 
         const float ln = logs * kLn2;
         lse = fused(top, a.scale, ln);
         logp = fused(at - top, a.scale, -ln);
-        if constexpr (W == kPolicy) policy_row(a, n, logp, loss, c);
+        if constexpr (W == kPolicy) policy_row(a, planes, logp, loss, c);
     }
     if (writes) {
         if (a.logp) a.logp[n] = logp;
@@ -187,13 +204,16 @@ __device__ __forceinline__ int one_of(int x) {
 }
 
 // Rows held whole in the registers of L lanes, NV vectors a lane: one read of the
-// logits for the loss and, where bar_logits is given, its gradient.  A workgroup
-// goes from row to row, and a vector's register takes the next row's as soon as
-// its gradient is stored, so loads run beside the second pass over the row.  The
-// row has more than half the vectors (NV > 1), so the first half needs no bounds.
-template <class T, int L, int NV, Work W, bool Grad, bool Stream>
+// logits for the loss and, where asked, its gradient.  A workgroup goes from row
+// to row, and a vector's register takes the next row's as soon as its gradient is
+// stored, so loads run beside the second pass over the row.  The row has no fewer
+// than half the vectors (NV > 1), so those before the half's last need no bounds.
+// Rows of whole waves pass as a stream (8192 rows of 131072 bfloat16 logits with
+// their gradient 841 us, 872 cached).
+template <class T, int L, int NV, Work W, bool Grad>
 __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(const RowArgs<T> a) {
     constexpr int V = kVec<T>, R = (L > kThreads ? L : kThreads) / L;
+    constexpr bool Stream = L >= 256;
     const int lane = threadIdx.x % L, sub = one_of<L>(threadIdx.x / L), mine = lane * V;
     const int vocab = static_cast<int>(a.vocab);
     const float k = a.scale * kLog2e;
@@ -208,14 +228,10 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
     // A row that is left out is not read: its lanes go on with what they hold, and
     // nothing of it is used.
     auto fetch = [&](Words& x, const T* row, int i) {
-        const int rest = vocab - i * L * V;     // what the row has from the lanes' first vector on
-        if (i < NV / 2) {
-            x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(row + i * L * V + static_cast<unsigned>(mine))));
-        } else {
-            x = __builtin_bit_cast(Words, (splat<T, V>(static_cast<T>(-INFINITY))));
-            if (mine + V <= rest) x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(row + i * L * V + static_cast<unsigned>(mine))));
-            else if (mine < rest) x = row_vector<T, Stream>(row + i * L * V, mine, rest, false);
-        }
+        const int lead = lead_of(row), rest = lead + vocab - i * L * V;   // the positions from lane 0's vector on
+        const T* from = row - lead + i * L * V;
+        if (i > 0 && i < NV / 2 - 1) x = __builtin_bit_cast(Words, (load_raw<T, V, Stream>(from + static_cast<unsigned>(mine))));
+        else x = row_vector<T, Stream>(from, mine, i == 0 ? lead : 0, rest);
     };
     int y = target(n);
     Words x[NV];
@@ -227,7 +243,9 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
     int turn = 0;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * R; base < a.rows; base += step, turn ^= 1) {
         const bool real = n < a.rows, out = y < 0;
-        float at = out ? 0.0f : y < vocab ? static_cast<float>(a.logits[n * a.row_stride + y]) : NAN;
+        const T* row = a.logits + n * a.row_stride;
+        float at = out ? 0.0f : y < vocab ? static_cast<float>(row[y]) : NAN;
+        const PolicyRow planes = policy_planes(a, n, W == kPolicy && !out);
         const int64_t next = n + step;
         const int next_y = target(next);
         float m = -INFINITY, s = 0.0f;
@@ -248,15 +266,16 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
         join_lanes<L>(m, s, k, turn);
         const float top = floor_of(m);
         float logs, c;
-        finish_row<W>(a, n, out, real && lane == 0, top, s, at, logs, c);
+        finish_row<W>(a, planes, n, out, real && lane == 0, top, s, at, logs, c);
         const T* ahead = a.logits + next * a.row_stride;
         if constexpr (Grad) {
-            T* bar = a.bar_logits + n * a.bar_stride;
+            const int lead = lead_of(row);
+            T* bar = a.bar_logits + n * a.bar_stride - lead;
             const bool zero = out || c == 0.0f;
             if (real) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int rest = vocab - i * L * V, hit = y - mine - i * L * V;
+                    const int hit = lead + y - mine - i * L * V;
                     float g[V];
                     forget(x[i]);
 #pragma unroll
@@ -269,8 +288,8 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
 #pragma unroll
                         for (int j = 0; j < V; ++j) g[j] = 0.0f;
                     }
-                    if (i < NV / 2 || mine + V <= rest) store<T, V, Stream>(bar + i * L * V + static_cast<unsigned>(mine), g);
-                    else put_vector<T, Stream>(bar + i * L * V, mine, rest, g);
+                    if (i > 0 && i < NV / 2 - 1) store<T, V, Stream>(bar + i * L * V + static_cast<unsigned>(mine), g);
+                    else put_vector<T, Stream>(bar + i * L * V, mine, i == 0 ? lead : 0, lead + vocab - i * L * V, g);
                     if (next_y >= 0) fetch(x[i], ahead, i);
                     asm volatile("" ::: "memory");     // a vector is stored before the next one is widened
                 }
@@ -289,22 +308,25 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
 // time: the log-sum-exp as a running (m, s), then, for the gradient, the row
 // once more.
 constexpr int kAhead = 4;
-template <class T, int L, Work W, bool Stream>
+template <class T, int L, Work W>
 __global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
     constexpr int V = kVec<T>;
     const int64_t n = blockIdx.x;
     const int lane = threadIdx.x;
     const float k = a.scale * kLog2e;
     const T* row = a.logits + n * a.row_stride;
+    const int lead = lead_of(row);
+    const int64_t high = lead + a.vocab;
     const int64_t y = target_of(a.target, a.target64, n);
     const bool out = y < 0;
     float at = out ? 0.0f : y < a.vocab ? static_cast<float>(row[y]) : NAN;
+    const PolicyRow planes = policy_planes(a, n, W == kPolicy && !out);
     float m = -INFINITY, s = 0.0f;
     if (!out) {
-        for (int64_t v0 = static_cast<int64_t>(lane) * V; v0 < a.vocab; v0 += kAhead * L * V) {
+        for (int64_t p = static_cast<int64_t>(lane) * V; p < high; p += kAhead * L * V) {
             Words x[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row, v0 + i * L * V, a.vocab, false);
+            for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, true>(row - lead, p + i * L * V, lead, high);
             float top = m;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
@@ -323,32 +345,36 @@ __global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
     join_lanes<L>(m, s, k, 0);
     const float top = floor_of(m);
     float logs, c;
-    finish_row<W>(a, n, out, lane == 0, top, s, at, logs, c);
+    finish_row<W>(a, planes, n, out, lane == 0, top, s, at, logs, c);
     if (W != kPolicy || !a.bar_logits) return;
-    T* bar = a.bar_logits + n * a.bar_stride;
+    T* bar = a.bar_logits + n * a.bar_stride - lead;
     const bool zero = out || c == 0.0f;
-    for (int64_t v = static_cast<int64_t>(lane) * V; v < a.vocab; v += L * V) {
-        const Words x = row_vector<T, Stream>(row, v, a.vocab, zero);
+    const int64_t at_y = out ? -1 : lead + y;
+    for (int64_t p = static_cast<int64_t>(lane) * V; p < high; p += L * V) {
+        const Words x = row_vector<T, true>(row - lead, p, lead, zero ? 0 : high);
         float g[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float p = exp2_fast(fused(element<T>(x, j) - top, k, -logs));
-            g[j] = zero ? 0.0f : v + j == y ? c - c * p : -c * p;
+            const float e = -c * exp2_fast(fused(element<T>(x, j) - top, k, -logs));
+            g[j] = zero ? 0.0f : p + j == at_y ? c + e : e;
         }
-        put_vector<T, Stream>(bar, v, a.vocab, g);
+        put_vector<T, true>(bar, p, lead, high, g);
     }
 }
 
 // The gradient from a saved lse: L lanes a row, kAhead vectors a lane at a time.
-template <class T, int L, Work W, bool Stream>
+template <class T, int L, Work W>
 __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradient(const RowArgs<T> a) {
     constexpr int V = kVec<T>, R = (L > kThreads ? L : kThreads) / L;
+    constexpr bool Stream = L >= 256;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / L;
     const int lane = threadIdx.x % L;
     if (n >= a.rows) return;
     const int64_t y = target_of(a.target, a.target64, n);
     const T* row = a.logits + n * a.row_stride;
-    T* bar = a.bar_logits + n * a.bar_stride;
+    const int lead = lead_of(row);
+    const int64_t high = lead + a.vocab, at_y = y < 0 ? -1 : lead + y;
+    T* bar = a.bar_logits + n * a.bar_stride - lead;
     float c = 0.0f, lse = 0.0f;
     if (y >= 0) {
         lse = a.lse[n];
@@ -356,51 +382,60 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
             c = a.bar_logp[n];
         } else {
             float loss;
-            policy_row(a, n, a.logp[n], loss, c);
+            policy_row(a, policy_planes(a, n, true), a.logp[n], loss, c);
         }
         c = (y < a.vocab ? c : NAN) * a.scale;
     }
     const bool zero = c == 0.0f;
-    for (int64_t v0 = static_cast<int64_t>(lane) * V; v0 < a.vocab; v0 += kAhead * L * V) {
+    for (int64_t p0 = static_cast<int64_t>(lane) * V; p0 < high; p0 += kAhead * L * V) {
         Words x[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row, v0 + i * L * V, a.vocab, zero);
+        for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row - lead, p0 + i * L * V, lead, zero ? 0 : high);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int64_t v = v0 + i * L * V;
+            const int64_t p = p0 + i * L * V;
             float g[V];
+            forget(x[i]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 // l - lse is rounded once, from the saved lse, before it is taken to base 2
-                const float p = exp2_fast(fused(element<T>(x[i], j), a.scale, -lse) * kLog2e);
-                g[j] = zero ? 0.0f : -c * p;
+                const float e = exp2_fast(fused(element<T>(x[i], j), a.scale, -lse) * kLog2e);
+                g[j] = zero ? 0.0f : -c * e;
             }
-            if (y >= v && y < v + V) {
+            if (at_y >= p && at_y < p + V) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) g[j] = v + j == y ? c + g[j] : g[j];
+                for (int j = 0; j < V; ++j) g[j] = p + j == at_y ? c + g[j] : g[j];
             }
-            put_vector<T, Stream>(bar, v, a.vocab, g);
+            put_vector<T, Stream>(bar, p, lead, high, g);
+            asm volatile("" ::: "memory");         // a vector is stored before the next one is widened
         }
     }
 }
 
-// The sum of `count` numbers in 64 bits: each thread its own stride in order,
-// then a fixed tree.
-__device__ __forceinline__ double sum_block(const float* x, int64_t count) {
-    __shared__ double lds[kWaves];
+// The sum of rows' losses in 64 bits: each workgroup its own run of kRun numbers
+// in a fixed order, and one more where there are several.  All of a thread's
+// loads are out at once (one after another, 65536 rows took 80 us).
+constexpr int kTotalThreads = 1024, kEach = 8, kRun = kTotalThreads * kEach;
+template <class In, class Out>
+__global__ void __launch_bounds__(kTotalThreads) hawk_row_total(const In* x, int64_t count, Out* out) {
+    __shared__ double lds[kTotalThreads / 64];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRun + threadIdx.x;
+    In v[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int64_t at = first + i * kTotalThreads;
+        v[i] = at < count ? x[at] : In(0);
+    }
     double t = 0.0;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads) t += static_cast<double>(x[i]);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) t += static_cast<double>(v[i]);
     for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = t;
     __syncthreads();
+    if (threadIdx.x != 0) return;
     t = 0.0;
-    for (int w = 0; w < kWaves; ++w) t += lds[w];
-    return t;
-}
-
-__global__ void __launch_bounds__(kThreads) hawk_row_total(const float* x, int64_t count, float* out) {
-    const double t = sum_block(x, count);
-    if (threadIdx.x == 0) *out = static_cast<float>(t);
+    for (int w = 0; w < kTotalThreads / 64; ++w) t += lds[w];
+    out[blockIdx.x] = static_cast<Out>(t);
 }
 
 struct PairArgs {
@@ -503,86 +538,68 @@ int launched(const char* what) {
     return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error(what, err);
 }
 
-// Rows that begin and end with 128-byte lines are passed as a stream.
-template <class T>
-bool whole_lines(const RowArgs<T>& a) {
-    auto whole = [&](const T* p, int64_t stride) {
-        return !p || (reinterpret_cast<uintptr_t>(p) % 128 == 0 && (stride * static_cast<int64_t>(sizeof(T))) % 128 == 0);
-    };
-    return whole(a.logits, a.row_stride) && whole(a.bar_logits, a.bar_stride);
-}
-
 constexpr int64_t kUnits = 256;  // compute units
 
-template <class T, int L, int NV, Work W, bool Grad, bool Stream>
+template <class T, int L, int NV, Work W, bool Grad>
 void launch_held(const RowArgs<T>& a, hipStream_t s) {
     constexpr int threads = L > kThreads ? L : kThreads, R = threads / L;
     const int64_t blocks = (a.rows + R - 1) / R;
     // as many workgroups as the card holds at once, each taking row after row
-    const int64_t most = kUnits * (L > kThreads ? 1 : NV >= 16 ? 4 : 8);
-    hipLaunchKernelGGL((hawk_row_held<T, L, NV, W, Grad, Stream>), dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
+    const int64_t most = kUnits * (L > kThreads ? (NV > 4 ? 1 : 2) : NV >= 16 ? 4 : NV >= 8 ? 6 : 8);
+    hipLaunchKernelGGL((hawk_row_held<T, L, NV, W, Grad>), dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
                        dim3(threads), 0, s, a);
 }
 
+template <int N> using Count = std::integral_constant<int, N>;
+
+// The lanes of a row by its vectors.  Its loss with the gradient holds rows of up
+// to 16384 vectors; without, those of up to 512 (several rows a workgroup, whose
+// reductions stay in a wave): a longer one needs no second pass, and a running
+// (m, s) holds nothing.  Fewer rows than two a unit take 1024 lanes each.
 template <class T, Work W>
 int rows_of(const RowArgs<T>& a, hipStream_t s) {
     if (a.rows == 0) return HK_OK;
-    const int64_t vectors = (a.vocab + kVec<T> - 1) / kVec<T>;
-    const bool stream = whole_lines(a), few = a.rows < 2 * kUnits;
+    constexpr int V = kVec<T>;
+    const auto off = [](const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(bytes)) % 16 != 0; };
+    const bool leads = off(a.logits, a.rows > 1 ? a.row_stride * static_cast<int64_t>(sizeof(T)) : 0);
+    const int64_t vectors = (a.vocab + (leads ? V - 1 : 0) + V - 1) / V;
+    const bool few = a.rows < 2 * kUnits;
     if constexpr (W == kGradient || W == kPolicyGradient) {
         auto go = [&](auto lanes) {
             constexpr int L = decltype(lanes)::value, R = (L > kThreads ? L : kThreads) / L;
-            const dim3 grid(static_cast<unsigned>((a.rows + R - 1) / R)), block(R * L);
-            if (stream) hipLaunchKernelGGL((hawk_row_gradient<T, L, W, true>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((hawk_row_gradient<T, L, W, false>), grid, block, 0, s, a);
+            hipLaunchKernelGGL((hawk_row_gradient<T, L, W>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)), dim3(R * L),
+                               0, s, a);
         };
-        if (vectors <= 32) go(std::integral_constant<int, 16>{});
-        else if (vectors <= 256) go(std::integral_constant<int, 64>{});
-        else if (few && vectors > 4096) go(std::integral_constant<int, 1024>{});
-        else go(std::integral_constant<int, 256>{});
+        if (vectors <= 32) go(Count<16>{});
+        else if (vectors <= 256) go(Count<64>{});
+        else if (few && vectors > 4096) go(Count<1024>{});
+        else go(Count<256>{});
     } else {
         const bool hold = W == kPolicy && a.bar_logits;
         auto held = [&](auto lanes, auto count) {
             constexpr int L = decltype(lanes)::value, NV = decltype(count)::value;
-            if constexpr (L >= 256) {         // taken for the gradient alone
-                if (stream) launch_held<T, L, NV, W, W == kPolicy, true>(a, s);
-                else launch_held<T, L, NV, W, W == kPolicy, false>(a, s);
-            } else {
-                if (hold) launch_held<T, L, NV, W, W == kPolicy, false>(a, s);
-                else launch_held<T, L, NV, W, false, false>(a, s);
-            }
+            if (hold) launch_held<T, L, NV, W, W == kPolicy>(a, s);
+            else if constexpr (L < 256) launch_held<T, L, NV, W, false>(a, s);
         };
-        std::integral_constant<int, 16> l16;
-        std::integral_constant<int, 64> l64;
-        std::integral_constant<int, 256> l256;
-        std::integral_constant<int, 1024> l1024;
-        std::integral_constant<int, 1> n1;
-        std::integral_constant<int, 2> n2;
-        std::integral_constant<int, 4> n4;
-        std::integral_constant<int, 8> n8;
-        std::integral_constant<int, 16> n16;
-        if (vectors <= 16) held(l16, n1);
-        else if (vectors <= 32) held(l16, n2);
-        else if (vectors <= 64) held(l16, n4);
-        else if (vectors <= 128) held(l64, n2);
-        else if (vectors <= 256) held(l64, n4);
-        else if (vectors <= 512) held(l64, n8);
-        else if (W == kPolicy && hold && vectors <= 16384) {
+        if (vectors <= 16) held(Count<16>{}, Count<1>{});
+        else if (vectors <= 32) held(Count<16>{}, Count<2>{});
+        else if (vectors <= 64) held(Count<16>{}, Count<4>{});
+        else if (vectors <= 128) held(Count<64>{}, Count<2>{});
+        else if (vectors <= 256) held(Count<64>{}, Count<4>{});
+        else if (vectors <= 512) held(Count<64>{}, Count<8>{});
+        else if (hold && vectors <= 16384) {
             if constexpr (W == kPolicy) {
-                if (vectors <= 1024) held(l256, n4);
-                else if (vectors <= 2048) held(l256, n8);
-                else if (vectors <= 4096 && few) held(l1024, n4);
-                else if (vectors <= 4096) held(l256, n16);
-                else if (vectors <= 8192) held(l1024, n8);
-                else held(l1024, n16);
+                if (vectors <= 1024) held(Count<256>{}, Count<4>{});
+                else if (vectors <= 2048) held(Count<256>{}, Count<8>{});
+                else if (vectors <= 4096 && few) held(Count<1024>{}, Count<4>{});
+                else if (vectors <= 4096) held(Count<256>{}, Count<16>{});
+                else if (vectors <= 8192) held(Count<1024>{}, Count<8>{});
+                else held(Count<1024>{}, Count<16>{});
             }
+        } else if (few || hold) {
+            hipLaunchKernelGGL((hawk_row_long<T, 1024, W>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
         } else {
-            const dim3 grid(static_cast<unsigned>(a.rows));
-            const bool big = few || (W == kPolicy && a.bar_logits);
-            if (big && stream) hipLaunchKernelGGL((hawk_row_long<T, 1024, W, true>), grid, dim3(1024), 0, s, a);
-            else if (big) hipLaunchKernelGGL((hawk_row_long<T, 1024, W, false>), grid, dim3(1024), 0, s, a);
-            else if (stream) hipLaunchKernelGGL((hawk_row_long<T, 256, W, true>), grid, dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((hawk_row_long<T, 256, W, false>), grid, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((hawk_row_long<T, 256, W>), dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, s, a);
         }
     }
     return launched("row kernel launch");
@@ -617,10 +634,33 @@ PairArgs pairs_of(const hk_row_loss_job& j) {
     return p;
 }
 
-int total(const float* x, int64_t count, float* out, hipStream_t s) {
-    hipLaunchKernelGGL(hawk_row_total, dim3(1), dim3(kThreads), 0, s, x, count, out);
+// *out = the sum of x, which takes `partial`'s doubles (2 * runs(count)) on the way.
+int64_t runs(int64_t count) { return (count + kRun - 1) / kRun; }
+int total(const float* x, int64_t count, float* out, double* partial, hipStream_t s) {
+    int64_t left = runs(count);
+    const dim3 block(kTotalThreads);
+    if (left <= 1) {
+        hipLaunchKernelGGL((hawk_row_total<float, float>), dim3(1), block, 0, s, x, count, out);
+        return launched("hawk_row_total launch");
+    }
+    hipLaunchKernelGGL((hawk_row_total<float, double>), dim3(static_cast<unsigned>(left)), block, 0, s, x, count, partial);
+    while (left > kRun) {                 // more than 2^26 numbers
+        double* next = partial + left;
+        hipLaunchKernelGGL((hawk_row_total<double, double>), dim3(static_cast<unsigned>(runs(left))), block, 0, s,
+                           static_cast<const double*>(partial), left, next);
+        partial = next;
+        left = runs(left);
+    }
+    hipLaunchKernelGGL((hawk_row_total<double, float>), dim3(1), block, 0, s, static_cast<const double*>(partial), left, out);
     return launched("hawk_row_total launch");
 }
+
+// Scratch: the sums' doubles, then a float a pair, then a float a row.
+double* partials(void* scratch) { return static_cast<double*>(scratch); }
+float* pair_floats(const hk_row_loss_job& j, void* scratch) {
+    return reinterpret_cast<float*>(partials(scratch) + 2 * runs(j.rows > j.pairs ? j.rows : j.pairs));
+}
+float* row_floats(const hk_row_loss_job& j, void* scratch) { return pair_floats(j, scratch) + j.pairs; }
 
 }  // namespace
 
@@ -628,7 +668,8 @@ extern "C" {
 
 size_t hk_row_loss_scratch_bytes(const hk_row_loss_job* job) {
     if (!job || job->rows < 0 || job->pairs < 0) return 0;
-    return sizeof(float) * static_cast<size_t>(job->rows + job->pairs + 1);
+    return sizeof(double) * 2 * static_cast<size_t>(runs(job->rows > job->pairs ? job->rows : job->pairs)) +
+           sizeof(float) * static_cast<size_t>(job->rows + job->pairs + 1);
 }
 
 int hk_token_logp(const hk_row_loss_job* job, void* scratch, void* stream) {
@@ -669,11 +710,11 @@ int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
     rc = typed(job->dtype, [&](auto t) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
-        a.row_loss = job->loss ? static_cast<float*>(scratch) : nullptr;
+        a.row_loss = job->loss ? row_floats(*job, scratch) : nullptr;
         return rows_of<T, kPolicy>(a, s);
     });
     if (rc != HK_OK || !job->loss) return rc;
-    return total(static_cast<const float*>(scratch), job->rows, job->loss, s);
+    return total(row_floats(*job, scratch), job->rows, job->loss, partials(scratch), s);
 }
 
 int hk_policy_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stream) {
@@ -702,8 +743,8 @@ int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) 
     int rc = check_pairs(job, scratch, "hk_preference_loss");
     if (rc != HK_OK) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    float* pair_loss = static_cast<float*>(scratch);
-    float* logp = job->logp ? job->logp : pair_loss + job->pairs;
+    float* pair_loss = pair_floats(*job, scratch);
+    float* logp = job->logp ? job->logp : row_floats(*job, scratch);
     rc = typed(job->dtype, [&](auto t) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
@@ -720,7 +761,7 @@ int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) 
         rc = launched("hawk_pair_loss launch");
         if (rc != HK_OK) return rc;
     }
-    return job->loss ? total(pair_loss, job->pairs, job->loss, s) : HK_OK;
+    return job->loss ? total(pair_loss, job->pairs, job->loss, partials(scratch), s) : HK_OK;
 }
 
 int hk_preference_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stream) {
@@ -731,7 +772,7 @@ int hk_preference_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stre
         return hawk_internal::set_error(HK_EVALUE, "hk_preference_loss_vjp: lse, margin and bar_logits are required");
     hipStream_t s = static_cast<hipStream_t>(stream);
     PairArgs p = pairs_of(*job);
-    p.bar_logp = static_cast<float*>(scratch);
+    p.bar_logp = row_floats(*job, scratch);
     hipLaunchKernelGGL(hawk_pair_slope, dim3(static_cast<unsigned>((job->pairs + kWaves - 1) / kWaves)), dim3(kThreads),
                        0, s, p);
     rc = launched("hawk_pair_slope launch");
