@@ -539,7 +539,7 @@ class RowLossJob(ctypes.Structure):
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "bar_logits", "target", "logp", "lse", "loss", "margin",
                                                 "bar_logp", "bar_loss", "old_logp", "ref_logp", "advantage", "weight",
-                                                "offsets")]
+                                                "offsets", "counter")]
                 + [(n, ctypes.c_int64) for n in ("rows", "vocab", "row_stride", "bar_stride", "pairs")]
                 + [(n, ctypes.c_float) for n in ("scale", "clip_low", "clip_high", "kl", "beta", "smoothing")]
                 + [(n, ctypes.c_int32) for n in ("dtype", "target64", "offsets64")])

@@ -33,6 +33,8 @@ struct RowArgs {
     const void* target;
     float *logp, *lse;
     float* row_loss;          // each row's weighted loss, or NULL
+    float* loss;              // their sum, taken by the last workgroup, or NULL
+    uint32_t* counter;        // workgroups done
     const float* bar_logp;    // the gradient's c (before scale), or NULL
     const float *bar_loss, *old_logp, *ref_logp, *advantage, *weight;
     int64_t rows, vocab, row_stride, bar_stride;
@@ -195,6 +197,41 @@ __device__ __forceinline__ void finish_row(const RowArgs<T>& a, const PolicyRow&
     c *= a.scale;
 }
 
+// The sum of rows' losses in 64 bits, each run of kRun numbers by one workgroup in a
+// fixed order.  All of a lane's loads are out at once (one after another, 65536
+// rows took 80 us).
+constexpr int kTotalThreads = 1024, kEach = 8, kRun = kTotalThreads * kEach;
+template <int Threads, class In>
+__device__ __forceinline__ double sum_run(const In* x, int64_t count) {
+    constexpr int each = kRun / Threads;
+    __shared__ double lds[Threads / 64];
+    double t = 0.0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < each; i0 += kEach) {
+        In v[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int64_t at = threadIdx.x + static_cast<int64_t>(i0 + i) * Threads;
+            v[i] = at < count ? x[at] : In(0);
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) t += static_cast<double>(v[i]);
+        if ((i0 + kEach) * static_cast<int64_t>(Threads) >= count) break;
+    }
+    for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = t;
+    __syncthreads();
+    t = 0.0;
+    for (int w = 0; w < Threads / 64; ++w) t += lds[w];
+    return t;
+}
+template <class In, class Out>
+__global__ void __launch_bounds__(kTotalThreads) hawk_row_total(const In* x, int64_t count, Out* out) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRun;
+    const double t = sum_run<kTotalThreads>(x + first, count - first < kRun ? count - first : kRun);
+    if (threadIdx.x == 0) out[blockIdx.x] = static_cast<Out>(t);
+}
+
 // A number that is one for the L lanes of a row, told to the compiler where they
 // are whole waves: rows are then addressed by a scalar and a lane's offset.
 template <int L>
@@ -301,6 +338,24 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
         }
         n = next;
         y = next_y;
+    }
+    if constexpr (W == kPolicy && L < 256) {
+        // few rows: the workgroup that is done last sums them all, instead of a
+        // launch of its own
+        if (a.loss) {
+            __shared__ int last;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last = atomicAdd(a.counter, 1u) == gridDim.x - 1;
+            __syncthreads();
+            if (!last) return;
+            __threadfence();
+            const double t = sum_run<kThreads>(a.row_loss, a.rows);
+            if (threadIdx.x == 0) {
+                *a.loss = static_cast<float>(t);
+                *a.counter = 0;
+            }
+        }
     }
 }
 
@@ -412,32 +467,6 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
     }
 }
 
-// The sum of rows' losses in 64 bits: each workgroup its own run of kRun numbers
-// in a fixed order, and one more where there are several.  All of a thread's
-// loads are out at once (one after another, 65536 rows took 80 us).
-constexpr int kTotalThreads = 1024, kEach = 8, kRun = kTotalThreads * kEach;
-template <class In, class Out>
-__global__ void __launch_bounds__(kTotalThreads) hawk_row_total(const In* x, int64_t count, Out* out) {
-    __shared__ double lds[kTotalThreads / 64];
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRun + threadIdx.x;
-    In v[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int64_t at = first + i * kTotalThreads;
-        v[i] = at < count ? x[at] : In(0);
-    }
-    double t = 0.0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) t += static_cast<double>(v[i]);
-    for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = t;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    t = 0.0;
-    for (int w = 0; w < kTotalThreads / 64; ++w) t += lds[w];
-    out[blockIdx.x] = static_cast<Out>(t);
-}
-
 struct PairArgs {
     const void *offsets, *target;
     const float *logp, *ref_logp, *weight, *bar_loss;
@@ -453,27 +482,55 @@ __device__ __forceinline__ int64_t cut_of(const PairArgs& a, int64_t k) {
 }
 
 // One wave a pair: both sequences' log ratios summed in 64 bits, then the loss.
-__global__ void __launch_bounds__(kThreads) hawk_pair_loss(const PairArgs a) {
-    const int64_t p = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+// A single workgroup takes all pairs and sums their losses too (Whole).
+constexpr int kPairThreads = 1024, kPairWaves = kPairThreads / 64, kPairs = 128;
+template <bool Whole>
+__global__ void __launch_bounds__(kPairThreads) hawk_pair_loss(const PairArgs a, float* total) {
     const int lane = threadIdx.x & 63;
-    if (p >= a.pairs) return;
-    const int64_t c0 = cut_of(a, 2 * p), c1 = cut_of(a, 2 * p + 1), c2 = cut_of(a, 2 * p + 2);
-    double t = 0.0;
-    for (int64_t n = c0 + lane; n < c2; n += 64) {
-        if (target_of(a.target, a.target64, n) < 0) continue;
-        const double r = static_cast<double>(a.logp[n]) - (a.ref_logp ? static_cast<double>(a.ref_logp[n]) : 0.0);
-        t += n < c1 ? r : -r;
+    double sum = 0.0;
+    for (int64_t p = static_cast<int64_t>(blockIdx.x) * kPairWaves + (threadIdx.x >> 6); p < a.pairs;
+         p += static_cast<int64_t>(gridDim.x) * kPairWaves) {
+        const int64_t c0 = cut_of(a, 2 * p), c1 = cut_of(a, 2 * p + 1), c2 = cut_of(a, 2 * p + 2);
+        double t = 0.0;
+        for (int64_t n0 = c0 + lane; n0 < c2; n0 += 4 * 64) {
+            float lp[4], ref[4];
+            int64_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t n = n0 + 64 * i;
+                y[i] = n < c2 ? target_of(a.target, a.target64, n) : -1;
+                lp[i] = n < c2 ? a.logp[n] : 0.0f;
+                ref[i] = n < c2 && a.ref_logp ? a.ref_logp[n] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double r = static_cast<double>(lp[i]) - static_cast<double>(ref[i]);
+                if (y[i] >= 0) t += n0 + 64 * i < c1 ? r : -r;
+            }
+        }
+        for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
+        const float w = a.weight ? a.weight[p] : a.even;
+        const double z = static_cast<double>(a.beta) * t;
+        // -log sigma(z) and -log sigma(-z) = z - log sigma(z), neither overflowing
+        const double soft = log1p(exp(-fabs(z)));
+        const double lose = soft + (z < 0.0 ? -z : 0.0), win = soft + (z > 0.0 ? z : 0.0);
+        const double loss = (z == z) ? (1.0 - a.smoothing) * lose + a.smoothing * win : z;
+        const float weighted = w == 0.0f ? 0.0f : static_cast<float>(w * loss);
+        sum += static_cast<double>(weighted);
+        if (lane == 0) {
+            if (a.margin) a.margin[p] = static_cast<float>(t);
+            if (!Whole && a.pair_loss) a.pair_loss[p] = weighted;
+        }
     }
-    for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
-    if (lane != 0) return;
-    const float w = a.weight ? a.weight[p] : a.even;
-    const double z = static_cast<double>(a.beta) * t;
-    // -log sigma(z) and -log sigma(-z) = z - log sigma(z), neither overflowing
-    const double soft = log1p(exp(-fabs(z)));
-    const double lose = soft + (z < 0.0 ? -z : 0.0), win = soft + (z > 0.0 ? z : 0.0);
-    const double loss = (z == z) ? (1.0 - a.smoothing) * lose + a.smoothing * win : z;
-    if (a.margin) a.margin[p] = static_cast<float>(t);
-    if (a.pair_loss) a.pair_loss[p] = w == 0.0f ? 0.0f : static_cast<float>(w * loss);
+    if constexpr (Whole) {
+        __shared__ double lds[kPairWaves];
+        if (lane == 0) lds[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        if (threadIdx.x != 0 || !total) return;
+        sum = 0.0;
+        for (int w = 0; w < kPairWaves; ++w) sum += lds[w];
+        *total = static_cast<float>(sum);
+    }
 }
 
 // The derivative of the loss by each row's log-probability: one wave a pair.
@@ -545,12 +602,22 @@ void launch_held(const RowArgs<T>& a, hipStream_t s) {
     constexpr int threads = L > kThreads ? L : kThreads, R = threads / L;
     const int64_t blocks = (a.rows + R - 1) / R;
     // as many workgroups as the card holds at once, each taking row after row
-    const int64_t most = kUnits * (L > kThreads ? (NV > 4 ? 1 : 2) : NV >= 16 ? 4 : NV >= 8 ? 6 : 8);
+    const int64_t most = kUnits * (L == 1024 ? 1 : L == 512 ? 2 : NV >= 16 ? 4 : NV >= 8 ? 6 : 8);
     hipLaunchKernelGGL((hawk_row_held<T, L, NV, W, Grad>), dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
                        dim3(threads), 0, s, a);
 }
 
 template <int N> using Count = std::integral_constant<int, N>;
+
+// A row's vectors, the most that its lead can make them.
+template <class T>
+int64_t vectors_of(const RowArgs<T>& a) {
+    constexpr int V = kVec<T>;
+    const uint64_t apart = a.rows > 1 ? static_cast<uint64_t>(a.row_stride) * sizeof(T) : 0;
+    const bool leads = (reinterpret_cast<uintptr_t>(a.logits) | apart) % 16 != 0;
+    return (a.vocab + (leads ? V - 1 : 0) + V - 1) / V;
+}
+constexpr int64_t kShortVectors = 512;     // rows that at most a wave holds
 
 // The lanes of a row by its vectors.  Its loss with the gradient holds rows of up
 // to 16384 vectors; without, those of up to 512 (several rows a workgroup, whose
@@ -559,10 +626,7 @@ template <int N> using Count = std::integral_constant<int, N>;
 template <class T, Work W>
 int rows_of(const RowArgs<T>& a, hipStream_t s) {
     if (a.rows == 0) return HK_OK;
-    constexpr int V = kVec<T>;
-    const auto off = [](const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(bytes)) % 16 != 0; };
-    const bool leads = off(a.logits, a.rows > 1 ? a.row_stride * static_cast<int64_t>(sizeof(T)) : 0);
-    const int64_t vectors = (a.vocab + (leads ? V - 1 : 0) + V - 1) / V;
+    const int64_t vectors = vectors_of(a);
     const bool few = a.rows < 2 * kUnits;
     if constexpr (W == kGradient || W == kPolicyGradient) {
         auto go = [&](auto lanes) {
@@ -586,14 +650,14 @@ int rows_of(const RowArgs<T>& a, hipStream_t s) {
         else if (vectors <= 64) held(Count<16>{}, Count<4>{});
         else if (vectors <= 128) held(Count<64>{}, Count<2>{});
         else if (vectors <= 256) held(Count<64>{}, Count<4>{});
-        else if (vectors <= 512) held(Count<64>{}, Count<8>{});
+        else if (vectors <= kShortVectors) held(Count<64>{}, Count<8>{});
         else if (hold && vectors <= 16384) {
             if constexpr (W == kPolicy) {
                 if (vectors <= 1024) held(Count<256>{}, Count<4>{});
                 else if (vectors <= 2048) held(Count<256>{}, Count<8>{});
                 else if (vectors <= 4096 && few) held(Count<1024>{}, Count<4>{});
                 else if (vectors <= 4096) held(Count<256>{}, Count<16>{});
-                else if (vectors <= 8192) held(Count<1024>{}, Count<8>{});
+                else if (vectors <= 8192) held(Count<512>{}, Count<16>{});
                 else held(Count<1024>{}, Count<16>{});
             }
         } else if (few || hold) {
@@ -707,13 +771,21 @@ int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
     if (rc != HK_OK) return rc;
     if (job->rows > 0 && job->loss && !scratch) return hawk_internal::set_error(HK_EVALUE, "hk_policy_loss: scratch is required");
     hipStream_t s = static_cast<hipStream_t>(stream);
+    bool summed = false;
     rc = typed(job->dtype, [&](auto t) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
         a.row_loss = job->loss ? row_floats(*job, scratch) : nullptr;
+        // in the rows' own launch where they are short and one run (200 rows of 48
+        // floats: 6.2 us a call against 7.7 with a launch more)
+        summed = job->loss && job->counter && job->rows > 0 && job->rows <= kRun && vectors_of(a) <= kShortVectors;
+        if (summed) {
+            a.loss = job->loss;
+            a.counter = static_cast<uint32_t*>(job->counter);
+        }
         return rows_of<T, kPolicy>(a, s);
     });
-    if (rc != HK_OK || !job->loss) return rc;
+    if (rc != HK_OK || !job->loss || summed) return rc;
     return total(row_floats(*job, scratch), job->rows, job->loss, partials(scratch), s);
 }
 
@@ -756,8 +828,12 @@ int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) 
         PairArgs p = pairs_of(*job);
         p.logp = logp;
         p.pair_loss = pair_loss;
-        hipLaunchKernelGGL(hawk_pair_loss, dim3(static_cast<unsigned>((job->pairs + kWaves - 1) / kWaves)),
-                           dim3(kThreads), 0, s, p);
+        if (job->pairs <= kPairs) {
+            hipLaunchKernelGGL(hawk_pair_loss<true>, dim3(1), dim3(kPairThreads), 0, s, p, job->loss);
+            return launched("hawk_pair_loss launch");
+        }
+        hipLaunchKernelGGL(hawk_pair_loss<false>, dim3(static_cast<unsigned>((job->pairs + kPairWaves - 1) / kPairWaves)),
+                           dim3(kPairThreads), 0, s, p, nullptr);
         rc = launched("hawk_pair_loss launch");
         if (rc != HK_OK) return rc;
     }

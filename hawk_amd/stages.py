@@ -27,11 +27,28 @@ import ctypes
 import math
 import threading
 
+import torch
+
 from . import _core
 from .ir import HawkError
-from .runtime import Stage, _on, _stream_of, _torch, _Workspace
+from .runtime import Stage, _on, _stream_of, _Workspace
+
+_Tensor = torch.Tensor
 
 __all__ = ["recurrence", "token_logp", "policy_loss", "preference_loss", "dropout"]
+
+def _current_device() -> int:
+    raw = getattr(torch._C, "_cuda_getDevice", None)
+    if raw is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_device() if torch.cuda.is_available() else -1
+    return raw()
+
+
+def _current_raw(device: int) -> int:
+    """The current HIP stream's handle on ``device``."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return torch.cuda.current_stream(device).cuda_stream if raw is None else raw(device)
+
 
 #: Plans a stage keeps (one a set of shapes, strides and types); past this the
 #: oldest half is dropped.
@@ -42,16 +59,19 @@ class _Plan:
     """One set of shapes, strides and types, checked: the job's fields that do
     not move between calls, and where the pointers go."""
 
-    __slots__ = ("job", "words", "slots", "fn", "ref", "scratch", "lock", "cells", "apart")
+    __slots__ = ("job", "words", "slots", "fn", "ref", "scratch", "counter", "lock", "cells", "apart", "order", "spaces")
 
-    def __init__(self, job, slots: dict, fn, scratch: int, cells=(), apart=()):
+    def __init__(self, job, slots: dict, fn, scratch: int, counter=None, cells=(), apart=()):
         self.job, self.fn, self.scratch = job, fn, scratch
         self.words = (ctypes.c_uint64 * (ctypes.sizeof(job) // 8)).from_buffer(job)
         self.slots = slots                  # plane -> word of the job that holds its address
         self.ref = ctypes.byref(job)
         self.lock = threading.Lock()
+        self.counter = counter              # the word that holds the stream's zeroed cell
         self.cells = cells                  # by-value words: (name, word)
         self.apart = apart                  # planes that may not start at one address
+        self.order = ()                     # (name, type, shape, strides, word) of a call's planes in turn
+        self.spaces: dict = {}              # stream -> _Space
 
 
 def _word(job_type, *path) -> int:
@@ -68,13 +88,25 @@ _spaces: dict = {}
 _spaces_lock = threading.Lock()
 
 
-def _space(device: int, stream: int) -> _Workspace:
-    key = device, stream
-    held = _spaces.get(key)
-    if held is None:
-        with _spaces_lock:
-            held = _spaces.setdefault(key, _Workspace(_torch().device("cuda", device)))
-    return held
+class _Space:
+    """What a stage's calls on a stream work in: scratch, shared by every stage
+    on it (a stream's calls run one after another), a zeroed cell that every call
+    leaves at zero, and the lock that keeps a call's launches together."""
+
+    __slots__ = ("scratch", "cell", "lock", "held")
+
+    def __init__(self, scratch, cell, lock):
+        self.held = scratch, cell
+        self.scratch, self.cell, self.lock = scratch.data_ptr(), cell.data_ptr(), lock
+
+
+def _space(device: int, stream: int, nbytes: int) -> _Space:
+    with _spaces_lock, _on(stream):
+        found = _spaces.get((device, stream))
+        if found is None:
+            found = _spaces[device, stream] = _Workspace(torch.device("cuda", device)), threading.Lock()
+        work, lock = found
+        return _Space(work.bytes(("stage", "scratch", nbytes), nbytes), work.bytes(("stage", "cell"), 8, zero=True), lock)
 
 
 class _Stage(Stage):
@@ -89,6 +121,7 @@ class _Stage(Stage):
 
     def __init__(self):
         self._plans: dict = {}
+        self._last = None                   # the plan of the call before
         self._lock = threading.Lock()
 
     @property
@@ -112,7 +145,6 @@ class _Stage(Stage):
     def _plan(self, key, arrays: dict):
         """The plan of ``key``, made and checked where there is none."""
         self._names(arrays)
-        torch = _torch()
         tensors = {n: x for n, x in arrays.items() if x is not None and n in self.planes}
         for n, x in tensors.items():
             if not isinstance(x, torch.Tensor):
@@ -146,51 +178,72 @@ class _Stage(Stage):
 
     def _found(self, arrays: dict):
         """``(plan, [(word, value)], device)`` of a call."""
-        key, at, device = [], [], -1
+        device = _current_device()
+        bound, plan = [], self._last
+        if plan is not None and len(plan.order) == len(arrays):     # the shapes of the call before, most often
+            for (name, x), (known, dtype, shape, strides, word) in zip(arrays.items(), plan.order):
+                if name is not known:
+                    break
+                if dtype is None:
+                    continue                # a by-value argument
+                if (type(x) is not _Tensor or x.dtype is not dtype or x.get_device() != device or x.shape != shape
+                        or x.stride() != strides):
+                    break
+                bound.append((word, x.data_ptr()))
+            else:
+                return self._finish(plan, bound, arrays, device)
+        key, bound = [device], []
         try:
             for name, x in arrays.items():
                 if x is None or name in self.values:
+                    key.append((name, x is None))
                     continue
-                device = x.get_device()
-                key.append((name, x.dtype, x.shape, x.stride(), device))
-                at.append((name, x.data_ptr()))
+                key.append((name, x.dtype, x.shape, x.stride(), x.get_device()))
             key = tuple(key)
             plan = self._plans.get(key)
         except (AttributeError, RuntimeError, TypeError):
             plan, key = None, None
-        if plan is None or device != _torch().cuda.current_device():
+        if plan is None:
             plan = self._plan(key, arrays)
             if key is None:
                 self._refuse("a plane is no dense tensor")
+            plan.order = tuple((name, None, None, None, 0) if x is None or name in self.values else
+                               (name, x.dtype, x.shape, x.stride(), plan.slots.get(name, -1))
+                               for name, x in arrays.items())
+        self._last = plan if all(x is not None for x in arrays.values()) else None
+        bound = [(plan.slots[name], x.data_ptr()) for name, x in arrays.items()
+                 if x is not None and name not in self.values]
+        return self._finish(plan, bound, arrays, device)
+
+    def _finish(self, plan, bound: list, arrays: dict, device: int):
         for one, two in plan.apart:
             a, b = arrays.get(one), arrays.get(two)
             if a is not None and b is not None and a.data_ptr() == b.data_ptr() and a.numel():
                 self._refuse(f"the output {one!r} and {two!r} are one tensor")
-        slots = plan.slots
-        bound = [(slots[name], ptr) for name, ptr in at if name in slots]
-        if self.values:
-            for name, word in plan.cells:
-                bound.append((word, self._value(name, arrays.get(name))))
+        for name, word in plan.cells:
+            bound.append((word, self._value(name, arrays.get(name))))
         return plan, bound, device
 
     def run(self, arrays: dict, stream=None) -> None:
         """Bind ``arrays`` and run once, in place (``hawk.run``)."""
         plan, bound, device = self._found(arrays)
-        stream = _stream_of(stream)
-        scratch = None
-        if plan.scratch:
-            space = _space(device, stream)
-            with space_lock(space):
-                held = space.get(("stage", "", plan.scratch))
-                if held is None:
-                    with _on(stream):
-                        held = space.take(("stage", "", plan.scratch), (plan.scratch,), _torch().uint8)
-            scratch = held.data_ptr()
-        with plan.lock:
-            words = plan.words
-            for word, value in bound:
-                words[word] = value
-            rc = plan.fn(plan.ref, scratch, stream or None)
+        stream = _current_raw(device) if stream is None else _stream_of(stream)
+        words = plan.words
+        if not plan.scratch:
+            with plan.lock:
+                for word, value in bound:
+                    words[word] = value
+                rc = plan.fn(plan.ref, None, stream or None)
+        else:
+            space = plan.spaces.get(stream)
+            if space is None:
+                space = plan.spaces[stream] = _space(device, stream, plan.scratch)
+            if plan.counter is not None:
+                bound.append((plan.counter, space.cell))
+            with plan.lock, space.lock:
+                for word, value in bound:
+                    words[word] = value
+                rc = plan.fn(plan.ref, space.scratch, stream or None)
         if rc:
             _core.check(rc)
 
@@ -201,32 +254,24 @@ class _Stage(Stage):
         stream = _stream_of(stream)
         job = type(plan.job).from_buffer_copy(plan.job)
         words = (ctypes.c_uint64 * (ctypes.sizeof(job) // 8)).from_buffer(job)
-        for word, value in bound:
-            words[word] = value
-        scratch = None
+        scratch = cell = None
         if plan.scratch:
             with _on(stream):
-                scratch = _torch().empty(plan.scratch, dtype=_torch().uint8, device=f"cuda:{device}")
-        return Launcher(plan.fn, job, scratch, stream, dict(arrays))
-
-
-_space_locks: dict = {}
-
-
-def space_lock(space):
-    """The lock of one stream's scratch."""
-    held = _space_locks.get(id(space))
-    if held is None:
-        held = _space_locks.setdefault(id(space), threading.Lock())
-    return held
+                scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=f"cuda:{device}")
+                if plan.counter is not None:
+                    cell = torch.zeros(8, dtype=torch.uint8, device=f"cuda:{device}")
+                    bound.append((plan.counter, cell.data_ptr()))
+        for word, value in bound:
+            words[word] = value
+        return Launcher(plan.fn, job, (scratch, cell), stream, dict(arrays))
 
 
 class Launcher:
     """A stage with its planes bound (:meth:`prepare <_Stage.prepare>`)."""
 
-    def __init__(self, fn, job, scratch, stream: int, arrays: dict):
+    def __init__(self, fn, job, scratch: tuple, stream: int, arrays: dict):
         self._held = job, scratch, arrays
-        self._args = fn, ctypes.byref(job), None if scratch is None else scratch.data_ptr(), stream or None
+        self._args = fn, ctypes.byref(job), None if scratch[0] is None else scratch[0].data_ptr(), stream or None
 
     def __call__(self) -> None:
         fn, job, scratch, stream = self._args
@@ -236,7 +281,6 @@ class Launcher:
 
 
 def _element(stage, dtype, allowed) -> int:
-    torch = _torch()
     code = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}.get(dtype)
     if code is None or code not in allowed:
         names = ", ".join(n for c, n in ((0, "float32"), (1, "float64"), (2, "bfloat16"), (3, "float16"))
@@ -247,7 +291,6 @@ def _element(stage, dtype, allowed) -> int:
 
 def _integer(stage, name: str, x) -> int:
     """1 for a contiguous 1-D int64 plane, 0 for an int32 one."""
-    torch = _torch()
     if x.dtype not in (torch.int32, torch.int64) or x.dim() != 1 or not x.is_contiguous():
         stage._refuse(f"{name!r} is a contiguous 1-D int32 or int64 tensor, got {x.dtype} {tuple(x.shape)}")
     return int(x.dtype == torch.int64)
@@ -255,7 +298,6 @@ def _integer(stage, name: str, x) -> int:
 
 def _vector(stage, name: str, x, count: int) -> None:
     """A contiguous float32 plane of ``count`` numbers (a cell may have no axis)."""
-    torch = _torch()
     fits = x.dim() == 1 and x.shape[0] == count or count == 1 and x.dim() == 0
     if x.dtype != torch.float32 or not fits or not x.is_contiguous():
         stage._refuse(f"{name!r} is a contiguous float32 tensor of {count}, got {x.dtype} {tuple(x.shape)}")
@@ -285,7 +327,6 @@ class _Recurrence(_Stage):
             self._refuse("the plane 'h' is not given")
 
     def _make(self, t: dict) -> _Plan:
-        torch = _torch()
         first = t["gate"]
         packed = t.get("offsets")
         job = _core.RecurrenceJob()
@@ -415,7 +456,8 @@ class _Rows(_Stage):
         for n in t:
             slots[n] = _word(_core.RowLossJob, n)
         L = _core.lib()
-        return _Plan(job, slots, getattr(L, self.entry), int(L.hk_row_loss_scratch_bytes(ctypes.byref(job))))
+        return _Plan(job, slots, getattr(L, self.entry), int(L.hk_row_loss_scratch_bytes(ctypes.byref(job))),
+                     counter=_word(_core.RowLossJob, "counter"))
 
     def _more(self, t: dict, job) -> None:
         if t.get("weight") is not None:
@@ -604,7 +646,6 @@ class _Dropout(_Stage):
         return x
 
     def _found(self, arrays: dict):
-        torch = _torch()
         cell = arrays.get("offset")
         if isinstance(cell, torch.Tensor) and (cell.dtype != torch.int64 or cell.numel() != 1 or not cell.is_cuda):
             self._refuse("offset= is an int or an int64 cell on the device")

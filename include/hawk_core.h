@@ -394,7 +394,8 @@ typedef struct hk_plane {
  *   a (1 - a), bar_x = (1 - a) G;  bar_h0 = C_0.
  * bar_x may be bar_h itself and bar_gate may be gate or x itself (h is read
  * a step away, so nothing may overwrite it).
- * Scratch: hk_recurrence_scratch_bytes(job, vjp) bytes, no contents needed.
+ * Scratch: hk_recurrence_scratch_bytes(job, vjp) bytes, 16-byte aligned, no
+ * contents needed.
  * HK_EVALUE for sizes below 0, a missing plane or another type. */
 typedef struct hk_recurrence_job {
     hk_plane gate, x, h, bar_h, bar_gate, bar_x;
@@ -442,8 +443,10 @@ int hk_recurrence_vjp(const hk_recurrence_job* job, void* scratch, void* stream)
  * hk_preference_loss_vjp reads logits, target, offsets, margin, lse and writes
  * bar_logits.
  *
- * Scratch: hk_row_loss_scratch_bytes(job) bytes, no contents needed.  The
- * sums over rows and pairs are taken in 64 bits in a fixed order. */
+ * Scratch: hk_row_loss_scratch_bytes(job) bytes, 16-byte aligned, no contents
+ * needed.  counter: a 32-bit word on the device, 0 before the first call and
+ * left at 0 by each (NULL: the policy loss of few rows takes one launch more).
+ * The sums over rows and pairs are taken in 64 bits in a fixed order. */
 typedef struct hk_row_loss_job {
     const void* logits;
     void* bar_logits;
@@ -451,6 +454,7 @@ typedef struct hk_row_loss_job {
     float *logp, *lse, *loss, *margin;
     const float *bar_logp, *bar_loss, *old_logp, *ref_logp, *advantage, *weight;
     const void* offsets;
+    void* counter;
     int64_t rows, vocab, row_stride, bar_stride, pairs;
     float scale, clip_low, clip_high, kl, beta, smoothing;
     int32_t dtype, target64, offsets64;

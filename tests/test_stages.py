@@ -925,5 +925,5 @@ def test_the_entries_refuse_bad_jobs():
 def test_the_jobs_are_laid_out_as_the_header_has_them():
     assert ctypes.sizeof(_core.SeqPlane) == 32
     assert ctypes.sizeof(_core.RecurrenceJob) == 6 * 32 + 5 * 8 + 3 * 8 + 4 * 4
-    assert ctypes.sizeof(_core.RowLossJob) == 14 * 8 + 5 * 8 + 6 * 4 + 3 * 4 + 4
+    assert ctypes.sizeof(_core.RowLossJob) == 15 * 8 + 5 * 8 + 6 * 4 + 3 * 4 + 4
     assert ctypes.sizeof(_core.DropoutJob) == 4 * 8 + 5 * 8 + 2 * 8 + 2 * 4
