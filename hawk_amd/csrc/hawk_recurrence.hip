@@ -59,9 +59,10 @@ struct RecArgs {
     uint32_t* counter;        // a strip's: hands its chunks out in order
     typename Word<Acc<T>>::type* agg;      // [chunk][states][2]: each tile's (P, H)
     typename Word<Acc<T>>::type* state;    // [chunk][states]: the state that leaves each tile
+    uint32_t* flag;                        // [strip][chunk]: 1 once that state is written
     int64_t seqs, chans, cols, states;   // states: those of one tile row, seqs * chans (packed: chans)
     int steps, groups;        // groups: threads across a row's channels
-    int lcol, nt, strips, chunks;   // a tile: 2^lcol columns by nt threads along the steps
+    int lcol, ncol, nt, strips, chunks;   // a tile: ncol columns (Dir 0: 2^lcol) by nt threads along the steps
     int counter_step;
     int rev, offsets64;       // rev: scan step i is row steps - 1 - i (packed planes)
 };
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
     __shared__ A lds_p[kMost<T, Dir> * V], lds_h[kMost<T, Dir> * V], lds_c[kMost<T, Dir> * V];
     __shared__ int lds_chunk, lds_from;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int ncol = 1 << a.lcol, nt = a.nt;
+    const int ncol = Dir == 0 ? 1 << a.lcol : a.ncol, nt = a.nt;
 
     // A strip's chunks are taken in the order of the strip's counter: whatever a
     // tile waits for has begun before it.  (One counter for all would hand out
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
         __syncthreads();
         chunk = __builtin_amdgcn_readfirstlane(lds_chunk);
     }
-    const int64_t col0 = static_cast<int64_t>(strip) << a.lcol;
+    const int64_t col0 = static_cast<int64_t>(strip) * ncol;
     const int here = Dir == 0 ? tid & (ncol - 1) : tid / nt;
     const int tl = Dir == 0 ? tid >> a.lcol : tid - here * nt;
     // a column's sequence and first channel; the row's last channels are a full
@@ -401,6 +402,9 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
             __syncthreads();
             typedef typename Word<A>::type W;
             const bool more = chunk + 1 < a.chunks;
+            uint32_t* flags = a.flag + static_cast<int64_t>(strip) * a.chunks;
+            auto raise = [&] { __hip_atomic_store(flags + chunk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+            bool cut_all = true;
             if (more) {
                 for (int i = tid; i < ncol * V; i += blockDim.x) {
                     const int64_t col = col0 + i / V;
@@ -409,37 +413,33 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                     if (col >= a.cols) break;
                     place(col, cs, cc, cskip);
                     if (i % V < cskip) continue;
-                    W* word = a.agg + 2 * (chunk * a.states + cs * a.chans + cc + i % V);
-                    publish<A>(word, lds_p[i]);
-                    publish<A>(word + 1, lds_h[i]);
+                    const int64_t state = chunk * a.states + cs * a.chans + cc + i % V;
+                    publish<A>(a.agg + 2 * state, lds_p[i]);
+                    publish<A>(a.agg + 2 * state + 1, lds_h[i]);
+                    // a cut in the tile: nothing before it matters to what leaves it
+                    if (Cut && lds_p[i] == A(0)) publish<A>(a.state + state, lds_h[i]);
+                    else cut_all = false;
                 }
             }
-            // How far back a state is known.  One wave looks at 64 chunks before
-            // this one, through a channel that the strip's tiles all write.
+            // a packed sequence that begins in the tile cuts every channel, so the
+            // tiles after it wait for nothing before it
+            if constexpr (Packed) {
+                if (more && __syncthreads_and(cut_all) && tid == 0) raise();
+            }
+            // How far back a state is known.  One wave looks at the strip's flags of
+            // the 64 chunks before this one: two lines a look, since every waiting
+            // tile looks again and again (at the states' own words, 64 lines a look,
+            // they took a third of the card's bandwidth).  A flag only says where to
+            // look; the words it is about are awaited for themselves.
             if (chunk > 0 && tid < 64) {
-                int64_t cs, cc;
-                int cskip;
-                place(col0, cs, cc, cskip);
-                const int64_t watch = cs * a.chans + cc + V - 1;
                 const int look = chunk - 1 - lane;
-                int from = 0;
+                uint64_t known;
                 for (;;) {
-                    A p, h, st;
-                    bool has_state = look < 0, has_agg = false;
-                    if (look >= 0) {
-                        const W* word = a.agg + 2 * (look * a.states + watch);
-                        has_agg = read<A>(word, p) & read<A>(word + 1, h);
-                        has_state = read<A>(a.state + look * a.states + watch, st);
-                    }
-                    const uint64_t states = __ballot(has_state), aggs = __ballot(has_agg);
-                    if (states) {
-                        from = __builtin_ctzll(states);
-                        const uint64_t need = (uint64_t(1) << from) - 1;
-                        if ((aggs & need) == need) break;
-                    }
-                    __builtin_amdgcn_s_sleep(2);
+                    known = __ballot(look < 0 || __hip_atomic_load(flags + look, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 1u);
+                    if (known) break;
+                    __builtin_amdgcn_s_sleep(4);
                 }
-                if (lane == 0) lds_from = chunk - 1 - from;     // -1: the state before the first chunk
+                if (lane == 0) lds_from = chunk - 1 - __builtin_ctzll(known);     // -1: the state before the first chunk
             }
             __syncthreads();
             // The state that enters: the known one, then the chunks since in
@@ -454,7 +454,9 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                 if (i % V < cskip) continue;
                 const int64_t state = cs * a.chans + cc + i % V;
                 A carry;
-                if (from >= 0) carry = await<A>(a.state + from * a.states + state);
+                const W* known = a.state + (from < 0 ? 0 : from) * a.states + state;
+                bool here_yet = true;             // asked for with the first aggregates, not before them
+                if (from >= 0) here_yet = read<A>(known, carry);
                 else carry = !Packed && a.init ? a.init[state] : A(0);
                 for (int k = from + 1; k < chunk; k += kBatch) {
                     A p[kBatch], h[kBatch];
@@ -463,6 +465,10 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                     for (int b = 0; b < kBatch; ++b) {
                         const W* word = a.agg + 2 * ((k + b < chunk ? k + b : k) * a.states + state);
                         ok[b] = read<A>(word, p[b]) & read<A>(word + 1, h[b]);
+                    }
+                    if (!here_yet) {
+                        carry = await<A>(known);
+                        here_yet = true;
                     }
 #pragma unroll
                     for (int b = 0; b < kBatch; ++b) {
@@ -475,10 +481,13 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                         carry = apply(p[b], carry, h[b]);
                     }
                 }
-                if (more) publish<A>(a.state + chunk * a.states + state, apply(lds_p[i], carry, lds_h[i]));
+                if (!here_yet) carry = await<A>(known);
+                if (more && !(Cut && lds_p[i] == A(0)))
+                    publish<A>(a.state + chunk * a.states + state, apply(lds_p[i], carry, lds_h[i]));
                 lds_c[i] = carry;
             }
             __syncthreads();
+            if (more && tid == 0) raise();
 #pragma unroll
             for (int v = 0; v < V; ++v) enter[v] = lds_c[(here < ncol ? here : 0) * V + v];
         }
@@ -580,10 +589,11 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
 }
 
 // Before tiles that tell each other states: the counters at 0, no word written.
-__global__ void __launch_bounds__(256) hawk_recurrence_clear(uint4* at, int64_t counters, int64_t count) {
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u), ones = make_uint4(~0u, ~0u, ~0u, ~0u);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += 256LL * gridDim.x)
-        at[i] = i < counters ? zero : ones;
+__global__ void __launch_bounds__(256) hawk_recurrence_clear(uint32_t* at, int64_t counters, int64_t count) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += 256LL * gridDim.x) {
+        const uint32_t w = i < counters ? 0u : ~0u;
+        store_raw<uint32_t, 4, true>(at + 4 * i, Raw<uint32_t, 4>{w, w, w, w});
+    }
 }
 
 // A few steps (a token at a time, or some): one thread takes V channels of a
@@ -656,7 +666,7 @@ int log2_up(int64_t n) {
 // sequences.
 struct Shape {
     int v, k, dir;
-    int lcol, nt, chunks, threads;
+    int lcol, ncol, nt, chunks, threads;
     int groups;
     int64_t cols, strips, states;
     bool stream;
@@ -675,8 +685,8 @@ template <class T, bool Vjp> struct Tile {
 // where few strips fill the card a tile waits for a state many tiles back:
 // forward of 1 x 65536 x 1024 (4 strips of 32 lanes) 169 us, 117 with 8 of 16
 // lanes; 16 x 4096 x 2048 (128 strips) 159 us, 177 with 256 of 16.
-constexpr int kAcross = 5, kAcrossFew = 4;
-constexpr int64_t kManyStrips = 64;
+constexpr int kAcross = 5, kAcrossFew = 4, kAcrossLeast = 3;
+constexpr int64_t kManyStrips = 64, kFewStrips = 16;
 
 template <class T, bool Vjp>
 Shape shape_of(const hk_recurrence_job& j) {
@@ -699,15 +709,15 @@ Shape shape_of(const hk_recurrence_job& j) {
         constexpr int most = kMost<T, 1>;
         s.chunks = static_cast<int>((need + most - 1) / most);
         s.nt = static_cast<int>((need + s.chunks - 1) / s.chunks);
-        s.lcol = 0;
-        while ((2 << s.lcol) * s.nt <= kThreads && (int64_t(1) << s.lcol) < s.cols) ++s.lcol;
+        s.ncol = s.nt < kThreads ? kThreads / s.nt : 1;
+        if (s.ncol > s.cols) s.ncol = static_cast<int>(s.cols);
     } else {
         s.dir = 0;
         s.v = chan && j.chans >= Tile<T, Vjp>::kVec ? Tile<T, Vjp>::kVec : 1;
         s.k = Tile<T, Vjp>::kSteps;
         s.groups = static_cast<int>((j.chans + s.v - 1) / s.v);
         s.cols = seqs * s.groups;
-        const int across = (s.cols >> kAcross) >= kManyStrips ? kAcross : kAcrossFew;
+        const int across = (s.cols >> kAcross) >= kManyStrips ? kAcross : (s.cols >> kAcrossFew) >= kFewStrips ? kAcrossFew : kAcrossLeast;
         s.lcol = log2_up(s.groups);
         if (s.lcol > across) s.lcol = across;
         const int64_t need = (j.steps + s.k - 1) / s.k;
@@ -722,6 +732,7 @@ Shape shape_of(const hk_recurrence_job& j) {
         s.nt = static_cast<int>((need + s.chunks - 1) / s.chunks);
         s.nt = (s.nt + wt - 1) / wt * wt;          // whole waves
         s.chunks = static_cast<int>((need + s.nt - 1) / s.nt);
+        s.ncol = 1 << s.lcol;
     }
     // Whole lines: a strip's part of a row begins and ends with a 128-byte line in
     // every plane, so nothing is read twice and it need not stay in the caches
@@ -734,8 +745,8 @@ Shape shape_of(const hk_recurrence_job& j) {
         s.stream &= (p->seq * static_cast<int64_t>(sizeof(T))) % 128 == 0 && (p->step * static_cast<int64_t>(sizeof(T))) % 128 == 0 &&
                     reinterpret_cast<uintptr_t>(p->data) % 128 == 0;
     }
-    s.threads = ((s.nt << s.lcol) + 63) / 64 * 64;
-    s.strips = (s.cols + (int64_t(1) << s.lcol) - 1) >> s.lcol;
+    s.threads = (s.nt * s.ncol + 63) / 64 * 64;
+    s.strips = (s.cols + s.ncol - 1) / s.ncol;
     s.states = seqs * j.chans;
     return s;
 }
@@ -771,9 +782,9 @@ Plane<T> plane_of(const hk_plane& p, int64_t steps, bool flip) {
 // A strip's counter lies on a line of its own unless there are many.
 int counter_step(const Shape& s) { return s.strips > 1024 ? 1 : 32; }
 size_t counter_bytes(const Shape& s) { return (4 * static_cast<size_t>(s.strips) * counter_step(s) + 255) / 256 * 256; }
-// (P, H) and the state of every (chunk, state), in whole 16-byte words
+// (P, H) and the state of every (chunk, state), then the flags, in whole 16-byte words
 size_t word_bytes(const Shape& s, size_t word) {
-    return (3 * word * static_cast<size_t>(s.states) * s.chunks + 15) / 16 * 16;
+    return (3 * word * static_cast<size_t>(s.states) * s.chunks + 4 * static_cast<size_t>(s.strips) * s.chunks + 15) / 16 * 16;
 }
 
 template <class T, bool Vjp>
@@ -838,6 +849,7 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
     a.steps = static_cast<int>(j.steps);
     a.groups = s.groups;
     a.lcol = s.lcol;
+    a.ncol = s.ncol;
     a.nt = s.nt;
     a.strips = static_cast<int>(s.strips);
     a.chunks = s.chunks;
@@ -849,11 +861,12 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
         a.counter_step = counter_step(s);
         a.agg = reinterpret_cast<W*>(static_cast<unsigned char*>(scratch) + counter_bytes(s));
         a.state = a.agg + 2 * s.states * s.chunks;
+        a.flag = reinterpret_cast<uint32_t*>(a.state + s.states * s.chunks);
         const int64_t counters = static_cast<int64_t>(counter_bytes(s) / 16);
         const int64_t words = counters + static_cast<int64_t>(word_bytes(s, sizeof(A)) / 16);
         const int64_t blocks = (words + 1023) / 1024;
         hipLaunchKernelGGL(hawk_recurrence_clear, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256),
-                           0, stream, static_cast<uint4*>(scratch), counters, words);
+                           0, stream, static_cast<uint32_t*>(scratch), counters, words);
         const int rc = launched("hawk_recurrence_clear launch");
         if (rc != HK_OK) return rc;
     }
