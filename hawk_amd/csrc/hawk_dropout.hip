@@ -112,23 +112,62 @@ __global__ void __launch_bounds__(kThreads) hawk_dropout(const DropArgs a, const
     }
 }
 
-// Rows apart whose counters run on from one row into the next: an element at a time.
-template <class T>
+// Rows apart whose counters run on from one row into the next: a thread's eight
+// elements of a row begin at any half of a counter, so it takes two of them and
+// shifts.  (16384 rows of 4093 bfloat16 elements, 4096 apart, with a residual: 79 us;
+// 222 an element at a time.)
+template <class T, bool Residual>
 __global__ void __launch_bounds__(kThreads) hawk_dropout_apart(const DropArgs a, const T* x, const T* residual, T* y,
                                                                const Acc<T> factor) {
-    const int64_t n = a.rows * a.cols;
-    const int64_t g = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (g * kNumbers >= n) return;
-    const Words u = numbers(a, offset_of(a), g);
-    int64_t row = g * kNumbers / a.cols, c = g * kNumbers - row * a.cols;
+    typedef Acc<T> A;
+    const int64_t per_row = (a.cols + kNumbers - 1) / kNumbers;
+    const int64_t v = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (v >= a.rows * per_row) return;
+    const int64_t row = v / per_row, c = (v - row * per_row) * kNumbers;
+    const int64_t left = a.cols - c, i = row * a.cols + c;
+    x += row * a.x_stride + c;
+    y += row * a.y_stride + c;
+    if (Residual) residual += row * a.residual_stride + c;
+    A in[kNumbers], add[kNumbers];
+    if (left >= kNumbers) {
+        load<T, kNumbers>(x, in);
+        if (Residual) load<T, kNumbers>(residual, add);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kNumbers; ++j) {
+            in[j] = j < left ? static_cast<A>(x[j]) : A(0);
+            add[j] = Residual && j < left ? static_cast<A>(residual[j]) : A(0);
+        }
+    }
+    const uint64_t offset = offset_of(a);
+    const int shift = static_cast<int>(i % kNumbers);        // halves of the first counter that are not this thread's
+    const Words one = numbers(a, offset, i / kNumbers), two = numbers(a, offset, i / kNumbers + 1);
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { w[j] = one.w[j]; w[4 + j] = two.w[j]; }
+    if (shift & 4) {
+#pragma unroll
+        for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+    }
+    if (shift & 2) {
+#pragma unroll
+        for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+    }
+    Words u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u.w[j] = shift & 1 ? w[j] >> 16 | w[j + 1] << 16 : w[j];
+    A out[kNumbers];
 #pragma unroll
     for (int j = 0; j < kNumbers; ++j) {
-        if (row < a.rows) {
-            Acc<T> v = dropped(a, u, j, static_cast<Acc<T>>(x[row * a.x_stride + c]), factor);
-            if (residual) v += static_cast<Acc<T>>(residual[row * a.residual_stride + c]);
-            y[row * a.y_stride + c] = static_cast<T>(v);
-        }
-        if (++c == a.cols) { c = 0; ++row; }
+        out[j] = dropped(a, u, j, in[j], factor);
+        if (Residual) out[j] += add[j];
+    }
+    if (left >= kNumbers) {
+        store<T, kNumbers>(y, out);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kNumbers; ++j)
+            if (j < left) y[j] = static_cast<T>(out[j]);
     }
 }
 
@@ -137,7 +176,8 @@ int dropout(const hk_dropout_job& j, hipStream_t stream) {
     const int64_t n = j.rows * j.cols;
     if (n == 0) return HK_OK;
     const bool whole = j.cols % kNumbers == 0, vectors = j.rows == 1 || whole;
-    const int64_t groups = (n + kNumbers - 1) / kNumbers, per = vectors ? kThreads * kSets : kThreads;
+    const int64_t groups = vectors ? (n + kNumbers - 1) / kNumbers : j.rows * ((j.cols + kNumbers - 1) / kNumbers);
+    const int64_t per = vectors ? kThreads * kSets : kThreads;
     const int64_t blocks = (groups + per - 1) / per;
     if (blocks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, "hk_dropout: the planes exceed the grid limit");
     const DropArgs a{j.offset_cell, j.seed, j.offset, j.rows, j.cols, j.x_stride, j.residual_stride, j.y_stride,
@@ -146,7 +186,8 @@ int dropout(const hk_dropout_job& j, hipStream_t stream) {
     const T *x = static_cast<const T*>(j.x), *residual = static_cast<const T*>(j.residual);
     T* y = static_cast<T*>(j.y);
     const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
-    if (!vectors) hipLaunchKernelGGL(hawk_dropout_apart<T>, grid, block, 0, stream, a, x, residual, y, factor);
+    if (!vectors && residual) hipLaunchKernelGGL((hawk_dropout_apart<T, true>), grid, block, 0, stream, a, x, residual, y, factor);
+    else if (!vectors) hipLaunchKernelGGL((hawk_dropout_apart<T, false>), grid, block, 0, stream, a, x, residual, y, factor);
     else if (j.rows == 1 && residual) hipLaunchKernelGGL((hawk_dropout<T, true, false>), grid, block, 0, stream, a, x, residual, y, factor);
     else if (j.rows == 1) hipLaunchKernelGGL((hawk_dropout<T, false, false>), grid, block, 0, stream, a, x, residual, y, factor);
     else if (residual) hipLaunchKernelGGL((hawk_dropout<T, true, true>), grid, block, 0, stream, a, x, residual, y, factor);

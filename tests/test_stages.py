@@ -927,3 +927,17 @@ def test_the_jobs_are_laid_out_as_the_header_has_them():
     assert ctypes.sizeof(_core.RecurrenceJob) == 6 * 32 + 5 * 8 + 3 * 8 + 4 * 4
     assert ctypes.sizeof(_core.RowLossJob) == 15 * 8 + 5 * 8 + 6 * 4 + 3 * 4 + 4
     assert ctypes.sizeof(_core.DropoutJob) == 4 * 8 + 5 * 8 + 2 * 8 + 2 * 4
+
+
+@pytest.mark.gpu
+def test_the_recurrent_policy_example_learns(gpu):
+    """All stages together: recall by chance is 1 in 16."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "recurrent_policy.py"
+    spec = importlib.util.spec_from_file_location("recurrent_policy", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.train(gpu, rounds=60)
+    assert got["rewards"][0] < 0.2 and got["rewards"][-1] > 0.5
+    assert got["right"] > 0.8 and got["preference"][-1] < got["preference"][0]
