@@ -32,7 +32,7 @@ constexpr int kThreads = 256;
 
 // A workgroup's most threads.  Where lanes lie along the steps a long sequence
 // takes large tiles, since each tile has one state to wait for (64 rows of 2^20
-// float steps: 352 us in tiles of 256 threads, 258 of 512, 261 of 1024).
+// float steps: 352 us in tiles of 256 threads, 258 of 512, 261 of 1024; 205 now).
 template <class T, int Dir> constexpr int kMost = Dir == 0 ? kThreads : 512;
 
 template <class T>
@@ -67,23 +67,24 @@ struct RecArgs {
     int rev, offsets64;       // rev: scan step i is row steps - 1 - i (packed planes)
 };
 
-__device__ __forceinline__ int64_t cut_at(const void* offsets, int wide, int64_t s) {
-    return wide ? static_cast<const int64_t*>(offsets)[s] : static_cast<const int32_t*>(offsets)[s];
+// A packed sequence's first row; there are at most 2^30 rows.
+__device__ __forceinline__ int cut_at(const void* offsets, int wide, int s) {
+    return wide ? static_cast<int>(static_cast<const int64_t*>(offsets)[s]) : static_cast<const int32_t*>(offsets)[s];
 }
 // The same of an s that is one for the workgroup: a scalar load, which does not
 // wait for the tile's loads.  (No kernel here writes offsets.)
-__device__ __forceinline__ int64_t cut_at_scalar(const void* offsets, int wide, int64_t s) {
+__device__ __forceinline__ int cut_at_scalar(const void* offsets, int wide, int s) {
     typedef const __attribute__((address_space(4))) int64_t* Wide;
     typedef const __attribute__((address_space(4))) int32_t* Narrow;
-    return wide ? ((Wide)(offsets))[s] : ((Narrow)(offsets))[s];
+    return wide ? static_cast<int>(((Wide)(offsets))[s]) : ((Narrow)(offsets))[s];
 }
 
 // The sequence of [low, high] whose rows hold `row`: the last one that starts at
 // or before it.
 template <class Cut>
-__device__ __forceinline__ int64_t sequence_of(Cut cut, int64_t low, int64_t high, int64_t row) {
+__device__ __forceinline__ int sequence_of(Cut cut, int low, int high, int row) {
     while (low < high) {
-        const int64_t mid = (low + high + 1) >> 1;
+        const int mid = low + (high - low + 1) / 2;
         if (cut(mid) <= row) low = mid;
         else high = mid - 1;
     }
@@ -239,19 +240,19 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
     // direction, which end one, and the sequence the first is in.  The tile's
     // own sequences are found once; most tiles lie within one or two.
     unsigned begins = 0, ends = 0;
-    int64_t seq_at = 0, seq_low = 0, seq_high = 0;
-    auto cut = [&](int64_t q) -> int64_t { return cut_at(a.offsets, a.offsets64, q); };
+    int seq_at = 0, seq_low = 0, seq_high = 0;
+    auto cut = [&](int q) -> int { return cut_at(a.offsets, a.offsets64, q); };
     if constexpr (Packed) {
         const int tile0 = chunk * (nt * K), tile1 = tile0 + nt * K < a.steps ? tile0 + nt * K - 1 : a.steps - 1;
-        const int64_t row_a = a.rev ? a.steps - 1 - tile1 : tile0, row_b = a.rev ? a.steps - 1 - tile0 : tile1;
-        auto scalar = [&](int64_t q) -> int64_t { return cut_at_scalar(a.offsets, a.offsets64, q); };
-        seq_low = sequence_of(scalar, 0, a.seqs - 1, row_a);
+        const int row_a = a.rev ? a.steps - 1 - tile1 : tile0, row_b = a.rev ? a.steps - 1 - tile0 : tile1;
+        auto scalar = [&](int q) -> int { return cut_at_scalar(a.offsets, a.offsets64, q); };
+        seq_low = sequence_of(scalar, 0, static_cast<int>(a.seqs) - 1, row_a);
         seq_high = seq_low;
-        if (scalar(seq_low + 1) <= row_b) seq_high = sequence_of(scalar, seq_low, a.seqs - 1, row_b);
-        int64_t low = scalar(seq_low), high = scalar(seq_low + 1);
+        if (scalar(seq_low + 1) <= row_b) seq_high = sequence_of(scalar, seq_low, static_cast<int>(a.seqs) - 1, row_b);
+        int low = scalar(seq_low), high = scalar(seq_low + 1);
         if (rows > 0) {
-            const int64_t row = a.rev ? a.steps - 1 - row0 : row0;
-            int64_t q = seq_low;
+            const int row = a.rev ? a.steps - 1 - row0 : row0;
+            int q = seq_low;
             if (seq_low != seq_high) {
                 q = sequence_of(cut, seq_low, seq_high, row);
                 low = cut(q);
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (k >= rows) continue;
-                const int64_t r = a.rev ? row - k : row + k;
+                const int r = a.rev ? row - k : row + k;
                 while (!a.rev && r >= high && q < seq_high) {
                     ++q;
                     low = high;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
         }
     }
     // The sequence of the k-th row where it begins one.
-    auto moved = [&](int k, int64_t q) -> int64_t {
+    auto moved = [&](int k, int q) -> int {
         return k == 0 ? q : sequence_of(cut, seq_low, seq_high, a.rev ? a.steps - 1 - row0 - k : row0 + k);
     };
     auto begin = [&](int64_t q, int v) -> A { return a.init ? a.init[q * a.chans + c0 + v] : A(0); };
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
     A P[V], H[V], least[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { P[v] = least[v] = A(1); H[v] = A(0); }
-    int64_t q = seq_at;
+    int q = seq_at;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if constexpr (Packed) {
@@ -399,6 +400,14 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                     lds_p[here * V + v] = join(P[v], earlier_p[v]);
                 }
             }
+        }
+        // what lies between the tile's first step and this thread's
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            before_h[v] = apply(before_p[v], earlier_h[v], before_h[v]);
+            before_p[v] = join(before_p[v], earlier_p[v]);
+        }
+        if (a.chunks > 1) {
             __syncthreads();
             typedef typename Word<A>::type W;
             const bool more = chunk + 1 < a.chunks;
@@ -482,18 +491,19 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                     }
                 }
                 if (!here_yet) carry = await<A>(known);
-                if (more && !(Cut && lds_p[i] == A(0)))
-                    publish<A>(a.state + chunk * a.states + state, apply(lds_p[i], carry, lds_h[i]));
+                if (more) {
+                    if (!(Cut && lds_p[i] == A(0)))
+                        publish<A>(a.state + chunk * a.states + state, apply(lds_p[i], carry, lds_h[i]));
+                    if (i == V - 1) raise();      // the first column's last channel, which every strip has
+                }
                 lds_c[i] = carry;
             }
             __syncthreads();
-            if (more && tid == 0) raise();
 #pragma unroll
             for (int v = 0; v < V; ++v) enter[v] = lds_c[(here < ncol ? here : 0) * V + v];
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-            enter[v] = apply(before_p[v], apply(earlier_p[v], enter[v], earlier_h[v]), before_h[v]);
+        for (int v = 0; v < V; ++v) enter[v] = apply(before_p[v], enter[v], before_h[v]);
     }
 
     // the steps again, from the state that enters them
@@ -578,8 +588,8 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
     }
     if constexpr (Packed) {               // a sequence without rows: its state passes through
         if (chunk == 0 && a.fin && live) {
-            for (int64_t e = tl; e < a.seqs; e += nt) {
-                if (cut_at(a.offsets, a.offsets64, e) < cut_at(a.offsets, a.offsets64, e + 1)) continue;
+            for (int e = tl; e < a.seqs; e += nt) {
+                if (cut(e) < cut(e + 1)) continue;
 #pragma unroll
                 for (int v = 0; v < V; ++v)
                     if (v >= skip) a.fin[e * a.chans + c0 + v] = begin(e, v);
@@ -683,8 +693,9 @@ template <class T, bool Vjp> struct Tile {
 // the planes of 16 x 4096 x 2048 bfloat16 elements at 6.07 TB/s, 16 lanes at
 // 4.84, 64 at 5.88 (a copy of the pattern), but give half the steps a tile, and
 // where few strips fill the card a tile waits for a state many tiles back:
-// forward of 1 x 65536 x 1024 (4 strips of 32 lanes) 169 us, 117 with 8 of 16
-// lanes; 16 x 4096 x 2048 (128 strips) 159 us, 177 with 256 of 16.
+// forward of 1 x 65536 x 1024 178 us in 4 strips of 32 lanes, 120 in 8 of 16, 110
+// in 16 of 8; 8 x 2048 x 1536 44 us in 96 of 16, 46 in 192 of 8; 16 x 4096 x 2048
+// 157 us in 128 of 32, 177 in 256 of 16.
 constexpr int kAcross = 5, kAcrossFew = 4, kAcrossLeast = 3;
 constexpr int64_t kManyStrips = 64, kFewStrips = 16;
 

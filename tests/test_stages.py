@@ -941,3 +941,173 @@ def test_the_recurrent_policy_example_learns(gpu):
     got = module.train(gpu, rounds=60)
     assert got["rewards"][0] < 0.2 and got["rewards"][-1] > 0.5
     assert got["right"] > 0.8 and got["preference"][-1] < got["preference"][0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,C,layout,packed,dtype", [
+    (70001, 8, "channels", False, "float32"), (150001, 1, "steps", False, "float32"),
+    (40003, 10, "channels", True, "bfloat16"), (30001, 3, "channels", True, "float64")], ids=str)
+def test_a_long_recurrence_is_many_tiles_in_order(gpu, T, C, layout, packed, dtype):
+    """More tiles than one look back sees, and the same bits every time."""
+    import torch
+    print(T, C, layout, packed, dtype, flush=True)
+    for reverse in (False, True):
+        got, held, offsets = recurrence_case(5 if packed else 1, T, C, dtype, "value", reverse, layout, True, packed, gpu,
+                                             seed=40)
+        # slow gates: a state reaches back over many tiles
+        gate = 1 - 0.001 * np.random.default_rng(3).random(held["gate"].shape)
+        if packed:
+            gate[T // 2] = 0.0
+        t, held["gate"] = plane(gate, dtype, gpu)
+        got["gate"] = t.transpose(-1, -2).contiguous().transpose(-1, -2) if layout == "steps" else t
+        stage = hawk.stages.recurrence(reverse=reverse)
+        planes = {n: got[n] for n in ("gate", "x", "h0")}
+        if packed:
+            planes["offsets"] = torch.from_numpy(offsets).to(gpu)
+        outs = []
+        for _ in range(3):
+            h, last = torch.empty_like(got["x"]), torch.empty_like(got["h0"])
+            hawk.run(stage, h=h, last=last, **planes)
+            bars = {n: torch.empty_like(got["x"]) for n in ("bar_gate", "bar_x")}
+            bars["bar_h0"] = torch.empty_like(got["h0"])
+            hawk.run(stage.vjp, h=h, bar_h=got["bar_h"], bar_last=got["bar_last"], **planes, **bars)
+            outs.append((h, last, *bars.values()))
+        assert all(torch.equal(a, b) for o in outs[1:] for a, b in zip(outs[0], o))
+        want, want_last, size = oracle_forward(held["gate"], held["x"], held["h0"], offsets, "value", reverse)
+        close(back(h), want, size, T, "value", dtype)
+        close(back(last), want_last, np.abs(size).max() + np.abs(want_last), T, "value", dtype, state=True)
+        wants, sizes = oracle_vjp(held["gate"], None, back(h), held["h0"], held["bar_h"], held["bar_last"], offsets,
+                                  "value", reverse)
+        for n, w, z in zip(("bar_gate", "bar_x", "bar_h0"), wants, sizes):
+            close(back(bars[n]), w, z, T, "value", dtype, state=n == "bar_h0")
+
+
+@pytest.mark.gpu
+def test_planes_whose_offsets_pass_32_bits(gpu):
+    """Two sequences, rows or steps more than 2^31 elements apart."""
+    import torch
+    far = (1 << 31) + 40
+    buffer = torch.empty(far + 4096, dtype=torch.bfloat16, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(6)
+
+    def apart(shape, strides):
+        t = buffer.as_strided(shape, strides)
+        t.copy_(torch.randn(shape, generator=g, device=gpu))
+        return t
+    # sequences apart, then steps apart
+    for strides in ((far, 24, 1), (24, far, 1)):
+        x = apart((2, 2, 24), strides)
+        gate = torch.rand(2, 2, 24, generator=g, device=gpu).bfloat16()
+        near, want = x.contiguous(), torch.empty(2, 2, 24, dtype=torch.bfloat16, device=gpu)
+        hawk.run(hawk.stages.recurrence(), gate=gate, x=near, h=want)
+        hawk.run(hawk.stages.recurrence(), gate=gate, x=x, h=x)
+        assert torch.equal(x, want)
+        hawk.run(hawk.stages.recurrence().vjp, gate=gate, h=x, bar_h=near, bar_x=near)
+        bar, again = torch.empty_like(want), x.clone()
+        hawk.run(hawk.stages.recurrence().vjp, gate=gate, h=want, bar_h=again, bar_x=bar)
+        hawk.run(hawk.stages.recurrence().vjp, gate=gate, h=want, bar_h=x, bar_x=x)
+        assert torch.equal(x, bar)
+    logits = apart((2, 300), (far, 1))
+    near = logits.contiguous()
+    target = torch.tensor([3, 299], device=gpu)
+    out, want, lse = (torch.empty(2, device=gpu) for _ in range(3))
+    hawk.run(hawk.stages.token_logp(), logits=near, target=target, logp=want, lse=lse)
+    hawk.run(hawk.stages.token_logp(), logits=logits, target=target, logp=out)
+    assert torch.equal(out, want)
+    c, bar = torch.ones(2, device=gpu), torch.empty_like(near)
+    hawk.run(hawk.stages.token_logp().vjp, logits=near, target=target, lse=lse, bar_logp=c, bar_logits=bar)
+    hawk.run(hawk.stages.token_logp().vjp, logits=logits, target=target, lse=lse, bar_logp=c, bar_logits=logits)
+    assert torch.equal(logits, bar)
+    for width in (300, 301):
+        x = apart((2, width), (far, 1))
+        near = x.contiguous()
+        hawk.run(hawk.stages.dropout(0.3), x=near, y=near, seed=5)
+        hawk.run(hawk.stages.dropout(0.3), x=x, y=x, seed=5)
+        assert torch.equal(x, near)
+
+
+@pytest.mark.gpu
+def test_a_stage_of_many_shapes_keeps_a_bounded_number_of_plans(gpu):
+    import torch
+    from hawk_amd import stages
+    scan = hawk.stages.recurrence()
+    for n in range(1, stages.PLANS + 60):
+        x = torch.ones(1, n, 2, device=gpu)
+        h = torch.empty_like(x)
+        hawk.run(scan, gate=x, x=x, h=h)
+        if n % 37 == 0:
+            assert torch.equal(h[0, :, 0], torch.arange(1, n + 1, device=gpu, dtype=torch.float32))
+    assert len(scan._plans) <= stages.PLANS
+    # planes in another order, of another type, and with a plane left out
+    h64 = torch.empty(1, 4, 2, dtype=torch.float64, device=gpu)
+    ones = torch.ones_like(h64)
+    hawk.run(scan, h=h64, x=ones, gate=ones, h0=None)
+    assert torch.equal(h64[0, :, 1], torch.arange(1, 5, device=gpu, dtype=torch.float64))
+    with pytest.raises(HawkError, match="'x' is not given"):
+        hawk.run(scan, h=h64, x=None, gate=ones)
+
+
+@pytest.mark.gpu
+def test_stages_from_several_threads(gpu):
+    """One stage, one stream, four threads: a call's launches and scratch stay together."""
+    import threading
+
+    import torch
+    scan, loss_of = hawk.stages.recurrence(), hawk.stages.policy_loss()
+    g = torch.Generator(device=gpu).manual_seed(12)
+    work = []
+    for k in range(4):
+        T = 700 + 300 * k
+        gate = torch.rand(2, T, 40, generator=g, device=gpu)
+        x = torch.randn(2, T, 40, generator=g, device=gpu)
+        logits = torch.randn(50 + k, 3000, generator=g, device=gpu)
+        n = len(logits)
+        planes = dict(logits=logits, target=torch.randint(0, 3000, (n,), generator=g, device=gpu),
+                      old_logp=torch.full((n,), -9.0, device=gpu), advantage=torch.randn(n, generator=g, device=gpu))
+        h, loss = torch.empty_like(x), torch.empty(1, device=gpu)
+        hawk.run(scan, gate=gate, x=x, h=h)
+        hawk.run(loss_of, loss=loss, **planes)
+        work.append((gate, x, h, planes, loss))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(k):
+        gate, x, want, planes, want_loss = work[k]
+        for _ in range(40):
+            h, loss = torch.empty_like(x), torch.empty(1, device=gpu)
+            hawk.run(scan, gate=gate, x=x, h=h)
+            hawk.run(loss_of, loss=loss, **planes)
+            if not torch.equal(h, want) or not torch.equal(loss, want_loss):
+                wrong.append(k)
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_run_of_the_loss_sum(gpu):
+    import torch
+    N, V = 70001, 5
+    g = np.random.default_rng(8)
+    logits = torch.from_numpy(g.normal(size=(N, V)).astype(np.float32)).to(gpu)
+    target = torch.from_numpy(g.integers(0, V, N)).to(gpu)
+    A = torch.from_numpy(g.normal(size=N).astype(np.float32)).to(gpu)
+    logp, loss, old = torch.empty(N, device=gpu), torch.empty(1, device=gpu), torch.full((N,), -1.6, device=gpu)
+    hawk.run(hawk.stages.policy_loss(), logits=logits, target=target, old_logp=old, advantage=A, logp=logp, loss=loss)
+    want, _ = oracle_policy(back(logp), target.cpu().numpy(), back(old), back(A), None, np.full(N, 1.0 / N), (0.2, 0.2),
+                            0.0, 1.0)
+    # each row's loss errs by 8 u of itself, their sum in 64 bits by nothing, the cell by u
+    assert abs(back(loss)[0] - want.sum()) <= 10 * 2.0 ** -24 * np.abs(want).sum()
+    # pairs past one workgroup's
+    P = 300
+    offsets = torch.arange(0, 2 * P + 1, device=gpu) * 3
+    n = 6 * P
+    out = {k: torch.empty(m, device=gpu) for k, m in (("loss", 1), ("margin", P), ("logp", n))}
+    hawk.run(hawk.stages.preference_loss(beta=0.5), logits=logits[:n], target=target[:n], offsets=offsets, **out)
+    margin, total, _ = oracle_pairs(back(out["logp"]), target[:n].cpu().numpy(), np.zeros(n), offsets.cpu().numpy(),
+                                    np.full(P, 1.0 / P), 0.5, 0.0)
+    assert np.abs(back(out["margin"]) - margin).max() <= 4 * 2.0 ** -24 * np.abs(margin).max()
+    assert abs(back(out["loss"])[0] - total) <= 16 * 2.0 ** -24 * (1 + total)
