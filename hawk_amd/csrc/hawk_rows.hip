@@ -26,6 +26,20 @@ using namespace hawk_vec;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 
+struct PairArgs {
+    const void *offsets, *target;
+    const float *logp, *ref_logp, *weight, *bar_loss;
+    float *margin, *pair_loss;
+    int64_t rows, pairs;
+    float beta, smoothing, even;
+    int offsets64, target64;
+};
+
+__device__ __forceinline__ int64_t cut_of(const PairArgs& a, int64_t k) {
+    const int64_t v = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[k] : static_cast<const int32_t*>(a.offsets)[k];
+    return v < 0 ? 0 : v > a.rows ? a.rows : v;
+}
+
 template <class T>
 struct RowArgs {
     const T* logits;
@@ -40,9 +54,10 @@ struct RowArgs {
     int64_t rows, vocab, row_stride, bar_stride;
     float scale, low, high, kl, even;   // low, high: the ratio's bounds; even: the weight where weight is NULL
     int target64;
+    PairArgs pairs;           // the preference loss's gradient
 };
 
-enum Work { kLogp, kPolicy, kGradient, kPolicyGradient };
+enum Work { kLogp, kPolicy, kGradient, kPolicyGradient, kPairGradient };
 
 // exp2 that flushes results below 2^-126 to 0, and a log2 to 1 ulp: the
 // hardware's own.
@@ -417,6 +432,26 @@ __global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
     }
 }
 
+// The derivative of the preference loss by a row's log-probability (times weight
+// and bar_loss): its sequence is the last that starts at or before it.
+__device__ __forceinline__ float pair_slope(const PairArgs& a, int64_t n) {
+    int64_t low = 0, high = 2 * a.pairs - 1;
+    while (low < high) {
+        const int64_t mid = (low + high + 1) >> 1;
+        if (cut_of(a, mid) <= n) low = mid;
+        else high = mid - 1;
+    }
+    if (n < cut_of(a, low) || n >= cut_of(a, low + 1)) return 0.0f;      // a row that no sequence holds
+    const int64_t p = low >> 1;
+    const float w = a.weight ? a.weight[p] : a.even;
+    if (w == 0.0f) return 0.0f;
+    float up, down;
+    sigmoid(a.beta * a.margin[p], up, down);
+    float slope = a.beta * w * (a.smoothing * up - (1.0f - a.smoothing) * down);
+    if (a.bar_loss) slope *= *a.bar_loss;
+    return low & 1 ? -slope : slope;
+}
+
 // The gradient from a saved lse: L lanes a row, kAhead vectors a lane at a time.
 template <class T, int L, Work W>
 __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradient(const RowArgs<T> a) {
@@ -435,17 +470,21 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
         lse = a.lse[n];
         if constexpr (W == kGradient) {
             c = a.bar_logp[n];
+        } else if constexpr (W == kPairGradient) {
+            c = pair_slope(a.pairs, n);
         } else {
             float loss;
             policy_row(a, policy_planes(a, n, true), a.logp[n], loss, c);
         }
         c = (y < a.vocab ? c : NAN) * a.scale;
     }
-    const bool zero = c == 0.0f;
+    // A row without a gradient is not read, unless to know it takes longer than to
+    // ask for the row's first vectors (a search for its pair).
+    const bool zero = c == 0.0f, unread = W == kPairGradient ? y < 0 : zero;
     for (int64_t p0 = static_cast<int64_t>(lane) * V; p0 < high; p0 += kAhead * L * V) {
         Words x[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row - lead, p0 + i * L * V, lead, zero ? 0 : high);
+        for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row - lead, p0 + i * L * V, lead, unread ? 0 : high);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t p = p0 + i * L * V;
@@ -465,20 +504,6 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
             asm volatile("" ::: "memory");         // a vector is stored before the next one is widened
         }
     }
-}
-
-struct PairArgs {
-    const void *offsets, *target;
-    const float *logp, *ref_logp, *weight, *bar_loss;
-    float *margin, *pair_loss, *bar_logp;
-    int64_t rows, pairs;
-    float beta, smoothing, even;
-    int offsets64, target64;
-};
-
-__device__ __forceinline__ int64_t cut_of(const PairArgs& a, int64_t k) {
-    const int64_t v = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[k] : static_cast<const int32_t*>(a.offsets)[k];
-    return v < 0 ? 0 : v > a.rows ? a.rows : v;
 }
 
 // One wave a pair: both sequences' log ratios summed in 64 bits, then the loss.
@@ -531,24 +556,6 @@ __global__ void __launch_bounds__(kPairThreads) hawk_pair_loss(const PairArgs a,
         for (int w = 0; w < kPairWaves; ++w) sum += lds[w];
         *total = static_cast<float>(sum);
     }
-}
-
-// The derivative of the loss by each row's log-probability: one wave a pair.
-__global__ void __launch_bounds__(kThreads) hawk_pair_slope(const PairArgs a) {
-    const int64_t p = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (p >= a.pairs) return;
-    const int64_t c0 = cut_of(a, 2 * p), c1 = cut_of(a, 2 * p + 1), c2 = cut_of(a, 2 * p + 2);
-    const float w = a.weight ? a.weight[p] : a.even;
-    float up, down;
-    sigmoid(a.beta * a.margin[p], up, down);
-    float slope = a.beta * w * (a.smoothing * up - (1.0f - a.smoothing) * down);
-    if (a.bar_loss) slope *= *a.bar_loss;
-    if (w == 0.0f) slope = 0.0f;
-    for (int64_t n = c0 + lane; n < c2; n += 64) a.bar_logp[n] = n < c1 ? slope : -slope;
-    // rows that no sequence holds
-    if (p == 0) for (int64_t n = lane; n < c0; n += 64) a.bar_logp[n] = 0.0f;
-    if (p == a.pairs - 1) for (int64_t n = c2 + lane; n < a.rows; n += 64) a.bar_logp[n] = 0.0f;
 }
 
 int check_job(const hk_row_loss_job* j, const std::string& who) {
@@ -618,6 +625,7 @@ int64_t vectors_of(const RowArgs<T>& a) {
     return (a.vocab + (leads ? V - 1 : 0) + V - 1) / V;
 }
 constexpr int64_t kShortVectors = 512;     // rows that at most a wave holds
+constexpr int64_t kFewVectors = 16384;     // 256 KiB of logits
 
 // The lanes of a row by its vectors.  Its loss with the gradient holds rows of up
 // to 16384 vectors; without, those of up to 512 (several rows a workgroup, whose
@@ -628,7 +636,7 @@ int rows_of(const RowArgs<T>& a, hipStream_t s) {
     if (a.rows == 0) return HK_OK;
     const int64_t vectors = vectors_of(a);
     const bool few = a.rows < 2 * kUnits;
-    if constexpr (W == kGradient || W == kPolicyGradient) {
+    if constexpr (W == kGradient || W == kPolicyGradient || W == kPairGradient) {
         auto go = [&](auto lanes) {
             constexpr int L = decltype(lanes)::value, R = (L > kThreads ? L : kThreads) / L;
             hipLaunchKernelGGL((hawk_row_gradient<T, L, W>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)), dim3(R * L),
@@ -651,6 +659,7 @@ int rows_of(const RowArgs<T>& a, hipStream_t s) {
         else if (vectors <= 128) held(Count<64>{}, Count<2>{});
         else if (vectors <= 256) held(Count<64>{}, Count<4>{});
         else if (vectors <= kShortVectors) held(Count<64>{}, Count<8>{});
+        else if (!hold && vectors <= 1024 && !few) launch_held<T, 64, 16, W, false>(a, s);
         else if (hold && vectors <= 16384) {
             if constexpr (W == kPolicy) {
                 if (vectors <= 1024) held(Count<256>{}, Count<4>{});
@@ -776,9 +785,11 @@ int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
         a.row_loss = job->loss ? row_floats(*job, scratch) : nullptr;
-        // in the rows' own launch where they are short and one run (200 rows of 48
-        // floats: 6.2 us a call against 7.7 with a launch more)
-        summed = job->loss && job->counter && job->rows > 0 && job->rows <= kRun && vectors_of(a) <= kShortVectors;
+        // in the rows' own launch where they are few: 200 rows of 48 floats 6.2 us a
+        // call against 7.7 with a launch more, but the workgroups' fences wait for
+        // what they stored: 4524 rows of 1660 float16 logits 123 us against 15
+        summed = job->loss && job->counter && job->rows > 0 && job->rows <= kRun && vectors_of(a) <= kShortVectors &&
+                 job->rows * vectors_of(a) <= kFewVectors;
         if (summed) {
             a.loss = job->loss;
             a.counter = static_cast<uint32_t*>(job->counter);
@@ -801,19 +812,20 @@ int hk_policy_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stream) 
     });
 }
 
-static int check_pairs(const hk_row_loss_job* j, const void* scratch, const std::string& who) {
+static int check_pairs(const hk_row_loss_job* j, const std::string& who) {
     using hawk_internal::set_error;
     const int rc = check_job(j, who);
     if (rc != HK_OK) return rc;
     if (j->pairs > 0 && !j->offsets) return set_error(HK_EVALUE, who + ": offsets are required");
     if (j->pairs == 0 && j->rows > 0) return set_error(HK_EVALUE, who + ": rows without a pair");
-    if ((j->rows > 0 || j->pairs > 0) && !scratch) return set_error(HK_EVALUE, who + ": scratch is required");
     return HK_OK;
 }
 
 int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
-    int rc = check_pairs(job, scratch, "hk_preference_loss");
+    int rc = check_pairs(job, "hk_preference_loss");
     if (rc != HK_OK) return rc;
+    if ((job->rows > 0 || job->pairs > 0) && !scratch)
+        return hawk_internal::set_error(HK_EVALUE, "hk_preference_loss: scratch is required");
     hipStream_t s = static_cast<hipStream_t>(stream);
     float* pair_loss = pair_floats(*job, scratch);
     float* logp = job->logp ? job->logp : row_floats(*job, scratch);
@@ -841,23 +853,18 @@ int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) 
 }
 
 int hk_preference_loss_vjp(const hk_row_loss_job* job, void* scratch, void* stream) {
-    int rc = check_pairs(job, scratch, "hk_preference_loss_vjp");
+    (void)scratch;
+    const int rc = check_pairs(job, "hk_preference_loss_vjp");
     if (rc != HK_OK) return rc;
     if (job->rows == 0) return HK_OK;
     if (!job->lse || !job->margin || !job->bar_logits)
         return hawk_internal::set_error(HK_EVALUE, "hk_preference_loss_vjp: lse, margin and bar_logits are required");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    PairArgs p = pairs_of(*job);
-    p.bar_logp = row_floats(*job, scratch);
-    hipLaunchKernelGGL(hawk_pair_slope, dim3(static_cast<unsigned>((job->pairs + kWaves - 1) / kWaves)), dim3(kThreads),
-                       0, s, p);
-    rc = launched("hawk_pair_slope launch");
-    if (rc != HK_OK) return rc;
     return typed(job->dtype, [&](auto t) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
-        a.bar_logp = p.bar_logp;
-        return rows_of<T, kGradient>(a, s);
+        a.pairs = pairs_of(*job);
+        return rows_of<T, kPairGradient>(a, s);
     });
 }
 
