@@ -24,11 +24,11 @@ namespace {
 using namespace hawk_vec;
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 
 struct PairArgs {
     const void *offsets, *target;
-    const float *logp, *ref_logp, *weight, *bar_loss;
+    const double* logp;       // before it is rounded
+    const float *ref_logp, *weight, *bar_loss;
     float *margin, *pair_loss;
     int64_t rows, pairs;
     float beta, smoothing, even;
@@ -48,6 +48,7 @@ struct RowArgs {
     float *logp, *lse;
     float* row_loss;          // each row's weighted loss, or NULL
     float* loss;              // their sum, taken by the last workgroup, or NULL
+    double* wide;             // logp before it is rounded to 32 bits, or NULL
     uint32_t* counter;        // workgroups done
     const float* bar_logp;    // the gradient's c (before scale), or NULL
     const float *bar_loss, *old_logp, *ref_logp, *advantage, *weight;
@@ -208,6 +209,10 @@ __device__ __forceinline__ void finish_row(const RowArgs<T>& a, const PolicyRow&
         if (a.logp) a.logp[n] = logp;
         if (a.lse) a.lse[n] = lse;
         if (W == kPolicy && a.row_loss) a.row_loss[n] = loss;
+        // A margin is a small difference of sums of these: rounding each to 32 bits
+        // (5e-7 of a logp of -10) would be most of its error.
+        if (W == kLogp && a.wide)
+            a.wide[n] = out ? 0.0 : (static_cast<double>(at) - top) * a.scale - log(static_cast<double>(s));
     }
     c *= a.scale;
 }
@@ -518,18 +523,19 @@ __global__ void __launch_bounds__(kPairThreads) hawk_pair_loss(const PairArgs a,
         const int64_t c0 = cut_of(a, 2 * p), c1 = cut_of(a, 2 * p + 1), c2 = cut_of(a, 2 * p + 2);
         double t = 0.0;
         for (int64_t n0 = c0 + lane; n0 < c2; n0 += 4 * 64) {
-            float lp[4], ref[4];
+            double lp[4];
+            float ref[4];
             int64_t y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int64_t n = n0 + 64 * i;
                 y[i] = n < c2 ? target_of(a.target, a.target64, n) : -1;
-                lp[i] = n < c2 ? a.logp[n] : 0.0f;
+                lp[i] = n < c2 ? a.logp[n] : 0.0;
                 ref[i] = n < c2 && a.ref_logp ? a.ref_logp[n] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const double r = static_cast<double>(lp[i]) - static_cast<double>(ref[i]);
+                const double r = lp[i] - static_cast<double>(ref[i]);
                 if (y[i] >= 0) t += n0 + 64 * i < c1 ? r : -r;
             }
         }
@@ -692,7 +698,6 @@ PairArgs pairs_of(const hk_row_loss_job& j) {
     PairArgs p{};
     p.offsets = j.offsets;
     p.target = j.target;
-    p.logp = j.logp;
     p.ref_logp = j.ref_logp;
     p.weight = j.weight;
     p.bar_loss = j.bar_loss;
@@ -728,12 +733,13 @@ int total(const float* x, int64_t count, float* out, double* partial, hipStream_
     return launched("hawk_row_total launch");
 }
 
-// Scratch: the sums' doubles, then a float a pair, then a float a row.
+// Scratch: the sums' doubles, a double a row (preference) or a float (policy),
+// then a float a pair.
+int64_t partial_count(const hk_row_loss_job& j) { return 2 * runs(j.rows > j.pairs ? j.rows : j.pairs); }
 double* partials(void* scratch) { return static_cast<double*>(scratch); }
-float* pair_floats(const hk_row_loss_job& j, void* scratch) {
-    return reinterpret_cast<float*>(partials(scratch) + 2 * runs(j.rows > j.pairs ? j.rows : j.pairs));
-}
-float* row_floats(const hk_row_loss_job& j, void* scratch) { return pair_floats(j, scratch) + j.pairs; }
+double* row_doubles(const hk_row_loss_job& j, void* scratch) { return partials(scratch) + partial_count(j); }
+float* row_floats(const hk_row_loss_job& j, void* scratch) { return reinterpret_cast<float*>(row_doubles(j, scratch)); }
+float* pair_floats(const hk_row_loss_job& j, void* scratch) { return reinterpret_cast<float*>(row_doubles(j, scratch) + j.rows); }
 
 }  // namespace
 
@@ -741,8 +747,7 @@ extern "C" {
 
 size_t hk_row_loss_scratch_bytes(const hk_row_loss_job* job) {
     if (!job || job->rows < 0 || job->pairs < 0) return 0;
-    return sizeof(double) * 2 * static_cast<size_t>(runs(job->rows > job->pairs ? job->rows : job->pairs)) +
-           sizeof(float) * static_cast<size_t>(job->rows + job->pairs + 1);
+    return sizeof(double) * static_cast<size_t>(partial_count(*job) + job->rows) + sizeof(float) * static_cast<size_t>(job->pairs + 1);
 }
 
 int hk_token_logp(const hk_row_loss_job* job, void* scratch, void* stream) {
@@ -828,17 +833,17 @@ int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) 
         return hawk_internal::set_error(HK_EVALUE, "hk_preference_loss: scratch is required");
     hipStream_t s = static_cast<hipStream_t>(stream);
     float* pair_loss = pair_floats(*job, scratch);
-    float* logp = job->logp ? job->logp : row_floats(*job, scratch);
+    double* wide = row_doubles(*job, scratch);
     rc = typed(job->dtype, [&](auto t) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
-        a.logp = logp;
+        a.wide = wide;
         return rows_of<T, kLogp>(a, s);
     });
     if (rc != HK_OK) return rc;
     if (job->pairs > 0) {
         PairArgs p = pairs_of(*job);
-        p.logp = logp;
+        p.logp = wide;
         p.pair_loss = pair_loss;
         if (job->pairs <= kPairs) {
             hipLaunchKernelGGL(hawk_pair_loss<true>, dim3(1), dim3(kPairThreads), 0, s, p, job->loss);

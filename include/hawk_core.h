@@ -436,7 +436,7 @@ int hk_recurrence_vjp(const hk_recurrence_job* job, void* scratch, void* stream)
  * hk_preference_loss: 2*pairs sequences of rows cut by offsets (2*pairs + 1
  * ascending row numbers from 0 to rows; 64-bit if offsets64 != 0); pair p
  * prefers sequence 2p to 2p + 1.  With s_k = sum over sequence k's kept rows of
- * (logp - ref_logp) (ref_logp NULL: 0): margin_p = s_2p - s_2p+1, z = beta margin,
+ * (logp - ref_logp) (ref_logp NULL: 0; each logp before it is rounded to 32 bits): margin_p = s_2p - s_2p+1, z = beta margin,
  *   *loss = sum_p weight_p (-(1 - smoothing) log sigma(z) - smoothing log sigma(-z)),
  * weight 1/pairs if NULL (a weight of 0 leaves the pair out).  It writes loss,
  * margin, logp, lse (each may be NULL).

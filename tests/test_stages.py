@@ -585,10 +585,10 @@ def test_the_policy_gradient_is_the_losss_difference_quotient(gpu):
         assert abs((ends[0] - ends[1]) / (2 * e) - float(bar[n, v])) < 1e-3, (n, v)
 
 
-def oracle_pairs(logp, target, ref, offsets, weight, beta, eps):
+def oracle_pairs(logp, target, ref, offsets, weight, beta, eps, margin=None):
     ratio = np.where(target >= 0, logp - ref, 0)
     sums = np.array([ratio[offsets[k]:offsets[k + 1]].sum() for k in range(len(offsets) - 1)])
-    margin = sums[0::2] - sums[1::2]
+    margin = sums[0::2] - sums[1::2] if margin is None else margin
     z = beta * margin
     soft = np.log1p(np.exp(-np.abs(z)))
     loss = (1 - eps) * (soft + np.maximum(-z, 0)) + eps * (soft + np.maximum(z, 0))
@@ -617,12 +617,19 @@ def test_preference_loss_and_its_gradient(gpu, lengths, V, dtype):
     out = {n: torch.empty(k, device=gpu) for n, k in (("loss", 1), ("margin", P), ("logp", N), ("lse", N))}
     w = torch.from_numpy(weight).to(gpu)
     hawk.run(stage, ref_logp=torch.from_numpy(ref).to(gpu), weight=w, **planes, **out)
-    margin, loss, slope = oracle_pairs(back(out["logp"]), target, ref.astype(np.float64), offsets,
-                                       weight.astype(np.float64), beta, eps)
+    margin, loss, slope = oracle_pairs(logp64, target, ref.astype(np.float64), offsets, weight.astype(np.float64), beta,
+                                       eps)
     close_row(back(out["logp"]), logp64, lse64)
-    # the sums are in 64 bits over the written log-probabilities: only the cells round
-    assert (np.abs(back(out["margin"]) - margin) <= 4 * 2.0 ** -24 * (np.abs(margin) + 1e-6)).all()
-    assert abs(back(out["loss"])[0] - loss) <= 16 * 2.0 ** -24 * (abs(loss) + weight.sum())
+    # the sums are in 64 bits over log-probabilities that are not rounded: each token's has the
+    # error of its row's sum of exponentials, whose terms err by their exponents' rounding,
+    # u log2(e) |x - m| each (|x - m| of the terms that weigh is below 16): 24 u; the cell rounds
+    tokens = np.add.reduceat(np.ones(N), np.minimum(offsets[:-1], N - 1)) * (np.diff(offsets) > 0)
+    allowed = 24 * 2.0 ** -24 * (tokens[0::2] + tokens[1::2]) + 2.0 ** -24 * np.abs(margin)
+    assert (np.abs(back(out["margin"]) - margin) <= allowed).all()
+    assert abs(back(out["loss"])[0] - loss) <= 16 * 2.0 ** -24 * (abs(loss) + weight.sum()) + beta * (weight * allowed).sum()
+    # the slope is the written margin's
+    _, _, slope = oracle_pairs(logp64, target, ref.astype(np.float64), offsets, weight.astype(np.float64), beta, eps,
+                               margin=back(out["margin"]))
     seq = np.searchsorted(offsets, np.arange(N), side="right") - 1
     c = 1.5 * np.where(seq % 2 == 0, slope[seq // 2], -slope[seq // 2])
     grad, size = oracle_gradient(l, target, back(out["lse"]), c, scale)
@@ -1109,5 +1116,6 @@ def test_more_rows_than_one_run_of_the_loss_sum(gpu):
     hawk.run(hawk.stages.preference_loss(beta=0.5), logits=logits[:n], target=target[:n], offsets=offsets, **out)
     margin, total, _ = oracle_pairs(back(out["logp"]), target[:n].cpu().numpy(), np.zeros(n), offsets.cpu().numpy(),
                                     np.full(P, 1.0 / P), 0.5, 0.0)
-    assert np.abs(back(out["margin"]) - margin).max() <= 4 * 2.0 ** -24 * np.abs(margin).max()
-    assert abs(back(out["loss"])[0] - total) <= 16 * 2.0 ** -24 * (1 + total)
+    # six written log-probabilities a pair, each rounded by u of itself
+    assert np.abs(back(out["margin"]) - margin).max() <= 2.0 ** -24 * (24 * 6 + 6 * np.abs(back(out["logp"])).max())
+    assert abs(back(out["loss"])[0] - total) <= 2.0 ** -24 * (16 * (1 + total) + 0.5 * (24 * 6 + 6 * 10))
