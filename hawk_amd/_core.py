@@ -534,12 +534,16 @@ class RecurrenceJob(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("dtype", "sigmoid", "reverse", "offsets64")])
 
 
+#: The zeroed bytes that a row loss's workgroups meet in (``HK_ROW_LOSS_STATE_BYTES``).
+STATE_BYTES = 8448
+
+
 class RowLossJob(ctypes.Structure):
     """The arguments of the losses over rows of logits (``hk_row_loss_job``)."""
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "bar_logits", "target", "logp", "lse", "loss", "margin",
                                                 "bar_logp", "bar_loss", "old_logp", "ref_logp", "advantage", "weight",
-                                                "offsets", "counter")]
+                                                "offsets", "state")]
                 + [(n, ctypes.c_int64) for n in ("rows", "vocab", "row_stride", "bar_stride", "pairs")]
                 + [(n, ctypes.c_float) for n in ("scale", "clip_low", "clip_high", "kl", "beta", "smoothing")]
                 + [(n, ctypes.c_int32) for n in ("dtype", "target64", "offsets64")])

@@ -24,6 +24,10 @@ namespace {
 using namespace hawk_vec;
 
 constexpr int kThreads = 256;
+constexpr int64_t kUnits = 256;            // compute units
+constexpr int64_t kWords = 4 * kUnits;     // parts of all rows that are split
+constexpr int64_t kSplitRows = kUnits / 4; // those rows at most
+static_assert(kWords * 8 + kSplitRows * 4 == HK_ROW_LOSS_STATE_BYTES, "a word a part, a counter a row");
 
 struct PairArgs {
     const void *offsets, *target;
@@ -49,11 +53,13 @@ struct RowArgs {
     float* row_loss;          // each row's weighted loss, or NULL
     float* loss;              // their sum, taken by the last workgroup, or NULL
     double* wide;             // logp before it is rounded to 32 bits, or NULL
-    uint32_t* counter;        // workgroups done
+    uint32_t* counter;        // workgroups done, a word a row (the sum: the first word)
+    uint64_t* run;            // the (m, s) of a row's parts, or NULL
     const float* bar_logp;    // the gradient's c (before scale), or NULL
     const float *bar_loss, *old_logp, *ref_logp, *advantage, *weight;
     int64_t rows, vocab, row_stride, bar_stride;
     float scale, low, high, kl, even;   // low, high: the ratio's bounds; even: the weight where weight is NULL
+    int64_t each;             // vectors of a row that a workgroup takes, where rows are split
     int target64;
     PairArgs pairs;           // the preference loss's gradient
 };
@@ -379,10 +385,84 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(c
     }
 }
 
-// Rows of any length, a workgroup of L lanes each, kAhead vectors a lane at a
-// time: the log-sum-exp as a running (m, s), then, for the gradient, the row
-// once more.
+// A lane's running (m, s) over positions first, first + L*V .. below end of a row
+// that starts at low, kAhead vectors at a time.
 constexpr int kAhead = 4;
+template <class T, int L>
+__device__ __forceinline__ void run_of(const T* from, int64_t first, int low, int64_t end, float k, float& m, float& s) {
+    constexpr int V = kVec<T>;
+    for (int64_t p = first; p < end; p += kAhead * L * V) {
+        Words x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, true>(from, p + i * L * V, low, end);
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) top = fmaxf(top, element<T>(x[i], j));
+        const float base = floor_of(top);
+        s *= exp2_fast((m - base) * k);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += exp2_fast((element<T>(x[i], j) - base) * k);
+        m = top;
+    }
+}
+
+// Few long rows: `parts` workgroups a row, a.each vectors a part.  A part leaves
+// its (m, s) in a word and counts itself; the last one counted joins the words in
+// their order and finishes the row.  A word is 0 until its part has come (no pair
+// is: s is 1 or more, a NaN, or 0 beside m = -inf), so nothing but the word itself
+// orders it: with a release and an acquire at each part's count, whose fences
+// write back and drop the caches, 512 rows of 131072 bfloat16 logits took 65 us
+// instead of 27.  The word waited for was sent before its part counted itself; if it
+// never shows (the state's words shared by two streams) the row is a NaN.
+constexpr int kMostParts = 64, kLooks = 1 << 20;
+template <class T, Work W>
+__global__ void __launch_bounds__(kThreads) hawk_row_parts(const RowArgs<T> a, int parts) {
+    constexpr int V = kVec<T>;
+    const int64_t n = blockIdx.x / parts;
+    const int part = static_cast<int>(blockIdx.x % parts), lane = threadIdx.x;
+    const float k = a.scale * kLog2e;
+    const int64_t y = target_of(a.target, a.target64, n);
+    const bool out = y < 0;
+    if (out && part > 0) return;
+    const T* row = a.logits + n * a.row_stride;
+    float at = out ? 0.0f : y < a.vocab ? static_cast<float>(row[y]) : NAN;
+    const PolicyRow planes = policy_planes(a, n, W == kPolicy && !out);
+    float m = -INFINITY, s = 0.0f;
+    if (!out) {
+        const int lead = lead_of(row);
+        const int64_t high = lead + a.vocab, end = (part + 1) * a.each * V;
+        run_of<T, kThreads>(row - lead, (part * a.each + lane) * V, lead, end < high ? end : high, k, m, s);
+        asm volatile("" : "+v"(at));
+        join_lanes<kThreads>(m, s, k, 0);
+        if (lane >= 64) return;
+        uint64_t* word = a.run + n * parts;
+        int done = 0;
+        if (lane == 0) {
+            const uint64_t pair = static_cast<uint64_t>(__builtin_bit_cast(uint32_t, m)) << 32 | __builtin_bit_cast(uint32_t, s);
+            __hip_atomic_store(word + part, pair, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            done = __hip_atomic_fetch_add(a.counter + n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1u;
+        }
+        if (!__builtin_amdgcn_readfirstlane(done)) return;
+        m = -INFINITY, s = 0.0f;
+        if (lane < parts) {
+            uint64_t pair = 0;
+            for (int i = 0; pair == 0 && i < kLooks; ++i) pair = __hip_atomic_load(word + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            word[lane] = 0;
+            m = __builtin_bit_cast(float, static_cast<uint32_t>(pair >> 32));
+            s = pair == 0 ? NAN : __builtin_bit_cast(float, static_cast<uint32_t>(pair));
+        }
+        if (lane == 0) a.counter[n] = 0;
+        join_lanes<64>(m, s, k, 0);
+    }
+    float logs, c;
+    finish_row<W>(a, planes, n, out, lane == 0, floor_of(m), s, at, logs, c);
+}
+
+// Rows of any length, a workgroup of L lanes each.
 template <class T, int L, Work W>
 __global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
     constexpr int V = kVec<T>;
@@ -391,50 +471,17 @@ __global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
     const float k = a.scale * kLog2e;
     const T* row = a.logits + n * a.row_stride;
     const int lead = lead_of(row);
-    const int64_t high = lead + a.vocab;
     const int64_t y = target_of(a.target, a.target64, n);
     const bool out = y < 0;
     float at = out ? 0.0f : y < a.vocab ? static_cast<float>(row[y]) : NAN;
     const PolicyRow planes = policy_planes(a, n, W == kPolicy && !out);
     float m = -INFINITY, s = 0.0f;
-    if (!out) {
-        for (int64_t p = static_cast<int64_t>(lane) * V; p < high; p += kAhead * L * V) {
-            Words x[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, true>(row - lead, p + i * L * V, lead, high);
-            float top = m;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) top = fmaxf(top, element<T>(x[i], j));
-            const float base = floor_of(top);
-            s *= exp2_fast((m - base) * k);
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) s += exp2_fast((element<T>(x[i], j) - base) * k);
-            m = top;
-        }
-    }
+    if (!out) run_of<T, L>(row - lead, static_cast<int64_t>(lane) * V, lead, lead + a.vocab, k, m, s);
     asm volatile("" : "+v"(at));
     join_lanes<L>(m, s, k, 0);
     const float top = floor_of(m);
     float logs, c;
     finish_row<W>(a, planes, n, out, lane == 0, top, s, at, logs, c);
-    if (W != kPolicy || !a.bar_logits) return;
-    T* bar = a.bar_logits + n * a.bar_stride - lead;
-    const bool zero = out || c == 0.0f;
-    const int64_t at_y = out ? -1 : lead + y;
-    for (int64_t p = static_cast<int64_t>(lane) * V; p < high; p += L * V) {
-        const Words x = row_vector<T, true>(row - lead, p, lead, zero ? 0 : high);
-        float g[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float e = -c * exp2_fast(fused(element<T>(x, j) - top, k, -logs));
-            g[j] = zero ? 0.0f : p + j == at_y ? c + e : e;
-        }
-        put_vector<T, true>(bar, p, lead, high, g);
-    }
 }
 
 // The derivative of the preference loss by a row's log-probability (times weight
@@ -460,7 +507,7 @@ __device__ __forceinline__ float pair_slope(const PairArgs& a, int64_t n) {
 // The gradient from a saved lse: L lanes a row, kAhead vectors a lane at a time.
 template <class T, int L, Work W>
 __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradient(const RowArgs<T> a) {
-    constexpr int V = kVec<T>, R = (L > kThreads ? L : kThreads) / L;
+    constexpr int V = kVec<T>, R = kThreads / L;
     constexpr bool Stream = L >= 256;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / L;
     const int lane = threadIdx.x % L;
@@ -468,7 +515,13 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
     const int64_t y = target_of(a.target, a.target64, n);
     const T* row = a.logits + n * a.row_stride;
     const int lead = lead_of(row);
-    const int64_t high = lead + a.vocab, at_y = y < 0 ? -1 : lead + y;
+    const int64_t last = lead + a.vocab, at_y = y < 0 ? -1 : lead + y;
+    int64_t high = last, first = static_cast<int64_t>(lane) * V;
+    if constexpr (L >= kThreads) {
+        const int64_t part = blockIdx.y * a.each * V, end = part + a.each * V;
+        first += part;
+        high = end < last ? end : last;
+    }
     T* bar = a.bar_logits + n * a.bar_stride - lead;
     float c = 0.0f, lse = 0.0f;
     if (y >= 0) {
@@ -486,7 +539,7 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
     // A row without a gradient is not read, unless to know it takes longer than to
     // ask for the row's first vectors (a search for its pair).
     const bool zero = c == 0.0f, unread = W == kPairGradient ? y < 0 : zero;
-    for (int64_t p0 = static_cast<int64_t>(lane) * V; p0 < high; p0 += kAhead * L * V) {
+    for (int64_t p0 = first; p0 < high; p0 += kAhead * L * V) {
         Words x[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) x[i] = row_vector<T, Stream>(row - lead, p0 + i * L * V, lead, unread ? 0 : high);
@@ -600,6 +653,8 @@ RowArgs<T> args_of(const hk_row_loss_job& j) {
     a.kl = j.kl;
     a.even = j.rows > 0 ? 1.0f / static_cast<float>(j.rows) : 0.0f;
     a.target64 = j.target64;
+    a.run = static_cast<uint64_t*>(j.state);
+    a.counter = j.state ? reinterpret_cast<uint32_t*>(a.run + kWords) : nullptr;
     return a;
 }
 
@@ -607,8 +662,6 @@ int launched(const char* what) {
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error(what, err);
 }
-
-constexpr int64_t kUnits = 256;  // compute units
 
 template <class T, int L, int NV, Work W, bool Grad>
 void launch_held(const RowArgs<T>& a, hipStream_t s) {
@@ -630,30 +683,52 @@ int64_t vectors_of(const RowArgs<T>& a) {
     const bool leads = (reinterpret_cast<uintptr_t>(a.logits) | apart) % 16 != 0;
     return (a.vocab + (leads ? V - 1 : 0) + V - 1) / V;
 }
+constexpr int64_t kHeldVectors = 16384;    // rows that a workgroup of 1024 lanes holds
+constexpr int64_t kSplitVectors = 16384;
 constexpr int64_t kShortVectors = 512;     // rows that at most a wave holds
 constexpr int64_t kFewVectors = 16384;     // 256 KiB of logits
+
+// The workgroups of a row: more than one where at most 64 rows have 16384 vectors
+// or more (one row of 131072 floats 8.0 us a call against 11.6 by one workgroup,
+// 52 of them 13.0 and 13.6, 52 of 200003 14.7 and 22.3), at most four a unit (eight:
+// the 52 rows 17.5 and 23.1).  Rows of 50001 floats lose up to 1 us by it, and so do
+// 256 rows of 131072 bfloat16.
+template <class T>
+int parts_of(const RowArgs<T>& a) {
+    const int64_t vectors = vectors_of(a);
+    if (a.rows == 0 || a.rows > kSplitRows || vectors < kSplitVectors || !a.run) return 1;
+    const int64_t by_length = vectors / (kAhead * kThreads), by_rows = kWords / a.rows;
+    const int64_t parts = by_length < by_rows ? by_length : by_rows;
+    return static_cast<int>(parts < kMostParts ? parts : kMostParts);
+}
 
 // The lanes of a row by its vectors.  Its loss with the gradient holds rows of up
 // to 16384 vectors; without, those of up to 512 (several rows a workgroup, whose
 // reductions stay in a wave): a longer one needs no second pass, and a running
-// (m, s) holds nothing.  Fewer rows than two a unit take 1024 lanes each.
+// (m, s) holds nothing.  Fewer rows than two a unit take 1024 lanes each.  A
+// gradient from a saved lse takes a workgroup for each 1024 vectors of a row: 4096
+// rows of 50001 floats 336 us against 368 with a workgroup a row, one row of 131072
+// 5.5 against 19.5 with 1024 lanes.
 template <class T, Work W>
-int rows_of(const RowArgs<T>& a, hipStream_t s) {
+int rows_of(RowArgs<T> a, hipStream_t s) {
     if (a.rows == 0) return HK_OK;
     const int64_t vectors = vectors_of(a);
     const bool few = a.rows < 2 * kUnits;
     if constexpr (W == kGradient || W == kPolicyGradient || W == kPairGradient) {
         auto go = [&](auto lanes) {
-            constexpr int L = decltype(lanes)::value, R = (L > kThreads ? L : kThreads) / L;
-            hipLaunchKernelGGL((hawk_row_gradient<T, L, W>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)), dim3(R * L),
-                               0, s, a);
+            constexpr int L = decltype(lanes)::value, R = kThreads / L;
+            const int64_t most = vectors / (kAhead * kThreads), parts = L < kThreads || most < 1 ? 1 : most < 65535 ? most : 65535;
+            a.each = (vectors + parts - 1) / parts;
+            hipLaunchKernelGGL((hawk_row_gradient<T, L, W>),
+                               dim3(static_cast<unsigned>((a.rows + R - 1) / R), static_cast<unsigned>(parts)), dim3(kThreads), 0, s, a);
         };
         if (vectors <= 32) go(Count<16>{});
         else if (vectors <= 256) go(Count<64>{});
-        else if (few && vectors > 4096) go(Count<1024>{});
         else go(Count<256>{});
     } else {
         const bool hold = W == kPolicy && a.bar_logits;
+        const int parts = parts_of(a);
+        a.each = (vectors + parts - 1) / parts;
         auto held = [&](auto lanes, auto count) {
             constexpr int L = decltype(lanes)::value, NV = decltype(count)::value;
             if (hold) launch_held<T, L, NV, W, W == kPolicy>(a, s);
@@ -666,7 +741,7 @@ int rows_of(const RowArgs<T>& a, hipStream_t s) {
         else if (vectors <= 256) held(Count<64>{}, Count<4>{});
         else if (vectors <= kShortVectors) held(Count<64>{}, Count<8>{});
         else if (!hold && vectors <= 1024 && !few) launch_held<T, 64, 16, W, false>(a, s);
-        else if (hold && vectors <= 16384) {
+        else if (hold) {
             if constexpr (W == kPolicy) {
                 if (vectors <= 1024) held(Count<256>{}, Count<4>{});
                 else if (vectors <= 2048) held(Count<256>{}, Count<8>{});
@@ -675,7 +750,9 @@ int rows_of(const RowArgs<T>& a, hipStream_t s) {
                 else if (vectors <= 8192) held(Count<512>{}, Count<16>{});
                 else held(Count<1024>{}, Count<16>{});
             }
-        } else if (few || hold) {
+        } else if (parts > 1) {
+            hipLaunchKernelGGL((hawk_row_parts<T, W>), dim3(static_cast<unsigned>(a.rows * parts)), dim3(kThreads), 0, s, a, parts);
+        } else if (few) {
             hipLaunchKernelGGL((hawk_row_long<T, 1024, W>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
         } else {
             hipLaunchKernelGGL((hawk_row_long<T, 256, W>), dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, s, a);
@@ -733,8 +810,8 @@ int total(const float* x, int64_t count, float* out, double* partial, hipStream_
     return launched("hawk_row_total launch");
 }
 
-// Scratch: the sums' doubles, a double a row (preference) or a float (policy),
-// then a float a pair.
+// Scratch: the sums' doubles, then a double a row and a float a pair (preference)
+// or three floats a row (policy).
 int64_t partial_count(const hk_row_loss_job& j) { return 2 * runs(j.rows > j.pairs ? j.rows : j.pairs); }
 double* partials(void* scratch) { return static_cast<double*>(scratch); }
 double* row_doubles(const hk_row_loss_job& j, void* scratch) { return partials(scratch) + partial_count(j); }
@@ -747,7 +824,7 @@ extern "C" {
 
 size_t hk_row_loss_scratch_bytes(const hk_row_loss_job* job) {
     if (!job || job->rows < 0 || job->pairs < 0) return 0;
-    return sizeof(double) * static_cast<size_t>(partial_count(*job) + job->rows) + sizeof(float) * static_cast<size_t>(job->pairs + 1);
+    return sizeof(double) * static_cast<size_t>(partial_count(*job) + 2 * job->rows + (job->pairs + 1) / 2);
 }
 
 int hk_token_logp(const hk_row_loss_job* job, void* scratch, void* stream) {
@@ -783,7 +860,7 @@ static int check_policy(const hk_row_loss_job* j, const std::string& who) {
 int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
     int rc = check_policy(job, "hk_policy_loss");
     if (rc != HK_OK) return rc;
-    if (job->rows > 0 && job->loss && !scratch) return hawk_internal::set_error(HK_EVALUE, "hk_policy_loss: scratch is required");
+    if (job->rows > 0 && (job->loss || job->bar_logits) && !scratch) return hawk_internal::set_error(HK_EVALUE, "hk_policy_loss: scratch is required");
     hipStream_t s = static_cast<hipStream_t>(stream);
     bool summed = false;
     rc = typed(job->dtype, [&](auto t) {
@@ -793,13 +870,20 @@ int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
         // in the rows' own launch where they are few: 200 rows of 48 floats 6.2 us a
         // call against 7.7 with a launch more, but the workgroups' fences wait for
         // what they stored: 4524 rows of 1660 float16 logits 123 us against 15
-        summed = job->loss && job->counter && job->rows > 0 && job->rows <= kRun && vectors_of(a) <= kShortVectors &&
+        summed = job->loss && job->state && job->rows > 0 && job->rows <= kRun && vectors_of(a) <= kShortVectors &&
                  job->rows * vectors_of(a) <= kFewVectors;
-        if (summed) {
-            a.loss = job->loss;
-            a.counter = static_cast<uint32_t*>(job->counter);
-        }
-        return rows_of<T, kPolicy>(a, s);
+        if (summed) a.loss = job->loss;
+        if (!a.bar_logits || vectors_of(a) <= kHeldVectors) return rows_of<T, kPolicy>(a, s);
+        // longer rows twice: all their losses, then all their gradients (4096 rows of
+        // 131072 floats 1080 us against 1091 with both in one workgroup's passes, 52 of
+        // them 30 against 46)
+        a.bar_logits = nullptr;
+        if (!a.logp) a.logp = row_floats(*job, scratch) + job->rows;
+        if (!a.lse) a.lse = row_floats(*job, scratch) + 2 * job->rows;
+        const int rc = rows_of<T, kPolicy>(a, s);
+        if (rc != HK_OK) return rc;
+        a.bar_logits = static_cast<T*>(job->bar_logits);
+        return rows_of<T, kPolicyGradient>(a, s);
     });
     if (rc != HK_OK || !job->loss || summed) return rc;
     return total(row_floats(*job, scratch), job->rows, job->loss, partials(scratch), s);

@@ -59,15 +59,15 @@ class _Plan:
     """One set of shapes, strides and types, checked: the job's fields that do
     not move between calls, and where the pointers go."""
 
-    __slots__ = ("job", "words", "slots", "fn", "ref", "scratch", "counter", "lock", "cells", "apart", "order", "spaces")
+    __slots__ = ("job", "words", "slots", "fn", "ref", "scratch", "state", "lock", "cells", "apart", "order", "spaces")
 
-    def __init__(self, job, slots: dict, fn, scratch: int, counter=None, cells=(), apart=()):
+    def __init__(self, job, slots: dict, fn, scratch: int, state=None, cells=(), apart=()):
         self.job, self.fn, self.scratch = job, fn, scratch
         self.words = (ctypes.c_uint64 * (ctypes.sizeof(job) // 8)).from_buffer(job)
         self.slots = slots                  # plane -> word of the job that holds its address
         self.ref = ctypes.byref(job)
         self.lock = threading.Lock()
-        self.counter = counter              # the word that holds the stream's zeroed cell
+        self.state = state                  # the job's word for the stream's zeroed state
         self.cells = cells                  # by-value words: (name, word)
         self.apart = apart                  # planes that may not start at one address
         self.order = ()                     # (name, type, shape, strides, word) of a call's planes in turn
@@ -90,14 +90,14 @@ _spaces_lock = threading.Lock()
 
 class _Space:
     """What a stage's calls on a stream work in: scratch, shared by every stage
-    on it (a stream's calls run one after another), a zeroed cell that every call
+    on it (a stream's calls run one after another), zeroed state that every call
     leaves at zero, and the lock that keeps a call's launches together."""
 
-    __slots__ = ("scratch", "cell", "lock", "held")
+    __slots__ = ("scratch", "state", "lock", "held")
 
-    def __init__(self, scratch, cell, lock):
-        self.held = scratch, cell
-        self.scratch, self.cell, self.lock = scratch.data_ptr(), cell.data_ptr(), lock
+    def __init__(self, scratch, state, lock):
+        self.held = scratch, state
+        self.scratch, self.state, self.lock = scratch.data_ptr(), state.data_ptr(), lock
 
 
 def _space(device: int, stream: int, nbytes: int) -> _Space:
@@ -106,7 +106,8 @@ def _space(device: int, stream: int, nbytes: int) -> _Space:
         if found is None:
             found = _spaces[device, stream] = _Workspace(torch.device("cuda", device)), threading.Lock()
         work, lock = found
-        return _Space(work.bytes(("stage", "scratch", nbytes), nbytes), work.bytes(("stage", "cell"), 8, zero=True), lock)
+        return _Space(work.bytes(("stage", "scratch", nbytes), nbytes),
+                      work.bytes(("stage", "state"), _core.STATE_BYTES, zero=True), lock)
 
 
 class _Stage(Stage):
@@ -238,8 +239,8 @@ class _Stage(Stage):
             space = plan.spaces.get(stream)
             if space is None:
                 space = plan.spaces[stream] = _space(device, stream, plan.scratch)
-            if plan.counter is not None:
-                bound.append((plan.counter, space.cell))
+            if plan.state is not None:
+                bound.append((plan.state, space.state))
             with plan.lock, space.lock:
                 for word, value in bound:
                     words[word] = value
@@ -254,16 +255,16 @@ class _Stage(Stage):
         stream = _stream_of(stream)
         job = type(plan.job).from_buffer_copy(plan.job)
         words = (ctypes.c_uint64 * (ctypes.sizeof(job) // 8)).from_buffer(job)
-        scratch = cell = None
+        scratch = state = None
         if plan.scratch:
             with _on(stream):
                 scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=f"cuda:{device}")
-                if plan.counter is not None:
-                    cell = torch.zeros(8, dtype=torch.uint8, device=f"cuda:{device}")
-                    bound.append((plan.counter, cell.data_ptr()))
+                if plan.state is not None:
+                    state = torch.zeros(_core.STATE_BYTES, dtype=torch.uint8, device=f"cuda:{device}")
+                    bound.append((plan.state, state.data_ptr()))
         for word, value in bound:
             words[word] = value
-        return Launcher(plan.fn, job, (scratch, cell), stream, dict(arrays))
+        return Launcher(plan.fn, job, (scratch, state), stream, dict(arrays))
 
 
 class Launcher:
@@ -457,7 +458,7 @@ class _Rows(_Stage):
             slots[n] = _word(_core.RowLossJob, n)
         L = _core.lib()
         return _Plan(job, slots, getattr(L, self.entry), int(L.hk_row_loss_scratch_bytes(ctypes.byref(job))),
-                     counter=_word(_core.RowLossJob, "counter"))
+                     state=_word(_core.RowLossJob, "state"))
 
     def _more(self, t: dict, job) -> None:
         if t.get("weight") is not None:

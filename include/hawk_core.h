@@ -436,7 +436,8 @@ int hk_recurrence_vjp(const hk_recurrence_job* job, void* scratch, void* stream)
  * hk_preference_loss: 2*pairs sequences of rows cut by offsets (2*pairs + 1
  * ascending row numbers from 0 to rows; 64-bit if offsets64 != 0); pair p
  * prefers sequence 2p to 2p + 1.  With s_k = sum over sequence k's kept rows of
- * (logp - ref_logp) (ref_logp NULL: 0; each logp before it is rounded to 32 bits): margin_p = s_2p - s_2p+1, z = beta margin,
+ * (logp - ref_logp) (ref_logp NULL: 0; each logp before it is rounded to 32
+ * bits): margin_p = s_2p - s_2p+1, z = beta margin,
  *   *loss = sum_p weight_p (-(1 - smoothing) log sigma(z) - smoothing log sigma(-z)),
  * weight 1/pairs if NULL (a weight of 0 leaves the pair out).  It writes loss,
  * margin, logp, lse (each may be NULL).
@@ -444,9 +445,12 @@ int hk_recurrence_vjp(const hk_recurrence_job* job, void* scratch, void* stream)
  * bar_logits.
  *
  * Scratch: hk_row_loss_scratch_bytes(job) bytes, 16-byte aligned, no contents
- * needed.  counter: a 32-bit word on the device, 0 before the first call and
- * left at 0 by each (NULL: the policy loss of few rows takes one launch more).
+ * needed (token_logp and the derivatives take none).  state:
+ * HK_ROW_LOSS_STATE_BYTES on the device, 0 before the first call and left at 0
+ * by each, one to a stream (NULL: no row is split over workgroups, and the
+ * policy loss of few rows takes one launch more).
  * The sums over rows and pairs are taken in 64 bits in a fixed order. */
+#define HK_ROW_LOSS_STATE_BYTES 8448
 typedef struct hk_row_loss_job {
     const void* logits;
     void* bar_logits;
@@ -454,7 +458,7 @@ typedef struct hk_row_loss_job {
     float *logp, *lse, *loss, *margin;
     const float *bar_logp, *bar_loss, *old_logp, *ref_logp, *advantage, *weight;
     const void* offsets;
-    void* counter;
+    void* state;
     int64_t rows, vocab, row_stride, bar_stride, pairs;
     float scale, clip_low, clip_high, kl, beta, smoothing;
     int32_t dtype, target64, offsets64;

@@ -692,6 +692,61 @@ def test_row_losses_replayed_from_a_graph_and_repeated(gpu):
         assert torch.equal(loss, want) and torch.equal(bar, wbar)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ROW_TYPES)
+@pytest.mark.parametrize("shape", [(2, 131072), (5, 262147), (64, 131081), (65, 131081)], ids=str)
+def test_few_long_rows_over_several_workgroups(gpu, shape, dtype):
+    """Rows whose first parts hold nothing, rows of the type's lowest value, and calls one
+    after another that find the workgroups' words as the call before left them."""
+    import torch
+    N, V = shape
+    g = np.random.default_rng([3, N, V])
+    x = g.normal(size=(N, V)) * 3
+    x[0, :V - 5] = -np.inf
+    target = g.integers(0, V, N)
+    target[0] = V - 2
+    if N > 2:
+        x[1] = float(torch.finfo(torch_type(dtype)).min) / 2
+        x[2, ::2] = -np.inf
+        target[2] |= 1
+        target[3] = -1
+    logits, held = plane(x, dtype, gpu)
+    del x
+    y = torch.from_numpy(target).to(gpu)
+    want, want_lse, l = oracle_rows(held, target, 1.0)
+    c = g.normal(size=N).astype(np.float32)
+    bar_logp = torch.from_numpy(c).to(gpu)
+    stage = hawk.stages.token_logp()
+    out = [torch.empty(N, device=gpu) for _ in range(2)]
+    held_launch = stage.prepare(logits=logits, target=y, logp=out[0], lse=out[1])
+    first = None
+    for k in range(3):
+        logp, lse = torch.empty(N, device=gpu), torch.empty(N, device=gpu)
+        hawk.run(stage, logits=logits, target=y, logp=logp, lse=lse)
+        held_launch()
+        close_row(back(logp), want, want_lse)
+        close_row(back(lse), want_lse, want_lse)
+        first = logp if first is None else first
+        assert torch.equal(logp, first) and torch.equal(logp, out[0]) and torch.equal(lse, out[1])
+    bar = torch.empty_like(logits)
+    hawk.run(stage.vjp, logits=logits, target=y, lse=lse, bar_logp=bar_logp, bar_logits=bar)
+    grad, size = oracle_gradient(l, target, back(lse), c.astype(np.float64), 1.0)
+    # a masked logit's gradient is 0, whatever its distance
+    reach = np.where(np.isinf(l), 0, l)
+    close_gradient(back(bar), grad, size, reach, back(lse), dtype)
+    del bar
+    # the policy loss of the same rows: its slope is -r A at r = 1, then in place
+    loss, both = torch.empty(1, device=gpu), torch.empty_like(logits)
+    planes = dict(target=y, old_logp=logp, advantage=-bar_logp, weight=torch.ones(N, device=gpu))
+    policy = hawk.stages.policy_loss()
+    hawk.run(policy, logits=logits, loss=loss, bar_logits=both, **planes)
+    close_gradient(back(both), grad, size, reach, back(lse), dtype, slack=8 * 2.0 ** -24 * (2 + 2 * np.abs(back(lse)).max()))
+    total = np.where(target >= 0, c, 0).astype(np.float64).sum()
+    assert abs(back(loss)[0] - total) <= 8 * 2.0 ** -24 * (2 + np.abs(want_lse)) @ np.abs(c) * 2
+    hawk.run(policy, logits=logits, bar_logits=logits, **planes)
+    assert torch.equal(logits, both)
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
