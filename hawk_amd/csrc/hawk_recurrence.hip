@@ -12,8 +12,8 @@
 //
 // A gate of 0 cuts, and so does the first row of a packed sequence: products
 // and their use take 0 times anything as 0 (cutmul), so neither an infinity
-// nor a NaN passes a cut; a product of gates is 0 only where one is (chain).  States and products are held in 32 bits (64 for
-// double planes).
+// nor a NaN passes a cut; a product of gates is 0 only where one is (chain).
+// States and products are held in 32 bits (64 for double planes).
 
 #include "hawk_core.h"
 #include "hawk_internal.h"
@@ -165,11 +165,14 @@ __device__ __forceinline__ bool read(const typename Word<A>::type* at, A& x) {
     return w != ~W(0);
 }
 // A word that its tile has written, or is about to: that tile has begun (see
-// the order of tiles below), so the wait ends.
+// the order of tiles below), so the wait ends.  Where it cannot (two streams
+// worked in one scratch) it ends after kLooks looks, seconds, with the unwritten
+// word, which is a NaN.
+constexpr int kLooks = 1 << 22;
 template <class A>
 __device__ __forceinline__ A await(const typename Word<A>::type* at) {
     A x;
-    while (!read<A>(at, x)) __builtin_amdgcn_s_sleep(1);
+    for (int looks = kLooks; !read<A>(at, x) && looks > 0; --looks) __builtin_amdgcn_s_sleep(1);
     return x;
 }
 
@@ -194,6 +197,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
         if (tid == 0) lds_chunk = static_cast<int>(atomicAdd(a.counter + strip * a.counter_step, 1u));
         __syncthreads();
         chunk = __builtin_amdgcn_readfirstlane(lds_chunk);
+        if (chunk >= a.chunks) return;             // only where two streams worked in one scratch
     }
     const int64_t col0 = static_cast<int64_t>(strip) * ncol;
     const int here = Dir == 0 ? tid & (ncol - 1) : tid / nt;
@@ -442,13 +446,14 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
             // look; the words it is about are awaited for themselves.
             if (chunk > 0 && tid < 64) {
                 const int look = chunk - 1 - lane;
-                uint64_t known;
-                for (;;) {
+                uint64_t known = 0;
+                for (int looks = kLooks; looks > 0; --looks) {
                     known = __ballot(look < 0 || __hip_atomic_load(flags + look, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 1u);
                     if (known) break;
                     __builtin_amdgcn_s_sleep(4);
                 }
-                if (lane == 0) lds_from = chunk - 1 - __builtin_ctzll(known);     // -1: the state before the first chunk
+                // -1: the state before the first chunk
+                if (lane == 0) lds_from = chunk - 1 - (known ? __builtin_ctzll(known) : 0);
             }
             __syncthreads();
             // The state that enters: the known one, then the chunks since in
