@@ -771,7 +771,7 @@ def kept(n, cut, offset, seed):
 
 
 def test_the_generator_is_philox_4x32_10():
-    """The published known answers (Random123's kat_vectors)."""
+    """The generator's published known answers."""
     assert philox(0, 0, 0) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
     ones = (1 << 64) - 1
     assert philox(ones, ones, ones) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
