@@ -3,7 +3,8 @@
 The library is the C-ABI launcher (``csrc/hawk_core.cpp``) plus the
 hand-written team-stage kernels (``csrc/hawk_team.hip``, ``csrc/hawk_linalg.hip``) and training stages
 (``csrc/hawk_recurrence.hip``, ``csrc/hawk_rows.hip``, ``csrc/hawk_dropout.hip``), built by ``hipcc``
-for gfx950 only, each file by a compiler of its own.  Its build digest is the sha256 of its own sources (each
+for gfx950 only, each file by a compiler of its own.  Beside it ``_bind.so`` (``csrc/hawk_bind.cpp``,
+built by the host compiler against PyTorch's headers) checks and binds a stage's tensors.  The build digest is the sha256 of its own sources (each
 file's name and sha256, in sorted order), stamped into the library and
 recomputed by :mod:`hawk_amd._core` at load, the same self-check the
 reference runs at import (reference ``hawk/__init__.py:146-212``).
@@ -13,6 +14,7 @@ from __future__ import annotations
 
 import hashlib
 import os
+import shutil
 import subprocess
 import sys
 import tempfile
@@ -24,6 +26,7 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 INCLUDE = ROOT / "include"
 LIBRARY = PACKAGE / "libhawk_core.so"
+BINDING = PACKAGE / "_bind.so"
 HIPCC = os.environ.get("HAWK_HIPCC", "/opt/rocm/bin/hipcc")
 
 #: The library's translation units.
@@ -52,8 +55,21 @@ def source_digest() -> str:
     return hashlib.sha256("".join(stream).encode()).hexdigest()
 
 
+def binding_command(digest: str, out: Path) -> list:
+    """The host compiler's command for ``_bind.so``."""
+    import sysconfig
+
+    import torch
+    at = Path(torch.__file__).resolve().parent
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DHAWK_BUILD_DIGEST="{digest}"',
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{sysconfig.get_paths()['include']}",
+            f"-I{at}/include", f"-I{at}/include/torch/csrc/api/include", str(CSRC / "hawk_bind.cpp"), "-o", str(out),
+            f"-L{at}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
 def build_library(verbose: bool = False) -> Path:
-    """Compile ``libhawk_core.so`` next to this file; returns its path."""
+    """Compile ``libhawk_core.so`` and ``_bind.so`` next to this file; returns the
+    library's path."""
     digest = source_digest()
     info = "compiler=" + HIPCC + "\\nflags=" + " ".join(HIP_FLAGS) + "\\noffload_arch=gfx950"
     tmp = LIBRARY.with_suffix(".so.tmp")
@@ -65,13 +81,18 @@ def build_library(verbose: bool = False) -> Path:
             print(" ".join(cmd), flush=True)
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
-            raise RuntimeError(f"hipcc failed building {LIBRARY.name}:\n{proc.stdout}\n{proc.stderr}")
+            raise RuntimeError(f"{cmd[0]} failed building {LIBRARY.name}:\n{proc.stdout}\n{proc.stderr}")
 
-    with tempfile.TemporaryDirectory() as made, ThreadPoolExecutor(len(UNITS)) as pool:
+    with tempfile.TemporaryDirectory() as made, ThreadPoolExecutor(len(UNITS) + 1) as pool:
+        binding = Path(made) / BINDING.name
+        bound = pool.submit(call, binding_command(digest, binding))
         objects = [str(Path(made) / f"{name}.o") for name in UNITS]
         list(pool.map(lambda pair: call([HIPCC, *flags, "-c", str(CSRC / pair[0]), "-o", pair[1]]),
                       zip(UNITS, objects)))
         call([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared", *objects, "-o", str(tmp), "-lhiprtc", "-lamdhip64"])
+        bound.result()
+        shutil.move(binding, BINDING.with_suffix(".so.tmp"))
+    os.replace(BINDING.with_suffix(".so.tmp"), BINDING)
     os.replace(tmp, LIBRARY)
     return LIBRARY
 

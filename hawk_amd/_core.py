@@ -147,6 +147,25 @@ def lib():
     return _lib
 
 
+_bind = None
+
+
+def bind():
+    """The module that binds a stage's planes (``csrc/hawk_bind.cpp``), built from
+    the sources that the library is."""
+    global _bind
+    if _bind is None:
+        digest = build_digest()
+        try:
+            from . import _bind as made
+        except ImportError as e:
+            raise HawkError(f"hawk_amd: _bind.so is not built; build it first (python hawk_amd/_build.py): {e}") from e
+        if made.digest != digest:
+            raise HawkError("hawk_amd: _bind.so was built from other sources; build again (python hawk_amd/_build.py)")
+        _bind = made
+    return _bind
+
+
 def library_path() -> Path:
     return _LIB_PATH
 

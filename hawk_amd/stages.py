@@ -59,19 +59,29 @@ class _Plan:
     """One set of shapes, strides and types, checked: the job's fields that do
     not move between calls, and where the pointers go."""
 
-    __slots__ = ("job", "words", "slots", "fn", "ref", "scratch", "state", "lock", "cells", "apart", "order", "spaces")
+    __slots__ = ("job", "slots", "fn", "entry", "scratch", "state", "cells", "apart", "spaces", "call")
 
-    def __init__(self, job, slots: dict, fn, scratch: int, state=None, cells=(), apart=()):
+    def __init__(self, job, slots: dict, fn, scratch: int, state=None, cells=(), apart=(), entry=None):
         self.job, self.fn, self.scratch = job, fn, scratch
-        self.words = (ctypes.c_uint64 * (ctypes.sizeof(job) // 8)).from_buffer(job)
+        self.entry = entry                  # the entry of a stage without scratch
         self.slots = slots                  # plane -> word of the job that holds its address
-        self.ref = ctypes.byref(job)
-        self.lock = threading.Lock()
         self.state = state                  # the job's word for the stream's zeroed state
         self.cells = cells                  # by-value words: (name, word)
         self.apart = apart                  # planes that may not start at one address
-        self.order = ()                     # (name, type, shape, strides, word) of a call's planes in turn
         self.spaces: dict = {}              # stream -> _Space
+        self.call = None
+
+    def bind(self, arrays: dict, values: tuple, device: int) -> None:
+        """``call``: what checks a call's planes against these ones and runs it."""
+        names = list(arrays)
+        cells = dict(self.cells)
+        planes = tuple((n, None, cells[n]) if n in values else (n, x, self.slots[n]) if x is not None else (n, None, -1)
+                       for n, x in arrays.items())
+        apart = tuple((names.index(a), names.index(b)) for a, b in self.apart
+                      if arrays.get(a) is not None and arrays.get(b) is not None)
+        entry = ctypes.cast(self.entry or self.fn, ctypes.c_void_p).value
+        self.call = _core.bind().Call(entry, self.entry is not None, bool(self.scratch), device, bytes(self.job),
+                                      -1 if self.state is None else self.state, planes, apart)
 
 
 def _word(job_type, *path) -> int:
@@ -90,24 +100,23 @@ _spaces_lock = threading.Lock()
 
 class _Space:
     """What a stage's calls on a stream work in: scratch, shared by every stage
-    on it (a stream's calls run one after another), zeroed state that every call
-    leaves at zero, and the lock that keeps a call's launches together."""
+    on it (a stream's calls run one after another), and zeroed state that every
+    call leaves at zero."""
 
-    __slots__ = ("scratch", "state", "lock", "held")
+    __slots__ = ("scratch", "state", "held")
 
-    def __init__(self, scratch, state, lock):
+    def __init__(self, scratch, state):
         self.held = scratch, state
-        self.scratch, self.state, self.lock = scratch.data_ptr(), state.data_ptr(), lock
+        self.scratch, self.state = scratch.data_ptr(), state.data_ptr()
 
 
 def _space(device: int, stream: int, nbytes: int) -> _Space:
     with _spaces_lock, _on(stream):
         found = _spaces.get((device, stream))
         if found is None:
-            found = _spaces[device, stream] = _Workspace(torch.device("cuda", device)), threading.Lock()
-        work, lock = found
-        return _Space(work.bytes(("stage", "scratch", nbytes), nbytes),
-                      work.bytes(("stage", "state"), _core.STATE_BYTES, zero=True), lock)
+            found = _spaces[device, stream] = _Workspace(torch.device("cuda", device))
+        return _Space(found.bytes(("stage", "scratch", nbytes), nbytes),
+                      found.bytes(("stage", "state"), _core.STATE_BYTES, zero=True))
 
 
 class _Stage(Stage):
@@ -180,20 +189,7 @@ class _Stage(Stage):
     def _found(self, arrays: dict):
         """``(plan, [(word, value)], device)`` of a call."""
         device = _current_device()
-        bound, plan = [], self._last
-        if plan is not None and len(plan.order) == len(arrays):     # the shapes of the call before, most often
-            for (name, x), (known, dtype, shape, strides, word) in zip(arrays.items(), plan.order):
-                if name is not known:
-                    break
-                if dtype is None:
-                    continue                # a by-value argument
-                if (type(x) is not _Tensor or x.dtype is not dtype or x.get_device() != device or x.shape != shape
-                        or x.stride() != strides):
-                    break
-                bound.append((word, x.data_ptr()))
-            else:
-                return self._finish(plan, bound, arrays, device)
-        key, bound = [device], []
+        key = [device]
         try:
             for name, x in arrays.items():
                 if x is None or name in self.values:
@@ -208,9 +204,7 @@ class _Stage(Stage):
             plan = self._plan(key, arrays)
             if key is None:
                 self._refuse("a plane is no dense tensor")
-            plan.order = tuple((name, None, None, None, 0) if x is None or name in self.values else
-                               (name, x.dtype, x.shape, x.stride(), plan.slots.get(name, -1))
-                               for name, x in arrays.items())
+            plan.bind(arrays, self.values, device)
         self._last = plan if all(x is not None for x in arrays.values()) else None
         bound = [(plan.slots[name], x.data_ptr()) for name, x in arrays.items()
                  if x is not None and name not in self.values]
@@ -227,24 +221,21 @@ class _Stage(Stage):
 
     def run(self, arrays: dict, stream=None) -> None:
         """Bind ``arrays`` and run once, in place (``hawk.run``)."""
-        plan, bound, device = self._found(arrays)
-        stream = _current_raw(device) if stream is None else _stream_of(stream)
-        words = plan.words
-        if not plan.scratch:
-            with plan.lock:
-                for word, value in bound:
-                    words[word] = value
-                rc = plan.fn(plan.ref, None, stream or None)
-        else:
-            space = plan.spaces.get(stream)
-            if space is None:
-                space = plan.spaces[stream] = _space(device, stream, plan.scratch)
-            if plan.state is not None:
-                bound.append((plan.state, space.state))
-            with plan.lock, space.lock:
-                for word, value in bound:
-                    words[word] = value
-                rc = plan.fn(plan.ref, space.scratch, stream or None)
+        device = _current_device()
+        raw = 0 if device < 0 else _current_raw(device) if stream is None else _stream_of(stream)
+        plan = self._last
+        rc = -1 if plan is None else plan.call.run(arrays, device, raw)      # the planes of the call before, most often
+        if rc < 0:
+            plan, bound, device = self._found(arrays)
+            space = None
+            if plan.scratch:
+                space = plan.spaces.get(raw)
+                if space is None:
+                    space = plan.spaces[raw] = _space(device, raw, plan.scratch)
+                    plan.call.space(raw, space.scratch, space.state)
+                if plan.state is not None:
+                    bound.append((plan.state, space.state))
+            rc = plan.call.launch(bound, 0 if space is None else space.scratch, raw)
         if rc:
             _core.check(rc)
 
@@ -624,7 +615,7 @@ class _Dropout(_Stage):
         slots["offset"] = _word(_core.DropoutJob, "offset_cell")
         cells = (("seed", _word(_core.DropoutJob, "seed")), ("offset", _word(_core.DropoutJob, "offset")))
         fn = _core.lib().hk_dropout
-        return _Plan(job, slots, lambda ref, scratch, stream: fn(ref, stream), 0, cells=cells)
+        return _Plan(job, slots, lambda ref, scratch, stream: fn(ref, stream), 0, cells=cells, entry=fn)
 
     def _row_stride(self, name: str, x) -> int:
         """The distance of rows that lie evenly apart, each contiguous."""

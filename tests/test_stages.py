@@ -991,6 +991,35 @@ def test_the_jobs_are_laid_out_as_the_header_has_them():
     assert ctypes.sizeof(_core.DropoutJob) == 4 * 8 + 5 * 8 + 2 * 8 + 2 * 4
 
 
+def test_the_binding_puts_words_where_they_belong_and_refuses_others():
+    import torch
+    seen = []
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p, ctypes.c_void_p)(
+        lambda job, scratch, stream: seen.append((job[0], job[1], job[2], scratch, stream)) or 5)
+    address = ctypes.cast(entry, ctypes.c_void_p).value
+    Call, x = _core.bind().Call, torch.zeros(3)
+    job = (1).to_bytes(8, "little") + (2).to_bytes(8, "little") + (3).to_bytes(8, "little")
+    call = Call(address, False, True, 0, job, 2, (("x", x, 0), ("seed", None, 1)), ())
+    assert call.launch([(1, 7), (2, 1 << 63)], 16, 32) == 5 and seen == [(1, 7, 1 << 63, 16, 32)]
+    with pytest.raises(ValueError):
+        call.launch([(3, 0)], 0, 0)
+    # no tensor of the plan's device, another count, another name: nothing runs
+    for arrays in ({"x": x, "seed": 4}, {"x": x}, {"seed": 4, "x": x}, {"x": 1, "seed": 4}, {}):
+        assert call.run(arrays, 0, 0) == -1
+    # by-value words alone: bound once the stream has its space, refused out of range
+    call = Call(address, False, True, 0, job, 2, (("seed", None, 1),), ())
+    assert call.run({"seed": 4}, 0, 32) == -1
+    call.space(32, 48, 64)
+    assert call.run({"seed": 4}, 0, 32) == 5 and seen[1:] == [(1, 4, 64, 48, 32)]
+    for bad in (True, -1, 1 << 64, 1.0, None):
+        assert call.run({"seed": bad}, 0, 32) == -1
+    assert call.run({"seed": 4}, 1, 32) == -1 and call.run({"seed": 4}, 0, 33) == -1
+    for planes, apart, size, error in (((("x", x, 3),), (), 24, ValueError), ((("x", 1, 0),), (), 24, TypeError),
+                                       ((("x", x, 0),), ((0, 1),), 24, ValueError), ((), (), 23, ValueError)):
+        with pytest.raises(error):
+            Call(address, False, True, 0, job[:size], 2, planes, apart)
+
+
 @pytest.mark.gpu
 def test_the_recurrent_policy_example_learns(gpu):
     """All stages together: recall by chance is 1 in 16."""
