@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(kShortThreads) hawk_recurrence_short(const Rec
     }
 }
 
-// No steps at all: every state passes through.
+// States as they are: of no steps at all, or aside before they are written over.
 template <class A>
 __global__ void __launch_bounds__(256) hawk_recurrence_pass(const A* init, A* fin, int64_t states) {
     const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -803,11 +803,23 @@ size_t word_bytes(const Shape& s, size_t word) {
     return (3 * word * static_cast<size_t>(s.states) * s.chunks + 4 * static_cast<size_t>(s.strips) * s.chunks + 15) / 16 * 16;
 }
 
+size_t tile_bytes(const Shape& s, size_t word) { return s.chunks > 1 ? counter_bytes(s) + word_bytes(s, word) : 0; }
+
+// States that leave may be written over those that enter.  One tile a sequence
+// has read these before a barrier; but a tile may still be to read them when the
+// last one, which took what lies between from the tiles' (P, H), has finished, and
+// packed rows read a sequence's state twice.  Such calls read a copy, which costs a
+// launch and only they pay.
+template <bool Vjp>
+bool may_copy(const hk_recurrence_job& j, const Shape& s) {
+    return (Vjp ? j.bar_last && j.bar_h0 : j.h0 && j.last) && (s.chunks > 1 || j.offsets);
+}
+
 template <class T, bool Vjp>
 size_t scratch_of(const hk_recurrence_job& j) {
     if (j.seqs <= 0 || j.steps <= 0 || j.chans <= 0) return 0;
     const Shape s = shape_of<T, Vjp>(j);
-    return s.chunks > 1 ? counter_bytes(s) + word_bytes(s, sizeof(Acc<T>)) : 0;
+    return tile_bytes(s, sizeof(Acc<T>)) + (may_copy<Vjp>(j, s) ? sizeof(Acc<T>) * static_cast<size_t>(j.seqs * j.chans) : 0);
 }
 
 int launched(const char* what) {
@@ -845,7 +857,17 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
     }
     const Shape s = shape_of<T, Vjp>(j);
     if (s.strips * s.chunks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, who + ": the planes exceed the grid limit");
-    if (s.chunks > 1 && !scratch) return hawk_internal::set_error(HK_EVALUE, who + ": scratch is required");
+    const int64_t entering = j.seqs * j.chans;
+    const bool copy = may_copy<Vjp>(j, s) && init < fin + entering && fin < init + entering;
+    if ((s.chunks > 1 || copy) && !scratch) return hawk_internal::set_error(HK_EVALUE, who + ": scratch is required");
+    if (copy) {
+        A* held = reinterpret_cast<A*>(static_cast<unsigned char*>(scratch) + tile_bytes(s, sizeof(A)));
+        hipLaunchKernelGGL(hawk_recurrence_pass<A>, dim3(static_cast<unsigned>((entering + 255) / 256)), dim3(256), 0,
+                           stream, init, held, entering);
+        const int rc = launched("hawk_recurrence_pass launch");
+        if (rc != HK_OK) return rc;
+        init = held;
+    }
     const bool flip = (j.reverse != 0) != Vjp;
     RecArgs<T> a{};
     a.gate = plane_of<T>(j.gate, j.steps, flip);

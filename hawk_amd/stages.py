@@ -361,6 +361,7 @@ class _Recurrence(_Stage):
                 self._refuse(f"the state {n!r} is a contiguous {state} tensor ({job.seqs}, {job.chans}), got "
                              f"{x.dtype} {tuple(x.shape)}")
             slots[n] = _word(_core.RecurrenceJob, n)
+            setattr(job, n, 8)
         if packed is not None:
             slots["offsets"] = _word(_core.RecurrenceJob, "offsets")
             job.offsets = 8
@@ -386,7 +387,8 @@ def recurrence(gate: str = "value", reverse: bool = False) -> Stage:
     than there are sequences, ascending from 0 to the rows; a sequence may be
     empty).  ``h0`` (state that enters, 0 if not given) and ``last`` (state that
     leaves, written) are ``(sequences, channels)`` in float32, float64 for
-    float64 planes; ``last`` may be ``h0``.  ``h`` may be ``x`` or ``gate``.
+    float64 planes; ``last`` may be ``h0``, and ``.vjp``'s ``bar_h0`` ``bar_last``.
+    ``h`` may be ``x`` or ``gate``.
     One token of running sequences is the same call with one step, ``h0`` and
     ``last``.
 

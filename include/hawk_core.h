@@ -386,7 +386,7 @@ typedef struct hk_plane {
  * is rows [offsets[s], offsets[s+1]) and may be empty (its last is its h0).
  *
  * hk_recurrence reads gate, x, h0 and writes h, last.  h may be x or gate
- * itself (same strides), last may be h0.
+ * itself (same strides), last may be h0, and the derivative's bar_h0 bar_last.
  * hk_recurrence_vjp reads gate, h (the forward's), x (sigmoid only), h0,
  * bar_h, bar_last and writes bar_gate, bar_x (either may be NULL data) and
  * bar_h0:  G_t = bar_h_t + C_(t+1), C_t = a_t G_t, C past the end = bar_last;
@@ -394,8 +394,8 @@ typedef struct hk_plane {
  *   a (1 - a), bar_x = (1 - a) G;  bar_h0 = C_0.
  * bar_x may be bar_h itself and bar_gate may be gate or x itself (h is read
  * a step away, so nothing may overwrite it).
- * Scratch: hk_recurrence_scratch_bytes(job, vjp) bytes, 16-byte aligned, no
- * contents needed.
+ * Scratch: hk_recurrence_scratch_bytes(job, vjp) bytes of the job with its
+ * pointers, 16-byte aligned, no contents needed.
  * HK_EVALUE for sizes below 0, a missing plane or another type. */
 typedef struct hk_recurrence_job {
     hk_plane gate, x, h, bar_h, bar_gate, bar_x;

@@ -345,6 +345,54 @@ def test_recurrences_in_place_replayed_and_on_two_streams(gpu):
         assert torch.equal(h, eager)
 
 
+def test_states_written_over_those_that_enter_have_room_for_a_copy():
+    L = _core.lib()
+    for steps, offsets, copied in ((4, None, False), (4, 8, True), (5000, None, True), (5000, 8, True)):
+        for vjp, names in ((0, ("h0", "last")), (1, ("bar_last", "bar_h0"))):
+            job = _core.RecurrenceJob()
+            job.seqs, job.steps, job.chans, job.offsets = 3, steps, 72, offsets
+            for n in ("gate", "x", "h", "bar_h", "bar_gate", "bar_x"):
+                plane = getattr(job, n)
+                plane.data, plane.seq, plane.step, plane.chan = 8, 72 * steps, 72, 1
+            without = L.hk_recurrence_scratch_bytes(ctypes.byref(job), vjp)
+            setattr(job, names[0], 8)
+            assert L.hk_recurrence_scratch_bytes(ctypes.byref(job), vjp) == without
+            setattr(job, names[1], 8)
+            assert L.hk_recurrence_scratch_bytes(ctypes.byref(job), vjp) == without + copied * 4 * 3 * 72
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("T", [40, 2500, 9000])
+def test_states_may_be_written_over_those_that_enter(gpu, T, dtype, packed):
+    """The bits of a call whose states that leave have a tensor of their own."""
+    import torch
+    S, C, d = 3, 72, getattr(torch, dtype)
+    g = torch.Generator(device=gpu).manual_seed(T)
+    shape = (T, C) if packed else (S, T, C)
+    gate = 0.9 + 0.1 * torch.rand(shape, generator=g, device=gpu, dtype=d)
+    x, bar = (torch.randn(shape, generator=g, device=gpu, dtype=d) for _ in range(2))
+    h0 = torch.randn(S, C, generator=g, device=gpu, dtype=d)
+    more = dict(offsets=torch.tensor([0, 13, T - 5, T], device=gpu)) if packed else {}
+    stage = hawk.stages.recurrence()
+    want, last, to_gate, to_x, to_h0 = (torch.empty_like(y) for y in (x, h0, x, x, h0))
+    hawk.run(stage, gate=gate, x=x, h=want, h0=h0, last=last, **more)
+    hawk.run(stage.vjp, gate=gate, h=want, bar_h=bar, h0=last, bar_last=h0, bar_gate=to_gate, bar_x=to_x, bar_h0=to_h0, **more)
+    for _ in range(4):
+        h, a, b = (torch.full_like(x, float("nan")) for _ in range(3))
+        state = h0.clone()
+        hawk.run(stage, gate=gate, x=x, h=h, h0=state, last=state, **more)
+        assert torch.equal(h, want) and torch.equal(state, last)
+        state = h0.clone()
+        hawk.run(stage.vjp, gate=gate, h=want, bar_h=bar, h0=last, bar_last=state, bar_gate=a, bar_x=b, bar_h0=state, **more)
+        assert torch.equal(a, to_gate) and torch.equal(b, to_x) and torch.equal(state, to_h0)
+    state = h0.clone()
+    launch = stage.prepare(gate=gate, x=x, h=h, h0=state, last=state, **more)
+    launch()
+    assert torch.equal(h, want) and torch.equal(state, last)
+
+
 @pytest.mark.gpu
 def test_recurrence_without_steps_sequences_or_channels(gpu):
     import torch
