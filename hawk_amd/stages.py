@@ -110,13 +110,20 @@ class _Space:
         self.scratch, self.state = scratch.data_ptr(), state.data_ptr()
 
 
-def _space(device: int, stream: int, nbytes: int) -> _Space:
+def _space(device: int, stream: int, nbytes: int, state: bool) -> tuple:
+    """``(space, kept)``: what the calls on ``stream`` work in.  One that is first
+    asked for while the stream is captured is that call's alone: its memory is the
+    graph's, and its state is cleared by the graph's replays, not before them."""
     with _spaces_lock, _on(stream):
+        if torch.cuda.is_current_stream_capturing():
+            clear = torch.zeros if state else torch.empty
+            return _Space(torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}"),
+                          clear(_core.STATE_BYTES if state else 0, dtype=torch.uint8, device=f"cuda:{device}")), False
         found = _spaces.get((device, stream))
         if found is None:
             found = _spaces[device, stream] = _Workspace(torch.device("cuda", device))
         return _Space(found.bytes(("stage", "scratch", nbytes), nbytes),
-                      found.bytes(("stage", "state"), _core.STATE_BYTES, zero=True))
+                      found.bytes(("stage", "state"), _core.STATE_BYTES, zero=True)), True
 
 
 class _Stage(Stage):
@@ -231,8 +238,10 @@ class _Stage(Stage):
             if plan.scratch:
                 space = plan.spaces.get(raw)
                 if space is None:
-                    space = plan.spaces[raw] = _space(device, raw, plan.scratch)
-                    plan.call.space(raw, space.scratch, space.state)
+                    space, kept = _space(device, raw, plan.scratch, plan.state is not None)
+                    if kept:
+                        plan.spaces[raw] = space
+                        plan.call.space(raw, space.scratch, space.state)
                 if plan.state is not None:
                     bound.append((plan.state, space.state))
             rc = plan.call.launch(bound, 0 if space is None else space.scratch, raw)
@@ -641,7 +650,8 @@ class _Dropout(_Stage):
 
     def _found(self, arrays: dict):
         cell = arrays.get("offset")
-        if isinstance(cell, torch.Tensor) and (cell.dtype != torch.int64 or cell.numel() != 1 or not cell.is_cuda):
+        if isinstance(cell, torch.Tensor) and (cell.dtype != torch.int64 or cell.numel() != 1
+                                               or not cell.is_cuda or cell.get_device() != _current_device()):
             self._refuse("offset= is an int or an int64 cell on the device")
         plan, bound, device = super()._found(arrays)
         bound.append((plan.slots["offset"], cell.data_ptr() if isinstance(cell, torch.Tensor) else 0))

@@ -741,6 +741,56 @@ def test_row_losses_replayed_from_a_graph_and_repeated(gpu):
 
 
 @pytest.mark.gpu
+def test_plain_calls_captured_on_a_stream_of_their_own(gpu):
+    """Two graphs captured on a stream that no call ran on before, replayed in
+    either order and between plain calls: none leans on what another cleared."""
+    import torch
+    N, V, T, C = 40, 48, 3000, 40
+    target = torch.randint(0, V, (N,), device=gpu)
+    old, A = -4.0 + torch.randn(N, device=gpu), torch.randn(N, device=gpu)
+    logits = torch.randn(N, V, device=gpu)
+    few = torch.randn(3, 200003, device=gpu)
+    gate, x = torch.rand(1, T, C, device=gpu), torch.randn(1, T, C, device=gpu)
+    loss_stage, logp_stage, scan = hawk.stages.policy_loss(), hawk.stages.token_logp(), hawk.stages.recurrence()
+
+    def calls():
+        loss, bar, logp, h = torch.empty(1, device=gpu), torch.empty_like(logits), torch.empty(3, device=gpu), torch.empty_like(x)
+
+        def run():
+            hawk.run(loss_stage, logits=logits, target=target, old_logp=old, advantage=A, loss=loss, bar_logits=bar)
+            hawk.run(logp_stage, logits=few, target=target[:3].contiguous(), logp=logp)
+            hawk.run(scan, gate=gate, x=x, h=h)
+        return run, (loss, bar, logp, h)
+
+    eager, want = calls()
+    eager()
+    torch.cuda.synchronize()
+    side, graphs = torch.cuda.Stream(), []
+    for _ in range(2):
+        run, outs = calls()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+        graphs.append((graph, outs))
+    for k in (1, 0, 1, 1, 0):
+        logits.copy_(torch.randn(N, V, device=gpu))
+        x.copy_(torch.randn(1, T, C, device=gpu))
+        eager()
+        graph, outs = graphs[k]
+        for o in outs:
+            o.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    with torch.cuda.stream(side):
+        for o in want:
+            o.fill_(float("nan"))
+        eager()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(graphs[0][1], want))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ROW_TYPES)
 @pytest.mark.parametrize("shape", [(2, 131072), (5, 262147), (64, 131081), (65, 131081)], ids=str)
 def test_few_long_rows_over_several_workgroups(gpu, shape, dtype):
