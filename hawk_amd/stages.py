@@ -612,7 +612,8 @@ class _Dropout(_Stage):
             if t[n].shape != shape or t[n].dtype != first.dtype:
                 self._refuse(f"{n!r} is {t[n].dtype} {tuple(t[n].shape)}, {self.source} is {first.dtype} "
                              f"{tuple(shape)}")
-        if all(t[n].is_contiguous() for n in used):
+        whole = all(t[n].is_contiguous() for n in used)
+        if whole:
             job.rows, job.cols = 1, first.numel()
         else:
             job.cols = shape[-1]
@@ -620,7 +621,7 @@ class _Dropout(_Stage):
         field = {self.source: "x", "residual": "residual", self.target: "y"}
         slots = {}
         for n in used:
-            if job.rows > 1:
+            if not whole:                   # one row alone is read as contiguous too
                 setattr(job, field[n] + "_stride", self._row_stride(n, t[n]))
             slots[n] = _word(_core.DropoutJob, field[n])
         slots["offset"] = _word(_core.DropoutJob, "offset_cell")

@@ -955,6 +955,24 @@ def test_dropout_draws_a_new_mask_a_replay(gpu):
         assert torch.equal(y, want)
 
 
+def test_dropout_refuses_a_single_row_that_is_not_contiguous():
+    """Planes are addressed by rows: one row with gaps, or of one element repeated, is refused as several are."""
+    import torch
+    base, m, one = torch.zeros(1000), torch.zeros(300, 7), torch.zeros(())
+    gaps = torch.zeros(1, 1000)[:, ::2]
+    for x in (base[::2], m[:, 3], gaps, one.expand(500), torch.zeros(1, 1, 1).expand(1, 1, 9)):
+        like = torch.zeros(x.shape)
+        drop = hawk.stages.dropout(0.5)
+        for stage, planes in ((drop, dict(x=x, y=like)), (drop, dict(x=like, y=x)), (drop, dict(x=like, residual=x, y=like)),
+                              (drop.vjp, dict(bar_y=x, bar_x=like)), (drop.vjp, dict(bar_y=like, bar_x=x))):
+            with pytest.raises(HawkError, match="is contiguous, got strides"):
+                stage._make(planes)
+    # one row that is contiguous, and rows of one element, are planes like any other
+    wide = torch.zeros(3, 64)
+    for x in (wide[1], wide[1:2, :7], wide[:, 3:4], torch.zeros(1, 1, 5)[:, :, 1:4], torch.zeros(4, 1).expand(4, 1), one):
+        assert hawk.stages.dropout(0.5)._make(dict(x=x, y=torch.zeros(x.shape))).job.cols > 0
+
+
 # -- refusals --------------------------------------------------------------------------------
 
 def test_options_out_of_range_are_refused():
