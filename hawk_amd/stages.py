@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import numbers
 import threading
 
 import torch
@@ -641,13 +642,12 @@ class _Dropout(_Stage):
         return dims[-1][1] if dims else 0
 
     def _value(self, name: str, x) -> int:
-        if x is None and name == "offset":
-            return 0
-        if name == "offset" and not isinstance(x, int):
-            return 0                        # a cell on the device, bound by address
-        if isinstance(x, bool) or not isinstance(x, int) or not 0 <= x < 1 << 64:
+        if name == "offset" and (x is None or isinstance(x, torch.Tensor)):
+            return 0                        # none, or a cell on the device, bound by address
+        number = int(x) if isinstance(x, numbers.Integral) and not isinstance(x, bool) else -1
+        if not 0 <= number < 1 << 64:
             self._refuse(f"{name}= is an int in [0, 2^64), got {x!r}")
-        return x
+        return number
 
     def _found(self, arrays: dict):
         cell = arrays.get("offset")
@@ -666,7 +666,7 @@ def dropout(p: float) -> Stage:
     Planes: ``x``, ``residual``, ``y`` (written) of one shape and type (float64,
     float32, bfloat16, float16), contiguous or with contiguous rows evenly apart;
     ``y`` may be ``x`` or ``residual``.  ``seed`` and ``offset`` (0 if not given)
-    are ints below 2^64: an element's number comes from them and its index in
+    are ints (numpy's too) below 2^64: an element's number comes from them and its index in
     row-major order alone, so the mask does not depend on strides.  ``offset`` may
     be an int64 cell on the device, read by the kernel: a captured call then
     draws a new mask a replay.  Philox4x32-10 gives the numbers.

@@ -973,6 +973,22 @@ def test_dropout_refuses_a_single_row_that_is_not_contiguous():
         assert hawk.stages.dropout(0.5)._make(dict(x=x, y=torch.zeros(x.shape))).job.cols > 0
 
 
+def test_dropout_takes_whole_numbers_as_they_are_and_refuses_others():
+    """An offset that is no cell is never taken for 0: a mask would repeat from step to step."""
+    import torch
+    stage = hawk.stages.dropout(0.5)
+    for name in ("seed", "offset"):
+        for x, want in ((5, 5), (np.int64(5), 5), (np.uint64((1 << 64) - 1), (1 << 64) - 1), (np.int32(0), 0)):
+            assert stage._value(name, x) == want
+        for x in (7.0, np.float64(7), "7", True, np.bool_(True), -1, np.int64(-1), 1 << 64, [5], np.array([5, 6])):
+            with pytest.raises(HawkError, match=f"{name}= is an int"):
+                stage._value(name, x)
+    assert stage._value("offset", None) == 0 and stage._value("offset", torch.zeros(1, dtype=torch.int64)) == 0
+    for x in (None, torch.zeros(1, dtype=torch.int64)):
+        with pytest.raises(HawkError, match="seed= is an int"):
+            stage._value("seed", x)
+
+
 # -- refusals --------------------------------------------------------------------------------
 
 def test_options_out_of_range_are_refused():
