@@ -160,9 +160,9 @@ class _Stage(Stage):
         if not any(arrays.get(name) is not None for name in self.writes):
             self._refuse(f"no output is given (one of {', '.join(self.writes)})")
 
-    def _plan(self, key, arrays: dict):
-        """The plan of ``key``, made and checked where there is none."""
-        self._names(arrays)
+    def _placed(self, arrays: dict) -> dict:
+        """The planes that are given: tensors of the current device, outputs that
+        repeat no memory."""
         tensors = {n: x for n, x in arrays.items() if x is not None and n in self.planes}
         for n, x in tensors.items():
             if not isinstance(x, torch.Tensor):
@@ -179,13 +179,21 @@ class _Stage(Stage):
             x = tensors.get(n)
             if x is not None and any(d > 1 and st == 0 for d, st in zip(x.shape, x.stride())):
                 self._refuse(f"the output {n!r} repeats memory (strides {tuple(x.stride())})")
-        plan = self._make(tensors)
+        return tensors
+
+    def _plan(self, key, arrays: dict, device: int) -> _Plan:
+        """A plan of ``key``, made, checked and bound before another thread may
+        find it."""
+        self._names(arrays)
+        plan = self._make(self._placed(arrays))
+        if key is None:
+            self._refuse("a plane is no dense tensor")
+        plan.bind(arrays, self.values, device)
         with self._lock:
-            if key is not None and len(self._plans) >= PLANS:
+            if len(self._plans) >= PLANS:
                 for old in list(self._plans)[:PLANS // 2]:
                     del self._plans[old]
-            if key is not None:
-                self._plans[key] = plan
+            self._plans[key] = plan
         return plan
 
     def _make(self, tensors: dict) -> _Plan:
@@ -209,10 +217,7 @@ class _Stage(Stage):
         except (AttributeError, RuntimeError, TypeError):
             plan, key = None, None
         if plan is None:
-            plan = self._plan(key, arrays)
-            if key is None:
-                self._refuse("a plane is no dense tensor")
-            plan.bind(arrays, self.values, device)
+            plan = self._plan(key, arrays, device)
         self._last = plan if all(x is not None for x in arrays.values()) else None
         bound = [(plan.slots[name], x.data_ptr()) for name, x in arrays.items()
                  if x is not None and name not in self.values]

@@ -1152,6 +1152,59 @@ def test_the_binding_puts_words_where_they_belong_and_refuses_others():
             Call(address, False, True, 0, job[:size], 2, planes, apart)
 
 
+def bare_stage(entry):
+    """A stage of planes ``x`` and ``y`` on the CPU, whose entry is the given function's address."""
+    from hawk_amd import stages
+
+    class Bare(stages._Stage):
+        name, reads, writes = "bare", ("x",), ("y",)
+
+        def _placed(self, arrays):
+            return {n: t for n, t in arrays.items() if t is not None}
+
+        def _make(self, t):
+            job = (ctypes.c_uint64 * 2)()
+            return stages._Plan(job, {"x": 0, "y": 1}, ctypes.cast(entry, ctypes.c_void_p), 0)
+    return Bare()
+
+
+def test_a_plan_is_found_once_it_can_be_called(monkeypatch):
+    """Threads that meet a new set of shapes at once each call a whole plan; a plan that could not be bound is
+    not kept."""
+    import threading
+
+    import torch
+    from hawk_amd import stages
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)(lambda *_: 0)
+    stage, x = bare_stage(entry), torch.zeros(3)
+    bind, inside, leave, seen = stages._Plan.bind, threading.Event(), threading.Event(), []
+
+    def slow(plan, *args):
+        inside.set()
+        leave.wait(10)
+        bind(plan, *args)
+    monkeypatch.setattr(stages._Plan, "bind", slow)
+    first = threading.Thread(target=lambda: seen.append(stage._found({"x": x, "y": x})[0]))
+    first.start()
+    assert inside.wait(10)
+    assert not stage._plans and stage._last is None
+    monkeypatch.setattr(stages._Plan, "bind", bind)
+    second = stage._found({"x": x, "y": x})[0]                 # meets the same shapes meanwhile
+    leave.set()
+    first.join()
+    assert second.call is not None and seen[0].call is not None
+    assert stage._found({"x": x, "y": x})[0].call is not None and len(stage._plans) == 1
+
+    def broken(plan, *args):
+        raise HawkError("the binding is not built")
+    monkeypatch.setattr(stages._Plan, "bind", broken)
+    stage = bare_stage(entry)
+    for _ in range(2):
+        with pytest.raises(HawkError, match="not built"):
+            stage._found({"x": x, "y": x})
+    assert not stage._plans and stage._last is None
+
+
 @pytest.mark.gpu
 def test_the_recurrent_policy_example_learns(gpu):
     """All stages together: recall by chance is 1 in 16."""
