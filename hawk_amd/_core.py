@@ -84,6 +84,7 @@ def _declare(lib) -> None:
         "hk_keyed_sample_sum_f32": (I, [V, I64, I64, V, V]),
         "hk_keyed_log_fold_f64": (I, [V, I64, V, I64, I64, ctypes.c_int32, V, I64, V, V, V]),
         "hk_keyed_log_fold_f32": (I, [V, I64, V, I64, I64, ctypes.c_int32, V, I64, V, V, V]),
+        "hk_stream_capturing": (I, [V]),
         "hk_recurrence_scratch_bytes": (SZ, [V, ctypes.c_int32]),
         "hk_recurrence": (I, [V, V, V]),
         "hk_recurrence_vjp": (I, [V, V, V]),
@@ -536,6 +537,16 @@ def band_ordered_sum_scratch_bytes() -> int:
 def band_ordered_sum(u: int, n: int, out: int, scratch: int, stream: int = 0) -> None:
     check(lib().hk_band_ordered_sum_f64(u or None, int(n), out,
                                         scratch, stream or None))
+
+
+def stream_capturing(stream: int) -> bool:
+    """Whether a graph is being captured on the stream of this handle."""
+    return bool(lib().hk_stream_capturing(stream or None))
+
+
+def stream_capturing_entry() -> int:
+    """The address of what :func:`stream_capturing` asks, for the binding."""
+    return ctypes.cast(lib().hk_stream_capturing, ctypes.c_void_p).value
 
 
 class SeqPlane(ctypes.Structure):

@@ -22,6 +22,7 @@ namespace {
 constexpr size_t kMostWords = 64;
 typedef int (*Entry)(const void* job, void* scratch, void* stream);
 typedef int (*PlainEntry)(const void* job, void* stream);
+typedef int (*Capturing)(void* stream);
 
 struct Plane {
     PyObject* name;          // held; a call's names are the same objects
@@ -40,6 +41,7 @@ struct Plan {
     bool plain;              // the entry takes no scratch
     bool needs_space;
     int device;
+    Capturing capturing;     // or NULL: no call is captured
     int64_t state_word;
     std::vector<uint64_t> job;
     std::vector<Plane> planes;
@@ -68,17 +70,18 @@ int enter(const Plan& plan, const uint64_t* job, uint64_t scratch, uint64_t stre
     return rc;
 }
 
-// Call(entry, plain, needs_space, device, job, state_word, planes, apart): planes is a
-// tuple of (name, tensor or None, word), apart one of (plane, plane) positions.
+// Call(entry, plain, needs_space, device, job, state_word, planes, apart, capturing):
+// planes is a tuple of (name, tensor or None, word), apart one of (plane, plane)
+// positions, capturing (may be left out) tells whether a stream is under capture.
 int call_init(PyObject* self, PyObject* args, PyObject*) {
-    unsigned long long entry;
+    unsigned long long entry, capturing = 0;
     int plain, needs_space, device;
     const char* job;
     Py_ssize_t job_bytes;
     long long state_word;
     PyObject *planes, *apart;
-    if (!PyArg_ParseTuple(args, "Kppiy#LO!O!", &entry, &plain, &needs_space, &device, &job, &job_bytes, &state_word,
-                          &PyTuple_Type, &planes, &PyTuple_Type, &apart))
+    if (!PyArg_ParseTuple(args, "Kppiy#LO!O!|K", &entry, &plain, &needs_space, &device, &job, &job_bytes, &state_word,
+                          &PyTuple_Type, &planes, &PyTuple_Type, &apart, &capturing))
         return -1;
     if (job_bytes % 8 != 0 || static_cast<size_t>(job_bytes) / 8 > kMostWords) {
         PyErr_SetString(PyExc_ValueError, "a job of whole words, 64 at most");
@@ -90,6 +93,7 @@ int call_init(PyObject* self, PyObject* args, PyObject*) {
     plan->plain = plain;
     plan->needs_space = needs_space;
     plan->device = device;
+    plan->capturing = reinterpret_cast<Capturing>(capturing);
     plan->state_word = state_word;
     plan->job.resize(job_bytes / 8);
     std::memcpy(plan->job.data(), job, job_bytes);
@@ -154,7 +158,8 @@ bool address_of(const Plan& plan, const Plane& p, PyObject* x, uint64_t& at) {
 }
 
 // run(arrays, device, stream): the entry's status, or -1 for a call that is not the
-// plan's (other planes, a stream without its space), of which nothing ran.
+// plan's (other planes, a stream without its space or under capture, whose space is
+// the graph's), of which nothing ran.
 PyObject* call_run(PyObject* self, PyObject* const* args, Py_ssize_t n) {
     if (n != 3 || !PyDict_CheckExact(args[0])) {
         PyErr_SetString(PyExc_TypeError, "run(arrays, device, stream)");
@@ -199,7 +204,7 @@ PyObject* call_run(PyObject* self, PyObject* const* args, Py_ssize_t n) {
         const Space* space = nullptr;
         for (const Space& s : plan.spaces)
             if (s.stream == stream) space = &s;
-        if (!space) return PyLong_FromLong(-1);
+        if (!space || (plan.capturing && plan.capturing(reinterpret_cast<void*>(stream)))) return PyLong_FromLong(-1);
         scratch = space->scratch;
         if (plan.state_word >= 0) job[plan.state_word] = space->state;
     }

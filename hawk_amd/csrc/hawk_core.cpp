@@ -509,4 +509,14 @@ int hk_launch_grid(const hk_entry* entry, const hk_argblock* ab, int64_t base,
     return launch_impl(entry, ab, base, count, n_samples, grid, block, stream);
 }
 
+int hk_stream_capturing(void* stream) {
+    if (!stream) return 0;              // the legacy default stream takes no capture
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return 1;
+    }
+    return status != hipStreamCaptureStatusNone;
+}
+
 }  // extern "C"

@@ -17,8 +17,10 @@ a stage whose planes are the primal's with ``bar_`` names for adjoints::
     hawk.run(scan, gate=z, x=x, h=h)
     hawk.run(scan.vjp, gate=z, x=x, h=h, bar_h=bar_h, bar_gate=bar_z, bar_x=bar_x)
 
-Planes are PyTorch-ROCm tensors, bound by address.  Scratch belongs to a stream:
-calls on several streams may run at once.  Nothing synchronises.
+Planes are PyTorch-ROCm tensors, bound by address.  Scratch belongs to a stream,
+or to the graph a call is captured in: calls on several streams and replays of
+several graphs may run at once (a launcher's own run one after another).  Nothing
+synchronises.
 """
 
 from __future__ import annotations
@@ -82,7 +84,8 @@ class _Plan:
                       if arrays.get(a) is not None and arrays.get(b) is not None)
         entry = ctypes.cast(self.entry or self.fn, ctypes.c_void_p).value
         self.call = _core.bind().Call(entry, self.entry is not None, bool(self.scratch), device, bytes(self.job),
-                                      -1 if self.state is None else self.state, planes, apart)
+                                      -1 if self.state is None else self.state, planes, apart,
+                                      _core.stream_capturing_entry())
 
 
 def _word(job_type, *path) -> int:
@@ -112,11 +115,11 @@ class _Space:
 
 
 def _space(device: int, stream: int, nbytes: int, state: bool) -> tuple:
-    """``(space, kept)``: what the calls on ``stream`` work in.  One that is first
-    asked for while the stream is captured is that call's alone: its memory is the
-    graph's, and its state is cleared by the graph's replays, not before them."""
+    """``(space, kept)``: what the calls on ``stream`` work in.  A captured call's is
+    its own: the memory is the graph's, which may be replayed on another stream
+    beside calls on this one, and its state is cleared by the graph's replays."""
     with _spaces_lock, _on(stream):
-        if torch.cuda.is_current_stream_capturing():
+        if _core.stream_capturing(stream):
             clear = torch.zeros if state else torch.empty
             return _Space(torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}"),
                           clear(_core.STATE_BYTES if state else 0, dtype=torch.uint8, device=f"cuda:{device}")), False
@@ -242,7 +245,7 @@ class _Stage(Stage):
             plan, bound, device = self._found(arrays)
             space = None
             if plan.scratch:
-                space = plan.spaces.get(raw)
+                space = None if _core.stream_capturing(raw) else plan.spaces.get(raw)
                 if space is None:
                     space, kept = _space(device, raw, plan.scratch, plan.state is not None)
                     if kept:
@@ -465,6 +468,8 @@ class _Rows(_Stage):
         for n in t:
             slots[n] = _word(_core.RowLossJob, n)
         L = _core.lib()
+        if self.vjp_of is not None:         # a derivative works in registers
+            return _Plan(job, slots, getattr(L, self.entry), 0)
         return _Plan(job, slots, getattr(L, self.entry), int(L.hk_row_loss_scratch_bytes(ctypes.byref(job))),
                      state=_word(_core.RowLossJob, "state"))
 

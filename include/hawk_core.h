@@ -363,6 +363,11 @@ int hk_mm16_f64(const double* const* in, int n_in, double* const* out, int n_out
 
 /* ---- training stages: recurrences, row losses, dropout ------------------- */
 
+/* Whether a graph is being captured on `stream` (1 or 0; 1 where the runtime
+ * cannot say).  What such a call works in is the graph's: its launches run when
+ * the graph is replayed, on any stream. */
+int hk_stream_capturing(void* stream);
+
 /* The element type of a stage's planes. */
 enum { HK_F32 = 0, HK_F64 = 1, HK_BF16 = 2, HK_F16 = 3 };
 

@@ -791,6 +791,66 @@ def test_plain_calls_captured_on_a_stream_of_their_own(gpu):
 
 
 @pytest.mark.gpu
+def test_plain_calls_captured_on_a_stream_that_ran_before(gpu):
+    """Graphs captured on a warmed stream, replayed on two others beside each other and beside plain calls on
+    that stream: each works in memory of its own."""
+    import torch
+    N, V, T, C = 40, 48, 6000, 40
+    target = torch.randint(0, V, (N,), device=gpu)
+    old, A = -4.0 + torch.randn(N, device=gpu), torch.randn(N, device=gpu)
+    logits, few = torch.randn(N, V, device=gpu), torch.randn(3, 200003, device=gpu)
+    gate, x = torch.rand(1, T, C, device=gpu), torch.randn(1, T, C, device=gpu)
+    offsets = torch.arange(0, N + 1, N // 8, device=gpu)[:9]
+    loss_stage, logp_stage, scan = hawk.stages.policy_loss(), hawk.stages.token_logp(), hawk.stages.recurrence()
+    pairs = hawk.stages.preference_loss()
+
+    def calls():
+        loss, bar, logp = torch.empty(1, device=gpu), torch.empty_like(logits), torch.empty(3, device=gpu)
+        h, to_gate, to_x = (torch.empty_like(x) for _ in range(3))
+        both = torch.empty(1, device=gpu)
+
+        def run():
+            hawk.run(loss_stage, logits=logits, target=target, old_logp=old, advantage=A, loss=loss, bar_logits=bar)
+            hawk.run(logp_stage, logits=few, target=target[:3].contiguous(), logp=logp)
+            hawk.run(scan, gate=gate, x=x, h=h)
+            hawk.run(scan.vjp, gate=gate, h=h, bar_h=x, bar_gate=to_gate, bar_x=to_x)
+            hawk.run(pairs, logits=logits, target=target, offsets=offsets, loss=both)
+        return run, (loss, bar, logp, h, to_gate, to_x, both)
+
+    eager, want = calls()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            eager()
+    torch.cuda.synchronize()
+    want = tuple(o.clone() for o in want)
+    graphs = []
+    for _ in range(2):
+        run, outs = calls()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+        graphs.append((graph, outs, torch.cuda.Stream()))
+    plain, plain_outs = calls()
+    for k in range(6):
+        for _, outs, _ in graphs:
+            for o in outs:
+                o.fill_(float("nan"))
+        for o in plain_outs:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(side):
+            plain()
+        torch.cuda.synchronize()
+        for outs in (graphs[0][1], graphs[1][1], plain_outs):
+            assert all(torch.equal(o, w) for o, w in zip(outs, want)), k
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ROW_TYPES)
 @pytest.mark.parametrize("shape", [(2, 131072), (5, 262147), (64, 131081), (65, 131081)], ids=str)
 def test_few_long_rows_over_several_workgroups(gpu, shape, dtype):
@@ -1203,6 +1263,49 @@ def test_a_plan_is_found_once_it_can_be_called(monkeypatch):
         with pytest.raises(HawkError, match="not built"):
             stage._found({"x": x, "y": x})
     assert not stage._plans and stage._last is None
+
+
+def test_a_captured_call_works_apart_from_the_streams_others(monkeypatch):
+    """A stream's space is not bound into a graph, which may be replayed on another stream: while the stream is
+    captured every call asks for space of its own, and none of it is kept."""
+    from types import SimpleNamespace
+
+    from hawk_amd import stages
+    seen, made, capturing = [], [], [False]
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p, ctypes.c_void_p)(
+        lambda job, scratch, stream: seen.append((scratch, job[2])) or 0)
+    asked = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(lambda stream: int(capturing[0]))
+    monkeypatch.setattr(_core, "stream_capturing", lambda stream: capturing[0])
+    monkeypatch.setattr(_core, "stream_capturing_entry", lambda: ctypes.cast(asked, ctypes.c_void_p).value)
+
+    def space(device, stream, nbytes, state):
+        made.append(SimpleNamespace(scratch=1000 + len(made), state=2000 + len(made)))
+        return made[-1], not capturing[0]
+    monkeypatch.setattr(stages, "_space", space)
+
+    class Fixed(stages._Stage):
+        """By-value words alone, which the binding's quick check takes on the CPU too."""
+        name, values = "fixed", ("seed",)
+
+        def _names(self, arrays):
+            pass
+
+        def _placed(self, arrays):
+            return {}
+
+        def _make(self, t):
+            return stages._Plan((ctypes.c_uint64 * 3)(), {}, ctypes.cast(entry, ctypes.c_void_p), 64, state=2,
+                                cells=(("seed", 1),))
+
+        def _value(self, name, x):
+            return x
+    stage, arrays = Fixed(), {"seed": 7}
+    for now in (False, False, True, True, False, True, False):
+        capturing[0] = now
+        stage.run(arrays, stream=96)
+    kept = (1000, 2000)
+    assert seen == [kept, kept, (1001, 2001), (1002, 2002), kept, (1003, 2003), kept] and len(made) == 4
+    assert _core.lib().hk_stream_capturing(None) == 0
 
 
 @pytest.mark.gpu
