@@ -268,7 +268,8 @@ class _Stage(Stage):
         if plan.scratch:
             with _on(stream):
                 scratch = torch.empty(plan.scratch, dtype=torch.uint8, device=f"cuda:{device}")
-                if plan.state is not None:
+                # under capture the clearing would wait for a replay: an entry does without
+                if plan.state is not None and not _core.stream_capturing(stream):
                     state = torch.zeros(_core.STATE_BYTES, dtype=torch.uint8, device=f"cuda:{device}")
                     bound.append((plan.state, state.data_ptr()))
         for word, value in bound:

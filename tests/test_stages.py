@@ -13,6 +13,7 @@ times itself.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -851,6 +852,37 @@ def test_plain_calls_captured_on_a_stream_that_ran_before(gpu):
 
 
 @pytest.mark.gpu
+def test_a_launcher_made_under_capture_runs_before_and_after_a_replay(gpu):
+    import torch
+    logits, few = torch.randn(40, 48, device=gpu), torch.randn(3, 200003, device=gpu)
+    target = torch.randint(0, 48, (40,), device=gpu)
+    planes = dict(logits=logits, target=target, old_logp=torch.full((40,), -4.0, device=gpu),
+                  advantage=torch.randn(40, device=gpu))
+    policy, rows = hawk.stages.policy_loss(), hawk.stages.token_logp()
+    loss, logp, want, want_logp = (torch.empty(k, device=gpu) for k in (1, 3, 1, 3))
+    hawk.run(policy, loss=want, **planes)
+    hawk.run(rows, logits=few, target=target[:3].contiguous(), logp=want_logp)
+    side, graph, y = torch.cuda.Stream(), torch.cuda.CUDAGraph(), target[:3].contiguous()
+    with torch.cuda.graph(graph, stream=side):
+        launches = policy.prepare(loss=loss, **planes), rows.prepare(logits=few, target=y, logp=logp)
+        for launch in launches:
+            launch()
+    for k in range(4):
+        loss.fill_(float("nan"))
+        logp.fill_(float("nan"))
+        torch.cuda.synchronize()
+        if k % 2:
+            graph.replay()
+        else:
+            for launch in launches:
+                launch()
+        torch.cuda.synchronize()
+        # a row in one piece or in parts: the terms are joined in another tree
+        assert abs(float(loss) - float(want)) <= 2.0 ** -20 * 10
+        assert (logp - want_logp).abs().max() <= 16 * 2.0 ** -24 * (2 + want_logp.abs().max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ROW_TYPES)
 @pytest.mark.parametrize("shape", [(2, 131072), (5, 262147), (64, 131081), (65, 131081)], ids=str)
 def test_few_long_rows_over_several_workgroups(gpu, shape, dtype):
@@ -1306,6 +1338,34 @@ def test_a_captured_call_works_apart_from_the_streams_others(monkeypatch):
     kept = (1000, 2000)
     assert seen == [kept, kept, (1001, 2001), (1002, 2002), kept, (1003, 2003), kept] and len(made) == 4
     assert _core.lib().hk_stream_capturing(None) == 0
+
+
+def test_a_launcher_made_under_capture_takes_no_state(monkeypatch):
+    """Its clearing would be the graph's: a call of the launcher before a replay would find what the memory held."""
+    import torch
+    from hawk_amd import stages
+    seen, capturing, made = [], [False], []
+    words = ctypes.POINTER(ctypes.c_uint64)
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)(
+        lambda job, scratch, stream: seen.append((scratch, ctypes.cast(job, words)[2])) or 0)
+    monkeypatch.setattr(_core, "stream_capturing", lambda stream: capturing[0])
+    monkeypatch.setattr(stages, "_on", lambda stream: contextlib.nullcontext())
+
+    def on_host(make):
+        def called(*args, device=None, **more):
+            made.append(make(*args, **more))
+            return made[-1]
+        return called
+    stage, x = bare_stage(entry), torch.zeros(3)
+    plan = stages._Plan((ctypes.c_uint64 * 3)(), {"x": 0, "y": 1}, entry, 64, state=2)
+    monkeypatch.setattr(stage, "_found", lambda arrays: (plan, [], -1))
+    monkeypatch.setattr(torch, "empty", on_host(torch.empty))
+    monkeypatch.setattr(torch, "zeros", on_host(torch.zeros))
+    for capturing[0], tensors in ((False, 2), (True, 1)):
+        made.clear()
+        stage.prepare(stream=96, x=x, y=x)()
+        assert len(made) == tensors
+        assert seen[-1] == (made[0].data_ptr(), made[1].data_ptr() if tensors == 2 else 0)
 
 
 @pytest.mark.gpu
