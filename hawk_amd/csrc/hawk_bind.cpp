@@ -13,6 +13,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <map>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -34,6 +35,7 @@ struct Plane {
 
 struct Space {
     uint64_t stream, scratch, state;
+    std::mutex* launches;
 };
 
 struct Plan {
@@ -54,14 +56,19 @@ struct Call {
     Plan* plan;
 };
 
-// Calls on one stream share its scratch, so a call's launches stay together.
-std::mutex launches;
+// Calls on one stream share its scratch, so each one's launches stay together; a
+// launch that blocks holds no other stream's.  (Found under the interpreter's lock.)
+std::mutex* launches_of(int device, uint64_t stream) {
+    static auto& all = *new std::map<std::pair<int, uint64_t>, std::mutex>;      // outlives every thread
+    return &all[{device, stream}];
+}
 
-int enter(const Plan& plan, const uint64_t* job, uint64_t scratch, uint64_t stream) {
+int enter(const Plan& plan, const uint64_t* job, uint64_t scratch, uint64_t stream, std::mutex* launches) {
     int rc;
     Py_BEGIN_ALLOW_THREADS
     {
-        std::lock_guard<std::mutex> hold(launches);
+        std::unique_lock<std::mutex> hold;
+        if (launches) hold = std::unique_lock<std::mutex>(*launches);
         void* s = reinterpret_cast<void*>(stream);
         rc = plan.plain ? reinterpret_cast<PlainEntry>(plan.entry)(job, s)
                         : reinterpret_cast<Entry>(plan.entry)(job, reinterpret_cast<void*>(scratch), s);
@@ -200,15 +207,17 @@ PyObject* call_run(PyObject* self, PyObject* const* args, Py_ssize_t n) {
     for (const auto& pair : plan.apart)
         if (at[pair.first] == at[pair.second]) return PyLong_FromLong(-1);
     uint64_t scratch = 0;
+    std::mutex* launches = nullptr;
     if (plan.needs_space) {
         const Space* space = nullptr;
         for (const Space& s : plan.spaces)
             if (s.stream == stream) space = &s;
         if (!space || (plan.capturing && plan.capturing(reinterpret_cast<void*>(stream)))) return PyLong_FromLong(-1);
         scratch = space->scratch;
+        launches = space->launches;
         if (plan.state_word >= 0) job[plan.state_word] = space->state;
     }
-    return PyLong_FromLong(enter(plan, job, scratch, stream));
+    return PyLong_FromLong(enter(plan, job, scratch, stream, launches));
 }
 
 // launch(bound, scratch, stream): the entry's status with the words of `bound`, a
@@ -230,14 +239,15 @@ PyObject* call_launch(PyObject* self, PyObject* args) {
         }
         job[word] = value;
     }
-    return PyLong_FromLong(enter(plan, job, scratch, stream));
+    return PyLong_FromLong(enter(plan, job, scratch, stream, plan.needs_space ? launches_of(plan.device, stream) : nullptr));
 }
 
 // space(stream, scratch, state): what the calls on a stream work in.
 PyObject* call_space(PyObject* self, PyObject* args) {
     unsigned long long stream, scratch, state;
     if (!PyArg_ParseTuple(args, "KKK", &stream, &scratch, &state)) return nullptr;
-    reinterpret_cast<Call*>(self)->plan->spaces.push_back({stream, scratch, state});
+    Plan& plan = *reinterpret_cast<Call*>(self)->plan;
+    plan.spaces.push_back({stream, scratch, state, launches_of(plan.device, stream)});
     Py_RETURN_NONE;
 }
 

@@ -1368,6 +1368,35 @@ def test_a_launcher_made_under_capture_takes_no_state(monkeypatch):
         assert seen[-1] == (made[0].data_ptr(), made[1].data_ptr() if tensors == 2 else 0)
 
 
+@pytest.mark.parametrize("one,two,apart", [((0, 32), (0, 64), True), ((0, 32), (1, 32), True), ((0, 32), (0, 32), False)], ids=str)
+def test_calls_wait_for_those_of_their_own_stream_alone(one, two, apart):
+    """A launch that blocks holds the calls of its stream, whose scratch it works in, and no others."""
+    import threading
+    inside, met, order = threading.Event(), threading.Event(), []
+
+    def first(job, scratch, stream):
+        inside.set()
+        order.append(("first", met.wait(20 if apart else 0.3)))
+        return 0
+
+    def second(job, scratch, stream):
+        order.append(("second", None))
+        met.set()
+        return 0
+    kind = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)
+    calls = []
+    for entry, (device, stream) in ((kind(first), one), (kind(second), two)):
+        call = _core.bind().Call(ctypes.cast(entry, ctypes.c_void_p).value, False, True, device, bytes(8), -1, (("seed", None, 0),), ())
+        call.space(stream, 48, 0)
+        calls.append((call, entry, device, stream))
+    running = threading.Thread(target=lambda: calls[0][0].run({"seed": 1}, *calls[0][2:]))
+    running.start()
+    assert inside.wait(20)
+    assert calls[1][0].run({"seed": 1}, *calls[1][2:]) == 0
+    running.join()
+    assert order == ([("second", None), ("first", True)] if apart else [("first", False), ("second", None)])
+
+
 @pytest.mark.gpu
 def test_the_recurrent_policy_example_learns(gpu):
     """All stages together: recall by chance is 1 in 16."""
