@@ -1,11 +1,12 @@
-"""Build step of hawk's gfx950 target: compile ``libhawk_core.so`` in-tree.
+"""Build step of hawk's gfx950 target: compile ``libhawk_core.so`` and ``_bind.so`` in-tree.
 
 The library is the C-ABI launcher (``csrc/hawk_core.cpp``) plus the
 hand-written team-stage kernels (``csrc/hawk_team.hip``, ``csrc/hawk_linalg.hip``) and training stages
 (``csrc/hawk_recurrence.hip``, ``csrc/hawk_rows.hip``, ``csrc/hawk_dropout.hip``), built by ``hipcc``
 for gfx950 only, each file by a compiler of its own.  Beside it ``_bind.so`` (``csrc/hawk_bind.cpp``,
-built by the host compiler against PyTorch's headers) checks and binds a stage's tensors.  The build digest is the sha256 of its own sources (each
-file's name and sha256, in sorted order), stamped into the library and
+built by the host compiler against PyTorch's headers) checks and binds a stage's tensors; the library
+is built and used without it.  The build digest is the sha256 of its own sources (each
+file's name and sha256, in sorted order), stamped into both and
 recomputed by :mod:`hawk_amd._core` at load, the same self-check the
 reference runs at import (reference ``hawk/__init__.py:146-212``).
 """
@@ -14,7 +15,6 @@ from __future__ import annotations
 
 import hashlib
 import os
-import shutil
 import subprocess
 import sys
 import tempfile
@@ -67,35 +67,47 @@ def binding_command(digest: str, out: Path) -> list:
             f"-L{at}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
+def _call(cmd: list, what: Path, verbose: bool) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed building {what.name}:\n{proc.stdout}\n{proc.stderr}")
+
+
 def build_library(verbose: bool = False) -> Path:
-    """Compile ``libhawk_core.so`` and ``_bind.so`` next to this file; returns the
-    library's path."""
+    """Compile ``libhawk_core.so`` next to this file; returns its path."""
     digest = source_digest()
     info = "compiler=" + HIPCC + "\\nflags=" + " ".join(HIP_FLAGS) + "\\noffload_arch=gfx950"
     tmp = LIBRARY.with_suffix(".so.tmp")
     flags = [*HIP_FLAGS, "-fPIC", "-std=c++17", f"-I{INCLUDE}", f"-I{CSRC}",
              f'-DHAWK_BUILD_DIGEST="{digest}"', f'-DHAWK_BUILD_INFO="{info}"']
-
-    def call(cmd: list) -> None:
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        proc = subprocess.run(cmd, capture_output=True, text=True)
-        if proc.returncode != 0:
-            raise RuntimeError(f"{cmd[0]} failed building {LIBRARY.name}:\n{proc.stdout}\n{proc.stderr}")
-
-    with tempfile.TemporaryDirectory() as made, ThreadPoolExecutor(len(UNITS) + 1) as pool:
-        binding = Path(made) / BINDING.name
-        bound = pool.submit(call, binding_command(digest, binding))
+    with tempfile.TemporaryDirectory() as made, ThreadPoolExecutor(len(UNITS)) as pool:
         objects = [str(Path(made) / f"{name}.o") for name in UNITS]
-        list(pool.map(lambda pair: call([HIPCC, *flags, "-c", str(CSRC / pair[0]), "-o", pair[1]]),
+        list(pool.map(lambda pair: _call([HIPCC, *flags, "-c", str(CSRC / pair[0]), "-o", pair[1]], LIBRARY, verbose),
                       zip(UNITS, objects)))
-        call([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared", *objects, "-o", str(tmp), "-lhiprtc", "-lamdhip64"])
-        bound.result()
-        shutil.move(binding, BINDING.with_suffix(".so.tmp"))
-    os.replace(BINDING.with_suffix(".so.tmp"), BINDING)
+        _call([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared", *objects, "-o", str(tmp), "-lhiprtc", "-lamdhip64"],
+              LIBRARY, verbose)
     os.replace(tmp, LIBRARY)
     return LIBRARY
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile ``_bind.so`` next to this file (the training stages need it, nothing
+    else does); returns its path."""
+    tmp = BINDING.with_suffix(".so.tmp")
+    _call(binding_command(source_digest(), tmp), BINDING, verbose)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
+def build(verbose: bool = False) -> list:
+    """Both, at the same time; returns their paths.  The library is in place where
+    only the binding fails."""
+    with ThreadPoolExecutor(1) as pool:
+        binding = pool.submit(build_binding, verbose)
+        return [build_library(verbose), binding.result()]
+
+
 if __name__ == "__main__":
-    print(build_library(verbose="-v" in sys.argv))
+    print(*build(verbose="-v" in sys.argv), sep="\n")

@@ -197,3 +197,35 @@ def test_launch_arguments_are_checked_before_hip():
     rc = L.hk_launch(fake, ab.handle, 0, 10, 10, 100, 1, None)
     assert rc != 0 and b"multiple of 64" in L.hk_last_error()
     assert L.hk_launch(fake, ab.handle, 0, 0, 10, 256, 1, None) == 0     # empty range: nothing launched
+
+
+def test_the_library_is_built_without_the_binding(monkeypatch, tmp_path):
+    """The launcher and its kernels need neither PyTorch's headers nor a host compiler: where these are missing the
+    library is built all the same, and the binding's failure is told."""
+    import subprocess
+    import types
+
+    from hawk_amd import _build
+    monkeypatch.setattr(_build, "LIBRARY", tmp_path / "libhawk_core.so")
+    monkeypatch.setattr(_build, "BINDING", tmp_path / "_bind.so")
+
+    def run(cmd, **more):
+        if cmd[0] == "g++":
+            return types.SimpleNamespace(returncode=1, stdout="", stderr="torch/csrc: no such file")
+        out = cmd[cmd.index("-o") + 1]
+        with open(out, "w") as f:
+            f.write("built")
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+    monkeypatch.setattr(subprocess, "run", run)
+    with pytest.raises(RuntimeError, match="_bind.so"):
+        _build.build()
+    assert (tmp_path / "libhawk_core.so").read_text() == "built" and not (tmp_path / "_bind.so").exists()
+    (tmp_path / "libhawk_core.so").unlink()
+
+    def missing(*_):
+        raise ImportError("no torch")
+    monkeypatch.setattr(_build, "binding_command", missing)
+    assert _build.build_library() == tmp_path / "libhawk_core.so"
+    assert (tmp_path / "libhawk_core.so").read_text() == "built"
+    with pytest.raises(ImportError):
+        _build.build()
