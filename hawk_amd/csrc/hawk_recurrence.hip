@@ -12,8 +12,10 @@
 //
 // A gate of 0 cuts, and so does the first row of a packed sequence: products
 // and their use take 0 times anything as 0 (cutmul), so neither an infinity
-// nor a NaN passes a cut; a product of gates is 0 only where one is (chain).
-// States and products are held in 32 bits (64 for double planes).
+// nor a NaN passes a cut.  States are held in 32 bits (64 for double planes), and
+// products as a mantissa of as many and an exponent of 32 (Gain), so that what a
+// state passes on is right also where the gates' product alone is no number of the
+// type: gates of 2 over 128 steps, or of 1/2 over 150.
 
 #include "hawk_core.h"
 #include "hawk_internal.h"
@@ -57,7 +59,8 @@ struct RecArgs {
     Acc<T>* fin;              // the state that leaves it: last, or bar_h0
     const void* offsets;
     uint32_t* counter;        // a strip's: hands its chunks out in order
-    typename Word<Acc<T>>::type* agg;      // [chunk][states][2]: each tile's (P, H)
+    uint64_t* agg;                         // [chunk][states]: each tile's (P's mantissa, H)
+    uint16_t* agg_exp;                     // [chunk][states]: and P's exponent
     typename Word<Acc<T>>::type* state;    // [chunk][states]: the state that leaves each tile
     uint32_t* flag;                        // [strip][chunk]: 1 once that state is written
     int64_t seqs, chans, cols, states;   // states: those of one tile row, seqs * chans (packed: chans)
@@ -176,7 +179,52 @@ __device__ __forceinline__ A await(const typename Word<A>::type* at) {
     return x;
 }
 
-constexpr int kBatch = 8;        // aggregates read at once
+// A tile's run for those behind it: (m, H) side by side, one word for 32-bit states,
+// and the exponent in 16 bits, none of them ever all bits.  (It is applied to a state
+// and joined to nothing, and at 2^+-32000 every state is an infinity or 0.)
+constexpr int kExponent = 1 << 15, kFar = 32000;
+template <class A> struct Run { Gain<A> p; A h; };
+__device__ __forceinline__ void publish_exponent(uint16_t* exps, int64_t at, int e) {
+    const int held = e < -kFar ? -kFar : e > kFar ? kFar : e;
+    __hip_atomic_store(exps + at, static_cast<uint16_t>(kExponent + held), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void publish_run(uint64_t* agg, uint16_t* exps, int64_t at, const Run<float>& r) {
+    typedef Word<float> W;
+    const uint32_t m = r.p.m == r.p.m ? __builtin_bit_cast(uint32_t, r.p.m) : W::kNan;
+    const uint32_t h = r.h == r.h ? __builtin_bit_cast(uint32_t, r.h) : W::kNan;
+    __hip_atomic_store(agg + at, static_cast<uint64_t>(h) << 32 | m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    publish_exponent(exps, at, r.p.e);
+}
+__device__ __forceinline__ void publish_run(uint64_t* agg, uint16_t* exps, int64_t at, const Run<double>& r) {
+    publish<double>(agg + 2 * at, r.p.m);
+    publish<double>(agg + 2 * at + 1, r.h);
+    publish_exponent(exps, at, r.p.e);
+}
+__device__ __forceinline__ bool read_exponent(const uint16_t* exps, int64_t at, int& e) {
+    const uint32_t w = __hip_atomic_load(exps + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    e = static_cast<int>(w) - kExponent;
+    return w != 0xffffu;
+}
+__device__ __forceinline__ bool read_run(const uint64_t* agg, const uint16_t* exps, int64_t at, Run<float>& r) {
+    const uint64_t w = __hip_atomic_load(agg + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool known = read_exponent(exps, at, r.p.e);
+    r.p.m = __builtin_bit_cast(float, static_cast<uint32_t>(w));
+    r.h = __builtin_bit_cast(float, static_cast<uint32_t>(w >> 32));
+    return (w != ~uint64_t(0)) & known;
+}
+__device__ __forceinline__ bool read_run(const uint64_t* agg, const uint16_t* exps, int64_t at, Run<double>& r) {
+    return read<double>(agg + 2 * at, r.p.m) & read<double>(agg + 2 * at + 1, r.h) & read_exponent(exps, at, r.p.e);
+}
+// As await; what never shows is a NaN.
+template <class A>
+__device__ __forceinline__ void await_run(const uint64_t* agg, const uint16_t* exps, int64_t at, Run<A>& r) {
+    for (int looks = kLooks; !read_run(agg, exps, at, r) && looks > 0; --looks) __builtin_amdgcn_s_sleep(1);
+}
+
+// Aggregates read at once.  Eight hide more of a wait, but cost 32-bit planes, and
+// lanes along the steps, a wave a SIMD: 1 x 65536 x 1024 bfloat16 100 us in eights,
+// 102 in fours; 64 x 2^20 float steps, derivative, 375 and 368.
+template <class T, int Dir> constexpr int kBatch = Dir == 0 && sizeof(T) == 2 ? 8 : 4;
 
 // Workgroups go to the dies in turn, each with an L2 of its own.  So tiles are
 // dealt out in windows in which a die takes some strips that lie beside each
@@ -192,9 +240,8 @@ constexpr unsigned kDies = 8, kBeside = 4, kBesideStream = 8;
 template <class T, int V, int K, int Dir, bool Sigmoid, bool Vjp, bool Packed, bool Stream>
 __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const RecArgs<T> a) {
     typedef Acc<T> A;
-    // A sigmoid gate is never 0, so only packed bounds and plain gates can cut.
-    constexpr bool Cut = !Sigmoid || Packed;
-    __shared__ A lds_p[kMost<T, Dir> * V], lds_h[kMost<T, Dir> * V], lds_c[kMost<T, Dir> * V];
+    __shared__ A lds_m[kMost<T, Dir> * V], lds_h[kMost<T, Dir> * V];
+    __shared__ int lds_e[kMost<T, Dir> * V];
     __shared__ int lds_chunk, lds_from;
     const int tid = threadIdx.x, lane = tid & 63;
     const int ncol = Dir == 0 ? 1 << a.lcol : a.ncol, nt = a.nt;
@@ -312,19 +359,22 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
         b = widen<T, V>(in[k], v);
         if constexpr (!Vjp && Sigmoid) b *= rest;
     };
-    // one step: the state after it, of the state before it
+    // one step: the state after it, of the state before it.  (A sigmoid gate that is
+    // NaN makes its step's outputs NaN by itself, so a product that takes 0 times
+    // anything as 0 is enough.)
+    auto through = [&](A g, A G) -> A { return Sigmoid ? cutmul(g, G) : g == A(0) ? A(0) : g * G; };
     auto step = [&](A g, A b, A h) -> A {
-        if constexpr (Vjp) return Cut && g == A(0) ? A(0) : g * (b + h);
-        else return Cut && g == A(0) ? b : fused(g, h, b);
+        if constexpr (Vjp) return through(g, b + h);
+        else if constexpr (Sigmoid) return cutmul(g, h) + b;
+        else return g == A(0) ? b : fused(g, h, b);
     };
-    auto join = [&](A p, A q) -> A { return Cut ? chain(p, q) : p * q; };
-    auto apply = [&](A p, A h, A add) -> A { return Cut ? add + cutmul(p, h) : fused(p, h, add); };
+    auto join = [&](const Gain<A>& p, const Gain<A>& q) -> Gain<A> { return normal(times(p, q)); };
 
-    // fold this thread's steps from a zero state; `least` tells a product that is
-    // 0 because a gate is from one too small for the type (see chain)
-    A P[V], H[V], least[V];
+    // fold this thread's steps from a zero state
+    Gain<A> P[V];
+    A H[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) { P[v] = least[v] = A(1); H[v] = A(0); }
+    for (int v = 0; v < V; ++v) { P[v] = {A(1), 0}; H[v] = A(0); }
     int q = seq_at;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -332,7 +382,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
             if (begins >> k & 1) {
                 q = moved(k, q);
 #pragma unroll
-                for (int v = 0; v < V; ++v) { P[v] = least[v] = A(0); H[v] = begin(q, v); }
+                for (int v = 0; v < V; ++v) { P[v] = {A(0), 0}; H[v] = begin(q, v); }
             }
         }
         forget(gate[k]);                  // values are widened a step at a time
@@ -342,16 +392,13 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
             A g, rest, b;
             coefficients(k, v, g, rest, b);
             H[v] = step(g, b, H[v]);
-            P[v] = Cut ? cutmul(P[v], g) : P[v] * g;
-            if constexpr (Cut) least[v] = smaller(least[v], g);
+            P[v] = times(P[v], g);
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) asm volatile("" : "+v"(P[v]), "+v"(H[v]));
+        for (int v = 0; v < V; ++v) asm volatile("" : "+v"(P[v].m), "+v"(P[v].e), "+v"(H[v]));
     }
-    if constexpr (Cut) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) P[v] = P[v] == A(0) && least[v] != A(0) ? least_normal(A(0)) : P[v];
-    }
+    for (int v = 0; v < V; ++v) P[v] = normal(P[v]);
 
     A enter[V];
 #pragma unroll
@@ -364,21 +411,13 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
         for (int d = 1; d < wt; d <<= 1) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const A p = __shfl_up(P[v], d * spacing), h = __shfl_up(H[v], d * spacing);
-                const A joined_h = apply(P[v], h, H[v]), joined_p = join(P[v], p);
+                const Gain<A> p{__shfl_up(P[v].m, d * spacing), __shfl_up(P[v].e, d * spacing)};
+                const A h = __shfl_up(H[v], d * spacing);
+                const A joined_h = passed(P[v], h, H[v]);
+                const Gain<A> joined_p = join(P[v], p);
                 H[v] = in_wave >= d ? joined_h : H[v];
-                P[v] = in_wave >= d ? joined_p : P[v];
-            }
-        }
-        A before_p[V], before_h[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            before_p[v] = A(1);
-            before_h[v] = A(0);
-            if (wt > 1) {
-                const A p = __shfl_up(P[v], spacing), h = __shfl_up(H[v], spacing);
-                before_p[v] = in_wave > 0 ? p : A(1);
-                before_h[v] = in_wave > 0 ? h : A(0);
+                P[v].m = in_wave >= d ? joined_p.m : P[v].m;
+                P[v].e = in_wave >= d ? joined_p.e : P[v].e;
             }
         }
         // Runs of a wave, in order: Dir 0, run r of a column is its threads r wt
@@ -392,20 +431,23 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
         if (Dir == 0 ? tl % wt == wt - 1 || tl == nt - 1 : lane == 63) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                lds_p[slot(run, here, v)] = P[v];
+                lds_m[slot(run, here, v)] = P[v].m;
+                lds_e[slot(run, here, v)] = P[v].e;
                 lds_h[slot(run, here, v)] = H[v];
             }
         }
         __syncthreads();
-        A earlier_p[V], earlier_h[V];
+        Gain<A> earlier_p[V];
+        A earlier_h[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) { earlier_p[v] = A(1); earlier_h[v] = A(0); }
+        for (int v = 0; v < V; ++v) { earlier_p[v] = {A(1), 0}; earlier_h[v] = A(0); }
         for (int r = first_run; r < run; ++r) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const A p = lds_p[slot(r, here, v)], h = lds_h[slot(r, here, v)];
-                earlier_h[v] = apply(p, earlier_h[v], h);
-                earlier_p[v] = join(p, earlier_p[v]);
+                const int at = slot(r, here, v);
+                const Gain<A> p{lds_m[at], lds_e[at]};
+                earlier_h[v] = passed(p, earlier_h[v], lds_h[at]);
+                earlier_p[v] = times(p, earlier_p[v]);        // at most eight runs
             }
         }
         if (a.chunks > 1) {
@@ -414,17 +456,30 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
             if (tl == nt - 1 && here < ncol) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    lds_h[here * V + v] = apply(P[v], earlier_h[v], H[v]);
-                    lds_p[here * V + v] = join(P[v], earlier_p[v]);
+                    const Gain<A> p = join(P[v], earlier_p[v]);
+                    lds_h[here * V + v] = passed(P[v], earlier_h[v], H[v]);
+                    lds_m[here * V + v] = p.m;
+                    lds_e[here * V + v] = p.e;
                 }
             }
         }
-        // what lies between the tile's first step and this thread's
+        // what lies between the tile's first step and this thread's: the runs before
+        // its own, then the threads of its own
+        auto before = [&] {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            before_h[v] = apply(before_p[v], earlier_h[v], before_h[v]);
-            before_p[v] = join(before_p[v], earlier_p[v]);
-        }
+            for (int v = 0; v < V; ++v) {
+                if (wt > 1) {
+                    const Gain<A> p{__shfl_up(P[v].m, spacing), __shfl_up(P[v].e, spacing)};
+                    const A joined_h = passed(p, earlier_h[v], __shfl_up(H[v], spacing));
+                    const Gain<A> joined_p = times(p, earlier_p[v]);
+                    earlier_h[v] = in_wave > 0 ? joined_h : earlier_h[v];
+                    earlier_p[v].m = in_wave > 0 ? joined_p.m : earlier_p[v].m;
+                    earlier_p[v].e = in_wave > 0 ? joined_p.e : earlier_p[v].e;
+                }
+                earlier_p[v] = normal(earlier_p[v]);
+            }
+        };
+        if (a.chunks <= 1) before();
         if (a.chunks > 1) {
             __syncthreads();
             typedef typename Word<A>::type W;
@@ -441,13 +496,13 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                     place(col, cs, cc, cskip);
                     if (i % V < cskip) continue;
                     const int64_t state = chunk * a.states + cs * a.chans + cc + i % V;
-                    publish<A>(a.agg + 2 * state, lds_p[i]);
-                    publish<A>(a.agg + 2 * state + 1, lds_h[i]);
+                    publish_run(a.agg, a.agg_exp, state, Run<A>{{lds_m[i], lds_e[i]}, lds_h[i]});
                     // a cut in the tile: nothing before it matters to what leaves it
-                    if (Cut && lds_p[i] == A(0)) publish<A>(a.state + state, lds_h[i]);
+                    if (lds_m[i] == A(0)) publish<A>(a.state + state, lds_h[i]);
                     else cut_all = false;
                 }
             }
+            before();                         // while the words are on their way
             // a packed sequence that begins in the tile cuts every channel, so the
             // tiles after it wait for nothing before it
             if constexpr (Packed) {
@@ -486,43 +541,37 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                 bool here_yet = true;             // asked for with the first aggregates, not before them
                 if (from >= 0) here_yet = read<A>(known, carry);
                 else carry = !Packed && a.init ? a.init[state] : A(0);
-                for (int k = from + 1; k < chunk; k += kBatch) {
-                    A p[kBatch], h[kBatch];
-                    bool ok[kBatch];
+                for (int k = from + 1; k < chunk; k += kBatch<T, Dir>) {
+                    Run<A> run_of[kBatch<T, Dir>];
+                    bool ok[kBatch<T, Dir>];
 #pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
-                        const W* word = a.agg + 2 * ((k + b < chunk ? k + b : k) * a.states + state);
-                        ok[b] = read<A>(word, p[b]) & read<A>(word + 1, h[b]);
-                    }
+                    for (int b = 0; b < kBatch<T, Dir>; ++b)
+                        ok[b] = read_run(a.agg, a.agg_exp, (k + b < chunk ? k + b : k) * a.states + state, run_of[b]);
                     if (!here_yet) {
                         carry = await<A>(known);
                         here_yet = true;
                     }
 #pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
+                    for (int b = 0; b < kBatch<T, Dir>; ++b) {
                         if (k + b >= chunk) continue;
-                        if (!ok[b]) {
-                            const W* word = a.agg + 2 * ((k + b) * a.states + state);
-                            p[b] = await<A>(word);
-                            h[b] = await<A>(word + 1);
-                        }
-                        carry = apply(p[b], carry, h[b]);
+                        if (!ok[b]) await_run<A>(a.agg, a.agg_exp, (k + b) * a.states + state, run_of[b]);
+                        carry = passed(run_of[b].p, carry, run_of[b].h);
                     }
                 }
                 if (!here_yet) carry = await<A>(known);
                 if (more) {
-                    if (!(Cut && lds_p[i] == A(0)))
-                        publish<A>(a.state + chunk * a.states + state, apply(lds_p[i], carry, lds_h[i]));
+                    if (lds_m[i] != A(0))
+                        publish<A>(a.state + chunk * a.states + state, passed({lds_m[i], lds_e[i]}, carry, lds_h[i]));
                     if (i == V - 1) raise();      // the first column's last channel, which every strip has
                 }
-                lds_c[i] = carry;
+                lds_h[i] = carry;                 // this thread's alone until the barrier
             }
             __syncthreads();
 #pragma unroll
-            for (int v = 0; v < V; ++v) enter[v] = lds_c[(here < ncol ? here : 0) * V + v];
+            for (int v = 0; v < V; ++v) enter[v] = lds_h[(here < ncol ? here : 0) * V + v];
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) enter[v] = apply(before_p[v], enter[v], before_h[v]);
+        for (int v = 0; v < V; ++v) enter[v] = passed(earlier_p[v], enter[v], earlier_h[v]);
     }
 
     // the steps again, from the state that enters them
@@ -568,7 +617,7 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
                     }
                     put<T, V>(to_gate, v, static_cast<T>(bar_gate));
                     put<T, V>(to_x, v, static_cast<T>(bar_x));
-                    enter[v] = Cut && g == A(0) ? A(0) : g * G;
+                    enter[v] = through(g, G);
                 }
                 if constexpr (Dir == 0) {
                     if (a.bar_gate.data) row_store<T, V, Stream>(out_gate, a.bar_gate.step, k, rows, skip, to_gate);
@@ -663,7 +712,7 @@ __global__ void __launch_bounds__(kShortThreads) hawk_recurrence_short(const Rec
                 sigmoid(ga, ga, rest);
                 b *= rest;
             }
-            h[v] = !Sigmoid && ga == A(0) ? b : fused(ga, h[v], b);
+            h[v] = Sigmoid ? cutmul(ga, h[v]) + b : ga == A(0) ? b : fused(ga, h[v], b);
             put<T, V>(h_now, v, static_cast<T>(h[v]));
         }
         row_store<T, V, false>(out, a.h.step, t, a.steps, skip, h_now);
@@ -812,9 +861,10 @@ Plane<T> plane_of(const hk_plane& p, int64_t steps, bool flip) {
 // A strip's counter lies on a line of its own unless there are many.
 int counter_step(const Shape& s) { return s.strips > 1024 ? 1 : 32; }
 size_t counter_bytes(const Shape& s) { return (4 * static_cast<size_t>(s.strips) * counter_step(s) + 255) / 256 * 256; }
-// (P, H) and the state of every (chunk, state), then the flags, in whole 16-byte words
+// The mantissa of P and H and the state of every (chunk, state), the flags, then P's
+// exponents, in whole 16-byte words
 size_t word_bytes(const Shape& s, size_t word) {
-    return (3 * word * static_cast<size_t>(s.states) * s.chunks + 4 * static_cast<size_t>(s.strips) * s.chunks + 15) / 16 * 16;
+    return ((3 * word + 2) * static_cast<size_t>(s.states) * s.chunks + 4 * static_cast<size_t>(s.strips) * s.chunks + 15) / 16 * 16;
 }
 
 size_t tile_bytes(const Shape& s, size_t word) { return s.chunks > 1 ? counter_bytes(s) + word_bytes(s, word) : 0; }
@@ -911,9 +961,11 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
         typedef typename Word<A>::type W;
         a.counter = static_cast<uint32_t*>(scratch);
         a.counter_step = counter_step(s);
-        a.agg = reinterpret_cast<W*>(static_cast<unsigned char*>(scratch) + counter_bytes(s));
-        a.state = a.agg + 2 * s.states * s.chunks;
-        a.flag = reinterpret_cast<uint32_t*>(a.state + s.states * s.chunks);
+        const int64_t words_each = s.states * s.chunks;
+        a.agg = reinterpret_cast<uint64_t*>(static_cast<unsigned char*>(scratch) + counter_bytes(s));
+        a.state = reinterpret_cast<W*>(a.agg) + 2 * words_each;
+        a.flag = reinterpret_cast<uint32_t*>(a.state + words_each);
+        a.agg_exp = reinterpret_cast<uint16_t*>(a.flag + s.strips * s.chunks);
         const int64_t counters = static_cast<int64_t>(counter_bytes(s) / 16);
         const int64_t words = counters + static_cast<int64_t>(word_bytes(s, sizeof(A)) / 16);
         const int64_t blocks = (words + 1023) / 1024;

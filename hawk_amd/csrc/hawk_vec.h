@@ -115,19 +115,30 @@ __device__ __forceinline__ float cutmul(float a, float b) {
 }
 __device__ __forceinline__ double cutmul(double a, double b) { return a == 0.0 || b == 0.0 ? 0.0 : a * b; }
 
-// The product of two gates' products.  It is 0 only where one of them is (a
-// cut): a product too small for the type stays the least normal number, so an
-// infinity or a NaN that enters a long run of small gates also leaves it.
-__device__ __forceinline__ float least_normal(float) { return 1.17549435e-38f; }
-__device__ __forceinline__ double least_normal(double) { return 2.2250738585072014e-308; }
+// x = mantissa(x) 2^exponent(x) with 1/2 <= |mantissa| < 1; 0, an infinity and a NaN
+// are their own mantissa, of exponent 0.
+__device__ __forceinline__ float mantissa(float x) { return __builtin_amdgcn_frexp_mantf(x); }
+__device__ __forceinline__ double mantissa(double x) { return __builtin_amdgcn_frexp_mant(x); }
+__device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }
+__device__ __forceinline__ int exponent(double x) { return __builtin_amdgcn_frexp_exp(x); }
+__device__ __forceinline__ float scaled(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+__device__ __forceinline__ double scaled(double x, int e) { return __builtin_amdgcn_ldexp(x, e); }
+
+// The product of a run of gates as m 2^e, which never leaves its range: a run of
+// gates may grow past the type's largest number, or fall below its least, and
+// still meet a state for which the result is an ordinary number.  m is 0 only
+// where a gate is (a cut), and it keeps its sign.
+template <class A> struct Gain { A m; int e; };
 template <class A>
-__device__ __forceinline__ A chain(A a, A b) {
-    const A p = cutmul(a, b);
-    return p == A(0) && a != A(0) && b != A(0) ? least_normal(A(0)) : p;
-}
-// The smaller of m and |g|; a NaN g leaves m.
-__device__ __forceinline__ float smaller(float m, float g) { return __builtin_fminf(m, __builtin_fabsf(g)); }
-__device__ __forceinline__ double smaller(double m, double g) { return __builtin_fmin(m, __builtin_fabs(g)); }
+__device__ __forceinline__ Gain<A> normal(const Gain<A>& p) { return {mantissa(p.m), p.e + exponent(p.m)}; }
+template <class A>
+__device__ __forceinline__ Gain<A> times(const Gain<A>& p, const Gain<A>& q) { return {cutmul(p.m, q.m), p.e + q.e}; }
+template <class A>
+__device__ __forceinline__ Gain<A> times(const Gain<A>& p, A g) { return times(p, Gain<A>{mantissa(g), exponent(g)}); }
+// add + p h of a normal p, the product rounded as a state of its size is; a cut
+// passes nothing.
+template <class A>
+__device__ __forceinline__ A passed(const Gain<A>& p, A h, A add) { return add + scaled(cutmul(p.m, h), p.e); }
 
 __device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
@@ -135,14 +146,15 @@ __device__ __forceinline__ double fused(double a, double b, double c) { return _
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// sigma(z) and 1 - sigma(z), each to its own relative accuracy: e = exp(-|z|)
-// never overflows and neither value is formed by a subtraction.
+// sigma(z) and 1 - sigma(z), each to its own relative accuracy: with e = exp(-z)
+// they are 1 / (1 + e) and e / (1 + e), neither formed by a subtraction.  e is held
+// at 2^125, where sigma is taken as 0 (z below -86.6): what is lost there and just
+// above it is 2^-125 in absolute terms.  A NaN z makes both values NaN.
 __device__ __forceinline__ void sigmoid(float z, float& a, float& rest) {
-    const float e = __builtin_amdgcn_exp2f(-kLog2e * __builtin_fabsf(z));
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(-kLog2e * z, 125.0f));
     const float r = __builtin_amdgcn_rcpf(1.0f + e);
-    const float small = e * r;
-    a = z >= 0.0f ? r : small;           // a NaN z makes both values NaN
-    rest = z >= 0.0f ? small : r;
+    rest = e * r;
+    a = r - 0x1p-125f;
 }
 __device__ __forceinline__ void sigmoid(double z, double& a, double& rest) {
     const double e = exp(-fabs(z));

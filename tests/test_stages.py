@@ -283,6 +283,123 @@ def test_a_gate_of_zero_and_a_sequences_start_cut_infinities_and_nan(gpu):
         assert torch.isnan(h[0, 5:]).all() and (h[0, :5] == 0).all()
 
 
+def far_gates(T, dtype, sign, seed):
+    """Gates that grow for a while and shrink for as long, (T, 1): a run's product passes the type's largest number,
+    or its least, while a state that starts low stays an ordinary number.  With the number it starts from."""
+    octaves, every = (1600, 1) if dtype == "float64" else (200, 1 if T < 3000 else 8)
+    t = np.arange(T)
+    gate = np.where(t % every == 0, np.where(t // (octaves * every) % 2 == 0, 2.0, 0.5), 1.0)
+    if sign:
+        gate = gate * np.where(np.random.default_rng(seed).random(T) < 0.5, -1, 1)
+    return gate[:, None], 2.0 ** (-octaves / 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["channels", "steps", "sliced", "packed"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float64"])
+@pytest.mark.parametrize("T,C", [(190, 16), (700, 40), (3500, 3), (9001, 8), (12001, 1)], ids=str)
+def test_gates_whose_product_leaves_the_types_range(gpu, T, C, dtype, layout):
+    """The states are ordinary numbers throughout, so the bounds are those of any recurrence."""
+    import torch
+    packed = layout == "packed"
+    for k, (sign, reverse) in enumerate([(False, False), (True, True), (True, False)]):
+        print(T, C, dtype, layout, sign, reverse, flush=True)
+        got, held, offsets = recurrence_case(1 if not packed else 2, T, C, dtype, "value", reverse,
+                                             "channels" if packed else layout, True, packed, gpu, seed=60 + k)
+        low = far_gates(T, dtype, sign, k)[1]
+        gate = np.tile(far_gates(T, dtype, sign, k)[0], (1, C))
+        if packed:                                             # both sequences start where the gates grow
+            offsets = np.array([0, T - 150, T])
+            gate = np.concatenate([gate[:T - 150], gate[:150]])
+            more = gate[T - 150:]
+            gate = np.concatenate([gate[:T - 150][::-1], more[::-1]]) if reverse else gate
+        elif reverse:
+            gate = gate[::-1]
+        g, held["gate"] = plane(np.ascontiguousarray(gate if packed else gate[None]), dtype, gpu)
+        got["gate"].copy_(g)
+        for n in ("x", "h0"):
+            t, held[n] = plane(held[n] * low, dtype if n == "x" else "float64" if dtype == "float64" else "float32", gpu)
+            got[n].copy_(t)
+        planes = {n: got[n] for n in ("gate", "x", "h0")}
+        if packed:
+            planes["offsets"] = torch.from_numpy(offsets).to(gpu)
+        stage = hawk.stages.recurrence(reverse=reverse)
+        h, last = torch.empty_like(got["x"]), torch.empty_like(got["h0"])
+        hawk.run(stage, h=h, last=last, **planes)
+        want, want_last, size = oracle_forward(held["gate"], held["x"], held["h0"], offsets, "value", reverse)
+        close(back(h), want, size, T, "value", dtype)
+        ends = np.array([np.abs(size[rows if packed else (0, rows)]).max(0) for _, rows in spans(1, T, offsets)])
+        close(back(last), want_last, ends, T, "value", dtype, state=True)
+        # the derivative: adjoints that start low where the gates grow in its direction
+        stage = hawk.stages.recurrence(reverse=not reverse)
+        bars = {n: torch.empty_like(got["x"]) for n in ("bar_gate", "bar_x")}
+        bars["bar_h0"] = torch.empty_like(got["h0"])
+        saved, held_h = plane(np.random.default_rng(k).normal(size=held["x"].shape), dtype, gpu)
+        hawk.run(stage.vjp, gate=got["gate"], h=saved, bar_h=got["x"], bar_last=got["h0"], h0=torch.ones_like(last),
+                 **{n: planes[n] for n in ("offsets",) if packed}, **bars)
+        wants, sizes = oracle_vjp(held["gate"], None, held_h, np.ones_like(held["h0"]), held["x"], held["h0"], offsets,
+                                  "value", not reverse)
+        for n, w, z in zip(("bar_gate", "bar_x", "bar_h0"), wants, sizes):
+            close(back(bars[n]), w, z, T, "value", dtype, state=n == "bar_h0")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,C,layout", [(200, 16, "channels"), (300, 1, "steps"), (9000, 8, "channels"), (9000, 2, "steps")],
+                         ids=str)
+def test_large_and_infinite_states_through_many_small_gates(gpu, T, C, layout):
+    import torch
+
+    def put(x):
+        return x.transpose(1, 2).contiguous().transpose(1, 2) if layout == "steps" else x
+    zero, h = put(torch.zeros(1, T, C, device=gpu)), put(torch.empty(1, T, C, device=gpu))
+    sign = torch.where(torch.arange(T, device=gpu) % 2 == 0, -1.0, 1.0)[None, :, None].expand(1, T, C)
+    steps = torch.arange(1, T + 1, device=gpu, dtype=torch.float64)[None, :, None]
+    for stage, gate in ((hawk.stages.recurrence(), torch.full_like(zero, -0.5)),
+                        (hawk.stages.recurrence("sigmoid"), torch.zeros_like(zero))):
+        alternating = stage.gate == "value"
+        # halved exactly while it is a normal number, gone below the least: no floor that a product is held at
+        hawk.run(stage, gate=put(gate), x=zero, h=h, h0=torch.full((1, C), 1e35, device=gpu))
+        want = float(torch.tensor(1e35)) * 0.5 ** steps * (sign if alternating else 1.0)
+        u = 2.0 ** -24 * (4 if alternating else 28 * T)
+        assert ((h.double() - want).abs() <= u * want.abs() + 2.0 ** -149).all()
+        # an infinity stays one, of the sign that the gates give it
+        hawk.run(stage, gate=put(gate), x=zero, h=h, h0=torch.full((1, C), math.inf, device=gpu))
+        assert torch.equal(h, put(torch.full_like(zero, math.inf) * (sign if alternating else 1.0)))
+        bar = put(torch.empty_like(zero))
+        hawk.run(stage.vjp, gate=put(gate), x=zero, h=put(torch.ones_like(zero)), bar_h=zero, bar_x=bar,
+                 bar_last=torch.full((1, C), math.inf, device=gpu))
+        assert torch.isinf(bar).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,C", [(1, 16), (8, 5), (40, 16), (9000, 8)], ids=str)
+def test_a_sigmoid_gate_below_the_least_number_cuts_in_every_form(gpu, T, C):
+    """sigma(-100) is no float32 of full precision and sigma(-inf) is 0: neither lets the state pass, dense or packed."""
+    import torch
+    x = torch.randn(1, T, C, device=gpu)
+    gate = torch.randn(1, T, C, device=gpu)
+    h0 = torch.full((1, C), math.inf, device=gpu)
+    stage, offsets = hawk.stages.recurrence("sigmoid"), torch.tensor([0, T], device=gpu)
+    for low in (-100.0, -math.inf):
+        for at in sorted({0, T // 2, T - 1}):
+            z = gate.clone()
+            z[0, at] = low
+            h, p = torch.empty_like(x), torch.empty(T, C, device=gpu)
+            hawk.run(stage, gate=z, x=x, h=h, h0=h0)
+            hawk.run(stage, gate=z[0], x=x[0], h=p, h0=h0, offsets=offsets)
+            for got in (h, p[None]):
+                assert torch.isinf(got[0, :at]).all()
+                want, _, size = oracle_forward(back(z[:, at:]), back(x[:, at:]), None, None, "sigmoid", False)
+                close(back(got[:, at:]), want, size, T - at, "sigmoid", "float32")
+            # the adjoint that would pass the cut, in both forms
+            bars = [torch.empty_like(x), torch.empty(T, C, device=gpu)]
+            hawk.run(stage.vjp, gate=z, x=x, h=h.nan_to_num(posinf=0, neginf=0), bar_h=torch.zeros_like(x), bar_last=h0, bar_x=bars[0])
+            hawk.run(stage.vjp, gate=z[0], x=x[0], h=p.nan_to_num(posinf=0, neginf=0), bar_h=torch.zeros(T, C, device=gpu), bar_last=h0,
+                     bar_x=bars[1], offsets=offsets)
+            for got in (bars[0][0], bars[1]):
+                assert torch.isinf(got[at:]).all() and (got[:at] == 0).all()
+
+
 @pytest.mark.gpu
 def test_one_token_at_a_time_is_the_whole_sequence(gpu):
     import torch
