@@ -98,11 +98,11 @@ __device__ __forceinline__ void policy_row(const RowArgs<T>& a, const PolicyRow&
     if (p.w == 0.0f) return;
     const float r = expf(logp - p.old);
     const float plain = r * p.A, clipped = fminf(fmaxf(r, a.low), a.high) * p.A;
-    // a NaN ratio stays one: fminf and fmaxf would drop it
-    if (!(r == r)) { loss = slope = r; return; }
+    // a NaN is the minimum (a NaN ratio or advantage, or an infinite one times 0):
+    // fminf, fmaxf and the comparison would drop it
+    if (!(plain == plain)) { loss = slope = plain; return; }
     loss = plain <= clipped ? -plain : -clipped;
     slope = plain <= clipped ? -plain : 0.0f;
-    if (!(p.A == p.A)) loss = slope = p.A;
     if (a.kl != 0.0f) {
         const float d = p.ref - logp;
         loss += a.kl * (expm1f(d) - d);

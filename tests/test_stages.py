@@ -1054,6 +1054,26 @@ def test_few_long_rows_over_several_workgroups(gpu, shape, dtype):
     assert torch.equal(logits, both)
 
 
+@pytest.mark.gpu
+def test_a_ratio_past_the_largest_number_is_the_minimums(gpu):
+    """r = inf: -min(r A, clamp(r) A) is bounded for A > 0, an infinity for A < 0 and, like inf * 0, a NaN for A = 0."""
+    import torch
+    logits, target = torch.zeros(4, 9, device=gpu), torch.arange(4, device=gpu)
+    A = torch.tensor([1.0, -1.0, 0.0, 0.5], device=gpu)
+    old = torch.tensor([-200.0, -200.0, -200.0, -2.0], device=gpu)
+    stage, loss, bar = hawk.stages.policy_loss(clip=0.2), torch.empty(1, device=gpu), torch.empty_like(logits)
+    for n, want in enumerate((-1.2, math.inf, math.nan, None)):
+        weight = torch.zeros(4, device=gpu)
+        weight[n] = 1.0
+        hawk.run(stage, logits=logits, target=target, old_logp=old, advantage=A, weight=weight, loss=loss, bar_logits=bar)
+        if want is None:
+            assert math.isfinite(float(loss)) and torch.isfinite(bar).all()
+        else:
+            assert float(loss) == pytest.approx(want, rel=1e-6, nan_ok=True)
+            assert torch.isnan(bar[n]).all() if math.isnan(want) else not math.isfinite(want) or (bar[n] == 0).all()
+        assert (bar[torch.arange(4) != n] == 0).all()
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
