@@ -104,9 +104,10 @@ __device__ __forceinline__ void policy_row(const RowArgs<T>& a, const PolicyRow&
     loss = plain <= clipped ? -plain : -clipped;
     slope = plain <= clipped ? -plain : 0.0f;
     if (a.kl != 0.0f) {
-        const float d = p.ref - logp;
-        loss += a.kl * (expm1f(d) - d);
-        slope -= a.kl * expm1f(d);
+        // e^d - 1 is an infinity before d is: a target without probability has both
+        const float d = p.ref - logp, grown = expm1f(d);
+        loss += a.kl * (grown == INFINITY ? grown : grown - d);
+        slope -= a.kl * grown;
     }
     loss *= p.w;
     slope *= a.bar_loss ? p.w * *a.bar_loss : p.w;

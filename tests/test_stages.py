@@ -1074,6 +1074,25 @@ def test_a_ratio_past_the_largest_number_is_the_minimums(gpu):
         assert (bar[torch.arange(4) != n] == 0).all()
 
 
+@pytest.mark.gpu
+def test_the_kl_term_of_a_target_without_probability_is_infinite(gpu):
+    import torch
+    logits, target = torch.randn(3, 50, device=gpu), torch.tensor([1, 2, 3], device=gpu)
+    logits[1, 2] = -math.inf
+    planes = dict(logits=logits, target=target, old_logp=torch.full((3,), -4.0, device=gpu),
+                  ref_logp=torch.full((3,), -4.0, device=gpu), advantage=torch.ones(3, device=gpu))
+    loss = torch.empty(1, device=gpu)
+    hawk.run(hawk.stages.policy_loss(kl=0.1), loss=loss, **planes)
+    assert float(loss) == math.inf
+    hawk.run(hawk.stages.policy_loss(), loss=loss, **{n: x for n, x in planes.items() if n != "ref_logp"})
+    assert math.isfinite(float(loss))
+    # a step of the policy that e^d overflows for
+    planes["ref_logp"][1] = 0.0
+    logits[1, 2] = -200.0
+    hawk.run(hawk.stages.policy_loss(kl=0.1), loss=loss, **planes)
+    assert float(loss) == math.inf
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
