@@ -115,8 +115,11 @@ __device__ __forceinline__ void policy_row(const RowArgs<T>& a, const PolicyRow&
 
 // A run of a row: its largest logit m and the sum s of 2^((x - m) k).  The
 // difference comes before the product, so a row of the type's lowest value is a
-// row of equal logits.  m = -inf with s = 0 where no logit is above -inf.
-__device__ __forceinline__ float floor_of(float m) { return m == -INFINITY ? 0.0f : m; }
+// row of equal logits.  m = -inf with s = 0 where no logit is above -inf, and
+// m = s = inf where one is +inf.  What is subtracted is always a number, so that
+// inf - inf comes up only for a target that is +inf itself.
+constexpr float kLargest = 3.40282347e+38f;
+__device__ __forceinline__ float floor_of(float m) { return m == -INFINITY ? 0.0f : fminf(m, kLargest); }
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, float k) {
     const float top = fmaxf(m, m2), base = floor_of(top);
     s = s * exp2_fast((m - base) * k) + s2 * exp2_fast((m2 - base) * k);

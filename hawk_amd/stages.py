@@ -502,7 +502,8 @@ def token_logp(scale: float = 1.0) -> Stage:
     a row contiguous, rows any distance apart; ``target`` int32 or int64;
     ``logp`` and ``lse`` (the row's log-sum-exp) float32, those given are
     written.  A target below 0 leaves its row out (``logp`` and ``lse`` 0, the
-    logits not read); one past the vocabulary gives a NaN.
+    logits not read); one past the vocabulary gives a NaN.  A logit of +inf makes
+    ``lse`` +inf: the other logits have probability 0, its own is a NaN.
 
     ``.vjp`` reads ``logits``, ``target``, ``lse``, ``bar_logp`` and writes
     ``bar_logits`` (it may be ``logits``)."""

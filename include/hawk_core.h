@@ -420,7 +420,8 @@ int hk_recurrence_vjp(const hk_recurrence_job* job, void* scratch, void* stream)
  *   lse_n = log sum_v exp(l[n, v]),  logp_n = l[n, target_n] - lse_n.
  * A row whose target is below 0 is left out: its logits are not read, its logp,
  * lse and loss are 0 and its gradient is 0.  A target of vocab or more gives a
- * NaN.  Every other plane is float.  bar_logits is [rows, vocab] of dtype,
+ * NaN.  A logit of +inf makes lse +inf: every other logit has probability 0, its
+ * own is a NaN.  Every other plane is float.  bar_logits is [rows, vocab] of dtype,
  * bar_stride elements a row, and may be logits itself.
  *
  * hk_token_logp writes logp and lse (either may be NULL).

@@ -1093,6 +1093,39 @@ def test_the_kl_term_of_a_target_without_probability_is_infinite(gpu):
     assert float(loss) == math.inf
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ROW_TYPES)
+@pytest.mark.parametrize("V", [5, 300, 3000, 9000, 70000, 200003])
+def test_an_infinite_logit_is_the_rows_sum(gpu, V, dtype):
+    """lse = +inf: every other logit has probability 0 and log-probability -inf, its own is inf - inf."""
+    import torch
+    for N in (6, 600) if V <= 9000 else (6,):
+        logits = torch.randn(N, V, device=gpu).to(torch_type(dtype))
+        target = torch.full((N,), 2, device=gpu)
+        logits[0, V - 1] = math.inf                        # another element's
+        logits[1, 2] = math.inf                            # the target's own
+        logits[2, 1], logits[2, 0] = math.inf, math.nan    # a NaN beside it
+        logits[3] = math.inf
+        logits[4, V - 1] = math.inf
+        logits[4, 2] = -math.inf
+        stage = hawk.stages.token_logp()
+        logp, lse, bar = torch.empty(N, device=gpu), torch.empty(N, device=gpu), torch.empty_like(logits)
+        hawk.run(stage, logits=logits, target=target, logp=logp, lse=lse)
+        assert (lse[[0, 1, 3, 4]] == math.inf).all() and torch.isnan(lse[2])
+        assert (logp[[0, 4]] == -math.inf).all() and torch.isnan(logp[[1, 2, 3]]).all()
+        assert torch.isfinite(lse[5:]).all() and torch.isfinite(logp[5:]).all()
+        hawk.run(stage.vjp, logits=logits, target=target, lse=lse, bar_logp=torch.ones(N, device=gpu), bar_logits=bar)
+        assert bar[0, 2] == 1 and (bar[0, 3:V - 1] == 0).all() and (bar[0, :2] == 0).all() and torch.isnan(bar[0, V - 1])
+        assert torch.isnan(bar[2]).all() and torch.isnan(bar[3]).all()
+        # the same sum in the other rows' kernels
+        both, again = torch.empty_like(logits), torch.empty(N, device=gpu)
+        hawk.run(hawk.stages.policy_loss(), logits=logits, target=target, old_logp=logp.nan_to_num(0.0, 0.0, 0.0),
+                 advantage=torch.ones(N, device=gpu), lse=again, bar_logits=both)
+        assert torch.equal(again.nan_to_num(-1.0), lse.nan_to_num(-1.0)) or (again - lse)[5:].abs().max() < 1e-4
+        assert (again[[0, 1, 3, 4]] == math.inf).all() and torch.isnan(again[2])
+        assert torch.isfinite(both[5:]).all() and (both[0] == 0).all()
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
