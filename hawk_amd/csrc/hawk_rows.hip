@@ -602,7 +602,9 @@ __global__ void __launch_bounds__(kPairThreads) hawk_pair_loss(const PairArgs a,
         // -log sigma(z) and -log sigma(-z) = z - log sigma(z), neither overflowing
         const double soft = log1p(exp(-fabs(z)));
         const double lose = soft + (z < 0.0 ? -z : 0.0), win = soft + (z > 0.0 ? z : 0.0);
-        const double loss = (z == z) ? (1.0 - a.smoothing) * lose + a.smoothing * win : z;
+        // a side of weight 0 costs nothing, be it infinite
+        const double one = a.smoothing < 1.0f ? (1.0 - a.smoothing) * lose : 0.0, other = a.smoothing > 0.0f ? a.smoothing * win : 0.0;
+        const double loss = (z == z) ? one + other : z;
         const float weighted = w == 0.0f ? 0.0f : static_cast<float>(w * loss);
         sum += static_cast<double>(weighted);
         if (lane == 0) {

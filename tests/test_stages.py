@@ -1126,6 +1126,30 @@ def test_an_infinite_logit_is_the_rows_sum(gpu, V, dtype):
         assert torch.isfinite(both[5:]).all() and (both[0] == 0).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairs", [1, 128, 129, 400])
+def test_an_infinite_margin_costs_what_its_side_of_the_loss_says(gpu, pairs):
+    """A sequence with a masked target has log-probability -inf.  Against it the preferred one's loss is 0, whatever the
+    weight 0 of the smoothing's other side; with smoothing it is infinite."""
+    import torch
+    logits = torch.zeros(2 * pairs, 8, device=gpu)
+    target = torch.zeros(2 * pairs, dtype=torch.int64, device=gpu)
+    planes = dict(logits=logits, target=target, offsets=torch.arange(2 * pairs + 1, device=gpu))
+    loss, margin, lse = torch.empty(1, device=gpu), torch.empty(pairs, device=gpu), torch.empty(2 * pairs, device=gpu)
+    rest = math.log(2) * (pairs - 1) / pairs               # every other margin is 0
+    for row, side, want in ((1, math.inf, {0.0: rest, 0.25: math.inf, 1.0: math.inf}),
+                            (0, -math.inf, {0.0: math.inf, 0.25: math.inf, 1.0: rest})):
+        logits.zero_()
+        logits[row, 0] = -math.inf
+        for smoothing, value in want.items():
+            stage, bar = hawk.stages.preference_loss(beta=0.5, smoothing=smoothing), torch.empty_like(logits)
+            hawk.run(stage, loss=loss, margin=margin, lse=lse, **planes)
+            assert float(margin[0]) == side and (margin[1:] == 0).all()
+            assert float(loss) == pytest.approx(value, rel=1e-6, abs=1e-7)
+            hawk.run(stage.vjp, margin=margin, lse=lse, bar_logits=bar, **planes)
+            assert torch.isfinite(bar).all()
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
