@@ -538,7 +538,9 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradie
             float loss;
             policy_row(a, policy_planes(a, n, true), a.logp[n], loss, c);
         }
-        c = (y < a.vocab ? c : NAN) * a.scale;
+        // past the vocabulary, unless its weight leaves the row out
+        if (y >= a.vocab && (W == kGradient || c != 0.0f)) c = NAN;
+        c *= a.scale;
     }
     // A row without a gradient is not read, unless to know it takes longer than to
     // ask for the row's first vectors (a search for its pair).

@@ -1150,6 +1150,41 @@ def test_an_infinite_margin_costs_what_its_side_of_the_loss_says(gpu, pairs):
             assert torch.isfinite(bar).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [7, 3000, 20000])
+def test_a_weight_of_zero_leaves_a_row_out_whatever_its_target(gpu, V):
+    """A target past the vocabulary is a NaN, in a row or pair of weight 0 nothing: in every form of the gradient."""
+    import torch
+    logits = torch.randn(6, V, device=gpu)
+    target = torch.tensor([1, V, 2, V + 5, 0, 3], device=gpu)
+    old = torch.full((6,), -5.0, device=gpu)
+    for weight, loud in (([1.0, 0.0, 1.0, 0.0, 1.0, 1.0], ()), ([1.0, 0.5, 1.0, 0.0, 1.0, 1.0], (1,))):
+        stage = hawk.stages.policy_loss()
+        planes = dict(logits=logits, target=target, old_logp=old, advantage=torch.ones(6, device=gpu),
+                      weight=torch.tensor(weight, device=gpu))
+        loss, logp, lse = (torch.empty(k, device=gpu) for k in (1, 6, 6))
+        one, two = torch.empty_like(logits), torch.empty_like(logits)
+        hawk.run(stage, loss=loss, logp=logp, lse=lse, bar_logits=one, **planes)
+        hawk.run(stage.vjp, logp=logp, lse=lse, bar_logits=two, **planes)
+        for bar in (one, two):
+            for n in range(6):
+                if n in loud:
+                    assert torch.isnan(bar[n]).all()
+                else:
+                    assert torch.isfinite(bar[n]).all() and (n not in (1, 3) or (bar[n] == 0).all())
+        assert math.isnan(float(loss)) == bool(loud)
+    pair, bar = hawk.stages.preference_loss(), torch.empty_like(logits)
+    planes = dict(logits=logits, target=target, offsets=torch.arange(7, device=gpu))
+    margin, lse = torch.empty(3, device=gpu), torch.empty(6, device=gpu)
+    for weight, loud in (([0.0, 0.0, 1.0], ()), ([0.0, 1.0, 1.0], (2, 3))):
+        planes["weight"] = torch.tensor(weight, device=gpu)
+        hawk.run(pair, margin=margin, lse=lse, loss=loss, **planes)
+        assert math.isnan(float(loss)) == bool(loud)
+        hawk.run(pair.vjp, margin=margin, lse=lse, bar_logits=bar, **planes)
+        for n in range(6):
+            assert torch.isnan(bar[n]).all() if n in loud else torch.isfinite(bar[n]).all()
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
