@@ -179,7 +179,7 @@ int dropout(const hk_dropout_job& j, hipStream_t stream) {
     const int64_t groups = vectors ? (n + kNumbers - 1) / kNumbers : j.rows * ((j.cols + kNumbers - 1) / kNumbers);
     const int64_t per = vectors ? kThreads * kSets : kThreads;
     const int64_t blocks = (groups + per - 1) / per;
-    if (blocks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, "hk_dropout: the planes exceed the grid limit");
+    if (blocks > UINT32_MAX / kThreads) return hawk_internal::set_error(HK_EVALUE, "hk_dropout: the planes exceed the grid limit");
     const DropArgs a{j.offset_cell, j.seed, j.offset, j.rows, j.cols, j.x_stride, j.residual_stride, j.y_stride,
                      static_cast<uint32_t>(j.cut)};
     const Acc<T> factor = j.cut < 65536 ? Acc<T>(65536) / Acc<T>(65536 - j.cut) : Acc<T>(0);

@@ -920,7 +920,7 @@ int recurrence(const hk_recurrence_job& j, void* scratch, hipStream_t stream, co
         return launched("hawk_recurrence_pass launch");
     }
     const Shape s = shape_of<T, Vjp>(j);
-    if (s.strips * s.chunks > INT32_MAX) return hawk_internal::set_error(HK_EVALUE, who + ": the planes exceed the grid limit");
+    if (s.strips * s.chunks > UINT32_MAX / s.threads) return hawk_internal::set_error(HK_EVALUE, who + ": the planes exceed the grid limit");
     const int64_t entering = j.seqs * j.chans;
     const bool copy = may_copy<Vjp>(j, s) && init < fin + entering && fin < init + entering;
     if ((s.chunks > 1 || copy) && !scratch) return hawk_internal::set_error(HK_EVALUE, who + ": scratch is required");

@@ -60,6 +60,7 @@ struct RowArgs {
     int64_t rows, vocab, row_stride, bar_stride;
     float scale, low, high, kl, even;   // low, high: the ratio's bounds; even: the weight where weight is NULL
     int64_t each;             // vectors of a row that a workgroup takes, where rows are split
+    int64_t first;            // the launch's first row
     int target64;
     PairArgs pairs;           // the preference loss's gradient
 };
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kThreads) hawk_row_parts(const RowArgs<T> a, i
 template <class T, int L, Work W>
 __global__ void __launch_bounds__(L) hawk_row_long(const RowArgs<T> a) {
     constexpr int V = kVec<T>;
-    const int64_t n = blockIdx.x;
+    const int64_t n = a.first + blockIdx.x;
     const int lane = threadIdx.x;
     const float k = a.scale * kLog2e;
     const T* row = a.logits + n * a.row_stride;
@@ -513,7 +514,7 @@ template <class T, int L, Work W>
 __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_gradient(const RowArgs<T> a) {
     constexpr int V = kVec<T>, R = kThreads / L;
     constexpr bool Stream = L >= 256;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / L;
+    const int64_t n = a.first + static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / L;
     const int lane = threadIdx.x % L;
     if (n >= a.rows) return;
     const int64_t y = target_of(a.target, a.target64, n);
@@ -683,6 +684,18 @@ void launch_held(const RowArgs<T>& a, hipStream_t s) {
 
 template <int N> using Count = std::integral_constant<int, N>;
 
+// A launch has fewer than 2^32 threads along an axis of its grid.  Rows of a
+// workgroup each, or R to one, go in launches of at most that many: calls
+// launch(blocks, first row).
+template <class Launch>
+void each_launch(int64_t rows, int64_t R, int threads, Launch&& launch) {
+    const int64_t most = UINT32_MAX / threads * R;
+    for (int64_t first = 0; first < rows; first += most) {
+        const int64_t here = rows - first < most ? rows - first : most;
+        launch(static_cast<unsigned>((here + R - 1) / R), first);
+    }
+}
+
 // A row's vectors, the most that its lead can make them.
 template <class T>
 int64_t vectors_of(const RowArgs<T>& a) {
@@ -727,8 +740,10 @@ int rows_of(RowArgs<T> a, hipStream_t s) {
             constexpr int L = decltype(lanes)::value, R = kThreads / L;
             const int64_t most = vectors / (kAhead * kThreads), parts = L < kThreads || most < 1 ? 1 : most < 65535 ? most : 65535;
             a.each = (vectors + parts - 1) / parts;
-            hipLaunchKernelGGL((hawk_row_gradient<T, L, W>),
-                               dim3(static_cast<unsigned>((a.rows + R - 1) / R), static_cast<unsigned>(parts)), dim3(kThreads), 0, s, a);
+            each_launch(a.rows, R, kThreads, [&](unsigned blocks, int64_t first) {
+                a.first = first;
+                hipLaunchKernelGGL((hawk_row_gradient<T, L, W>), dim3(blocks, static_cast<unsigned>(parts)), dim3(kThreads), 0, s, a);
+            });
         };
         if (vectors <= 32) go(Count<16>{});
         else if (vectors <= 256) go(Count<64>{});
@@ -763,7 +778,10 @@ int rows_of(RowArgs<T> a, hipStream_t s) {
         } else if (few) {
             hipLaunchKernelGGL((hawk_row_long<T, 1024, W>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
         } else {
-            hipLaunchKernelGGL((hawk_row_long<T, 256, W>), dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, s, a);
+            each_launch(a.rows, 1, 256, [&](unsigned blocks, int64_t first) {
+                a.first = first;
+                hipLaunchKernelGGL((hawk_row_long<T, 256, W>), dim3(blocks), dim3(256), 0, s, a);
+            });
         }
     }
     return launched("row kernel launch");
@@ -941,8 +959,9 @@ int hk_preference_loss(const hk_row_loss_job* job, void* scratch, void* stream) 
             hipLaunchKernelGGL(hawk_pair_loss<true>, dim3(1), dim3(kPairThreads), 0, s, p, job->loss);
             return launched("hawk_pair_loss launch");
         }
-        hipLaunchKernelGGL(hawk_pair_loss<false>, dim3(static_cast<unsigned>((job->pairs + kPairWaves - 1) / kPairWaves)),
-                           dim3(kPairThreads), 0, s, p, nullptr);
+        const int64_t blocks = (job->pairs + kPairWaves - 1) / kPairWaves, most = UINT32_MAX / kPairThreads;
+        hipLaunchKernelGGL(hawk_pair_loss<false>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(kPairThreads), 0, s,
+                           p, nullptr);
         rc = launched("hawk_pair_loss launch");
         if (rc != HK_OK) return rc;
     }

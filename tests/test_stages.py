@@ -1185,6 +1185,36 @@ def test_a_weight_of_zero_leaves_a_row_out_whatever_its_target(gpu, V):
             assert torch.isnan(bar[n]).all() if n in loud else torch.isfinite(bar[n]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V", [((1 << 28) + 3, 2), ((1 << 26) + 5, 280)], ids=str)
+def test_more_rows_than_one_launch_has_threads_for(gpu, N, V):
+    """A launch has fewer than 2^32 threads along its grid: 2^28 rows of 16 lanes each, 2^26 of 64, are past that."""
+    import torch
+    block = torch.randn(1 << 16, V, device=gpu).bfloat16()
+    logits = torch.empty(N, V, dtype=torch.bfloat16, device=gpu)
+    for first in range(0, N, len(block)):
+        part = logits[first:first + len(block)]
+        part.copy_(block[:len(part)])
+    target = torch.zeros(N, dtype=torch.int32, device=gpu)
+    target[1::2] = 1
+    logp, lse = torch.empty(N, device=gpu), torch.empty(N, device=gpu)
+    stage = hawk.stages.token_logp()
+    hawk.run(stage, logits=logits, target=target, logp=logp, lse=lse)
+    want = torch.log_softmax(block.double(), 1)
+    at = torch.arange(len(block), device=gpu) % 2
+    for first in (0, N - N % len(block) - len(block), N // 2 // len(block) * len(block)):
+        rows = slice(first, first + len(block))
+        assert (logp[rows].double() - want[torch.arange(len(block), device=gpu), at]).abs().max() < 1e-5
+    tail = N % len(block)
+    assert (logp[N - tail:].double() - want[torch.arange(tail, device=gpu), at[:tail]]).abs().max() < 1e-5
+    hawk.run(stage.vjp, logits=logits, target=target, lse=lse, bar_logp=torch.ones(N, device=gpu), bar_logits=logits)
+    grad = -want.exp()
+    grad[torch.arange(len(block), device=gpu), at] += 1
+    for first in list(range(0, N - len(block), len(block) * 331)) + [N - tail - len(block)]:
+        assert (logits[first:first + len(block)].double() - grad).abs().max() < 2.0 ** -8
+    assert (logits[N - tail:].double() - grad[:tail]).abs().max() < 2.0 ** -8
+
+
 # -- dropout ---------------------------------------------------------------------------------
 
 def philox(group, offset, seed):
@@ -1454,6 +1484,23 @@ def test_the_entries_refuse_bad_jobs():
     assert L.hk_recurrence(ctypes.byref(r), None, None) == 0
     w.dtype, w.rows = 0, 0
     assert L.hk_token_logp(ctypes.byref(w), None, None) == 0
+
+
+def test_planes_past_the_grids_threads_are_refused_before_the_launch():
+    """Dropout and the recurrence cut their launches no finer: what does not fit one is told by the entry."""
+    L = _core.lib()
+    d = _core.DropoutJob()
+    d.rows, d.cols, d.cut, d.dtype = 1, 1 << 37, 5, 2
+    d.x = d.y = 16
+    assert L.hk_dropout(ctypes.byref(d), None) == 1 and b"grid limit" in L.hk_last_error()
+    d.rows, d.cols = 1 << 34, 9
+    assert L.hk_dropout(ctypes.byref(d), None) == 1 and b"grid limit" in L.hk_last_error()
+    r = _core.RecurrenceJob()
+    r.seqs, r.steps, r.chans, r.dtype = 1 << 29, 1 << 10, 1, 2
+    for n in ("gate", "x", "h"):
+        plane = getattr(r, n)
+        plane.data, plane.seq, plane.step, plane.chan = 16, 2 << 10, 2, 3
+    assert L.hk_recurrence(ctypes.byref(r), 16, None) == 1 and b"grid limit" in L.hk_last_error()
 
 
 def test_the_jobs_are_laid_out_as_the_header_has_them():
