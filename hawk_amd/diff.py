@@ -631,7 +631,10 @@ class _Forward:
 def jvp(kernel, wrt=None) -> Program:
     """The forward-mode derivative: a program reading the primal inputs and a
     tangent plane ``dot_<x>`` per input of ``wrt``, and writing ``dot_<y>``
-    for each per-sample sink ``y``."""
+    for each per-sample sink ``y``.  A stage (:mod:`hawk_amd.stages`) has none."""
+    from .runtime import Stage
+    if isinstance(kernel, Stage):
+        raise HawkError(f"{kernel.name}: a stage has no forward-mode derivative (hawk.diff.vjp gives its reverse)")
     program = _program_of(kernel)
     _refuse_prior_reads(program, "jvp")
     _refuse_extremes(program, "jvp")

@@ -17,6 +17,9 @@ a stage whose planes are the primal's with ``bar_`` names for adjoints::
     hawk.run(scan, gate=z, x=x, h=h)
     hawk.run(scan.vjp, gate=z, x=x, h=h, bar_h=bar_h, bar_gate=bar_z, bar_x=bar_x)
 
+A stage is no traced kernel: it has no ``hawk.diff.jvp`` and is no member of a
+``hawk.chain`` or ``hawk.steps``; it takes the planes that kernels write and read.
+
 Planes are PyTorch-ROCm tensors, bound by address.  Scratch belongs to a stream,
 or to the graph a call is captured in: calls on several streams and replays of
 several graphs may run at once (a launcher's own run one after another).  Nothing

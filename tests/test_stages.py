@@ -1397,6 +1397,16 @@ def test_names_missing_planes_and_launch_options_are_refused():
         diff.vjp(scan.vjp)
 
 
+def test_a_stage_is_no_traced_kernel():
+    for stage in (hawk.stages.recurrence(), hawk.stages.policy_loss().vjp, hawk.stages.dropout(0.5)):
+        with pytest.raises(HawkError, match=f"{stage.name}: a stage has no forward-mode derivative"):
+            diff.jvp(stage)
+        with pytest.raises(HawkError, match="not a traced kernel"):
+            hawk.chain(stage, name="both")
+        with pytest.raises(HawkError, match="takes a traced kernel"):
+            hawk.steps(stage, 2)
+
+
 @pytest.mark.gpu
 def test_planes_that_do_not_fit_are_refused(gpu):
     import torch
