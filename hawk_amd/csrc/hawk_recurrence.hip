@@ -10,6 +10,10 @@
 // entered.  The derivative is the same recurrence run the other way: C_t =
 // a_t (bar_h_t + C_(t+1)) has the gate a_t and the input a_t bar_h_t.
 //
+// The tiles join theirs in one pass over the data, by the published decoupled
+// look-back (Merrill and Garland, Single-pass parallel prefix scan with decoupled
+// look-back, 2016): each publishes its run, then folds those published before it.
+//
 // A gate of 0 cuts, and so does the first row of a packed sequence: products
 // and their use take 0 times anything as 0 (cutmul), so neither an infinity
 // nor a NaN passes a cut.  States are held in 32 bits (64 for double planes), and
@@ -34,7 +38,7 @@ constexpr int kThreads = 256;
 
 // A workgroup's most threads.  Where lanes lie along the steps a long sequence
 // takes large tiles, since each tile has one state to wait for (64 rows of 2^20
-// float steps: 352 us in tiles of 256 threads, 258 of 512, 261 of 1024; 205 now).
+// float steps: 238 us in tiles of 256 threads, 211 of 512, 232 of 1024).
 template <class T, int Dir> constexpr int kMost = Dir == 0 ? kThreads : 512;
 
 template <class T>
@@ -222,7 +226,7 @@ __device__ __forceinline__ void await_run(const uint64_t* agg, const uint16_t* e
 }
 
 // Aggregates read at once.  Eight hide more of a wait, but cost 32-bit planes, and
-// lanes along the steps, a wave a SIMD: 1 x 65536 x 1024 bfloat16 100 us in eights,
+// lanes along the steps, a wave a SIMD: 1 x 65536 x 1024 bfloat16 101 us in eights,
 // 102 in fours; 64 x 2^20 float steps, derivative, 375 and 368.
 template <class T, int Dir> constexpr int kBatch = Dir == 0 && sizeof(T) == 2 ? 8 : 4;
 
@@ -231,10 +235,10 @@ template <class T, int Dir> constexpr int kBatch = Dir == 0 && sizeof(T) == 2 ? 
 // other: what two of them share of a line is fetched once (every grid's last part
 // window in plain order; which die takes a tile does not matter to what it waits
 // for).  One, 2, 4, 8, 16 strips, forward in us: 37 sequences, 65793 x 1001 bfloat16
-// 151, 140, 136, 140, 142; 5, 30000 x 997 float 117, 106, 99, 104, 109; 64,
-// 100000 x 511 130, 114, 112, 112, 113.  Streams share no line, but words that their
-// tiles wait for: 1 x 65536 x 1024 101, 99, 98, 96, 97 and its derivative 168, 168,
-// 161, 152, 152; 16 x 4096 x 2048 157, 156, 159, 157, 157.
+// 151, 142, 138, 141, 143; 5, 30000 x 997 float 118, 111, 107, 109, 114; 64,
+// 100000 x 511 125, 119, 117, 116, 116.  Streams share no line, but words that their
+// tiles wait for: 1 x 65536 x 1024 103, 103, 103, 101, 102 and its derivative 164,
+// 167, 165, 156, 157; 16 x 4096 x 2048 156, 155, 160, 156, 156.
 constexpr unsigned kDies = 8, kBeside = 4, kBesideStream = 8;
 
 template <class T, int V, int K, int Dir, bool Sigmoid, bool Vjp, bool Packed, bool Stream>
@@ -350,9 +354,9 @@ __global__ void __launch_bounds__((kMost<T, Dir>)) hawk_recurrence_tile(const Re
     auto begin = [&](int64_t q, int v) -> A { return a.init ? a.init[q * a.chans + c0 + v] : A(0); };
 
     // Gates and inputs cost less to convert twice than to hold twice as wide: the
-    // bfloat16 forward of 8 steps keeps 64 registers of them instead of 128, and
-    // even the sigmoid's second evaluation is won back by the third wave a SIMD
-    // (16 x 4096 x 2048: 182 us against 186 with its value kept).
+    // bfloat16 forward of 8 steps keeps 64 registers of them instead of 128, and three
+    // waves a SIMD win back even the sigmoid's second evaluation (16 x 4096 x 2048:
+    // 178 us; 356 with both its values kept, at one wave).
     auto coefficients = [&](int k, int v, A& g, A& rest, A& b) {
         g = widen<T, V>(gate[k], v);
         if constexpr (Sigmoid) sigmoid(g, g, rest);
@@ -676,8 +680,9 @@ __global__ void __launch_bounds__(256) hawk_recurrence_clear(uint32_t* at, int64
 
 // A few steps (a token at a time, or some): one thread takes V channels of a
 // sequence from step to step, with nothing to join.  Bounded by a launch and one
-// round trip to memory: 64 x 1 x 2048 bfloat16 3.4 us a call against 8.2 for a
-// tile, 512 x 8 x 8192 38 against 47; at 16 steps 91 against 79, the other way.
+// round trip to memory.  bfloat16, us a call, against a tile: 64 x 1 x 2048 4.7 and
+// 8.4, 512 x 4 x 8192 15.7 and 21.5, 512 x 8 x 2048 8.7 and 9.7; the other way from
+// 8 steps of 512 x 8192 on (39 and 35; 16 steps 80 and 68).
 constexpr int kShort = 8, kShortThreads = 64;
 template <class T, int V, bool Sigmoid>
 __global__ void __launch_bounds__(kShortThreads) hawk_recurrence_short(const RecArgs<T> a) {
@@ -761,9 +766,9 @@ template <class T, bool Vjp> struct Tile {
 // the planes of 16 x 4096 x 2048 bfloat16 elements at 6.07 TB/s, 16 lanes at
 // 4.84, 64 at 5.88 (a copy of the pattern), but give half the steps a tile, and
 // where few strips fill the card a tile waits for a state many tiles back:
-// forward of 1 x 65536 x 1024 178 us in 4 strips of 32 lanes, 120 in 8 of 16, 110
-// in 16 of 8; 8 x 2048 x 1536 44 us in 96 of 16, 46 in 192 of 8; 16 x 4096 x 2048
-// 157 us in 128 of 32, 177 in 256 of 16.
+// forward of 1 x 65536 x 1024 152 us in 4 strips of 32 lanes, 111 in 8 of 16, 101
+// in 16 of 8; 8 x 2048 x 1536 44 us in 48 of 32, 42 in 96 of 16 and in 192 of 8;
+// 16 x 4096 x 2048 157 us in 128 of 32, 168 in 256 of 16.
 constexpr int kAcross = 5, kAcrossFew = 4, kAcrossLeast = 3;
 constexpr int64_t kManyStrips = 64, kFewStrips = 16;
 
@@ -815,9 +820,9 @@ Shape shape_of(const hk_recurrence_job& j) {
     }
     // Whole lines: a strip's part of a row begins and ends with a 128-byte line in
     // every plane, so nothing is read twice and it need not stay in the caches
-    // (16 x 4096 x 2048 forward 159 us as a stream, 176 cached).  Otherwise the
+    // (16 x 4096 x 2048 forward 157 us as a stream, 170 cached).  Otherwise the
     // neighbouring strip finds its share of a line there (65793 packed rows of
-    // 1001 bfloat16 channels: 154 us cached, 167 as a stream).
+    // 1001 bfloat16 channels: 138 us cached, 168 as a stream).
     s.stream = s.dir == 0 && s.v > 1;
     for (const hk_plane* p : planes) {
         if (!p->data) continue;

@@ -8,6 +8,9 @@
 // k = scale log2(e) rounded once and used for every term of a row, the target's
 // l_y k - m - log2(sum) is exact in k (a different scale by 6e-8), so nothing
 // is lost between the target's term and the sum's.
+// Where a row does not fit the registers, (m, sum) run along in one pass and are
+// rescaled as m grows: the published online softmax (Milakov and Gimelshein, Online
+// normalizer calculation for softmax, 2018).
 
 #include "hawk_core.h"
 #include "hawk_internal.h"
@@ -276,8 +279,8 @@ __device__ __forceinline__ int one_of(int x) {
 // to row, and a vector's register takes the next row's as soon as its gradient is
 // stored, so loads run beside the second pass over the row.  The row has no fewer
 // than half the vectors (NV > 1), so those before the half's last need no bounds.
-// Rows of whole waves pass as a stream (8192 rows of 131072 bfloat16 logits with
-// their gradient 841 us, 872 cached).
+// Rows of whole waves pass as a stream (with their gradient, 512 rows of 131072
+// bfloat16 logits 58 us, 63 cached; 8192 of them 828 and 832).
 template <class T, int L, int NV, Work W, bool Grad>
 __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_row_held(const RowArgs<T> a) {
     constexpr int V = kVec<T>, R = (L > kThreads ? L : kThreads) / L;
@@ -420,8 +423,8 @@ __device__ __forceinline__ void run_of(const T* from, int64_t first, int low, in
 // their order and finishes the row.  A word is 0 until its part has come (no pair
 // is: s is 1 or more, a NaN, or 0 beside m = -inf), so nothing but the word itself
 // orders it: with a release and an acquire at each part's count, whose fences
-// write back and drop the caches, 512 rows of 131072 bfloat16 logits took 65 us
-// instead of 27.  The word waited for was sent before its part counted itself; if it
+// write back and drop the caches, 64 rows of 262144 bfloat16 logits take 33 us
+// instead of 13.  The word waited for was sent before its part counted itself; if it
 // never shows (the state's words shared by two streams) the row is a NaN.
 constexpr int kMostParts = 64, kLooks = 1 << 20;
 template <class T, Work W>
@@ -710,10 +713,10 @@ constexpr int64_t kShortVectors = 512;     // rows that at most a wave holds
 constexpr int64_t kFewVectors = 16384;     // 256 KiB of logits
 
 // The workgroups of a row: more than one where at most 64 rows have 16384 vectors
-// or more (one row of 131072 floats 8.0 us a call against 11.6 by one workgroup,
-// 52 of them 13.0 and 13.6, 52 of 200003 14.7 and 22.3), at most four a unit (eight:
-// the 52 rows 17.5 and 23.1).  Rows of 50001 floats lose up to 1 us by it, and so do
-// 256 rows of 131072 bfloat16.
+// or more (one row of 131072 floats 4.7 us a call against 9.7 by one workgroup,
+// 52 of them 10.7 and 13.4, 52 of 200003 12.0 and 21.5), at most four a unit (eight:
+// the 52 rows 14.5 and 18.3).  52 rows of 50001 floats lose 0.4 us by it, 256 of
+// 131072 bfloat16 0.3.
 template <class T>
 int parts_of(const RowArgs<T>& a) {
     const int64_t vectors = vectors_of(a);
@@ -729,7 +732,7 @@ int parts_of(const RowArgs<T>& a) {
 // (m, s) holds nothing.  Fewer rows than two a unit take 1024 lanes each.  A
 // gradient from a saved lse takes a workgroup for each 1024 vectors of a row: 4096
 // rows of 50001 floats 336 us against 368 with a workgroup a row, one row of 131072
-// 5.5 against 19.5 with 1024 lanes.
+// 4.6 against 40.
 template <class T, Work W>
 int rows_of(RowArgs<T> a, hipStream_t s) {
     if (a.rows == 0) return HK_OK;
@@ -893,16 +896,16 @@ int hk_policy_loss(const hk_row_loss_job* job, void* scratch, void* stream) {
         typedef decltype(t) T;
         RowArgs<T> a = args_of<T>(*job);
         a.row_loss = job->loss ? row_floats(*job, scratch) : nullptr;
-        // in the rows' own launch where they are few: 200 rows of 48 floats 6.2 us a
-        // call against 7.7 with a launch more, but the workgroups' fences wait for
-        // what they stored: 4524 rows of 1660 float16 logits 123 us against 15
+        // in the rows' own launch where they are few: 200 rows of 48 floats 6.5 us a
+        // call against 7.9 with a launch more, but the workgroups' fences wait for
+        // what they stored: 4524 rows of 1660 float16 logits 126 us against 16
         summed = job->loss && job->state && job->rows > 0 && job->rows <= kRun && vectors_of(a) <= kShortVectors &&
                  job->rows * vectors_of(a) <= kFewVectors;
         if (summed) a.loss = job->loss;
         if (!a.bar_logits || vectors_of(a) <= kHeldVectors) return rows_of<T, kPolicy>(a, s);
         // longer rows twice: all their losses, then all their gradients (4096 rows of
-        // 131072 floats 1080 us against 1091 with both in one workgroup's passes, 52 of
-        // them 30 against 46)
+        // 131072 floats 1077 us against 1091 with both in one workgroup's passes, 52 of
+        // them 26 against 46)
         a.bar_logits = nullptr;
         if (!a.logp) a.logp = row_floats(*job, scratch) + job->rows;
         if (!a.lse) a.lse = row_floats(*job, scratch) + 2 * job->rows;
