@@ -3,11 +3,12 @@
 The task is recall: a sequence shows a token, then noise, and at every step the
 policy is rewarded for naming the first token.  One layer holds a gated
 recurrence on a residual branch with dropout; the products by its weights are
-torch's, everything between them is ``hawk.stages``:
+torch's, everything between them is hawk's, a traced kernel and its stages:
 
 * the forward and its reverse: ``recurrence`` (sigmoid gates) and ``dropout``;
-* rollouts: ``token_logp`` of the sampled actions, discounted rewards by a
-  reversed ``recurrence`` whose gate holds the discount and the ends;
+* rollouts: ``token_logp`` of the sampled actions; a traced kernel, a sample a
+  step, turns rewards and ends into the planes of a reversed ``recurrence``, which
+  sums the discounted rewards;
 * the update: ``policy_loss`` (clipped, with a KL term to the first policy),
   its gradient in the same pass over the logits;
 * then a few steps of ``preference_loss`` on pairs of answers;
@@ -19,6 +20,7 @@ Run it on a ROCm device: ``python examples/recurrent_policy.py``.
 from __future__ import annotations
 
 import sys
+import tempfile
 from pathlib import Path
 
 import torch
@@ -26,9 +28,17 @@ import torch
 sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 import hawk_amd as hawk  # noqa: E402
+from hawk_amd import Mutable, Param, Scalar  # noqa: E402
 
-TOKENS, WIDTH, STEPS, SEQUENCES = 16, 64, 12, 256
+TOKENS, WIDTH, STEPS, SEQUENCES = 16, 64, 12, 250
 DISCOUNT = 0.5
+
+
+@hawk.kernel
+def gains(reward: Scalar, ends: Scalar, baseline: Param, gate: Mutable[Scalar], x: Mutable[Scalar]):
+    """One step's part of the discounted sum: what comes after an end is cut."""
+    gate = DISCOUNT * (1.0 - ends)
+    x = reward - baseline
 
 
 class Policy:
@@ -108,8 +118,11 @@ def train(device="cuda:0", rounds: int = 60, seed: int = 0, tell=None) -> dict:
     policy, first = Policy(device, seed), Policy(device, seed)
     returns = hawk.stages.recurrence(reverse=True)
     loss_of = hawk.stages.policy_loss(clip=(0.2, 0.28), kl=0.01)
-    gate = torch.full((SEQUENCES, STEPS, 1), DISCOUNT, device=device)
-    gate[:, -1] = 0.0                                            # the episode ends here
+    with tempfile.TemporaryDirectory() as unit:
+        hawk.build([gains], unit, mode="float32")
+        step_gains = hawk.load(unit, "gains")
+    ends, (gate, x) = torch.zeros(SEQUENCES, STEPS, 1, device=device), torch.empty(2, SEQUENCES, STEPS, 1, device=device)
+    ends[:, -1] = 1.0                                            # the episode ends here
     rewards = []
     for k in range(rounds):
         tokens = episodes(SEQUENCES)
@@ -117,8 +130,10 @@ def train(device="cuda:0", rounds: int = 60, seed: int = 0, tell=None) -> dict:
         actions = torch.multinomial(torch.softmax(logits, 1), 1, generator=g)[:, 0]
         reward = (actions.view(SEQUENCES, STEPS) == tokens[:, :1]).float()
         rewards.append(float(reward.mean()))
+        hawk.run(step_gains, reward=reward.flatten(), ends=ends.flatten(), baseline=rewards[-1], gate=gate.flatten(),
+                 x=x.flatten())
         gain = torch.empty_like(gate)
-        hawk.run(returns, gate=gate, x=(reward - reward.mean()).unsqueeze(-1), h=gain)
+        hawk.run(returns, gate=gate, x=x, h=gain)
         planes = dict(target=actions, old_logp=logp_of(logits, actions), advantage=gain.flatten() / (gain.std() + 1e-6),
                       ref_logp=logp_of(first.forward(tokens, train=False)[0], actions))
         loss = torch.empty(1, device=device)
