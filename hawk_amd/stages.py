@@ -415,8 +415,8 @@ def recurrence(gate: str = "value", reverse: bool = False) -> Stage:
     ``last``.
 
     A gate of exactly 0 cuts: nothing before it reaches the state, not even an
-    infinity or a NaN.  A sigmoid gate is 0 below -86.6 (-745 in float64).  Gates of
-    any size are taken: their products are held past the range of the type.  Runs of
+    infinity or a NaN.  A sigmoid gate is 0 below -86.6 (-745 in float64).  Finite
+    gates of any size are taken: their products are held past the type's range.  Runs of
     steps are joined, so where gates grow, a run's own sum from a zero state has to
     stay in that range, and rounding errors grow as the gates' product does.
 

@@ -372,6 +372,27 @@ def test_large_and_infinite_states_through_many_small_gates(gpu, T, C, layout):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["channels", "steps"])
+@pytest.mark.parametrize("T,C", [(7, 16), (100, 16), (5000, 3)], ids=str)
+def test_gates_below_the_least_normal_number(gpu, T, C, layout):
+    """A gate of few bits is the number it holds, in a thread's own steps and in the products that are joined."""
+    import torch
+
+    def put(x):
+        return x.transpose(1, 2).contiguous().transpose(1, 2) if layout == "steps" else x
+    gate = torch.ones(1, T, C, device=gpu)
+    gate[0, T // 2], gate[0, T // 2 + 1] = 1e-40, -3e35
+    x, h, h0 = put(torch.zeros_like(gate)), put(torch.empty_like(gate)), torch.full((1, C), 1e35, device=gpu)
+    hawk.run(hawk.stages.recurrence(), gate=put(gate), x=x, h=h, h0=h0)
+    want = h0.double() * torch.cumprod(gate.double(), 1)
+    assert ((h.double() - want).abs() <= 8 * 2.0 ** -24 * want.abs()).all()
+    bar = put(torch.empty_like(gate))
+    hawk.run(hawk.stages.recurrence(reverse=True).vjp, gate=put(gate), h=x, bar_h=x, bar_last=h0, bar_x=bar)
+    want = torch.cat([h0.double()[:, None], want[:, :-1]], 1)            # the adjoint before each step's gate
+    assert ((bar.double() - want).abs() <= 8 * 2.0 ** -24 * want.abs()).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T,C", [(1, 16), (8, 5), (40, 16), (9000, 8)], ids=str)
 def test_a_sigmoid_gate_below_the_least_number_cuts_in_every_form(gpu, T, C):
     """sigma(-100) is no float32 of full precision and sigma(-inf) is 0: neither lets the state pass, dense or packed."""
