@@ -219,10 +219,15 @@ __device__ __forceinline__ bool read_run(const uint64_t* agg, const uint16_t* ex
 __device__ __forceinline__ bool read_run(const uint64_t* agg, const uint16_t* exps, int64_t at, Run<double>& r) {
     return read<double>(agg + 2 * at, r.p.m) & read<double>(agg + 2 * at + 1, r.h) & read_exponent(exps, at, r.p.e);
 }
-// As await; what never shows is a NaN.
+// As await; a run of which a part never shows is a NaN.
 template <class A>
 __device__ __forceinline__ void await_run(const uint64_t* agg, const uint16_t* exps, int64_t at, Run<A>& r) {
-    for (int looks = kLooks; !read_run(agg, exps, at, r) && looks > 0; --looks) __builtin_amdgcn_s_sleep(1);
+    bool known = false;
+    for (int looks = kLooks; !known && looks > 0; --looks) {
+        known = read_run(agg, exps, at, r);
+        if (!known) __builtin_amdgcn_s_sleep(1);
+    }
+    if (!known) r.h = NAN;
 }
 
 // Aggregates read at once.  Eight hide more of a wait, but cost 32-bit planes, and
