@@ -477,8 +477,8 @@ class _Rows(_Stage):
         L = _core.lib()
         if self.vjp_of is not None:         # a derivative works in registers
             return _Plan(job, slots, getattr(L, self.entry), 0)
-        return _Plan(job, slots, getattr(L, self.entry), int(L.hk_row_loss_scratch_bytes(ctypes.byref(job))),
-                     state=_word(_core.RowLossJob, "state"))
+        scratch = int(L.hk_row_loss_scratch_bytes(ctypes.byref(job))) if "loss" in self.writes else min(job.rows, 1)
+        return _Plan(job, slots, getattr(L, self.entry), scratch, state=_word(_core.RowLossJob, "state"))
 
     def _more(self, t: dict, job) -> None:
         if t.get("weight") is not None:

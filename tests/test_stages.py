@@ -1534,6 +1534,21 @@ def test_planes_past_the_grids_threads_are_refused_before_the_launch():
     assert L.hk_recurrence(ctypes.byref(r), 16, None) == 1 and b"grid limit" in L.hk_last_error()
 
 
+def test_a_stage_takes_the_scratch_its_entry_works_in():
+    """Rows without a sum over them work in the stream's state alone, their gradients in neither."""
+    import torch
+    N = 4096
+    l, t, f = torch.zeros(N, 8), torch.zeros(N, dtype=torch.int64), torch.zeros(N)
+    logp, policy = hawk.stages.token_logp(), hawk.stages.policy_loss()
+    plan = logp._make(dict(logits=l, target=t, logp=f))
+    assert plan.scratch == 1 and plan.state is not None
+    plan = logp.vjp._make(dict(logits=l, target=t, lse=f, bar_logp=f, bar_logits=l))
+    assert plan.scratch == 0 and plan.state is None
+    plan = policy._make(dict(logits=l, target=t, old_logp=f, advantage=f, logp=f))
+    assert plan.scratch >= 12 * N and plan.state is not None
+    assert logp._make(dict(logits=l[:0], target=t[:0], logp=f[:0])).scratch == 0
+
+
 def test_the_jobs_are_laid_out_as_the_header_has_them():
     assert ctypes.sizeof(_core.SeqPlane) == 32
     assert ctypes.sizeof(_core.RecurrenceJob) == 6 * 32 + 5 * 8 + 3 * 8 + 4 * 4
