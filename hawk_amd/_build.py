@@ -2,8 +2,8 @@
 
 The library is the C-ABI launcher (``csrc/hawk_core.cpp``) plus the
 hand-written team-stage kernels (``csrc/hawk_team.hip``, ``csrc/hawk_linalg.hip``) and training stages
-(``csrc/hawk_recurrence.hip``, ``csrc/hawk_rows.hip``, ``csrc/hawk_dropout.hip``), built by ``hipcc``
-for gfx950 only, each file by a compiler of its own.  Beside it ``_bind.so`` (``csrc/hawk_bind.cpp``,
+(``csrc/hawk_recurrence.hip``, ``csrc/hawk_rows.hip``, ``csrc/hawk_dropout.hip``, ``csrc/hawk_norm.hip``,
+``csrc/hawk_sample.hip``, ``csrc/hawk_linear.hip``), built by ``hipcc`` for gfx950 only, each file by a compiler of its own.  Beside it ``_bind.so`` (``csrc/hawk_bind.cpp``,
 built by the host compiler against PyTorch's headers) checks and binds a stage's tensors; the library
 is built and used without it.  The build digest is the sha256 of its own sources (each
 file's name and sha256, in sorted order), stamped into both and
@@ -31,7 +31,7 @@ HIPCC = os.environ.get("HAWK_HIPCC", "/opt/rocm/bin/hipcc")
 
 #: The library's translation units.
 UNITS = ("hawk_core.cpp", "hawk_team.hip", "hawk_linalg.hip", "hawk_recurrence.hip", "hawk_rows.hip",
-         "hawk_dropout.hip")
+         "hawk_dropout.hip", "hawk_norm.hip", "hawk_sample.hip", "hawk_linear.hip")
 
 #: Flags every HIP translation unit of this target is built with: gfx950
 #: only, no floating-point contraction (the host oracle's ``native`` profile

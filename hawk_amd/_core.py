@@ -96,6 +96,14 @@ def _declare(lib) -> None:
         "hk_preference_loss": (I, [V, V, V]),
         "hk_preference_loss_vjp": (I, [V, V, V]),
         "hk_dropout": (I, [V, V]),
+        "hk_layer_norm_scratch_bytes": (SZ, [V, ctypes.c_int32]),
+        "hk_layer_norm": (I, [V, V, V]),
+        "hk_layer_norm_vjp": (I, [V, V, V]),
+        "hk_sample_scratch_bytes": (SZ, [V]),
+        "hk_sample": (I, [V, V, V]),
+        "hk_linear_attention_scratch_bytes": (SZ, [V, ctypes.c_int32]),
+        "hk_linear_attention": (I, [V, V, V]),
+        "hk_linear_attention_vjp": (I, [V, V, V]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -586,3 +594,38 @@ class DropoutJob(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("rows", "cols", "x_stride", "residual_stride", "y_stride")]
                 + [(n, ctypes.c_uint64) for n in ("seed", "offset")]
                 + [(n, ctypes.c_int32) for n in ("cut", "dtype")])
+
+
+class LayerNormJob(ctypes.Structure):
+    """The arguments of ``hk_layer_norm`` and its derivative (``hk_layer_norm_job``)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "bar_y", "y", "bar_x", "bar_weight", "bar_bias",
+                                                "mean", "rstd")]
+                + [(n, ctypes.c_int64) for n in ("rows", "cols", "x_stride", "y_stride", "bar_y_stride", "bar_x_stride")]
+                + [("eps", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "reserved")])
+
+
+class SampleJob(ctypes.Structure):
+    """The arguments of ``hk_sample`` (``hk_sample_job``)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "u", "row_temperature", "row_top_p", "row_min_p", "row_top_k",
+                                                "token", "logp")]
+                + [(n, ctypes.c_int64) for n in ("rows", "vocab", "row_stride", "top_k")]
+                + [(n, ctypes.c_double) for n in ("temperature", "top_p", "min_p")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "u64bits", "token64", "reserved")])
+
+
+class HeadPlane(ctypes.Structure):
+    """A (sequence, step, head, channel) plane (``hk_head_plane``): strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("seq", ctypes.c_int64), ("step", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class LinearAttentionJob(ctypes.Structure):
+    """The arguments of ``hk_linear_attention`` and its derivative (``hk_linear_attention_job``)."""
+
+    _fields_ = ([(n, HeadPlane) for n in ("q", "k", "v", "o", "bar_o", "bar_q", "bar_k", "bar_v")]
+                + [(n, ctypes.c_void_p) for n in ("decay", "h0", "bar_last", "last", "bar_h0", "offsets")]
+                + [(n, ctypes.c_int64) for n in ("seqs", "steps", "heads")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("keys", "values", "dtype", "offsets64", "reserved")])

@@ -1,0 +1,682 @@
+// hawk_linear.hip — linear attention with a decay for each head on gfx950, and its
+// derivative.
+//
+// The mathematics.  S_t = g S_(t-1) + k_t v_t^T, o_t = scale q_t S_t.  Written out,
+//   o_i = scale sum_(j <= i) g^(i-j) (q_i . k_j) v_j + scale g^(i+1) q_i h0,
+// one form A(a, b, c) of three planes, whose derivative is the same form with the
+// planes in other places: bar_q = A(bar_o, v, k), and with time reversed
+// bar_k = A(v, bar_o, q), bar_v = A(k, q, bar_o).  One kernel computes all four.
+//
+// In chunks of C tokens, with X what the tokens before a chunk have left, as its
+// first token sees it,
+//   out_i = g^i (a_i X) + sum_(j <= i in the chunk) g^(i-j) (a_i . b_j) c_j,
+//   X' = g^C X + sum_j g^(C-j) b_j c_j^T :
+// products for the matrix cores.  A workgroup walks a run of chunks with its columns
+// of X in registers: a wave has 16 columns of c.  X as the matrix cores leave it is
+// an operand of the next chunk's product as it stands, if that product takes its
+// terms in the order in which X lies in the lanes; a's columns are staged in that order.
+//
+// The numbers.  X and every sum are held in 32 bits.  The matrix cores multiply bf16;
+// a number of more digits is a sum of bf16 parts (three make 24 bits), and a product is
+// the sum of the parts' products down to 2^-17 of it where the result is rounded to 16
+// bits, 2^-25 otherwise, and always 2^-25 in X.
+
+#include "hawk_core.h"
+#include "hawk_internal.h"
+#include "hawk_vec.h"
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include <string>
+
+namespace {
+
+using namespace hawk_vec;
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kSlice = 16 * kWaves;        // columns of c that a workgroup has
+constexpr int kMostWidth = 256;
+constexpr int64_t kUnits = 256, kDies = 8;
+
+typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
+typedef float F4 __attribute__((ext_vector_type(4)));
+typedef uint16_t H4 __attribute__((ext_vector_type(4)));
+typedef uint16_t H8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ F4 product(const H8& a, const H8& b, const F4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf8, a), __builtin_bit_cast(Bf8, b), c, 0, 0, 0);
+}
+
+// The N bf16 parts of a number, each the nearest to what the ones before leave: two are
+// within 2^-18 of it, three are a number of 24 bits.
+template <int N>
+__device__ __forceinline__ void cut(float x, uint16_t (&out)[N]) {
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+        const bf16 h = static_cast<bf16>(x);
+        out[p] = __builtin_bit_cast(uint16_t, h);
+        if (p + 1 < N) x -= static_cast<float>(h);
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ void parts_of(T x, uint16_t (&out)[N]) {
+    if constexpr (N == 1) {
+        out[0] = __builtin_bit_cast(uint16_t, x);
+    } else if constexpr (sizeof(T) == 2) {
+        cut<N>(static_cast<float>(x), out);
+    } else {
+        // above bf16's largest number the nearest one is an infinity: the next below is taken
+        const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+        const bf16 near = static_cast<bf16>(x);
+        const uint16_t h = fabsf(static_cast<float>(near)) < INFINITY ? __builtin_bit_cast(uint16_t, near) : static_cast<uint16_t>(bits >> 16);
+        uint16_t rest[N - 1];
+        cut<N - 1>(x - __builtin_bit_cast(float, static_cast<uint32_t>(h) << 16), rest);
+        out[0] = h;
+#pragma unroll
+        for (int p = 1; p < N; ++p) out[p] = rest[p - 1];
+    }
+}
+__device__ __forceinline__ float part(uint16_t h) { return __builtin_bit_cast(float, static_cast<uint32_t>(h) << 16); }
+
+// The parts of a type's elements, and of what is computed from them.
+template <class T> struct Parts;
+template <> struct Parts<bf16> { static constexpr int in = 1, made = 2, reach = 2; };
+template <> struct Parts<f16> { static constexpr int in = 2, made = 2, reach = 2; };
+template <> struct Parts<float> { static constexpr int in = 3, made = 3, reach = 3; };
+constexpr int kExact = 3;                  // X is kept to 24 bits
+
+// sum over pairs of parts (p, q) with p + q < Reach
+template <int Reach, int N, int M>
+__device__ __forceinline__ F4 product(const H8 (&a)[N], const H8 (&b)[M], F4 c) {
+#pragma unroll
+    for (int s = Reach - 1; s >= 0; --s)   // the smallest first
+#pragma unroll
+        for (int p = 0; p < N; ++p)
+            if (s - p >= 0 && s - p < M) c = product(a[p], b[s - p], c);
+    return c;
+}
+
+template <class T>
+struct Plane {
+    T* at;
+    int64_t seq, step, head;
+};
+
+template <class T>
+struct LinearArgs {
+    Plane<const T> a, b, c;
+    Plane<T> out;              // at may be NULL
+    const float* decay;
+    const float* start;        // the state that enters, element (d, e) at d*state_d + e*state_e of a head's; or NULL
+    float* end;                // the state that leaves, or NULL
+    float* cuts;               // the segments' states, [slot][head][width][columns], or NULL
+    const void* offsets;
+    int64_t seqs, steps, heads, slots, segment, segments;    // segments: of a dense sequence
+    int state_d, state_e, width, columns, slices;
+    float inner, outer;        // factors of b's products and of the result
+    int offsets64, reverse;
+};
+
+struct Span {
+    int64_t seq, first, length, begin, end;    // tokens [begin, end) of a sequence that starts at row `first`
+    bool real, last;
+};
+template <class T>
+__device__ __forceinline__ int64_t bound_of(const LinearArgs<T>& a, int64_t k) {
+    const int64_t v = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[k] : static_cast<const int32_t*>(a.offsets)[k];
+    return v < 0 ? 0 : v > a.steps ? a.steps : v;
+}
+// Sequence s's segments have the slots from bound(s) / segment + s on: more than it needs
+// by one at most, and none of two sequences.
+template <class T>
+__device__ __forceinline__ Span span_of(const LinearArgs<T>& a, int64_t slot) {
+    Span s;
+    int64_t segment;
+    if (!a.offsets) {
+        s.seq = slot / a.segments;
+        segment = slot - s.seq * a.segments;
+        s.first = 0;
+        s.length = a.steps;
+    } else {
+        int64_t low = 0, high = a.seqs - 1;
+        while (low < high) {
+            const int64_t mid = (low + high + 1) / 2;
+            if (bound_of(a, mid) / a.segment + mid <= slot) low = mid;
+            else high = mid - 1;
+        }
+        s.seq = low;
+        s.first = bound_of(a, low);
+        s.length = bound_of(a, low + 1) - s.first;
+        if (s.length < 0) s.length = 0;
+        segment = slot - (s.first / a.segment + low);
+    }
+    s.begin = segment * a.segment;
+    s.real = segment >= 0 && (segment == 0 || s.begin < s.length);
+    s.end = s.begin + a.segment < s.length ? s.begin + a.segment : s.length;
+    s.last = s.end == s.length;
+    return s;
+}
+
+__device__ __forceinline__ double octaves_of(float g) {
+    if (!(g >= 0.0f && g <= 1.0f)) return NAN;
+    return g == 0.0f ? -1e30 : log2(static_cast<double>(g));
+}
+__device__ __forceinline__ float power(double octaves, int64_t n) { return exp2f(static_cast<float>(octaves * static_cast<double>(n))); }
+
+// Where column d of a is staged: the order in which X's rows lie in the lanes, two
+// tiles of 16 after each other.
+__device__ __forceinline__ int staged(int d) { return (d & ~31) | (d >> 2 & 3) << 3 | (d >> 4 & 1) << 2 | (d & 3); }
+
+// Eight tokens by four channels, a thread's share of a chunk's plane.
+template <class T> struct Block { Raw<T, 4> x[8]; };
+template <class T>
+__device__ __forceinline__ void fetch(Block<T>& x, const T* head, int64_t step, int64_t row, int way, int i, int count, int d, int width) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        x.x[r] = splat<T, 4>(static_cast<T>(0.0f));
+        if (i + r >= count) continue;
+        const T* at = head + (row + way * static_cast<int64_t>(i + r)) * step + d;
+        if (d + 4 <= width) {
+            x.x[r] = load_raw<T, 4>(at);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < width) x.x[r][j] = at[j];
+        }
+    }
+}
+
+template <class T, int DP, int C>
+struct Tiles {
+    static constexpr int N = Parts<T>::in, M = Parts<T>::made;
+    static constexpr int Wide = DP + 8, Long = C + 8;      // rows are 16 bytes apart in the banks
+    uint16_t a[N][C][Wide];
+    union {
+        uint16_t b[N][C][Wide];                            // rows of tokens, until the products of a and b are made
+        uint16_t turned[N][DP][Long];                      // rows of channels
+    };
+    uint16_t c[N][kSlice][Long];
+    uint16_t inside[M][C][Long];                           // g^(i-j) a_i . b_j
+    float power[C + 1];
+    int odd;                                               // c holds what is no number
+};
+// Eight tokens' unit of a row of channels lies turned by d / 4: lanes that write, or read,
+// neighbouring rows then meet different banks.
+template <int C>
+__device__ __forceinline__ int unit(int d, int eight) { return ((eight + (d >> 2)) & (C / 8 - 1)) * 8; }
+
+template <class T, int DP, int C>
+__device__ __forceinline__ void stage_rows(uint16_t (&to)[Parts<T>::in][C][DP + 8], const Block<T>& x, int eight, int d) {
+    constexpr int N = Parts<T>::in;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        H4 h[N];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint16_t p[N];
+            parts_of<T, N>(x.x[r][j], p);
+#pragma unroll
+            for (int n = 0; n < N; ++n) h[n][j] = p[n];
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) *reinterpret_cast<H4*>(&to[n][eight * 8 + r][staged(d)]) = h[n];
+    }
+}
+template <class T, int R, int C>
+__device__ __forceinline__ void stage_turned(uint16_t (&to)[Parts<T>::in][R][C + 8], const Block<T>& x, int eight, int d) {
+    constexpr int N = Parts<T>::in;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        H8 h[N];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            uint16_t p[N];
+            parts_of<T, N>(x.x[r][j], p);
+#pragma unroll
+            for (int n = 0; n < N; ++n) h[n][r] = p[n];
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) *reinterpret_cast<H8*>(&to[n][d + j][unit<C>(d, eight)]) = h[n];
+    }
+}
+template <int N, int R, int W>
+__device__ __forceinline__ void take(H8 (&out)[N], const uint16_t (&from)[N][R][W], int row, int at) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = *reinterpret_cast<const H8*>(&from[n][row][at]);
+}
+
+// Workgroup (slot, head, slice).  Whole: the walk over a segment; otherwise what the
+// segment leaves of its own, for the sum over the segments before another.
+template <class T, int DP, int C, bool Whole>
+__global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
+    constexpr int N = Parts<T>::in, M = Parts<T>::made, Reach = Parts<T>::reach;
+    constexpr int Blocks = C / 8 * (DP / 4), SliceBlocks = C / 8 * (kSlice / 4);
+    static_assert(Blocks <= kThreads && SliceBlocks <= kThreads, "a block a thread");
+    __shared__ Tiles<T, DP, C> s;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, quad = lane >> 4;
+    const int64_t pairs = a.slots * a.heads, group = kDies * a.slices;
+    const int64_t total = (pairs + kDies - 1) / kDies * group;
+    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+        // a pair's slices go to one die, whose L2 has a and b for all of them
+        const int64_t pair = id / group * kDies + id % kDies;
+        const int slice = static_cast<int>(id / kDies % a.slices);
+        if (pair >= pairs) continue;
+        const int64_t slot = pair / a.heads, head = pair - slot * a.heads;
+        const Span span = span_of(a, slot);
+        if (!span.real || (!Whole && span.last)) continue;
+        const double octaves = octaves_of(a.decay[head]);
+        const int e0 = slice * kSlice;
+        const int64_t plane = static_cast<int64_t>(a.width) * a.columns;
+        const int64_t state = (span.seq * a.heads + head) * plane, mark = pair * plane;
+        const int way = a.reverse ? -1 : 1;
+        const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
+        const T* pa = Whole ? a.a.at + span.seq * a.a.seq + head * a.a.head : nullptr;
+        const T* pb = a.b.at + span.seq * a.b.seq + head * a.b.head;
+        const T* pc = a.c.at + span.seq * a.c.seq + head * a.c.head + e0;
+        __syncthreads();                                   // the run before is done with the tiles
+        for (int n = tid; n <= C; n += kThreads) s.power[n] = power(octaves, n);
+
+        // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
+        F4 X[DP / 16];
+        const int e = e0 + wave * 16 + col;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int d = i * 16 + quad * 4 + k;
+                float x = 0.0f;
+                if (Whole && d < a.width && e < a.columns) {
+                    if (a.cuts) x = a.cuts[mark + static_cast<int64_t>(d) * a.columns + e];
+                    else if (a.start) x = a.start[state + static_cast<int64_t>(d) * a.state_d + static_cast<int64_t>(e) * a.state_e] * (a.reverse ? 1.0f : power(octaves, 1));
+                }
+                X[i][k] = x;
+            }
+        if (Whole && a.end && span.length == 0) {          // no token: what enters leaves
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int d = i * 16 + quad * 4 + k;
+                    if (d >= a.width || e >= a.columns) continue;
+                    const int64_t at = state + static_cast<int64_t>(d) * a.state_d + static_cast<int64_t>(e) * a.state_e;
+                    a.end[at] = a.start ? a.start[at] : 0.0f;
+                }
+        }
+
+        const int eight = tid / (DP / 4), d4 = tid % (DP / 4) * 4;          // this thread's block of a and b
+        const int ceight = tid / (kSlice / 4), c4 = tid % (kSlice / 4) * 4;  // and of c
+        Block<T> xa, xb, xc;
+        auto load_chunk = [&](int64_t at) {
+            const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
+            const int64_t row = row0 + way * at;
+            if (tid < Blocks) {
+                if (Whole) fetch(xa, pa, a.a.step, row, way, eight * 8, count, d4, a.width);
+                fetch(xb, pb, a.b.step, row, way, eight * 8, count, d4, a.width);
+            }
+            if (tid < SliceBlocks) fetch(xc, pc, a.c.step, row, way, ceight * 8, count, c4, a.columns - e0);
+        };
+        if (span.begin < span.end) load_chunk(span.begin);
+        for (int64_t at = span.begin; at < span.end; at += C) {
+            const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
+            const int64_t row = row0 + way * at;
+            __syncthreads();
+            if (tid == 0) s.odd = 0;
+            if (tid < Blocks) {
+                if (Whole) {
+                    stage_rows<T, DP, C>(s.a, xa, eight, d4);
+                    stage_rows<T, DP, C>(s.b, xb, eight, d4);
+                } else {
+                    stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+                }
+            }
+            bool odd = false;
+            if (tid < SliceBlocks) {
+                stage_turned<T, kSlice, C>(s.c, xc, ceight, c4);
+                if (Whole) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) odd |= !(fabsf(static_cast<float>(xc.x[r][j])) < INFINITY);
+                }
+            }
+            __syncthreads();
+            if constexpr (Whole) {
+                if (odd) s.odd = 1;
+                // tiles of 16 x 16: inside = g^(i-j) a_i . b_j, rows j, columns i >= j
+                constexpr int Side = C / 16, Pairs = Side * (Side + 1) / 2;
+                for (int t = wave; t < Pairs; t += kWaves) {
+                    int ti = 0;
+                    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+                    const int tj = t - ti * (ti + 1) / 2;
+                    F4 p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int d = 0; d < DP; d += 32) {
+                        H8 fa[N], fb[N];
+                        take(fa, s.a, ti * 16 + col, d + quad * 8);
+                        take(fb, s.b, tj * 16 + col, d + quad * 8);
+                        p = product<Reach>(fb, fa, p);
+                    }
+                    const int i = ti * 16 + col, j = tj * 16 + quad * 4;
+                    H4 h[M];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float v = i >= j + k ? p[k] * (s.power[i >= j + k ? i - j - k : 0] * a.inner) : 0.0f;
+                        uint16_t q[M];
+                        cut<M>(v, q);
+#pragma unroll
+                        for (int n = 0; n < M; ++n) h[n][k] = q[n];
+                    }
+#pragma unroll
+                    for (int n = 0; n < M; ++n) *reinterpret_cast<H4*>(&s.inside[n][i][j]) = h[n];
+                    // a block of 32 tokens j is taken whole: its half past the diagonal is 0
+                    if (ti == tj && (ti & 1) == 0) {
+#pragma unroll
+                        for (int n = 0; n < M; ++n) *reinterpret_cast<H4*>(&s.inside[n][i][j + 16]) = H4{0, 0, 0, 0};
+                    }
+                }
+                __syncthreads();
+                if (tid < Blocks) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+            }
+            if (at + C < span.end) load_chunk(at + C);
+            if constexpr (Whole) {
+                // out^T: rows e, columns i.  First a X, in X's own order of channels.
+                F4 o[C / 16];
+#pragma unroll
+                for (int t = 0; t < C / 16; ++t) o[t] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int d = 0; d < DP; d += 32) {
+                    H8 fx[M];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        uint16_t q[M];
+                        cut<M>(X[d / 16 + k / 4][k & 3], q);
+#pragma unroll
+                        for (int n = 0; n < M; ++n) fx[n][k] = q[n];
+                    }
+#pragma unroll
+                    for (int t = 0; t < C / 16; ++t) {
+                        H8 fa[N];
+                        take(fa, s.a, t * 16 + col, d + quad * 8);
+                        o[t] = product<Reach>(fx, fa, o[t]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < C / 16; ++t) {
+                    const float g = s.power[t * 16 + col];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[t][k] *= g;
+                }
+                if (!s.odd) {
+#pragma unroll
+                    for (int j = 0; j < C; j += 32) {
+                        H8 fc[N];
+                        take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+#pragma unroll
+                        for (int t = j / 16; t < C / 16; ++t) {
+                            H8 fp[M];
+                            take(fp, s.inside, t * 16 + col, j + quad * 8);
+                            o[t] = product<Reach>(fc, fp, o[t]);
+                        }
+                    }
+                } else {
+                    // An infinity or a NaN in c, times the 0 of a token before it, would be a
+                    // NaN there: such a chunk is summed term by term.
+                    for (int t = 0; t < C / 16; ++t)
+                        for (int j = 0; j <= t * 16 + col; ++j) {
+                            float p = 0.0f;
+                            for (int n = M - 1; n >= 0; --n) p += part(s.inside[n][t * 16 + col][j]);
+                            for (int k = 0; k < 4; ++k) {
+                                const int r = wave * 16 + quad * 4 + k;
+                                float c = 0.0f;
+                                for (int n = N - 1; n >= 0; --n) c += part(s.c[n][r][unit<C>(r, j / 8) + (j & 7)]);
+#pragma unroll
+                                for (int u = 0; u < C / 16; ++u)
+                                    if (u == t) o[u][k] = fused(p, c, o[u][k]);
+                            }
+                        }
+                }
+                if (a.out.at) {
+                    T* po = a.out.at + span.seq * a.out.seq + head * a.out.head + e0 + wave * 16 + quad * 4;
+                    const int left = a.columns - (e0 + wave * 16 + quad * 4);
+#pragma unroll
+                    for (int t = 0; t < C / 16; ++t) {
+                        const int i = t * 16 + col;
+                        if (i >= count) continue;
+                        T* to = po + (row + way * static_cast<int64_t>(i)) * a.out.step;
+                        const float x[4] = {o[t][0] * a.outer, o[t][1] * a.outer, o[t][2] * a.outer, o[t][3] * a.outer};
+                        if (left >= 4) {
+                            store<T, 4>(to, x);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (k < left) to[k] = static_cast<T>(x[k]);
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            // X' = g^n X + sum_j g^(n-j) b_j c_j, n the chunk's tokens; one power less where
+            // the state leaves a forward walk
+            const int n = count - (Whole && !a.reverse && span.last && at + C >= span.end ? 1 : 0);
+            const float keep = s.power[n];
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) X[i][k] *= keep;
+#pragma unroll
+            for (int j = 0; j < C; j += 32) {
+                H8 fc[N], fw[kExact];
+                take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int far = n - (j + quad * 8 + k);
+                    const float w = s.power[far < 0 ? 0 : far] * a.inner;
+                    float c = 0.0f;
+#pragma unroll
+                    for (int p = N - 1; p >= 0; --p) c += part(fc[p][k]);
+                    uint16_t q[kExact];
+                    cut<kExact>(w * c, q);
+#pragma unroll
+                    for (int p = 0; p < kExact; ++p) fw[p][k] = q[p];
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    H8 fb[N];
+                    take(fb, s.turned, i * 16 + col, unit<C>(i * 16 + col, j / 8 + quad));
+                    X[i] = product<kExact>(fb, fw, X[i]);
+                }
+            }
+        }
+        if (Whole ? a.end && span.last && span.length > 0 : true) {
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int d = i * 16 + quad * 4 + k;
+                    if (d >= a.width || e >= a.columns) continue;
+                    if (Whole) a.end[state + static_cast<int64_t>(d) * a.state_d + static_cast<int64_t>(e) * a.state_e] = X[i][k];
+                    else a.cuts[mark + static_cast<int64_t>(d) * a.columns + e] = X[i][k];
+                }
+        }
+    }
+}
+
+// Each segment's own state becomes the one that enters it.
+template <class T>
+__global__ void __launch_bounds__(kThreads) hawk_linear_join(const LinearArgs<T> a) {
+    const int64_t plane = static_cast<int64_t>(a.width) * a.columns, blocks = (plane + kThreads - 1) / kThreads;
+    const int64_t total = a.seqs * a.heads * blocks;
+    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+        const int64_t pair = id / blocks, i = (id - pair * blocks) * kThreads + threadIdx.x;
+        if (i >= plane) continue;
+        const int64_t seq = pair / a.heads, head = pair - seq * a.heads;
+        int64_t length = a.steps, slot = seq * a.segments;
+        if (a.offsets) {
+            const int64_t first = bound_of(a, seq);
+            length = bound_of(a, seq + 1) - first;
+            slot = first / a.segment + seq;
+        }
+        const double octaves = octaves_of(a.decay[head]);
+        const float keep = power(octaves, a.segment);
+        const int64_t d = i / a.columns, e = i - d * a.columns;
+        float x = 0.0f;
+        if (a.start) x = a.start[pair * plane + d * a.state_d + e * a.state_e] * (a.reverse ? 1.0f : power(octaves, 1));
+        for (int64_t t = 0; t == 0 || t < length; t += a.segment, ++slot) {
+            if (slot >= a.slots) break;                    // offsets that do not ascend
+            float* at = a.cuts + (slot * a.heads + head) * plane + i;
+            const float own = t + a.segment < length ? *at : 0.0f;
+            *at = x;
+            x = fused(keep, x, own);
+        }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+// One walk: which planes it reads as a, b and c.
+struct Walk {
+    const hk_head_plane *a, *b, *c, *out;
+    const float* start;
+    float* end;
+    int width, columns, state_d, state_e, reverse;
+    float inner, outer;
+};
+int walks_of(const hk_linear_attention_job& j, int vjp, Walk (&w)[3]) {
+    const int K = j.keys, V = j.values;
+    int n = 0;
+    if (!vjp) {
+        w[n++] = Walk{&j.q, &j.k, &j.v, &j.o, j.h0, j.last, K, V, V, 1, 0, 1.0f, j.scale};
+        return n;
+    }
+    if (j.bar_q.data) w[n++] = Walk{&j.bar_o, &j.v, &j.k, &j.bar_q, j.h0, nullptr, V, K, 1, V, 0, 1.0f, j.scale};
+    if (j.bar_k.data) w[n++] = Walk{&j.v, &j.bar_o, &j.q, &j.bar_k, j.bar_last, nullptr, V, K, 1, V, 1, j.scale, 1.0f};
+    if (j.bar_v.data || j.bar_h0) w[n++] = Walk{&j.k, &j.q, &j.bar_o, &j.bar_v, j.bar_last, j.bar_h0, K, V, V, 1, 1, j.scale, 1.0f};
+    return n;
+}
+
+// The tokens of a segment: one a workgroup that walks a whole sequence if that gives the
+// units four workgroups each, otherwise as many as do, 256 at least.
+struct Cut { int64_t segment, segments, slots; };
+Cut cut_of(const hk_linear_attention_job& j, int columns) {
+    const int64_t slices = (columns + kSlice - 1) / kSlice, most = j.steps > 1 ? j.steps : 1;
+    const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps;
+    int64_t each = tokens / (4 * kUnits) * j.heads * slices + 1;
+    each = each < 256 ? 256 : (each + 63) / 64 * 64;
+    if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1} : Cut{most, 1, j.seqs};
+    if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs};
+    const int64_t n = (j.steps + each - 1) / each;
+    return Cut{each, n, n * j.seqs};
+}
+size_t cuts_bytes(const hk_linear_attention_job& j, const Walk& w) {
+    const Cut c = cut_of(j, w.columns);
+    if (c.segment >= j.steps) return 0;
+    return static_cast<size_t>(c.slots) * static_cast<size_t>(j.heads) * w.width * w.columns * sizeof(float);
+}
+
+template <class T>
+Plane<const T> in(const hk_head_plane& p) { return {static_cast<const T*>(p.data), p.seq, p.step, p.head}; }
+
+int launched(const char* what) {
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error(what, err);
+}
+
+template <class T, int DP, int C>
+void launch(const LinearArgs<T>& a, hipStream_t stream) {
+    const int64_t pairs = a.slots * a.heads, total = (pairs + kDies - 1) / kDies * kDies * a.slices, most = 1 << 22;
+    const dim3 grid(static_cast<unsigned>(total < most ? total : most)), block(kThreads);
+    if (a.cuts) {
+        hipLaunchKernelGGL((hawk_linear<T, DP, C, false>), grid, block, 0, stream, a);
+        const int64_t plane = static_cast<int64_t>(a.width) * a.columns, joins = a.seqs * a.heads * ((plane + kThreads - 1) / kThreads);
+        hipLaunchKernelGGL((hawk_linear_join<T>), dim3(static_cast<unsigned>(joins < most ? joins : most)), block, 0, stream, a);
+    }
+    hipLaunchKernelGGL((hawk_linear<T, DP, C, true>), grid, block, 0, stream, a);
+}
+
+template <class T>
+int walk(const hk_linear_attention_job& j, const Walk& w, void* scratch, hipStream_t stream) {
+    LinearArgs<T> a;
+    a.a = in<T>(*w.a);
+    a.b = in<T>(*w.b);
+    a.c = in<T>(*w.c);
+    a.out = Plane<T>{static_cast<T*>(w.out->data), w.out->seq, w.out->step, w.out->head};
+    a.decay = j.decay;
+    a.start = w.start;
+    a.end = w.end;
+    a.offsets = j.offsets;
+    a.seqs = j.seqs;
+    a.steps = j.steps;
+    a.heads = j.heads;
+    const Cut c = cut_of(j, w.columns);
+    a.segment = c.segment;
+    a.segments = c.segments;
+    a.slots = c.slots;
+    a.cuts = cuts_bytes(j, w) ? static_cast<float*>(scratch) : nullptr;
+    a.state_d = w.state_d;
+    a.state_e = w.state_e;
+    a.width = w.width;
+    a.columns = w.columns;
+    a.slices = (w.columns + kSlice - 1) / kSlice;
+    a.inner = w.inner;
+    a.outer = w.outer;
+    a.offsets64 = j.offsets64;
+    a.reverse = w.reverse;
+    // more tokens a chunk cost more products inside it, fewer more passes over X
+    constexpr int C = Parts<T>::in == 1 ? 64 : 32;
+    if (w.width <= 32) launch<T, 32, C>(a, stream);
+    else if (w.width <= 64) launch<T, 64, C>(a, stream);
+    else if (w.width <= 128) launch<T, 128, C>(a, stream);
+    else launch<T, 256, 32>(a, stream);
+    return launched("hawk_linear launch");
+}
+
+template <class T>
+int all(const hk_linear_attention_job& j, int vjp, void* scratch, hipStream_t stream) {
+    Walk w[3];
+    const int n = walks_of(j, vjp, w);
+    for (int i = 0; i < n; ++i) {
+        const int rc = walk<T>(j, w[i], scratch, stream);
+        if (rc != HK_OK) return rc;
+    }
+    return HK_OK;
+}
+
+int run(const hk_linear_attention_job* job, int vjp, void* scratch, void* stream) {
+    using hawk_internal::set_error;
+    if (!job) return set_error(HK_EVALUE, "hk_linear_attention: a job is required");
+    const hk_linear_attention_job& j = *job;
+    if (j.seqs < 0 || j.steps < 0 || j.heads < 0) return set_error(HK_EVALUE, "hk_linear_attention: sizes must be >= 0");
+    if (j.keys < 1 || j.keys > kMostWidth || j.values < 1 || j.values > kMostWidth)
+        return set_error(HK_EVALUE, "hk_linear_attention: a head has 1 to 256 channels");
+    if (j.dtype != HK_F32 && j.dtype != HK_BF16 && j.dtype != HK_F16)
+        return set_error(HK_EVALUE, "hk_linear_attention: the planes' element type is 32-bit or 16-bit");
+    if (j.seqs == 0 || j.heads == 0) return HK_OK;
+    const bool tokens = j.steps > 0;
+    if (!j.decay || (tokens && (!j.q.data || !j.k.data || !j.v.data || (vjp && !j.bar_o.data))))
+        return set_error(HK_EVALUE, "hk_linear_attention: a plane is missing");
+    if (j.steps > INT64_MAX / 16 / j.seqs / j.heads)
+        return set_error(HK_EVALUE, "hk_linear_attention: the planes exceed the grid limit");
+    if (hk_linear_attention_scratch_bytes(job, vjp) && !scratch)
+        return set_error(HK_EVALUE, "hk_linear_attention: scratch is required");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (j.dtype == HK_F32) return all<float>(j, vjp, scratch, s);
+    return j.dtype == HK_BF16 ? all<bf16>(j, vjp, scratch, s) : all<f16>(j, vjp, scratch, s);
+}
+
+}  // namespace
+
+extern "C" size_t hk_linear_attention_scratch_bytes(const hk_linear_attention_job* job, int32_t vjp) {
+    if (!job || job->seqs <= 0 || job->steps <= 0 || job->heads <= 0) return 0;
+    if (job->keys < 1 || job->keys > kMostWidth || job->values < 1 || job->values > kMostWidth) return 0;
+    Walk w[3];
+    const int n = walks_of(*job, vjp, w);
+    size_t most = 0;
+    for (int i = 0; i < n; ++i) {
+        const size_t bytes = cuts_bytes(*job, w[i]);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
+
+extern "C" int hk_linear_attention(const hk_linear_attention_job* job, void* scratch, void* stream) { return run(job, 0, scratch, stream); }
+extern "C" int hk_linear_attention_vjp(const hk_linear_attention_job* job, void* scratch, void* stream) { return run(job, 1, scratch, stream); }

@@ -5,7 +5,10 @@ hold in one lane.
 * :func:`token_logp`       the log-probability of each row's target;
 * :func:`policy_loss`      the clipped policy loss with a KL term;
 * :func:`preference_loss`  the loss of pairs of sequences;
-* :func:`dropout`          dropout from a counter-based generator, no mask stored.
+* :func:`dropout`          dropout from a counter-based generator, no mask stored;
+* :func:`layer_norm`       layer norm over rows, its derivative with the weights' sums;
+* :func:`linear_attention` linear attention with a decay for each head;
+* :func:`sample`           a token drawn from each row of logits.
 
 A stage is run as a loaded kernel is: ``hawk.run(stage, **planes)`` writes the
 caller's output planes in place, on the current HIP stream or ``stream=``, and
@@ -41,7 +44,8 @@ from .runtime import Stage, _on, _stream_of, _Workspace
 
 _Tensor = torch.Tensor
 
-__all__ = ["recurrence", "token_logp", "policy_loss", "preference_loss", "dropout"]
+__all__ = ["recurrence", "token_logp", "policy_loss", "preference_loss", "dropout", "layer_norm", "linear_attention",
+           "sample"]
 
 def _current_device() -> int:
     raw = getattr(torch._C, "_cuda_getDevice", None)
@@ -183,7 +187,7 @@ class _Stage(Stage):
                          f"{torch.cuda.current_device()}")
         for n in self.writes:
             x = tensors.get(n)
-            if x is not None and any(d > 1 and st == 0 for d, st in zip(x.shape, x.stride())):
+            if x is not None and x.numel() and any(d > 1 and st == 0 for d, st in zip(x.shape, x.stride())):
                 self._refuse(f"the output {n!r} repeats memory (strides {tuple(x.stride())})")
         return tensors
 
@@ -601,6 +605,20 @@ def preference_loss(beta: float = 0.1, smoothing: float = 0.0, scale: float = 1.
 
 # -- dropout -------------------------------------------------------------------------------
 
+def _row_stride(stage, name: str, x) -> int:
+    """The distance of rows that lie evenly apart, each contiguous."""
+    if not x.numel():
+        return 0
+    dims = [(d, st) for d, st in zip(x.shape[:-1], x.stride()[:-1]) if d != 1]
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        stage._refuse(f"a row of {name!r} is contiguous, got strides {tuple(x.stride())}")
+    for (_, outer), (d, inner) in zip(dims, dims[1:]):
+        if outer != d * inner:
+            stage._refuse(f"the rows of {name!r} are not evenly apart (shape {tuple(x.shape)}, strides "
+                          f"{tuple(x.stride())})")
+    return dims[-1][1] if dims else 0
+
+
 class _Dropout(_Stage):
     values = ("seed", "offset")
 
@@ -641,23 +659,12 @@ class _Dropout(_Stage):
         slots = {}
         for n in used:
             if not whole:                   # one row alone is read as contiguous too
-                setattr(job, field[n] + "_stride", self._row_stride(n, t[n]))
+                setattr(job, field[n] + "_stride", _row_stride(self, n, t[n]))
             slots[n] = _word(_core.DropoutJob, field[n])
         slots["offset"] = _word(_core.DropoutJob, "offset_cell")
         cells = (("seed", _word(_core.DropoutJob, "seed")), ("offset", _word(_core.DropoutJob, "offset")))
         fn = _core.lib().hk_dropout
         return _Plan(job, slots, lambda ref, scratch, stream: fn(ref, stream), 0, cells=cells, entry=fn)
-
-    def _row_stride(self, name: str, x) -> int:
-        """The distance of rows that lie evenly apart, each contiguous."""
-        dims = [(d, st) for d, st in zip(x.shape[:-1], x.stride()[:-1]) if d != 1]
-        if x.shape[-1] > 1 and x.stride(-1) != 1:
-            self._refuse(f"a row of {name!r} is contiguous, got strides {tuple(x.stride())}")
-        for (_, outer), (d, inner) in zip(dims, dims[1:]):
-            if outer != d * inner:
-                self._refuse(f"the rows of {name!r} are not evenly apart (shape {tuple(x.shape)}, strides "
-                             f"{tuple(x.stride())})")
-        return dims[-1][1] if dims else 0
 
     def _value(self, name: str, x) -> int:
         if name == "offset" and (x is None or isinstance(x, torch.Tensor)):
@@ -697,3 +704,264 @@ def dropout(p: float) -> Stage:
     if (cut == 0) != (p == 0) or (cut == 65536) != (p == 1):
         raise HawkError(f"dropout: p={p!r} rounds to {cut // 65536} at the generator's resolution of 2^-16")
     return _Dropout(float(p), False)
+
+
+# -- layer norm ----------------------------------------------------------------------------
+
+class _LayerNorm(_Stage):
+    def __init__(self, eps: float, derivative: bool):
+        super().__init__()
+        self.eps, self.derivative = eps, derivative
+        self.name = "layer_norm_vjp" if derivative else "layer_norm"
+        if derivative:
+            self.reads, self.may_read = ("x", "mean", "rstd", "bar_y"), ("weight",)
+            self.writes = ("bar_x", "bar_weight", "bar_bias")
+        else:
+            self.reads, self.may_read, self.writes = ("x",), ("weight", "bias"), ("y", "mean", "rstd")
+            self.vjp = _LayerNorm(eps, True)
+            self.vjp.vjp_of = self
+
+    def _make(self, t: dict) -> _Plan:
+        job, x = _core.LayerNormJob(), t["x"]
+        job.dtype = _element(self, x.dtype, (0, 2, 3))
+        if x.dim() < 1:
+            self._refuse("x has rows of at least one axis")
+        job.cols = x.shape[-1]
+        job.rows = x.numel() // job.cols if job.cols else 0
+        for n in ("x", "y", "bar_y", "bar_x"):
+            if n not in t:
+                continue
+            if t[n].shape != x.shape or t[n].dtype != x.dtype:
+                self._refuse(f"{n!r} is {t[n].dtype} {tuple(t[n].shape)}, x is {x.dtype} {tuple(x.shape)}")
+            stride = _row_stride(self, n, t[n])
+            if n in self.writes and job.rows > 1 and stride < job.cols:
+                self._refuse(f"the rows of {n!r} overlap (strides {tuple(t[n].stride())})")
+            setattr(job, n + "_stride", stride)
+        for n in ("mean", "rstd"):
+            if n in t:
+                _vector(self, n, t[n], x.shape[:-1].numel())
+        weights = [n for n in ("weight", "bias", "bar_weight", "bar_bias") if n in t]
+        kind = t[weights[0]].dtype if weights else x.dtype
+        if kind not in (torch.float32, x.dtype):
+            self._refuse(f"{weights[0]!r} is float32 or {x.dtype}, got {kind}")
+        for n in weights:
+            if t[n].dtype != kind or tuple(t[n].shape) != (job.cols,) or not t[n].is_contiguous():
+                self._refuse(f"{n!r} is a contiguous {kind} tensor of {job.cols}, got {t[n].dtype} {tuple(t[n].shape)}")
+        job.weight_dtype = _element(self, kind, (0, 2, 3))
+        job.eps = self.eps
+        slots = {}
+        for n in t:
+            slots[n] = _word(_core.LayerNormJob, n)
+            setattr(job, n, 16)             # any address: which planes there are decides what a call works in
+        L = _core.lib()
+        fn = L.hk_layer_norm_vjp if self.derivative else L.hk_layer_norm
+        apart = tuple((out, n) for out in ("y", "mean", "rstd") for n in ("weight", "bias")) if not self.derivative else \
+            (("bar_weight", "weight"), ("bar_weight", "bar_bias"), ("bar_bias", "weight"), ("bar_x", "weight"))
+        return _Plan(job, slots, fn, int(L.hk_layer_norm_scratch_bytes(ctypes.byref(job), int(self.derivative))),
+                     apart=apart)
+
+
+def layer_norm(eps: float = 1e-5) -> Stage:
+    """Layer norm over the last axis: ``y = (x - mean) rstd weight + bias`` with
+    ``rstd = 1 / sqrt(var + eps)``.
+
+    Planes: ``x``, ``y`` (written, it may be ``x``) of one shape and type (float32,
+    bfloat16, float16), rows contiguous and evenly apart; ``weight`` and ``bias``
+    (1 and 0 if not given) of one number a column, in float32 or the planes' type;
+    ``mean`` and ``rstd`` float32, one a row, as a contiguous 1-D tensor, written
+    where given.
+
+    ``.vjp`` reads ``x``, ``weight``, ``mean``, ``rstd``, ``bar_y`` and writes those
+    given of ``bar_x`` (it may be ``x`` or ``bar_y``), ``bar_weight`` and
+    ``bar_bias`` (of the weight's type).  The sums over rows are taken in a fixed
+    order, 0 where there are no rows."""
+    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 0 <= eps < math.inf:
+        raise HawkError(f"layer_norm: eps= is a finite number from 0, got {eps!r}")
+    return _LayerNorm(float(eps), False)
+
+
+# -- linear attention ----------------------------------------------------------------------
+
+class _LinearAttention(_Stage):
+    def __init__(self, scale: float, derivative: bool):
+        super().__init__()
+        self.scale, self.derivative = scale, derivative
+        self.name = "linear_attention_vjp" if derivative else "linear_attention"
+        if derivative:
+            self.reads, self.may_read = ("q", "k", "v", "decay", "bar_o"), ("h0", "bar_last", "offsets")
+            self.writes = ("bar_q", "bar_k", "bar_v", "bar_h0")
+        else:
+            self.reads, self.may_read, self.writes = ("q", "k", "v", "decay"), ("h0", "offsets"), ("o", "last")
+            self.vjp = _LinearAttention(scale, True)
+            self.vjp.vjp_of = self
+
+    def _make(self, t: dict) -> _Plan:
+        job, q, packed = _core.LinearAttentionJob(), t["q"], t.get("offsets")
+        job.dtype = _element(self, q.dtype, (0, 2, 3))
+        if packed is None and q.dim() != 4:
+            self._refuse(f"dense planes are (sequences, steps, heads, channels), got q {tuple(q.shape)}; packed ones "
+                         "(rows, heads, channels) come with offsets")
+        if packed is not None:
+            if q.dim() != 3:
+                self._refuse(f"packed planes are (rows, heads, channels), got q {tuple(q.shape)}")
+            job.offsets64 = _integer(self, "offsets", packed)
+            if packed.numel() < 1:
+                self._refuse("offsets holds one number more than there are sequences")
+            job.seqs = packed.numel() - 1
+            job.steps, job.heads = q.shape[:2]
+        else:
+            job.seqs, job.steps, job.heads = q.shape[:3]
+        job.keys, job.values = q.shape[-1], t["v"].shape[-1] if t["v"].dim() else 0
+        for n, channels in (("q", job.keys), ("v", job.values)):
+            if not 1 <= channels <= 256:
+                self._refuse(f"a head of {n!r} has 1 to 256 channels, got {tuple(t[n].shape)}")
+        slots = {}
+        for n in ("q", "k", "v", "o", "bar_o", "bar_q", "bar_k", "bar_v"):
+            x = t.get(n)
+            if x is None:
+                continue
+            shape = (*q.shape[:-1], job.keys if n[-1] in "qk" else job.values)
+            if tuple(x.shape) != shape or x.dtype != q.dtype:
+                self._refuse(f"{n!r} is {x.dtype} {tuple(x.shape)}, where {q.dtype} {shape} goes with q "
+                             f"{tuple(q.shape)} and v {tuple(t['v'].shape)}")
+            if shape[-1] > 1 and x.stride(-1) != 1:
+                self._refuse(f"a head of {n!r} is contiguous, got strides {tuple(x.stride())}")
+            plane, strides = getattr(job, n), x.stride()
+            plane.seq = 0 if packed is not None else strides[0]
+            plane.step, plane.head = strides[-3], strides[-2]
+            plane.data = 16                 # any address: which planes there are decides what a call works in
+            slots[n] = _word(_core.LinearAttentionJob, n, "data")
+        _vector(self, "decay", t["decay"], job.heads)
+        for n in ("h0", "bar_last", "last", "bar_h0"):
+            x = t.get(n)
+            if x is None:
+                continue
+            shape = (job.seqs, job.heads, job.keys, job.values)
+            if x.dtype != torch.float32 or tuple(x.shape) != shape or not x.is_contiguous():
+                self._refuse(f"the state {n!r} is a contiguous float32 tensor {shape}, got {x.dtype} {tuple(x.shape)}")
+        for n in ("decay", "h0", "bar_last", "last", "bar_h0", "offsets"):
+            if n in t:
+                slots[n] = _word(_core.LinearAttentionJob, n)
+                setattr(job, n, 16)
+        job.scale = self.scale
+        L = _core.lib()
+        fn = L.hk_linear_attention_vjp if self.derivative else L.hk_linear_attention
+        scratch = int(L.hk_linear_attention_scratch_bytes(ctypes.byref(job), int(self.derivative)))
+        given = [n for n in self.writes if n in t]
+        read = [n for n in self.reads + self.may_read if n in t]
+        apart = [(out, n) for out in given for n in read if (out, n) != ("last", "h0")]
+        apart += [(a, b) for i, a in enumerate(given) for b in given[i + 1:]]
+        return _Plan(job, slots, fn, scratch, apart=tuple(apart))
+
+
+def linear_attention(scale: float = 1.0) -> Stage:
+    """Linear attention with a decay for each head: ``S_t = decay S_(t-1) + k_t v_t^T``,
+    ``o_t = scale q_t S_t``, from the state ``h0``.
+
+    Planes: ``q``, ``k`` ``(sequences, steps, heads, keys)`` and ``v``, ``o``
+    (written) ``(..., values)`` of one type (float32, bfloat16, float16), 1 to 256
+    channels a head, those of a head contiguous, the other axes in any order; or
+    packed ``(rows, heads, channels)`` with ``offsets``, the sequences' bounds as in
+    :func:`recurrence`.  ``decay`` float32, one a head, in [0, 1] (another gives
+    NaN); it is a constant and has no gradient.  ``h0`` (state that enters, 0 if not
+    given) and ``last`` (state that leaves, written where given; it may be ``h0``)
+    are ``(sequences, heads, keys, values)`` in float32.  One token of running
+    sequences is the same call with one step, ``h0`` and ``last``.
+
+    States and sums are held in 32 bits; products are taken to 2^-24 in the states and
+    for float32 planes, to 2^-16 of each where ``o`` is rounded to 16 bits.  A token
+    with an infinity or a NaN makes what it reaches no number (an infinity may come
+    out as a NaN) and leaves earlier tokens as they are.
+
+    ``.vjp`` reads ``q``, ``k``, ``v``, ``decay``, ``bar_o``, ``h0``, ``bar_last``,
+    ``offsets`` and writes those given of ``bar_q``, ``bar_k``, ``bar_v``,
+    ``bar_h0``.  A plane that was expanded along an axis (heads that share keys and
+    values) gets its full gradient; its own is the sum along that axis.  No output
+    may be an input or another output."""
+    if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not math.isfinite(scale):
+        raise HawkError(f"linear_attention: scale= is a finite number, got {scale!r}")
+    return _LinearAttention(float(scale), False)
+
+
+# -- sampling ------------------------------------------------------------------------------
+
+class _Sample(_Stage):
+    reads, writes = ("logits", "u"), ("token", "logp")
+    may_read = ("temperature", "top_k", "top_p", "min_p")
+
+    def __init__(self, **options):
+        self.name = "sample"
+        super().__init__()
+        self.options = options
+
+    def _make(self, t: dict) -> _Plan:
+        job, logits = _core.SampleJob(), t["logits"]
+        if logits.dim() != 2:
+            self._refuse(f"logits are (rows, vocabulary), got {tuple(logits.shape)}")
+        job.dtype = _element(self, logits.dtype, (0, 2, 3))
+        job.rows, job.vocab = logits.shape
+        if job.vocab > 1 << 22:
+            self._refuse(f"a vocabulary has at most 2^22 tokens, got {job.vocab}")
+        if job.vocab > 1 and logits.stride(1) != 1:
+            self._refuse(f"a row of 'logits' is contiguous, got strides {tuple(logits.stride())}")
+        job.row_stride = logits.stride(0)
+        u = t["u"]
+        if u.dtype not in (torch.float32, torch.float64) or tuple(u.shape) != (job.rows,) or not u.is_contiguous():
+            self._refuse(f"'u' is a contiguous float32 or float64 tensor of {job.rows}, got {u.dtype} {tuple(u.shape)}")
+        job.u64bits = int(u.dtype == torch.float64)
+        for n in ("logp", "temperature", "top_p", "min_p"):
+            if n in t:
+                _vector(self, n, t[n], job.rows)
+        for n in ("token", "top_k"):
+            if n not in t:
+                continue
+            wide = _integer(self, n, t[n])
+            if t[n].shape[0] != job.rows:
+                self._refuse(f"{n!r} has {t[n].shape[0]} rows, logits {job.rows}")
+            if n == "token":
+                job.token64 = wide
+            elif wide:
+                self._refuse("'top_k' is a contiguous 1-D int32 tensor, got torch.int64")
+        for n, v in self.options.items():
+            setattr(job, n, v)
+        slots = {n: _word(_core.SampleJob, "row_" + n if n in self.may_read else n) for n in t}
+        L = _core.lib()
+        return _Plan(job, slots, L.hk_sample, int(L.hk_sample_scratch_bytes(ctypes.byref(job))),
+                     apart=tuple((out, n) for out in self.writes for n in self.reads + self.may_read) + (("token", "logp"),))
+
+
+def sample(temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> Stage:
+    """A token drawn from each row of logits by a given random number.
+
+    With ``w = exp((logit - max) / temperature)`` and a row's tokens in descending
+    order (equal ones by index), the tokens kept are those that every filter keeps:
+    the first ``top_k`` (0: all); of these the ones before which less than ``top_p`` of
+    their whole weight has passed (1: all); those with ``w >= min_p`` (0: all); the
+    highest in any case.  The token is the first, by index, at which the kept
+    tokens' running weight passes ``u`` times their whole weight.
+
+    Planes: ``logits`` ``(rows, vocabulary)`` in float32, bfloat16 or float16, a row
+    contiguous, rows any distance apart, 2^22 tokens at most; ``u`` float32 or
+    float64, one a row in [0, 1) (below draws the first kept token, above the last);
+    written where given: ``token`` (int32 or int64) and ``logp`` (float32), the
+    token's log-probability among those kept.  ``temperature``, ``top_p``, ``min_p``
+    (float32) and ``top_k`` (int32), one a row, stand for the stage's own where given.
+
+    A temperature of 0 takes the highest logit, the first of equal ones, with a
+    ``logp`` of 0.  A row that holds a NaN, or whose ``u`` is one or whose
+    temperature is below 0 or one, gives token -1 and a NaN; a row of -inf alone
+    (nothing is allowed) token -1 and -inf; logits of +inf share the whole.  Weights
+    are summed exactly, as whole numbers of 2^-40 of the highest or less, so a call
+    repeats bit for bit.  There is no derivative: the loss reads the token's
+    ``token_logp``."""
+    def number(x):
+        return isinstance(x, (int, float)) and not isinstance(x, bool) and x == x
+    if not number(temperature) or temperature < 0:
+        raise HawkError(f"sample: temperature= is a number from 0, got {temperature!r}")
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k < 1 << 63:
+        raise HawkError(f"sample: top_k= is an int from 0, got {top_k!r}")
+    if not number(top_p) or top_p < 0:
+        raise HawkError(f"sample: top_p= is a number from 0, got {top_p!r}")
+    if not number(min_p):
+        raise HawkError(f"sample: min_p= is a number, got {min_p!r}")
+    return _Sample(temperature=float(temperature), top_k=top_k, top_p=float(top_p), min_p=float(min_p))

@@ -497,6 +497,98 @@ typedef struct hk_dropout_job {
 } hk_dropout_job;
 int hk_dropout(const hk_dropout_job* job, void* stream);
 
+/* Layer norm over the rows of [rows, cols] planes, strides in elements, a row
+ * contiguous:  xh = (x - mean) rstd, rstd = 1 / sqrt(var + eps), var the mean of
+ * (x - mean)^2,  y = xh weight + bias (NULL: 1 and 0).  dtype HK_F32, HK_BF16 or
+ * HK_F16; weight, bias and their gradients are of weight_dtype, HK_F32 or the
+ * planes' own; mean and rstd are float, one a row.
+ * hk_layer_norm reads x, weight, bias and writes y, mean, rstd (each may be NULL;
+ * y may be x).
+ * hk_layer_norm_vjp reads x, weight, mean, rstd, bar_y and writes, each may be NULL,
+ *   bar_x = rstd (g - mean(g) - xh mean(g xh)), g = bar_y weight  (it may be x or bar_y),
+ *   bar_weight = sum over rows of bar_y xh, bar_bias = sum over rows of bar_y
+ * (sums in a fixed order; 0 where there are no rows).
+ * Scratch: hk_layer_norm_scratch_bytes(job, vjp) bytes of the job with its pointers,
+ * 16-byte aligned, no contents needed. */
+typedef struct hk_layer_norm_job {
+    const void *x, *weight, *bias, *bar_y;
+    void *y, *bar_x, *bar_weight, *bar_bias;
+    float *mean, *rstd;
+    int64_t rows, cols, x_stride, y_stride, bar_y_stride, bar_x_stride;
+    float eps;
+    int32_t dtype, weight_dtype, reserved;
+} hk_layer_norm_job;
+size_t hk_layer_norm_scratch_bytes(const hk_layer_norm_job* job, int32_t vjp);
+int hk_layer_norm(const hk_layer_norm_job* job, void* scratch, void* stream);
+int hk_layer_norm_vjp(const hk_layer_norm_job* job, void* scratch, void* stream);
+
+/* A token drawn from each row of logits ([rows, vocab], element (n, v) at
+ * logits + n*row_stride + v; HK_F32, HK_BF16 or HK_F16; vocab at most 2^22) by the
+ * number u_n (double if u64bits != 0, else float).  With w_v = exp((l_v - max) / T)
+ * and a row's tokens in descending order, equal ones by index, what is kept is the
+ * shortest of
+ *   top_k tokens (0 or below, or vocab and above: all),
+ *   the tokens before which those of top_k have summed to less than top_p of their
+ *   whole sum (1 and above, or a NaN: all),
+ *   the tokens with w >= min_p (0 and below, or a NaN: all),
+ * and the highest in any case.  token is the first by index at which the sum of the
+ * kept w passes u times their whole sum (u below 0: the first kept, 1 and above: the
+ * last), logp = log(w_token / sum).  T = 0 takes the highest, the first of equal
+ * ones, and logp 0.  A row with a NaN, a NaN u or a T below 0 or NaN gives token -1 and a
+ * NaN; one of -inf alone, or without tokens, token -1 and -inf; logits of +inf share the
+ * whole.  row_temperature, row_top_p, row_min_p (float) and row_top_k (int32) are one
+ * a row and stand for temperature, top_p, min_p and top_k where not NULL.
+ * token is 64-bit if token64 != 0 else 32-bit; token and logp may be NULL.
+ * Scratch: hk_sample_scratch_bytes(job) bytes, 16-byte aligned, no contents needed. */
+typedef struct hk_sample_job {
+    const void *logits, *u;
+    const float *row_temperature, *row_top_p, *row_min_p;
+    const int32_t* row_top_k;
+    void* token;
+    float* logp;
+    int64_t rows, vocab, row_stride, top_k;
+    double temperature, top_p, min_p;
+    int32_t dtype, u64bits, token64, reserved;
+} hk_sample_job;
+size_t hk_sample_scratch_bytes(const hk_sample_job* job);
+int hk_sample(const hk_sample_job* job, void* scratch, void* stream);
+
+/* A (sequence, step, head, channel) plane: element (s, t, h, c) at
+ * data + s*seq + t*step + h*head + c elements.  A packed plane has no sequence
+ * axis (seq unused): its steps are the rows of all sequences in turn. */
+typedef struct hk_head_plane {
+    void* data;
+    int64_t seq, step, head;
+} hk_head_plane;
+
+/* Linear attention with a decay for each head: from S_(-1) = h0 (0 if NULL),
+ *   S_t = decay S_(t-1) + k_t v_t^T,  o_t = scale q_t S_t,  last = S_(T-1).
+ * q, k have `keys` channels, v, o `values`, both 1 to 256; dtype HK_F32, HK_BF16 or
+ * HK_F16.  decay is a float for each head in [0, 1] (another gives NaN); states (h0,
+ * last, bar_last, bar_h0) are [seqs, heads, keys, values] row-major float, each may
+ * be NULL.  offsets as in hk_recurrence_job.  What a token that is no number (or
+ * infinite) reaches is no number, earlier tokens stay what they are.
+ * hk_linear_attention writes o (data may be NULL) and last, which may be h0.
+ * hk_linear_attention_vjp reads q, k, v, bar_o, h0, bar_last and writes, each may be
+ * NULL:  W_t = decay W_(t+1) + scale q_t bar_o_t^T with decay W_T = bar_last,
+ *   bar_q_t = scale S_t bar_o_t, bar_k_t = W_t v_t, bar_v_t = k_t W_t,
+ *   bar_h0 = decay W_0.
+ * No output may be an input (but last h0), nor bar_h0 bar_last.
+ * Scratch: hk_linear_attention_scratch_bytes(job, vjp) bytes of the job with its
+ * pointers, 16-byte aligned, no contents needed. */
+typedef struct hk_linear_attention_job {
+    hk_head_plane q, k, v, o, bar_o, bar_q, bar_k, bar_v;
+    const float *decay, *h0, *bar_last;
+    float *last, *bar_h0;
+    const void* offsets;
+    int64_t seqs, steps, heads;
+    float scale;
+    int32_t keys, values, dtype, offsets64, reserved;
+} hk_linear_attention_job;
+size_t hk_linear_attention_scratch_bytes(const hk_linear_attention_job* job, int32_t vjp);
+int hk_linear_attention(const hk_linear_attention_job* job, void* scratch, void* stream);
+int hk_linear_attention_vjp(const hk_linear_attention_job* job, void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
