@@ -33,9 +33,8 @@ namespace {
 
 using namespace hawk_vec;
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kSlice = 16 * kWaves;        // columns of c that a workgroup has
-constexpr int kMostWidth = 256;
+constexpr int kJoinThreads = 256;
+constexpr int kMostWidth = 256, kMostWalks = 3;
 constexpr int64_t kUnits = 256, kDies = 8;
 
 typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
@@ -167,26 +166,51 @@ __device__ __forceinline__ float power(double octaves, int64_t n) { return exp2f
 // tiles of 16 after each other.
 __device__ __forceinline__ int staged(int d) { return (d & ~31) | (d >> 2 & 3) << 3 | (d >> 4 & 1) << 2 | (d & 3); }
 
-// Eight tokens by four channels, a thread's share of a chunk's plane.
+// Eight tokens by four channels, a thread's share of a chunk's plane: of `count` tokens
+// from `chunk` on those from i, of `width` channels those from d.  What is not there is 0.
 template <class T> struct Block { Raw<T, 4> x[8]; };
-template <class T>
-__device__ __forceinline__ void fetch(Block<T>& x, const T* head, int64_t step, int64_t row, int way, int i, int count, int d, int width) {
+template <class R>
+__device__ __forceinline__ void shift_down(R& x, int n) {
+    if constexpr (sizeof(R) == 8) {
+        x = __builtin_bit_cast(R, __builtin_bit_cast(uint64_t, x) >> (16 * n));
+    } else {
+        if (n & 1) x = R{x[1], x[2], x[3], 0.0f};
+        if (n & 2) x = R{x[2], x[3], 0.0f, 0.0f};
+    }
+}
+template <class T, int C>
+__device__ __forceinline__ void fetch(Block<T>& x, const T* chunk, int64_t step, int i, int count, int d, int width) {
+    const Raw<T, 4> zero = splat<T, 4>(static_cast<T>(0.0f));
+    if (count == C && (width & 3) == 0) {
+        const T* at = chunk + i * step + d;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x.x[r] = zero;
+        if (d < width)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x.x[r] = load_raw<T, 4>(at + r * step);
+        return;
+    }
+    // Every load is of a token and of channels that are there; a row's last channels are
+    // read from its end and moved down.
+    const int from = d < width - 4 ? d : width < 4 ? 0 : width - 4;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        x.x[r] = splat<T, 4>(static_cast<T>(0.0f));
-        if (i + r >= count) continue;
-        const T* at = head + (row + way * static_cast<int64_t>(i + r)) * step + d;
-        if (d + 4 <= width) {
-            x.x[r] = load_raw<T, 4>(at);
+        const T* at = chunk + (i + r < count ? i + r : count - 1) * step + from;
+        Raw<T, 4> v = zero;
+        if (width >= 4) {
+            v = load_raw<T, 4>(at);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (d + j < width) x.x[r][j] = at[j];
+            for (int j = 0; j < 3; ++j)
+                if (j < width) v[j] = at[j];
         }
+        shift_down(v, (d - from) & 3);
+        x.x[r] = i + r < count && d < width ? v : zero;
     }
 }
 
-template <class T, int DP, int C>
+// A workgroup of W waves has 16 W columns of c.
+template <class T, int DP, int C, int W>
 struct Tiles {
     static constexpr int N = Parts<T>::in, M = Parts<T>::made;
     static constexpr int Wide = DP + 8, Long = C + 8;      // rows are 16 bytes apart in the banks
@@ -195,7 +219,7 @@ struct Tiles {
         uint16_t b[N][C][Wide];                            // rows of tokens, until the products of a and b are made
         uint16_t turned[N][DP][Long];                      // rows of channels
     };
-    uint16_t c[N][kSlice][Long];
+    uint16_t c[N][16 * W][Long];
     uint16_t inside[M][C][Long];                           // g^(i-j) a_i . b_j
     float power[C + 1];
     int odd;                                               // c holds what is no number
@@ -245,15 +269,22 @@ __device__ __forceinline__ void take(H8 (&out)[N], const uint16_t (&from)[N][R][
     for (int n = 0; n < N; ++n) out[n] = *reinterpret_cast<const H8*>(&from[n][row][at]);
 }
 
-// Workgroup (slot, head, slice).  Whole: the walk over a segment; otherwise what the
-// segment leaves of its own, for the sum over the segments before another.
-template <class T, int DP, int C, bool Whole>
-__global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
+template <class T>
+struct Walks { LinearArgs<T> walk[kMostWalks]; };
+
+// Workgroup (slot, head, slice) of a walk.  Whole: the walk over a segment; otherwise
+// what the segment leaves of its own, for the sum over the segments before another.
+template <class T, int DP, int C, int W, bool Whole>
+__global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 ? 4 : 2)) hawk_linear(const Walks<T> walks) {
     constexpr int N = Parts<T>::in, M = Parts<T>::made, Reach = Parts<T>::reach;
-    constexpr int Blocks = C / 8 * (DP / 4), SliceBlocks = C / 8 * (kSlice / 4);
-    static_assert(Blocks <= kThreads && SliceBlocks <= kThreads, "a block a thread");
-    __shared__ Tiles<T, DP, C> s;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, quad = lane >> 4;
+    constexpr int Threads = 64 * W, Slice = 16 * W;
+    constexpr int Blocks = C / 8 * (DP / 4), SliceBlocks = C / 8 * (Slice / 4);
+    static_assert(Blocks <= Threads && SliceBlocks <= Threads, "a block a thread");
+    // Where the threads are twice b's blocks, the upper half has a's, in the same registers.
+    constexpr bool Halves = 2 * Blocks <= Threads;
+    const LinearArgs<T>& a = walks.walk[blockIdx.y];
+    __shared__ Tiles<T, DP, C, W> s;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, quad = lane >> 4;
     const int64_t pairs = a.slots * a.heads, group = kDies * a.slices;
     const int64_t total = (pairs + kDies - 1) / kDies * group;
     for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
@@ -265,73 +296,67 @@ __global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
         const Span span = span_of(a, slot);
         if (!span.real || (!Whole && span.last)) continue;
         const double octaves = octaves_of(a.decay[head]);
-        const int e0 = slice * kSlice;
+        const int e0 = slice * Slice, columns = a.columns - e0;
         const int64_t plane = static_cast<int64_t>(a.width) * a.columns;
         const int64_t state = (span.seq * a.heads + head) * plane, mark = pair * plane;
         const int way = a.reverse ? -1 : 1;
         const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
-        const T* pa = Whole ? a.a.at + span.seq * a.a.seq + head * a.a.head : nullptr;
-        const T* pb = a.b.at + span.seq * a.b.seq + head * a.b.head;
-        const T* pc = a.c.at + span.seq * a.c.seq + head * a.c.head + e0;
         __syncthreads();                                   // the run before is done with the tiles
-        for (int n = tid; n <= C; n += kThreads) s.power[n] = power(octaves, n);
+        for (int n = tid; n <= C; n += Threads) s.power[n] = power(octaves, n);
 
         // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
         F4 X[DP / 16];
         const int e = e0 + wave * 16 + col;
+        const float* enters = Whole ? a.cuts && span.length > 0 ? a.cuts + mark : a.start ? a.start + state : nullptr : nullptr;
+        const bool joined = enters && a.cuts && span.length > 0;
+        const int enters_d = joined ? a.columns : a.state_d, enters_e = joined ? 1 : a.state_e;
+        const float once = joined || a.reverse || span.length == 0 ? 1.0f : power(octaves, 1);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int d = i * 16 + quad * 4 + k;
-                float x = 0.0f;
-                if (Whole && d < a.width && e < a.columns) {
-                    if (a.cuts) x = a.cuts[mark + static_cast<int64_t>(d) * a.columns + e];
-                    else if (a.start) x = a.start[state + static_cast<int64_t>(d) * a.state_d + static_cast<int64_t>(e) * a.state_e] * (a.reverse ? 1.0f : power(octaves, 1));
-                }
-                X[i][k] = x;
-            }
-        if (Whole && a.end && span.length == 0) {          // no token: what enters leaves
+        for (int i = 0; i < DP / 16; ++i) X[i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (enters)
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int d = i * 16 + quad * 4 + k;
-                    if (d >= a.width || e >= a.columns) continue;
-                    const int64_t at = state + static_cast<int64_t>(d) * a.state_d + static_cast<int64_t>(e) * a.state_e;
-                    a.end[at] = a.start ? a.start[at] : 0.0f;
+                    const float x = enters[(d < a.width ? d : 0) * enters_d + (e < a.columns ? e : 0) * enters_e];
+                    X[i][k] = d < a.width && e < a.columns ? x * once : 0.0f;
                 }
-        }
 
-        const int eight = tid / (DP / 4), d4 = tid % (DP / 4) * 4;          // this thread's block of a and b
-        const int ceight = tid / (kSlice / 4), c4 = tid % (kSlice / 4) * 4;  // and of c
+        // this thread's blocks
+        const bool upper = Halves && tid >= Blocks;
+        const int btid = upper ? tid - Blocks : tid, ctid = tid - (Threads - SliceBlocks);
+        const int eight = btid / (DP / 4), d4 = btid % (DP / 4) * 4, ceight = ctid / (Slice / 4), c4 = ctid % (Slice / 4) * 4;
+        const bool has = btid < Blocks;
+        const Plane<const T>&pa = a.a, &pb = upper ? a.a : a.b, &pc = a.c;
         Block<T> xa, xb, xc;
+        auto fetch_from = [&](Block<T>& x, const Plane<const T>& p, int64_t at, int i, int count, int d, int width, int first) {
+            fetch<T, C>(x, p.at + span.seq * p.seq + head * p.head + (row0 + way * at) * p.step + first, way * p.step, i, count, d, width);
+        };
         auto load_chunk = [&](int64_t at) {
             const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
-            const int64_t row = row0 + way * at;
-            if (tid < Blocks) {
-                if (Whole) fetch(xa, pa, a.a.step, row, way, eight * 8, count, d4, a.width);
-                fetch(xb, pb, a.b.step, row, way, eight * 8, count, d4, a.width);
+            if (has) {
+                if (Whole && !Halves) fetch_from(xa, pa, at, eight * 8, count, d4, a.width, 0);
+                if (Whole || !upper) fetch_from(xb, pb, at, eight * 8, count, d4, a.width, 0);
             }
-            if (tid < SliceBlocks) fetch(xc, pc, a.c.step, row, way, ceight * 8, count, c4, a.columns - e0);
+            if (ctid >= 0) fetch_from(xc, pc, at, ceight * 8, count, c4, columns, e0);
         };
         if (span.begin < span.end) load_chunk(span.begin);
         for (int64_t at = span.begin; at < span.end; at += C) {
             const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
-            const int64_t row = row0 + way * at;
             __syncthreads();
             if (tid == 0) s.odd = 0;
-            if (tid < Blocks) {
-                if (Whole) {
-                    stage_rows<T, DP, C>(s.a, xa, eight, d4);
-                    stage_rows<T, DP, C>(s.b, xb, eight, d4);
+            if (has) {
+                if constexpr (Whole) {
+                    if (!Halves) stage_rows<T, DP, C>(s.a, xa, eight, d4);
+                    stage_rows<T, DP, C>(upper ? s.a : s.b, xb, eight, d4);
                 } else {
-                    stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+                    if (!upper) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
                 }
             }
             bool odd = false;
-            if (tid < SliceBlocks) {
-                stage_turned<T, kSlice, C>(s.c, xc, ceight, c4);
+            if (ctid >= 0) {
+                stage_turned<T, Slice, C>(s.c, xc, ceight, c4);
                 if (Whole) {
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
@@ -344,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
                 if (odd) s.odd = 1;
                 // tiles of 16 x 16: inside = g^(i-j) a_i . b_j, rows j, columns i >= j
                 constexpr int Side = C / 16, Pairs = Side * (Side + 1) / 2;
-                for (int t = wave; t < Pairs; t += kWaves) {
+                for (int t = wave; t < Pairs; t += W) {
                     int ti = 0;
                     while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
                     const int tj = t - ti * (ti + 1) / 2;
@@ -375,7 +400,7 @@ __global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
                     }
                 }
                 __syncthreads();
-                if (tid < Blocks) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+                if (has && !upper) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
             }
             if (at + C < span.end) load_chunk(at + C);
             if constexpr (Whole) {
@@ -421,35 +446,41 @@ __global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
                 } else {
                     // An infinity or a NaN in c, times the 0 of a token before it, would be a
                     // NaN there: such a chunk is summed term by term.
-                    for (int t = 0; t < C / 16; ++t)
-                        for (int j = 0; j <= t * 16 + col; ++j) {
-                            float p = 0.0f;
-                            for (int n = M - 1; n >= 0; --n) p += part(s.inside[n][t * 16 + col][j]);
-                            for (int k = 0; k < 4; ++k) {
-                                const int r = wave * 16 + quad * 4 + k;
-                                float c = 0.0f;
-                                for (int n = N - 1; n >= 0; --n) c += part(s.c[n][r][unit<C>(r, j / 8) + (j & 7)]);
+#pragma unroll 1
+                    for (int j = 0; j < C; ++j) {
+                        float c[4];
 #pragma unroll
-                                for (int u = 0; u < C / 16; ++u)
-                                    if (u == t) o[u][k] = fused(p, c, o[u][k]);
-                            }
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = wave * 16 + quad * 4 + k;
+                            c[k] = 0.0f;
+#pragma unroll
+                            for (int n = N - 1; n >= 0; --n) c[k] += part(s.c[n][r][unit<C>(r, j / 8) + (j & 7)]);
                         }
+#pragma unroll
+                        for (int t = 0; t < C / 16; ++t) {
+                            float p = 0.0f;
+#pragma unroll
+                            for (int n = M - 1; n >= 0; --n) p += part(s.inside[n][t * 16 + col][j]);
+                            if (j <= t * 16 + col)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) o[t][k] = fused(p, c[k], o[t][k]);
+                        }
+                    }
                 }
-                if (a.out.at) {
-                    T* po = a.out.at + span.seq * a.out.seq + head * a.out.head + e0 + wave * 16 + quad * 4;
-                    const int left = a.columns - (e0 + wave * 16 + quad * 4);
+                const int left = columns - (wave * 16 + quad * 4);
+                if (a.out.at && left > 0) {
+                    T* to = a.out.at + span.seq * a.out.seq + head * a.out.head + (row0 + way * (at + col)) * a.out.step + e0 + wave * 16 + quad * 4;
 #pragma unroll
                     for (int t = 0; t < C / 16; ++t) {
-                        const int i = t * 16 + col;
-                        if (i >= count) continue;
-                        T* to = po + (row + way * static_cast<int64_t>(i)) * a.out.step;
+                        if (t * 16 + col >= count) continue;
                         const float x[4] = {o[t][0] * a.outer, o[t][1] * a.outer, o[t][2] * a.outer, o[t][3] * a.outer};
+                        T* here = to + (way * t * 16) * a.out.step;
                         if (left >= 4) {
-                            store<T, 4>(to, x);
+                            store<T, 4>(here, x);
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (k < left) to[k] = static_cast<T>(x[k]);
+                            for (int k = 0; k < 3; ++k)
+                                if (k < left) here[k] = static_cast<T>(x[k]);
                         }
                     }
                 }
@@ -487,27 +518,27 @@ __global__ void __launch_bounds__(kThreads) hawk_linear(const LinearArgs<T> a) {
                 }
             }
         }
-        if (Whole ? a.end && span.last && span.length > 0 : true) {
+        float* leaves = !Whole ? a.cuts + mark : a.end && span.last ? a.end + state : nullptr;
+        const int leaves_d = Whole ? a.state_d : a.columns, leaves_e = Whole ? a.state_e : 1;
+        if (leaves && e < a.columns)
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int d = i * 16 + quad * 4 + k;
-                    if (d >= a.width || e >= a.columns) continue;
-                    if (Whole) a.end[state + static_cast<int64_t>(d) * a.state_d + static_cast<int64_t>(e) * a.state_e] = X[i][k];
-                    else a.cuts[mark + static_cast<int64_t>(d) * a.columns + e] = X[i][k];
+                    if (d < a.width) leaves[d * leaves_d + e * leaves_e] = X[i][k];
                 }
-        }
     }
 }
 
 // Each segment's own state becomes the one that enters it.
 template <class T>
-__global__ void __launch_bounds__(kThreads) hawk_linear_join(const LinearArgs<T> a) {
-    const int64_t plane = static_cast<int64_t>(a.width) * a.columns, blocks = (plane + kThreads - 1) / kThreads;
+__global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> walks) {
+    const LinearArgs<T>& a = walks.walk[blockIdx.y];
+    const int64_t plane = static_cast<int64_t>(a.width) * a.columns, blocks = (plane + kJoinThreads - 1) / kJoinThreads;
     const int64_t total = a.seqs * a.heads * blocks;
     for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
-        const int64_t pair = id / blocks, i = (id - pair * blocks) * kThreads + threadIdx.x;
+        const int64_t pair = id / blocks, i = (id - pair * blocks) * kJoinThreads + threadIdx.x;
         if (i >= plane) continue;
         const int64_t seq = pair / a.heads, head = pair - seq * a.heads;
         int64_t length = a.steps, slot = seq * a.segments;
@@ -541,7 +572,7 @@ struct Walk {
     int width, columns, state_d, state_e, reverse;
     float inner, outer;
 };
-int walks_of(const hk_linear_attention_job& j, int vjp, Walk (&w)[3]) {
+int walks_of(const hk_linear_attention_job& j, int vjp, Walk (&w)[kMostWalks]) {
     const int K = j.keys, V = j.values;
     int n = 0;
     if (!vjp) {
@@ -554,13 +585,18 @@ int walks_of(const hk_linear_attention_job& j, int vjp, Walk (&w)[3]) {
     return n;
 }
 
-// The tokens of a segment: one a workgroup that walks a whole sequence if that gives the
-// units four workgroups each, otherwise as many as do, 256 at least.
+// The columns of a workgroup: 128 where there are more than 64, which shares what is
+// staged of a and b, and the products of the two, among twice the waves.
+int slice_of(int columns) { return columns > 64 ? 128 : 64; }
+int bucket_of(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : width <= 128 ? 128 : 256; }
+
+// The tokens of a segment: a whole sequence if that gives the units two workgroups each,
+// otherwise as many as do, 256 at least.
 struct Cut { int64_t segment, segments, slots; };
 Cut cut_of(const hk_linear_attention_job& j, int columns) {
-    const int64_t slices = (columns + kSlice - 1) / kSlice, most = j.steps > 1 ? j.steps : 1;
+    const int64_t slices = (columns + slice_of(columns) - 1) / slice_of(columns), most = j.steps > 1 ? j.steps : 1;
     const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps;
-    int64_t each = tokens / (4 * kUnits) * j.heads * slices + 1;
+    int64_t each = tokens / (2 * kUnits) * j.heads * slices + 1;
     each = each < 256 ? 256 : (each + 63) / 64 * 64;
     if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1} : Cut{most, 1, j.seqs};
     if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs};
@@ -581,20 +617,39 @@ int launched(const char* what) {
     return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error(what, err);
 }
 
-template <class T, int DP, int C>
-void launch(const LinearArgs<T>& a, hipStream_t stream) {
-    const int64_t pairs = a.slots * a.heads, total = (pairs + kDies - 1) / kDies * kDies * a.slices, most = 1 << 22;
-    const dim3 grid(static_cast<unsigned>(total < most ? total : most)), block(kThreads);
-    if (a.cuts) {
-        hipLaunchKernelGGL((hawk_linear<T, DP, C, false>), grid, block, 0, stream, a);
-        const int64_t plane = static_cast<int64_t>(a.width) * a.columns, joins = a.seqs * a.heads * ((plane + kThreads - 1) / kThreads);
-        hipLaunchKernelGGL((hawk_linear_join<T>), dim3(static_cast<unsigned>(joins < most ? joins : most)), block, 0, stream, a);
+template <class T, int DP, int C, int W>
+void launch(const Walks<T>& walks, int n, hipStream_t stream) {
+    int64_t total = 0, joins = 0;
+    bool cuts = false;
+    for (int i = 0; i < n; ++i) {
+        const LinearArgs<T>& a = walks.walk[i];
+        const int64_t each = (a.slots * a.heads + kDies - 1) / kDies * kDies * a.slices;
+        const int64_t plane = static_cast<int64_t>(a.width) * a.columns, parts = a.seqs * a.heads * ((plane + kJoinThreads - 1) / kJoinThreads);
+        total = each > total ? each : total;
+        joins = parts > joins ? parts : joins;
+        cuts = cuts || a.cuts;
     }
-    hipLaunchKernelGGL((hawk_linear<T, DP, C, true>), grid, block, 0, stream, a);
+    const int64_t most = 1 << 20;
+    const dim3 grid(static_cast<unsigned>(total < most ? total : most), static_cast<unsigned>(n)), block(64 * W);
+    if (cuts) {
+        hipLaunchKernelGGL((hawk_linear<T, DP, C, W, false>), grid, block, 0, stream, walks);
+        hipLaunchKernelGGL((hawk_linear_join<T>), dim3(static_cast<unsigned>(joins < most ? joins : most), static_cast<unsigned>(n)),
+                           dim3(kJoinThreads), 0, stream, walks);
+    }
+    hipLaunchKernelGGL((hawk_linear<T, DP, C, W, true>), grid, block, 0, stream, walks);
+}
+template <class T, int W>
+void launch(const Walks<T>& walks, int n, int bucket, hipStream_t stream) {
+    // more tokens a chunk cost more products inside it, fewer more passes over X
+    constexpr int C = Parts<T>::in == 1 ? 64 : 32;
+    if (bucket == 32) launch<T, 32, C, W>(walks, n, stream);
+    else if (bucket == 64) launch<T, 64, C, W>(walks, n, stream);
+    else if (bucket == 128) launch<T, 128, C, W>(walks, n, stream);
+    else launch<T, 256, 32, W>(walks, n, stream);
 }
 
 template <class T>
-int walk(const hk_linear_attention_job& j, const Walk& w, void* scratch, hipStream_t stream) {
+LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w) {
     LinearArgs<T> a;
     a.a = in<T>(*w.a);
     a.b = in<T>(*w.b);
@@ -611,31 +666,43 @@ int walk(const hk_linear_attention_job& j, const Walk& w, void* scratch, hipStre
     a.segment = c.segment;
     a.segments = c.segments;
     a.slots = c.slots;
-    a.cuts = cuts_bytes(j, w) ? static_cast<float*>(scratch) : nullptr;
     a.state_d = w.state_d;
     a.state_e = w.state_e;
     a.width = w.width;
     a.columns = w.columns;
-    a.slices = (w.columns + kSlice - 1) / kSlice;
+    a.slices = (w.columns + slice_of(w.columns) - 1) / slice_of(w.columns);
     a.inner = w.inner;
     a.outer = w.outer;
     a.offsets64 = j.offsets64;
     a.reverse = w.reverse;
-    // more tokens a chunk cost more products inside it, fewer more passes over X
-    constexpr int C = Parts<T>::in == 1 ? 64 : 32;
-    if (w.width <= 32) launch<T, 32, C>(a, stream);
-    else if (w.width <= 64) launch<T, 64, C>(a, stream);
-    else if (w.width <= 128) launch<T, 128, C>(a, stream);
-    else launch<T, 256, 32>(a, stream);
-    return launched("hawk_linear launch");
+    a.cuts = nullptr;
+    return a;
 }
 
+// Walks of one form are one launch.
 template <class T>
 int all(const hk_linear_attention_job& j, int vjp, void* scratch, hipStream_t stream) {
-    Walk w[3];
+    Walk w[kMostWalks];
     const int n = walks_of(j, vjp, w);
+    char* room = static_cast<char*>(scratch);
+    bool done[kMostWalks] = {};
     for (int i = 0; i < n; ++i) {
-        const int rc = walk<T>(j, w[i], scratch, stream);
+        if (done[i]) continue;
+        Walks<T> walks = {};
+        int count = 0;
+        const int bucket = bucket_of(w[i].width), slice = slice_of(w[i].columns);
+        for (int k = i; k < n; ++k) {
+            if (done[k] || bucket_of(w[k].width) != bucket || slice_of(w[k].columns) != slice) continue;
+            done[k] = true;
+            walks.walk[count] = args_of<T>(j, w[k]);
+            const size_t bytes = cuts_bytes(j, w[k]);
+            if (bytes) walks.walk[count].cuts = reinterpret_cast<float*>(room);
+            room += bytes;
+            ++count;
+        }
+        if (slice == 64) launch<T, 4>(walks, count, bucket, stream);
+        else launch<T, 8>(walks, count, bucket, stream);
+        const int rc = launched("hawk_linear launch");
         if (rc != HK_OK) return rc;
     }
     return HK_OK;
@@ -668,14 +735,11 @@ int run(const hk_linear_attention_job* job, int vjp, void* scratch, void* stream
 extern "C" size_t hk_linear_attention_scratch_bytes(const hk_linear_attention_job* job, int32_t vjp) {
     if (!job || job->seqs <= 0 || job->steps <= 0 || job->heads <= 0) return 0;
     if (job->keys < 1 || job->keys > kMostWidth || job->values < 1 || job->values > kMostWidth) return 0;
-    Walk w[3];
+    Walk w[kMostWalks];
     const int n = walks_of(*job, vjp, w);
-    size_t most = 0;
-    for (int i = 0; i < n; ++i) {
-        const size_t bytes = cuts_bytes(*job, w[i]);
-        most = bytes > most ? bytes : most;
-    }
-    return most;
+    size_t bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += cuts_bytes(*job, w[i]);
+    return bytes;
 }
 
 extern "C" int hk_linear_attention(const hk_linear_attention_job* job, void* scratch, void* stream) { return run(job, 0, scratch, stream); }
