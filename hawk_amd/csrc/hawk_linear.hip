@@ -46,6 +46,10 @@ __device__ __forceinline__ F4 product(const H8& a, const H8& b, const F4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf8, a), __builtin_bit_cast(Bf8, b), c, 0, 0, 0);
 }
 
+// What is written before is scheduled before: the reads of a loop that is unrolled are
+// not all made first, which would take the registers of all of them.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // The N bf16 parts of a number, each the nearest to what the ones before leave: two are
 // within 2^-18 of it, three are a number of 24 bits.
 template <int N>
@@ -166,48 +170,57 @@ __device__ __forceinline__ float power(double octaves, int64_t n) { return exp2f
 // tiles of 16 after each other.
 __device__ __forceinline__ int staged(int d) { return (d & ~31) | (d >> 2 & 3) << 3 | (d >> 4 & 1) << 2 | (d & 3); }
 
-// Eight tokens by four channels, a thread's share of a chunk's plane: of `count` tokens
-// from `chunk` on those from i, of `width` channels those from d.  What is not there is 0.
+// Eight tokens by four channels, a thread's share of a chunk's plane.  A load is always of
+// tokens and channels that are there: past a chunk's last token it is that token's, past a
+// row's last channels the row's last four.  settle() makes of it what the share is, when
+// it is staged: the loads of the next chunk are under way meanwhile.
 template <class T> struct Block { Raw<T, 4> x[8]; };
-template <class R>
-__device__ __forceinline__ void shift_down(R& x, int n) {
-    if constexpr (sizeof(R) == 8) {
-        x = __builtin_bit_cast(R, __builtin_bit_cast(uint64_t, x) >> (16 * n));
+template <class T, int C, bool Narrow>
+__device__ __forceinline__ void fetch(Block<T>& x, const T* at, int64_t step, int i, int count, int width) {
+    if (Narrow && width < 4) {             // rows without four channels
+        at += (i < count ? 0 : count - 1 - i) * step;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            x.x[r] = Raw<T, 4>{at[0], at[width > 1], at[width > 2 ? 2 : 0], static_cast<T>(0.0f)};
+            at += i + r + 1 < count ? step : 0;
+        }
+    } else if (count == C) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x.x[r] = load_raw<T, 4>(at + r * step);
     } else {
-        if (n & 1) x = R{x[1], x[2], x[3], 0.0f};
-        if (n & 2) x = R{x[2], x[3], 0.0f, 0.0f};
+        at += (i < count ? 0 : count - 1 - i) * step;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            x.x[r] = load_raw<T, 4>(at);
+            at += i + r + 1 < count ? step : 0;
+        }
     }
 }
-template <class T, int C>
-__device__ __forceinline__ void fetch(Block<T>& x, const T* chunk, int64_t step, int i, int count, int d, int width) {
-    const Raw<T, 4> zero = splat<T, 4>(static_cast<T>(0.0f));
-    if (count == C && (width & 3) == 0) {
-        const T* at = chunk + i * step + d;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) x.x[r] = zero;
-        if (d < width)
-#pragma unroll
-            for (int r = 0; r < 8; ++r) x.x[r] = load_raw<T, 4>(at + r * step);
-        return;
+template <class R>
+__device__ __forceinline__ R moved_down(const R& x, int n) {
+    if constexpr (sizeof(R) == 8) {
+        return __builtin_bit_cast(R, __builtin_bit_cast(uint64_t, x) >> (16 * n));
+    } else {
+        const R y = n & 1 ? R{x[1], x[2], x[3], 0.0f} : x;
+        return n & 2 ? R{y[2], y[3], 0.0f, 0.0f} : y;
     }
-    // Every load is of a token and of channels that are there; a row's last channels are
-    // read from its end and moved down.
-    const int from = d < width - 4 ? d : width < 4 ? 0 : width - 4;
+}
+// left: the channels of the share that are in the row, 4 at most.
+template <class T>
+__device__ __forceinline__ void settle(Block<T>& x, int i, int count, int left, int width) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        const T* at = chunk + (i + r < count ? i + r : count - 1) * step + from;
-        Raw<T, 4> v = zero;
-        if (width >= 4) {
-            v = load_raw<T, 4>(at);
-        } else {
+        const Raw<T, 4> v = width < 4 ? x.x[r] : moved_down(x.x[r], left > 0 ? 4 - left : 0);
+        x.x[r] = i + r < count && left > 0 ? v : splat<T, 4>(static_cast<T>(0.0f));
+        if (width < 4)
 #pragma unroll
-            for (int j = 0; j < 3; ++j)
-                if (j < width) v[j] = at[j];
-        }
-        shift_down(v, (d - from) & 3);
-        x.x[r] = i + r < count && d < width ? v : zero;
+            for (int j = 1; j < 4; ++j)
+                if (j >= width) x.x[r][j] = static_cast<T>(0.0f);
     }
 }
+// The channel a share's load begins at, from the one it is of.
+__device__ __forceinline__ int loaded(int d, int width) { return d + 4 <= width ? d : width < 4 ? 0 : width - 4; }
+__device__ __forceinline__ int left_of(int d, int width) { return width - d < 4 ? width - d : 4; }
 
 // A workgroup of W waves has 16 W columns of c.
 template <class T, int DP, int C, int W>
@@ -275,260 +288,274 @@ struct Walks { LinearArgs<T> walk[kMostWalks]; };
 // Workgroup (slot, head, slice) of a walk.  Whole: the walk over a segment; otherwise
 // what the segment leaves of its own, for the sum over the segments before another.
 template <class T, int DP, int C, int W, bool Whole>
-__global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 ? 4 : 2)) hawk_linear(const Walks<T> walks) {
+__global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 ? 4 : 2)) hawk_linear(const Walks<T> walks, const int64_t before) {
     constexpr int N = Parts<T>::in, M = Parts<T>::made, Reach = Parts<T>::reach;
     constexpr int Threads = 64 * W, Slice = 16 * W;
     constexpr int Blocks = C / 8 * (DP / 4), SliceBlocks = C / 8 * (Slice / 4);
     static_assert(Blocks <= Threads && SliceBlocks <= Threads, "a block a thread");
-    // Where the threads are twice b's blocks, the upper half has a's, in the same registers.
-    constexpr bool Halves = 2 * Blocks <= Threads;
+    // Where the waves are twice b's, the upper half has a's shares, in the same registers.
+    constexpr bool Halves = 2 * Blocks <= Threads && Blocks % 64 == 0;
     const LinearArgs<T>& a = walks.walk[blockIdx.y];
     __shared__ Tiles<T, DP, C, W> s;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, quad = lane >> 4;
     const int64_t pairs = a.slots * a.heads, group = kDies * a.slices;
-    const int64_t total = (pairs + kDies - 1) / kDies * group;
-    for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
-        // a pair's slices go to one die, whose L2 has a and b for all of them
-        const int64_t pair = id / group * kDies + id % kDies;
-        const int slice = static_cast<int>(id / kDies % a.slices);
-        if (pair >= pairs) continue;
-        const int64_t slot = pair / a.heads, head = pair - slot * a.heads;
-        const Span span = span_of(a, slot);
-        if (!span.real || (!Whole && span.last)) continue;
-        const double octaves = octaves_of(a.decay[head]);
-        const int e0 = slice * Slice, columns = a.columns - e0;
-        const int64_t plane = static_cast<int64_t>(a.width) * a.columns;
-        const int64_t state = (span.seq * a.heads + head) * plane, mark = pair * plane;
-        const int way = a.reverse ? -1 : 1;
-        const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
-        __syncthreads();                                   // the run before is done with the tiles
-        for (int n = tid; n <= C; n += Threads) s.power[n] = power(octaves, n);
+    // a pair's slices go to one die, whose L2 has a and b for all of them
+    const int64_t id = before + blockIdx.x, pair = id / group * kDies + id % kDies;
+    const int slice = static_cast<int>(id / kDies % a.slices);
+    if (pair >= pairs) return;
+    const int64_t slot = pair / a.heads, head = pair - slot * a.heads;
+    const Span span = span_of(a, slot);
+    if (!span.real || (!Whole && span.last)) return;
+    const double octaves = octaves_of(a.decay[head]);
+    const int e0 = slice * Slice, columns = a.columns - e0;
+    const int64_t plane = static_cast<int64_t>(a.width) * a.columns;
+    const int64_t state = (span.seq * a.heads + head) * plane, mark = pair * plane;
+    const int way = a.reverse ? -1 : 1;
+    const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
+    for (int n = tid; n <= C; n += Threads) s.power[n] = power(octaves, n);
 
-        // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
-        F4 X[DP / 16];
-        const int e = e0 + wave * 16 + col;
-        const float* enters = Whole ? a.cuts && span.length > 0 ? a.cuts + mark : a.start ? a.start + state : nullptr : nullptr;
-        const bool joined = enters && a.cuts && span.length > 0;
-        const int enters_d = joined ? a.columns : a.state_d, enters_e = joined ? 1 : a.state_e;
-        const float once = joined || a.reverse || span.length == 0 ? 1.0f : power(octaves, 1);
+    // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
+    F4 X[DP / 16];
+    const int e = e0 + wave * 16 + col;
+    const float* enters = Whole ? a.cuts && span.length > 0 ? a.cuts + mark : a.start ? a.start + state : nullptr : nullptr;
+    const bool joined = enters && a.cuts && span.length > 0;
+    const int enters_d = joined ? a.columns : a.state_d, enters_e = joined ? 1 : a.state_e;
+    const float once = joined || a.reverse || span.length == 0 ? 1.0f : power(octaves, 1);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) X[i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (enters)
+    for (int i = 0; i < DP / 16; ++i) X[i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (enters)
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
+        for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int d = i * 16 + quad * 4 + k;
-                    const float x = enters[(d < a.width ? d : 0) * enters_d + (e < a.columns ? e : 0) * enters_e];
-                    X[i][k] = d < a.width && e < a.columns ? x * once : 0.0f;
-                }
+            for (int k = 0; k < 4; ++k) {
+                const int d = i * 16 + quad * 4 + k;
+                const float x = enters[(d < a.width ? d : 0) * enters_d + (e < a.columns ? e : 0) * enters_e];
+                X[i][k] = d < a.width && e < a.columns ? x * once : 0.0f;
+            }
 
-        // this thread's blocks
-        const bool upper = Halves && tid >= Blocks;
-        const int btid = upper ? tid - Blocks : tid, ctid = tid - (Threads - SliceBlocks);
-        const int eight = btid / (DP / 4), d4 = btid % (DP / 4) * 4, ceight = ctid / (Slice / 4), c4 = ctid % (Slice / 4) * 4;
-        const bool has = btid < Blocks;
-        const Plane<const T>&pa = a.a, &pb = upper ? a.a : a.b, &pc = a.c;
-        Block<T> xa, xb, xc;
-        auto fetch_from = [&](Block<T>& x, const Plane<const T>& p, int64_t at, int i, int count, int d, int width, int first) {
-            fetch<T, C>(x, p.at + span.seq * p.seq + head * p.head + (row0 + way * at) * p.step + first, way * p.step, i, count, d, width);
-        };
-        auto load_chunk = [&](int64_t at) {
-            const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
-            if (has) {
-                if (Whole && !Halves) fetch_from(xa, pa, at, eight * 8, count, d4, a.width, 0);
-                if (Whole || !upper) fetch_from(xb, pb, at, eight * 8, count, d4, a.width, 0);
+    // this thread's shares, and where the chunk to be loaded has them
+    const bool upper = Halves && wave * 64 >= Blocks;
+    const int btid = upper ? tid - Blocks : tid, ctid = tid - (Threads - SliceBlocks);
+    const int eight = btid / (DP / 4), d4 = btid % (DP / 4) * 4, ceight = ctid / (Slice / 4), c4 = ctid % (Slice / 4) * 4;
+    const bool has = btid < Blocks && (Whole || !upper);
+    Block<T> xa, xb, xc;
+    auto first = [&](const Plane<const T>& p, int i, int d, int width) {
+        return p.at + span.seq * p.seq + head * p.head + (row0 + way * (span.begin + i)) * p.step + loaded(d, width);
+    };
+    const int64_t step_a = way * a.a.step, step_b = way * (upper ? a.a.step : a.b.step), step_c = way * a.c.step;
+    const T *at_a = nullptr, *at_b = nullptr, *at_c = nullptr;
+    if (has) {
+        if (Whole && !Halves) at_a = first(a.a, eight * 8, d4, a.width);
+        at_b = first(upper ? a.a : a.b, eight * 8, d4, a.width);
+    }
+    if (ctid >= 0) at_c = first(a.c, ceight * 8, e0 + c4, a.columns);
+    auto load_chunk = [&](int64_t at) {
+        const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
+        if (has) {
+            if (Whole && !Halves) fetch<T, C, DP == 32>(xa, at_a, step_a, eight * 8, count, a.width);
+            fetch<T, C, DP == 32>(xb, at_b, step_b, eight * 8, count, a.width);
+        }
+        if (ctid >= 0) fetch<T, C, W == 4>(xc, at_c, step_c, ceight * 8, count, a.columns);
+        at_a += C * step_a;
+        at_b += C * step_b;
+        at_c += C * step_c;
+    };
+    if (span.begin < span.end) load_chunk(span.begin);
+    for (int64_t at = span.begin; at < span.end; at += C) {
+        const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
+        __syncthreads();
+        if (tid == 0) s.odd = 0;
+        if (has) {
+            if (count < C || a.width < DP) {
+                if (Whole && !Halves) settle(xa, eight * 8, count, left_of(d4, a.width), a.width);
+                settle(xb, eight * 8, count, left_of(d4, a.width), a.width);
             }
-            if (ctid >= 0) fetch_from(xc, pc, at, ceight * 8, count, c4, columns, e0);
-        };
-        if (span.begin < span.end) load_chunk(span.begin);
-        for (int64_t at = span.begin; at < span.end; at += C) {
-            const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
-            __syncthreads();
-            if (tid == 0) s.odd = 0;
-            if (has) {
-                if constexpr (Whole) {
-                    if (!Halves) stage_rows<T, DP, C>(s.a, xa, eight, d4);
-                    stage_rows<T, DP, C>(upper ? s.a : s.b, xb, eight, d4);
-                } else {
-                    if (!upper) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
-                }
-            }
-            bool odd = false;
-            if (ctid >= 0) {
-                stage_turned<T, Slice, C>(s.c, xc, ceight, c4);
-                if (Whole) {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) odd |= !(fabsf(static_cast<float>(xc.x[r][j])) < INFINITY);
-                }
-            }
-            __syncthreads();
             if constexpr (Whole) {
-                if (odd) s.odd = 1;
-                // tiles of 16 x 16: inside = g^(i-j) a_i . b_j, rows j, columns i >= j
-                constexpr int Side = C / 16, Pairs = Side * (Side + 1) / 2;
-                for (int t = wave; t < Pairs; t += W) {
-                    int ti = 0;
-                    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-                    const int tj = t - ti * (ti + 1) / 2;
-                    F4 p = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int d = 0; d < DP; d += 32) {
-                        H8 fa[N], fb[N];
-                        take(fa, s.a, ti * 16 + col, d + quad * 8);
-                        take(fb, s.b, tj * 16 + col, d + quad * 8);
-                        p = product<Reach>(fb, fa, p);
-                    }
-                    const int i = ti * 16 + col, j = tj * 16 + quad * 4;
-                    H4 h[M];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float v = i >= j + k ? p[k] * (s.power[i >= j + k ? i - j - k : 0] * a.inner) : 0.0f;
-                        uint16_t q[M];
-                        cut<M>(v, q);
-#pragma unroll
-                        for (int n = 0; n < M; ++n) h[n][k] = q[n];
-                    }
-#pragma unroll
-                    for (int n = 0; n < M; ++n) *reinterpret_cast<H4*>(&s.inside[n][i][j]) = h[n];
-                    // a block of 32 tokens j is taken whole: its half past the diagonal is 0
-                    if (ti == tj && (ti & 1) == 0) {
-#pragma unroll
-                        for (int n = 0; n < M; ++n) *reinterpret_cast<H4*>(&s.inside[n][i][j + 16]) = H4{0, 0, 0, 0};
-                    }
-                }
-                __syncthreads();
-                if (has && !upper) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+                if (!Halves) stage_rows<T, DP, C>(s.a, xa, eight, d4);
+                stage_rows<T, DP, C>(upper ? s.a : s.b, xb, eight, d4);
+            } else {
+                stage_turned<T, DP, C>(s.turned, xb, eight, d4);
             }
-            if (at + C < span.end) load_chunk(at + C);
-            if constexpr (Whole) {
-                // out^T: rows e, columns i.  First a X, in X's own order of channels.
-                F4 o[C / 16];
+        }
+        bool odd = false;
+        if (ctid >= 0) {
+            if (count < C || columns < Slice) settle(xc, ceight * 8, count, left_of(e0 + c4, a.columns), a.columns);
+            stage_turned<T, Slice, C>(s.c, xc, ceight, c4);
+            if (Whole) {
 #pragma unroll
-                for (int t = 0; t < C / 16; ++t) o[t] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int r = 0; r < 8; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) odd |= !(fabsf(static_cast<float>(xc.x[r][j])) < INFINITY);
+            }
+        }
+        __syncthreads();
+        if constexpr (Whole) {
+            if (odd) s.odd = 1;
+            // tiles of 16 x 16: inside = g^(i-j) a_i . b_j, rows j, columns i >= j
+            constexpr int Side = C / 16, Pairs = Side * (Side + 1) / 2;
+            for (int t = wave; t < Pairs; t += W) {
+                int ti = 0;
+                while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+                const int tj = t - ti * (ti + 1) / 2;
+                F4 p = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int d = 0; d < DP; d += 32) {
-                    H8 fx[M];
+                    H8 fa[N], fb[N];
+                    take(fa, s.a, ti * 16 + col, d + quad * 8);
+                    take(fb, s.b, tj * 16 + col, d + quad * 8);
+                    p = product<Reach>(fb, fa, p);
+                    in_order();
+                }
+                const int i = ti * 16 + col, j = tj * 16 + quad * 4;
+                H4 h[M];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        uint16_t q[M];
-                        cut<M>(X[d / 16 + k / 4][k & 3], q);
+                for (int k = 0; k < 4; ++k) {
+                    const float v = i >= j + k ? p[k] * (s.power[i >= j + k ? i - j - k : 0] * a.inner) : 0.0f;
+                    uint16_t q[M];
+                    cut<M>(v, q);
 #pragma unroll
-                        for (int n = 0; n < M; ++n) fx[n][k] = q[n];
-                    }
+                    for (int n = 0; n < M; ++n) h[n][k] = q[n];
+                }
 #pragma unroll
-                    for (int t = 0; t < C / 16; ++t) {
-                        H8 fa[N];
-                        take(fa, s.a, t * 16 + col, d + quad * 8);
-                        o[t] = product<Reach>(fx, fa, o[t]);
-                    }
+                for (int n = 0; n < M; ++n) *reinterpret_cast<H4*>(&s.inside[n][i][j]) = h[n];
+                // a block of 32 tokens j is taken whole: its half past the diagonal is 0
+                if (ti == tj && (ti & 1) == 0) {
+#pragma unroll
+                    for (int n = 0; n < M; ++n) *reinterpret_cast<H4*>(&s.inside[n][i][j + 16]) = H4{0, 0, 0, 0};
+                }
+            }
+            __syncthreads();
+            if (has && !upper) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+        }
+        if (at + C < span.end) load_chunk(at + C);
+        if constexpr (Whole) {
+            // out^T: rows e, columns i.  First a X, in X's own order of channels.
+            F4 o[C / 16];
+#pragma unroll
+            for (int t = 0; t < C / 16; ++t) o[t] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int d = 0; d < DP; d += 32) {
+                H8 fx[M];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    uint16_t q[M];
+                    cut<M>(X[d / 16 + k / 4][k & 3], q);
+#pragma unroll
+                    for (int n = 0; n < M; ++n) fx[n][k] = q[n];
                 }
 #pragma unroll
                 for (int t = 0; t < C / 16; ++t) {
-                    const float g = s.power[t * 16 + col];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[t][k] *= g;
+                    H8 fa[N];
+                    take(fa, s.a, t * 16 + col, d + quad * 8);
+                    o[t] = product<Reach>(fx, fa, o[t]);
                 }
-                if (!s.odd) {
+                in_order();
+            }
 #pragma unroll
-                    for (int j = 0; j < C; j += 32) {
-                        H8 fc[N];
-                        take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+            for (int t = 0; t < C / 16; ++t) {
+                const float g = s.power[t * 16 + col];
 #pragma unroll
-                        for (int t = j / 16; t < C / 16; ++t) {
-                            H8 fp[M];
-                            take(fp, s.inside, t * 16 + col, j + quad * 8);
-                            o[t] = product<Reach>(fc, fp, o[t]);
-                        }
+                for (int k = 0; k < 4; ++k) o[t][k] *= g;
+            }
+            if (!s.odd) {
+#pragma unroll
+                for (int j = 0; j < C; j += 32) {
+                    H8 fc[N];
+                    take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+#pragma unroll
+                    for (int t = j / 16; t < C / 16; ++t) {
+                        H8 fp[M];
+                        take(fp, s.inside, t * 16 + col, j + quad * 8);
+                        o[t] = product<Reach>(fc, fp, o[t]);
                     }
-                } else {
-                    // An infinity or a NaN in c, times the 0 of a token before it, would be a
-                    // NaN there: such a chunk is summed term by term.
+                    in_order();
+                }
+            } else {
+                // An infinity or a NaN in c, times the 0 of a token before it, would be a
+                // NaN there: such a chunk is summed term by term.
 #pragma unroll 1
-                    for (int j = 0; j < C; ++j) {
-                        float c[4];
+                for (int j = 0; j < C; ++j) {
+                    float c[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int r = wave * 16 + quad * 4 + k;
-                            c[k] = 0.0f;
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = wave * 16 + quad * 4 + k;
+                        c[k] = 0.0f;
 #pragma unroll
-                            for (int n = N - 1; n >= 0; --n) c[k] += part(s.c[n][r][unit<C>(r, j / 8) + (j & 7)]);
-                        }
-#pragma unroll
-                        for (int t = 0; t < C / 16; ++t) {
-                            float p = 0.0f;
-#pragma unroll
-                            for (int n = M - 1; n >= 0; --n) p += part(s.inside[n][t * 16 + col][j]);
-                            if (j <= t * 16 + col)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) o[t][k] = fused(p, c[k], o[t][k]);
-                        }
+                        for (int n = N - 1; n >= 0; --n) c[k] += part(s.c[n][r][unit<C>(r, j / 8) + (j & 7)]);
                     }
-                }
-                const int left = columns - (wave * 16 + quad * 4);
-                if (a.out.at && left > 0) {
-                    T* to = a.out.at + span.seq * a.out.seq + head * a.out.head + (row0 + way * (at + col)) * a.out.step + e0 + wave * 16 + quad * 4;
 #pragma unroll
                     for (int t = 0; t < C / 16; ++t) {
-                        if (t * 16 + col >= count) continue;
-                        const float x[4] = {o[t][0] * a.outer, o[t][1] * a.outer, o[t][2] * a.outer, o[t][3] * a.outer};
-                        T* here = to + (way * t * 16) * a.out.step;
-                        if (left >= 4) {
-                            store<T, 4>(here, x);
-                        } else {
+                        float p = 0.0f;
 #pragma unroll
-                            for (int k = 0; k < 3; ++k)
-                                if (k < left) here[k] = static_cast<T>(x[k]);
-                        }
+                        for (int n = M - 1; n >= 0; --n) p += part(s.inside[n][t * 16 + col][j]);
+                        if (j <= t * 16 + col)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[t][k] = fused(p, c[k], o[t][k]);
                     }
                 }
-                __syncthreads();
             }
-            // X' = g^n X + sum_j g^(n-j) b_j c_j, n the chunk's tokens; one power less where
-            // the state leaves a forward walk
-            const int n = count - (Whole && !a.reverse && span.last && at + C >= span.end ? 1 : 0);
-            const float keep = s.power[n];
+            const int left = columns - (wave * 16 + quad * 4);
+            if (a.out.at && left > 0) {
+                T* to = a.out.at + span.seq * a.out.seq + head * a.out.head + (row0 + way * (at + col)) * a.out.step + e0 + wave * 16 + quad * 4;
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
+                for (int t = 0; t < C / 16; ++t) {
+                    if (t * 16 + col >= count) continue;
+                    const float x[4] = {o[t][0] * a.outer, o[t][1] * a.outer, o[t][2] * a.outer, o[t][3] * a.outer};
+                    T* here = to + (way * t * 16) * a.out.step;
+                    if (left >= 4) {
+                        store<T, 4>(here, x);
+                    } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) X[i][k] *= keep;
-#pragma unroll
-            for (int j = 0; j < C; j += 32) {
-                H8 fc[N], fw[kExact];
-                take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int far = n - (j + quad * 8 + k);
-                    const float w = s.power[far < 0 ? 0 : far] * a.inner;
-                    float c = 0.0f;
-#pragma unroll
-                    for (int p = N - 1; p >= 0; --p) c += part(fc[p][k]);
-                    uint16_t q[kExact];
-                    cut<kExact>(w * c, q);
-#pragma unroll
-                    for (int p = 0; p < kExact; ++p) fw[p][k] = q[p];
+                        for (int k = 0; k < 3; ++k)
+                            if (k < left) here[k] = static_cast<T>(x[k]);
+                    }
                 }
+            }
+            __syncthreads();
+        }
+        // X' = g^n X + sum_j g^(n-j) b_j c_j, n the chunk's tokens; one power less where
+        // the state leaves a forward walk
+        const int n = count - (Whole && !a.reverse && span.last && at + C >= span.end ? 1 : 0);
+        const float keep = s.power[n];
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    H8 fb[N];
-                    take(fb, s.turned, i * 16 + col, unit<C>(i * 16 + col, j / 8 + quad));
-                    X[i] = product<kExact>(fb, fw, X[i]);
-                }
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) X[i][k] *= keep;
+#pragma unroll
+        for (int j = 0; j < C; j += 32) {
+            H8 fc[N], fw[kExact];
+            take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int far = n - (j + quad * 8 + k);
+                const float w = s.power[far < 0 ? 0 : far] * a.inner;
+                float c = 0.0f;
+#pragma unroll
+                for (int p = N - 1; p >= 0; --p) c += part(fc[p][k]);
+                uint16_t q[kExact];
+                cut<kExact>(w * c, q);
+#pragma unroll
+                for (int p = 0; p < kExact; ++p) fw[p][k] = q[p];
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                H8 fb[N];
+                take(fb, s.turned, i * 16 + col, unit<C>(i * 16 + col, j / 8 + quad));
+                X[i] = product<kExact>(fb, fw, X[i]);
+                if (i & 1) in_order();
             }
         }
-        float* leaves = !Whole ? a.cuts + mark : a.end && span.last ? a.end + state : nullptr;
-        const int leaves_d = Whole ? a.state_d : a.columns, leaves_e = Whole ? a.state_e : 1;
-        if (leaves && e < a.columns)
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int d = i * 16 + quad * 4 + k;
-                    if (d < a.width) leaves[d * leaves_d + e * leaves_e] = X[i][k];
-                }
     }
+    float* leaves = !Whole ? a.cuts + mark : a.end && span.last ? a.end + state : nullptr;
+    const int leaves_d = Whole ? a.state_d : a.columns, leaves_e = Whole ? a.state_e : 1;
+    if (leaves && e < a.columns)
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int d = i * 16 + quad * 4 + k;
+                if (d < a.width) leaves[d * leaves_d + e * leaves_e] = X[i][k];
+            }
 }
 
 // Each segment's own state becomes the one that enters it.
@@ -630,13 +657,19 @@ void launch(const Walks<T>& walks, int n, hipStream_t stream) {
         cuts = cuts || a.cuts;
     }
     const int64_t most = 1 << 20;
-    const dim3 grid(static_cast<unsigned>(total < most ? total : most), static_cast<unsigned>(n)), block(64 * W);
+    auto each = [&](auto kernel) {                         // launches stay below 2^32 threads
+        for (int64_t before = 0; before < total; before += most) {
+            const int64_t left = total - before;
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(left < most ? left : most), static_cast<unsigned>(n)), dim3(64 * W), 0, stream,
+                               walks, before);
+        }
+    };
     if (cuts) {
-        hipLaunchKernelGGL((hawk_linear<T, DP, C, W, false>), grid, block, 0, stream, walks);
+        each(hawk_linear<T, DP, C, W, false>);
         hipLaunchKernelGGL((hawk_linear_join<T>), dim3(static_cast<unsigned>(joins < most ? joins : most), static_cast<unsigned>(n)),
                            dim3(kJoinThreads), 0, stream, walks);
     }
-    hipLaunchKernelGGL((hawk_linear<T, DP, C, W, true>), grid, block, 0, stream, walks);
+    each(hawk_linear<T, DP, C, W, true>);
 }
 template <class T, int W>
 void launch(const Walks<T>& walks, int n, int bucket, hipStream_t stream) {
