@@ -237,6 +237,33 @@ struct Tiles {
     float power[C + 1];
     int odd;                                               // c holds what is no number
 };
+// A number told to the compiler anew, so that what is computed from it (the tiles'
+// addresses) is computed where it is used, and holds no registers through a loop.
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// A thread's shares of the planes: of a and b, and of c.
+template <int DP, int C, int W>
+struct Shares {
+    static constexpr int Threads = 64 * W, Slice = 16 * W, Blocks = C / 8 * (DP / 4), SliceBlocks = C / 8 * (Slice / 4);
+    static_assert(Blocks <= Threads && SliceBlocks <= Threads, "a share a thread");
+    // Where the waves are twice b's, the upper half has a's shares, in the same registers.
+    static constexpr bool Halves = 2 * Blocks <= Threads && Blocks % 64 == 0;
+    int eight, d, c_eight, c;      // the eight tokens and the four channels
+    bool has, has_c;
+    __device__ __forceinline__ Shares(int tid, int wave) {
+        const int b = Halves ? tid % Blocks : tid, k = tid - (Threads - SliceBlocks);
+        eight = b / (DP / 4);
+        d = b % (DP / 4) * 4;
+        c_eight = k / (Slice / 4);
+        c = k % (Slice / 4) * 4;
+        has = Blocks % 64 == 0 ? Halves ? wave * 64 < 2 * Blocks : wave * 64 < Blocks : b < Blocks;
+        has_c = SliceBlocks % 64 == 0 ? wave * 64 >= Threads - SliceBlocks : k >= 0;
+    }
+};
+
 // Eight tokens' unit of a row of channels lies turned by d / 4: lanes that write, or read,
 // neighbouring rows then meet different banks.
 template <int C>
@@ -290,11 +317,9 @@ struct Walks { LinearArgs<T> walk[kMostWalks]; };
 template <class T, int DP, int C, int W, bool Whole>
 __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 ? 4 : 2)) hawk_linear(const Walks<T> walks, const int64_t before) {
     constexpr int N = Parts<T>::in, M = Parts<T>::made, Reach = Parts<T>::reach;
-    constexpr int Threads = 64 * W, Slice = 16 * W;
-    constexpr int Blocks = C / 8 * (DP / 4), SliceBlocks = C / 8 * (Slice / 4);
-    static_assert(Blocks <= Threads && SliceBlocks <= Threads, "a block a thread");
-    // Where the waves are twice b's, the upper half has a's shares, in the same registers.
-    constexpr bool Halves = 2 * Blocks <= Threads && Blocks % 64 == 0;
+    typedef Shares<DP, C, W> Mine;
+    constexpr int Threads = Mine::Threads, Slice = Mine::Slice;
+    constexpr bool Halves = Mine::Halves;
     const LinearArgs<T>& a = walks.walk[blockIdx.y];
     __shared__ Tiles<T, DP, C, W> s;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, quad = lane >> 4;
@@ -334,53 +359,53 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             }
 
     // this thread's shares, and where the chunk to be loaded has them
-    const bool upper = Halves && wave * 64 >= Blocks;
-    const int btid = upper ? tid - Blocks : tid, ctid = tid - (Threads - SliceBlocks);
-    const int eight = btid / (DP / 4), d4 = btid % (DP / 4) * 4, ceight = ctid / (Slice / 4), c4 = ctid % (Slice / 4) * 4;
-    const bool has = btid < Blocks && (Whole || !upper);
+    const bool upper = Halves && wave * 64 >= Mine::Blocks;
+    const Mine at_first(tid, wave);
     Block<T> xa, xb, xc;
     auto first = [&](const Plane<const T>& p, int i, int d, int width) {
         return p.at + span.seq * p.seq + head * p.head + (row0 + way * (span.begin + i)) * p.step + loaded(d, width);
     };
     const int64_t step_a = way * a.a.step, step_b = way * (upper ? a.a.step : a.b.step), step_c = way * a.c.step;
     const T *at_a = nullptr, *at_b = nullptr, *at_c = nullptr;
-    if (has) {
-        if (Whole && !Halves) at_a = first(a.a, eight * 8, d4, a.width);
-        at_b = first(upper ? a.a : a.b, eight * 8, d4, a.width);
+    if (at_first.has) {
+        if (Whole && !Halves) at_a = first(a.a, at_first.eight * 8, at_first.d, a.width);
+        at_b = first(upper ? a.a : a.b, at_first.eight * 8, at_first.d, a.width);
     }
-    if (ctid >= 0) at_c = first(a.c, ceight * 8, e0 + c4, a.columns);
-    auto load_chunk = [&](int64_t at) {
+    if (at_first.has_c) at_c = first(a.c, at_first.c_eight * 8, e0 + at_first.c, a.columns);
+    auto load_chunk = [&](const Mine& my, int64_t at) {
         const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
-        if (has) {
-            if (Whole && !Halves) fetch<T, C, DP == 32>(xa, at_a, step_a, eight * 8, count, a.width);
-            fetch<T, C, DP == 32>(xb, at_b, step_b, eight * 8, count, a.width);
+        if (my.has && (Whole || !upper)) {
+            if (Whole && !Halves) fetch<T, C, DP == 32>(xa, at_a, step_a, my.eight * 8, count, a.width);
+            fetch<T, C, DP == 32>(xb, at_b, step_b, my.eight * 8, count, a.width);
         }
-        if (ctid >= 0) fetch<T, C, W == 4>(xc, at_c, step_c, ceight * 8, count, a.columns);
+        if (my.has_c) fetch<T, C, W == 4>(xc, at_c, step_c, my.c_eight * 8, count, a.columns);
         at_a += C * step_a;
         at_b += C * step_b;
         at_c += C * step_c;
     };
-    if (span.begin < span.end) load_chunk(span.begin);
+    if (span.begin < span.end) load_chunk(at_first, span.begin);
     for (int64_t at = span.begin; at < span.end; at += C) {
         const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
         __syncthreads();
         if (tid == 0) s.odd = 0;
-        if (has) {
+        const int now = afresh(tid), col = now & 15, quad = now >> 4 & 3;
+        const Mine my(now, wave);
+        if (my.has && (Whole || !upper)) {
             if (count < C || a.width < DP) {
-                if (Whole && !Halves) settle(xa, eight * 8, count, left_of(d4, a.width), a.width);
-                settle(xb, eight * 8, count, left_of(d4, a.width), a.width);
+                if (Whole && !Halves) settle(xa, my.eight * 8, count, left_of(my.d, a.width), a.width);
+                settle(xb, my.eight * 8, count, left_of(my.d, a.width), a.width);
             }
             if constexpr (Whole) {
-                if (!Halves) stage_rows<T, DP, C>(s.a, xa, eight, d4);
-                stage_rows<T, DP, C>(upper ? s.a : s.b, xb, eight, d4);
+                if (!Halves) stage_rows<T, DP, C>(s.a, xa, my.eight, my.d);
+                stage_rows<T, DP, C>(upper ? s.a : s.b, xb, my.eight, my.d);
             } else {
-                stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+                stage_turned<T, DP, C>(s.turned, xb, my.eight, my.d);
             }
         }
         bool odd = false;
-        if (ctid >= 0) {
-            if (count < C || columns < Slice) settle(xc, ceight * 8, count, left_of(e0 + c4, a.columns), a.columns);
-            stage_turned<T, Slice, C>(s.c, xc, ceight, c4);
+        if (my.has_c) {
+            if (count < C || columns < Slice) settle(xc, my.c_eight * 8, count, left_of(e0 + my.c, a.columns), a.columns);
+            stage_turned<T, Slice, C>(s.c, xc, my.c_eight, my.c);
             if (Whole) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
@@ -425,9 +450,9 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
                 }
             }
             __syncthreads();
-            if (has && !upper) stage_turned<T, DP, C>(s.turned, xb, eight, d4);
+            if (my.has && !upper) stage_turned<T, DP, C>(s.turned, xb, my.eight, my.d);
         }
-        if (at + C < span.end) load_chunk(at + C);
+        if (at + C < span.end) load_chunk(my, at + C);
         if constexpr (Whole) {
             // out^T: rows e, columns i.  First a X, in X's own order of channels.
             F4 o[C / 16];
