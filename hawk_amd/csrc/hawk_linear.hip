@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 namespace {
 
@@ -218,6 +219,30 @@ __device__ __forceinline__ void settle(Block<T>& x, int i, int count, int left, 
                 if (j >= width) x.x[r][j] = static_cast<T>(0.0f);
     }
 }
+// Whether a share holds what is no number: the largest of its magnitudes as whole numbers.
+template <class T>
+__device__ __forceinline__ bool no_number(const Block<T>& x) {
+    if constexpr (sizeof(T) == 2) {
+        typedef uint16_t H2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t W2 __attribute__((ext_vector_type(2)));
+        constexpr uint16_t least = std::is_same_v<T, bf16> ? 0x7f80 : 0x7c00;
+        H2 most = {0, 0};
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const W2 w = __builtin_bit_cast(W2, x.x[r]) & 0x7fff7fffu;
+            const uint32_t one = w[0], two = w[1];
+            most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_bit_cast(H2, one), __builtin_bit_cast(H2, two)));
+        }
+        return most[0] >= least || most[1] >= least;
+    } else {
+        uint32_t most = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(uint32_t, static_cast<float>(x.x[r][j])) & 0x7fffffffu);
+        return most >= 0x7f800000u;
+    }
+}
 // The channel a share's load begins at, from the one it is of.
 __device__ __forceinline__ int loaded(int d, int width) { return d + 4 <= width ? d : width < 4 ? 0 : width - 4; }
 __device__ __forceinline__ int left_of(int d, int width) { return width - d < 4 ? width - d : 4; }
@@ -235,6 +260,7 @@ struct Tiles {
     uint16_t c[N][16 * W][Long];
     uint16_t inside[M][C][Long];                           // g^(i-j) a_i . b_j
     float power[C + 1];
+    alignas(16) float weight[C];                           // what a token of the chunk has in X'
     int odd;                                               // c holds what is no number
 };
 // A number told to the compiler anew, so that what is computed from it (the tiles'
@@ -264,10 +290,9 @@ struct Shares {
     }
 };
 
-// Eight tokens' unit of a row of channels lies turned by d / 4: lanes that write, or read,
-// neighbouring rows then meet different banks.
-template <int C>
-__device__ __forceinline__ int unit(int d, int eight) { return ((eight + (d >> 2)) & (C / 8 - 1)) * 8; }
+// Where eight tokens' unit of a row of channels lies: eight lanes that read neighbouring
+// rows, or write every fourth one, meet the banks once each.
+__device__ __forceinline__ int unit(int d, int eight) { return (eight ^ (d >> 4 & 1)) * 8; }
 
 template <class T, int DP, int C>
 __device__ __forceinline__ void stage_rows(uint16_t (&to)[Parts<T>::in][C][DP + 8], const Block<T>& x, int eight, int d) {
@@ -300,7 +325,7 @@ __device__ __forceinline__ void stage_turned(uint16_t (&to)[Parts<T>::in][R][C +
             for (int n = 0; n < N; ++n) h[n][r] = p[n];
         }
 #pragma unroll
-        for (int n = 0; n < N; ++n) *reinterpret_cast<H8*>(&to[n][d + j][unit<C>(d, eight)]) = h[n];
+        for (int n = 0; n < N; ++n) *reinterpret_cast<H8*>(&to[n][d + j][unit(d, eight)]) = h[n];
     }
 }
 template <int N, int R, int W>
@@ -362,32 +387,29 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
     const bool upper = Halves && wave * 64 >= Mine::Blocks;
     const Mine at_first(tid, wave);
     Block<T> xa, xb, xc;
-    auto first = [&](const Plane<const T>& p, int i, int d, int width) {
-        return p.at + span.seq * p.seq + head * p.head + (row0 + way * (span.begin + i)) * p.step + loaded(d, width);
-    };
-    const int64_t step_a = way * a.a.step, step_b = way * (upper ? a.a.step : a.b.step), step_c = way * a.c.step;
-    const T *at_a = nullptr, *at_b = nullptr, *at_c = nullptr;
-    if (at_first.has) {
-        if (Whole && !Halves) at_a = first(a.a, at_first.eight * 8, at_first.d, a.width);
-        at_b = first(upper ? a.a : a.b, at_first.eight * 8, at_first.d, a.width);
-    }
-    if (at_first.has_c) at_c = first(a.c, at_first.c_eight * 8, e0 + at_first.c, a.columns);
     auto load_chunk = [&](const Mine& my, int64_t at) {
         const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
+        auto row = [&](const Plane<const T>& p) { return p.at + span.seq * p.seq + head * p.head + (row0 + way * at) * p.step; };
         if (my.has && (Whole || !upper)) {
-            if (Whole && !Halves) fetch<T, C, DP == 32>(xa, at_a, step_a, my.eight * 8, count, a.width);
-            fetch<T, C, DP == 32>(xb, at_b, step_b, my.eight * 8, count, a.width);
+            const int64_t step_a = way * a.a.step, step_b = way * (upper ? a.a.step : a.b.step);
+            const int d = loaded(my.d, a.width);
+            if (Whole && !Halves) fetch<T, C, DP == 32>(xa, row(a.a) + my.eight * 8 * step_a + d, step_a, my.eight * 8, count, a.width);
+            fetch<T, C, DP == 32>(xb, row(upper ? a.a : a.b) + my.eight * 8 * step_b + d, step_b, my.eight * 8, count, a.width);
         }
-        if (my.has_c) fetch<T, C, W == 4>(xc, at_c, step_c, my.c_eight * 8, count, a.columns);
-        at_a += C * step_a;
-        at_b += C * step_b;
-        at_c += C * step_c;
+        if (my.has_c) {
+            const int64_t step = way * a.c.step;
+            fetch<T, C, W == 4>(xc, row(a.c) + my.c_eight * 8 * step + loaded(e0 + my.c, a.columns), step, my.c_eight * 8, count, a.columns);
+        }
     };
     if (span.begin < span.end) load_chunk(at_first, span.begin);
     for (int64_t at = span.begin; at < span.end; at += C) {
         const int count = static_cast<int>(span.end - at < C ? span.end - at : C);
+        // the tokens that X' decays by; one less where the state leaves a forward walk
+        const int n = count - (Whole && !a.reverse && span.last && at + C >= span.end ? 1 : 0);
         __syncthreads();
         if (tid == 0) s.odd = 0;
+        if (at == span.begin || n < C)
+            for (int j = tid; j < C; j += Threads) s.weight[j] = s.power[j < n ? n - j : 0] * a.inner;
         const int now = afresh(tid), col = now & 15, quad = now >> 4 & 3;
         const Mine my(now, wave);
         if (my.has && (Whole || !upper)) {
@@ -406,12 +428,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
         if (my.has_c) {
             if (count < C || columns < Slice) settle(xc, my.c_eight * 8, count, left_of(e0 + my.c, a.columns), a.columns);
             stage_turned<T, Slice, C>(s.c, xc, my.c_eight, my.c);
-            if (Whole) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) odd |= !(fabsf(static_cast<float>(xc.x[r][j])) < INFINITY);
-            }
+            if (Whole) odd = no_number(xc);
         }
         __syncthreads();
         if constexpr (Whole) {
@@ -486,7 +503,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
 #pragma unroll
                 for (int j = 0; j < C; j += 32) {
                     H8 fc[N];
-                    take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+                    take(fc, s.c, wave * 16 + col, unit(wave * 16 + col, j / 8 + quad));
 #pragma unroll
                     for (int t = j / 16; t < C / 16; ++t) {
                         H8 fp[M];
@@ -506,7 +523,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
                         const int r = wave * 16 + quad * 4 + k;
                         c[k] = 0.0f;
 #pragma unroll
-                        for (int n = N - 1; n >= 0; --n) c[k] += part(s.c[n][r][unit<C>(r, j / 8) + (j & 7)]);
+                        for (int n = N - 1; n >= 0; --n) c[k] += part(s.c[n][r][unit(r, j / 8) + (j & 7)]);
                     }
 #pragma unroll
                     for (int t = 0; t < C / 16; ++t) {
@@ -538,9 +555,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             }
             __syncthreads();
         }
-        // X' = g^n X + sum_j g^(n-j) b_j c_j, n the chunk's tokens; one power less where
-        // the state leaves a forward walk
-        const int n = count - (Whole && !a.reverse && span.last && at + C >= span.end ? 1 : 0);
+        // X' = g^n X + sum_j g^(n-j) b_j c_j
         const float keep = s.power[n];
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i)
@@ -549,23 +564,24 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
 #pragma unroll
         for (int j = 0; j < C; j += 32) {
             H8 fc[N], fw[kExact];
-            take(fc, s.c, wave * 16 + col, unit<C>(wave * 16 + col, j / 8 + quad));
+            take(fc, s.c, wave * 16 + col, unit(wave * 16 + col, j / 8 + quad));
+            F4 w[2];
+            w[0] = *reinterpret_cast<const F4*>(&s.weight[j + quad * 8]);
+            w[1] = *reinterpret_cast<const F4*>(&s.weight[j + quad * 8 + 4]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const int far = n - (j + quad * 8 + k);
-                const float w = s.power[far < 0 ? 0 : far] * a.inner;
                 float c = 0.0f;
 #pragma unroll
                 for (int p = N - 1; p >= 0; --p) c += part(fc[p][k]);
                 uint16_t q[kExact];
-                cut<kExact>(w * c, q);
+                cut<kExact>(w[k / 4][k & 3] * c, q);
 #pragma unroll
                 for (int p = 0; p < kExact; ++p) fw[p][k] = q[p];
             }
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 H8 fb[N];
-                take(fb, s.turned, i * 16 + col, unit<C>(i * 16 + col, j / 8 + quad));
+                take(fb, s.turned, i * 16 + col, unit(i * 16 + col, j / 8 + quad));
                 X[i] = product<kExact>(fb, fw, X[i]);
                 if (i & 1) in_order();
             }
