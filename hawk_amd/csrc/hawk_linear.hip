@@ -194,6 +194,7 @@ __device__ __forceinline__ void fetch(Block<T>& x, const T* at, int64_t step, in
         for (int r = 0; r < 8; ++r) {
             x.x[r] = load_raw<T, 4>(at);
             at += i + r + 1 < count ? step : 0;
+            in_order();                    // this form's addresses are not the other's work
         }
     }
 }
@@ -259,7 +260,8 @@ struct Tiles {
     };
     uint16_t c[N][16 * W][Long];
     uint16_t inside[M][C][Long];                           // g^(i-j) a_i . b_j
-    float power[C + 1];
+    float power[C + 1];                                    // g^n
+    float scaled[C];                                       // the same, times what inside is scaled by
     alignas(16) float weight[C];                           // what a token of the chunk has in X'
     int odd;                                               // c holds what is no number
 };
@@ -362,7 +364,10 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
     const int64_t state = (span.seq * a.heads + head) * plane, mark = pair * plane;
     const int way = a.reverse ? -1 : 1;
     const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
-    for (int n = tid; n <= C; n += Threads) s.power[n] = power(octaves, n);
+    for (int n = tid; n <= C; n += Threads) {
+        s.power[n] = power(octaves, n);
+        if (n < C) s.scaled[n] = s.power[n] * (a.inner * a.outer);
+    }
 
     // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
     F4 X[DP / 16];
@@ -450,11 +455,18 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
                 }
                 const int i = ti * 16 + col, j = tj * 16 + quad * 4;
                 H4 h[M];
+                float v[4];
+                if (ti > tj) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = p[k] * s.scaled[i - j - k];
+                } else {                                   // what p is past the diagonal is not looked at
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = i >= j + k ? p[k] * s.scaled[i >= j + k ? i - j - k : 0] : 0.0f;
+                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float v = i >= j + k ? p[k] * (s.power[i >= j + k ? i - j - k : 0] * a.inner) : 0.0f;
                     uint16_t q[M];
-                    cut<M>(v, q);
+                    cut<M>(v[k], q);
 #pragma unroll
                     for (int n = 0; n < M; ++n) h[n][k] = q[n];
                 }
@@ -495,7 +507,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             }
 #pragma unroll
             for (int t = 0; t < C / 16; ++t) {
-                const float g = s.power[t * 16 + col];
+                const float g = s.power[t * 16 + col] * a.outer;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[t][k] *= g;
             }
@@ -542,7 +554,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
 #pragma unroll
                 for (int t = 0; t < C / 16; ++t) {
                     if (t * 16 + col >= count) continue;
-                    const float x[4] = {o[t][0] * a.outer, o[t][1] * a.outer, o[t][2] * a.outer, o[t][3] * a.outer};
+                    const float x[4] = {o[t][0], o[t][1], o[t][2], o[t][3]};
                     T* here = to + (way * t * 16) * a.out.step;
                     if (left >= 4) {
                         store<T, 4>(here, x);
@@ -570,19 +582,32 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             w[1] = *reinterpret_cast<const F4*>(&s.weight[j + quad * 8 + 4]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                float c = 0.0f;
+                float c = part(fc[N - 1][k]);
 #pragma unroll
-                for (int p = N - 1; p >= 0; --p) c += part(fc[p][k]);
+                for (int p = N - 2; p >= 0; --p) c += part(fc[p][k]);
                 uint16_t q[kExact];
                 cut<kExact>(w[k / 4][k & 3] * c, q);
 #pragma unroll
                 for (int p = 0; p < kExact; ++p) fw[p][k] = q[p];
             }
+            // X's last digits show in the state that leaves, not in results of 16 bits
+            if (Reach < kExact && a.end) {
+                in_order();
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    H8 fb[N];
+                    take(fb, s.turned, i * 16 + col, unit(i * 16 + col, j / 8 + quad));
+#pragma unroll
+                    for (int p = 0; p < N; ++p) X[i] = product(fb[p], fw[kExact - 1 - p], X[i]);
+                    if (i & 1) in_order();
+                }
+            }
+            in_order();
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 H8 fb[N];
                 take(fb, s.turned, i * 16 + col, unit(i * 16 + col, j / 8 + quad));
-                X[i] = product<kExact>(fb, fw, X[i]);
+                X[i] = product<Reach>(fb, fw, X[i]);
                 if (i & 1) in_order();
             }
         }
@@ -658,21 +683,24 @@ int walks_of(const hk_linear_attention_job& j, int vjp, Walk (&w)[kMostWalks]) {
 int slice_of(int columns) { return columns > 64 ? 128 : 64; }
 int bucket_of(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : width <= 128 ? 128 : 256; }
 
-// The tokens of a segment: a whole sequence if that gives the units two workgroups each,
-// otherwise as many as do, 256 at least.
+// The tokens of a segment.  Walks that are enough for most of the units go whole: what
+// cutting costs, the segments' own states first, is about half a walk.  Otherwise, and
+// where sequences are of any length, as many as give the units two workgroups each, 256
+// at least.
 struct Cut { int64_t segment, segments, slots; };
-Cut cut_of(const hk_linear_attention_job& j, int columns) {
+Cut cut_of(const hk_linear_attention_job& j, int columns, int walks) {
     const int64_t slices = (columns + slice_of(columns) - 1) / slice_of(columns), most = j.steps > 1 ? j.steps : 1;
-    const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps;
-    int64_t each = tokens / (2 * kUnits) * j.heads * slices + 1;
+    const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps, beside = j.heads * slices * walks;
+    int64_t each = tokens / (2 * kUnits) * beside + 1;
     each = each < 256 ? 256 : (each + 63) / 64 * 64;
+    if (!j.offsets && j.seqs * beside >= kUnits * 3 / 4) each = most;
     if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1} : Cut{most, 1, j.seqs};
     if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs};
     const int64_t n = (j.steps + each - 1) / each;
     return Cut{each, n, n * j.seqs};
 }
-size_t cuts_bytes(const hk_linear_attention_job& j, const Walk& w) {
-    const Cut c = cut_of(j, w.columns);
+size_t cuts_bytes(const hk_linear_attention_job& j, const Walk& w, int walks) {
+    const Cut c = cut_of(j, w.columns, walks);
     if (c.segment >= j.steps) return 0;
     return static_cast<size_t>(c.slots) * static_cast<size_t>(j.heads) * w.width * w.columns * sizeof(float);
 }
@@ -723,7 +751,7 @@ void launch(const Walks<T>& walks, int n, int bucket, hipStream_t stream) {
 }
 
 template <class T>
-LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w) {
+LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w, int walks) {
     LinearArgs<T> a;
     a.a = in<T>(*w.a);
     a.b = in<T>(*w.b);
@@ -736,7 +764,7 @@ LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w) {
     a.seqs = j.seqs;
     a.steps = j.steps;
     a.heads = j.heads;
-    const Cut c = cut_of(j, w.columns);
+    const Cut c = cut_of(j, w.columns, walks);
     a.segment = c.segment;
     a.segments = c.segments;
     a.slots = c.slots;
@@ -768,8 +796,8 @@ int all(const hk_linear_attention_job& j, int vjp, void* scratch, hipStream_t st
         for (int k = i; k < n; ++k) {
             if (done[k] || bucket_of(w[k].width) != bucket || slice_of(w[k].columns) != slice) continue;
             done[k] = true;
-            walks.walk[count] = args_of<T>(j, w[k]);
-            const size_t bytes = cuts_bytes(j, w[k]);
+            walks.walk[count] = args_of<T>(j, w[k], n);
+            const size_t bytes = cuts_bytes(j, w[k], n);
             if (bytes) walks.walk[count].cuts = reinterpret_cast<float*>(room);
             room += bytes;
             ++count;
@@ -812,7 +840,7 @@ extern "C" size_t hk_linear_attention_scratch_bytes(const hk_linear_attention_jo
     Walk w[kMostWalks];
     const int n = walks_of(*job, vjp, w);
     size_t bytes = 0;
-    for (int i = 0; i < n; ++i) bytes += cuts_bytes(*job, w[i]);
+    for (int i = 0; i < n; ++i) bytes += cuts_bytes(*job, w[i], n);
     return bytes;
 }
 
