@@ -72,8 +72,9 @@ __device__ __forceinline__ u64 weight_of(const Weights& k, float x) {
     p = __builtin_fma(r, p, ln2 * ln2 / 2.0);
     p = __builtin_fma(r, p, ln2);
     p = __builtin_fma(r, p, 1.0);
-    const double w = scaled(p * k.table[n & (kTable - 1)], n >> 7);
-    return __builtin_bit_cast(uint64_t, w + 0x1p52) - kUnit;
+    // n / 128 octaves more: the numbers are normal, so their exponents are added to
+    const uint64_t w = __builtin_bit_cast(uint64_t, p * k.table[n & (kTable - 1)]) + (static_cast<uint64_t>(static_cast<uint32_t>(n & -kTable) << 13) << 32);
+    return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, w) + 0x1p52) - kUnit;
 }
 
 
@@ -135,22 +136,21 @@ __device__ __forceinline__ u64 block_before(Sums<NT>& s, u64 own, u64& all) {
     return before;
 }
 
-// A row, read by NT threads: wave w has the vectors [w, w + 1) * steps * 64 of it, so the
-// waves' parts, and a wave's steps, follow each other by index.  Every pass reads the row;
-// all but the first find it in the caches.
+// A row, or a part of one, read by NT threads: from vector `begin` on, wave w has the
+// vectors [w, w + 1) * steps * 64, so the waves' shares, and a wave's steps, follow each
+// other by index.  Every pass reads the row; all but the first find it in the caches.
 template <class T, int NT>
 struct Row {
     const T* at;               // the row's address less its lead, 16-byte aligned
-    int low, steps;            // the row's first position; vectors of a lane
-    int64_t high;              // past its last
+    int low, high;             // the row's first position, and past its last
+    int begin, steps;          // the part's first vector; vectors of a lane
 
     __device__ __forceinline__ int position(int i) const {
-        return ((static_cast<int>(threadIdx.x >> 6) * steps + i) * 64 + static_cast<int>(threadIdx.x & 63)) * kVec<T>;
+        return (begin + (static_cast<int>(threadIdx.x >> 6) * steps + i) * 64 + static_cast<int>(threadIdx.x & 63)) * kVec<T>;
     }
     // What lies before the row or past its end is -inf.
-    __device__ __forceinline__ Raw<T, kVec<T>> vector(int i) const {
+    __device__ __forceinline__ Raw<T, kVec<T>> vector(int p) const {
         constexpr int V = kVec<T>;
-        const int p = position(i);
         if (p >= low && p + V <= high) return load_raw<T, V>(at + p);
         Raw<T, V> x = splat<T, V>(static_cast<T>(-INFINITY));
 #pragma unroll
@@ -158,25 +158,31 @@ struct Row {
             if (p + j >= low && p + j < high) put<T, V>(x, j, at[p + j]);
         return x;
     }
-    // f(step, first index, vector) of every step from `from` up to `end`, kAhead loads at a time.
+    // f(first index, vector) of every step from `from` up to `end`, kAhead loads at a time;
+    // a wave whose vectors are all in the row asks that once.
     template <class F> __device__ __forceinline__ void each(int from, int end, F&& f) const {
-        constexpr int kAhead = 4;
+        constexpr int V = kVec<T>, kAhead = 4;
         for (int i = from; i < end; i += kAhead) {
-            Raw<T, kVec<T>> x[kAhead];
+            Raw<T, V> x[kAhead];
+            const int p = position(i), first = __builtin_amdgcn_readfirstlane(p);
+            if (i + kAhead <= end && first >= low && first + kAhead * 64 * V <= high) {
 #pragma unroll
-            for (int b = 0; b < kAhead; ++b)
-                if (i + b < end) x[b] = vector(i + b);
+                for (int b = 0; b < kAhead; ++b) x[b] = load_raw<T, V>(at + p + b * 64 * V);
+            } else {
 #pragma unroll
-            for (int b = 0; b < kAhead; ++b)
-                if (i + b < end) {
-                    f(i + b, position(i + b) - low, x[b]);
-                    __builtin_amdgcn_sched_barrier(0);     // a vector at a time: fewer registers, more waves
-                }
+                for (int b = 0; b < kAhead; ++b)
+                    if (i + b < end) x[b] = vector(p + b * 64 * V);
+            }
+#pragma unroll
+            for (int b = 0; b < kAhead; ++b) {
+                if (i + b < end) f(p + b * 64 * V - low, x[b]);
+                __builtin_amdgcn_sched_barrier(0);         // a vector at a time: fewer registers, more waves
+            }
         }
     }
     // f(index, number) of every token.
     template <class F> __device__ __forceinline__ void tokens(int vocab, F&& f) const {
-        each(0, steps, [&](int, int first, const Raw<T, kVec<T>>& v) {
+        each(0, steps, [&](int first, const Raw<T, kVec<T>>& v) {
 #pragma unroll
             for (int j = 0; j < kVec<T>; ++j) {
                 const int i = first + j;
@@ -210,10 +216,21 @@ __device__ __forceinline__ void fill(Shared<NT, true>& s, const Row<T, NT>& row,
     for (int b = threadIdx.x; b < kBins; b += NT) s.bins[b] = 0;
     if (threadIdx.x == 0) s.found = kBins, s.listed = 0, s.low = kAll, s.high = 0;
     __syncthreads();
+    u64 rest = 0;                                         // the last bin's, which may have most of a row (what is barred)
     row.tokens(vocab, [&](uint32_t i, float x) {
         const int b = bins.of(code_of(i, x), x);
-        if (b >= 0) atomicAdd(&s.bins[b], mass ? weight_of(k, x) : 1);
+        if (b < 0) return;
+        if (mass) {
+            const u64 w = weight_of(k, x);
+            if (b == kBins - 1) rest += w;
+            else atomicAdd(&s.bins[b], w);
+        } else {
+            if (b == kBins - 1) ++rest;
+            else atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[b]), 1u);
+        }
     });
+    rest = wave_sum(rest);
+    if ((threadIdx.x & 63) == 0 && rest) atomicAdd(&s.bins[kBins - 1], rest);
     __syncthreads();
     constexpr int Each = kBins / NT;
     u64 own = 0, all;
@@ -439,7 +456,7 @@ __device__ __forceinline__ u64 from_row(Sums<NT>& s, const Row<T, NT>& row, doub
     for (int c = 0, i = 0; i < row.steps; ++c) {
         const int end = i + run < row.steps ? i + run : row.steps;
         u64 sum = 0;
-        row.each(i, end, [&](int, int first, const Raw<T, V>& v) {
+        row.each(i, end, [&](int first, const Raw<T, V>& v) {
 #pragma unroll
             for (int j = 0; j < V; ++j) sum += kept(first, v, j);
         });
@@ -465,7 +482,7 @@ __device__ __forceinline__ u64 from_row(Sums<NT>& s, const Row<T, NT>& row, doub
         const int end = (c + 1) * run < row.steps ? (c + 1) * run : row.steps;
 #pragma unroll 1
         for (int i = c * run; i < end; ++i) {
-            const Raw<T, V> v = row.vector(i);
+            const Raw<T, V> v = row.vector(row.position(i));
             const int first = row.position(i) - row.low;
             u64 w[V], own = 0;
 #pragma unroll
@@ -500,7 +517,8 @@ __global__ void __launch_bounds__(NT, 4) hawk_sample(const SampleArgs<T> a) {
         Row<T, NT> row;
         row.low = static_cast<int>(reinterpret_cast<uintptr_t>(from) % 16 / sizeof(T));
         row.at = from - row.low;
-        row.high = row.low + a.vocab;
+        row.high = row.low + vocab;
+        row.begin = 0;
         row.steps = static_cast<int>((row.high + V * NT - 1) / (V * NT));
         const double heat = a.temperature ? static_cast<double>(a.temperature[n]) : a.temperature_all;
         const double u = a.u64bits ? static_cast<const double*>(a.u)[n] : static_cast<double>(static_cast<const float*>(a.u)[n]);
@@ -508,7 +526,7 @@ __global__ void __launch_bounds__(NT, 4) hawk_sample(const SampleArgs<T> a) {
         // the highest logit, and whether one is a NaN
         float m = -INFINITY;
         bool bad = false;
-        row.each(0, row.steps, [&](int, int, const Raw<T, V>& v) {
+        row.each(0, row.steps, [&](int, const Raw<T, V>& v) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float x = widen<T, V>(v, j);
