@@ -32,6 +32,7 @@ constexpr int64_t kMostVocab = 1 << 22;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;                // candidates that are ranked against each other
 constexpr u64 kAll = ~0ull;
+constexpr int64_t kUnits = 256;            // compute units
 
 template <class T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 
@@ -144,9 +145,18 @@ struct Row {
     const T* at;               // the row's address less its lead, 16-byte aligned
     int low, high;             // the row's first position, and past its last
     int begin, steps;          // the part's first vector; vectors of a lane
+    int wave;                  // whose share this is
 
+    // `part` of the parts of row n, each of NT * steps vectors.
+    __device__ __forceinline__ Row(const SampleArgs<T>& a, int64_t n, int part, int steps_, int wave_) : steps(steps_), wave(wave_) {
+        const T* from = a.logits + n * a.row_stride;
+        low = static_cast<int>(reinterpret_cast<uintptr_t>(from) % 16 / sizeof(T));
+        at = from - low;
+        high = low + static_cast<int>(a.vocab);
+        begin = part * (NT * steps);
+    }
     __device__ __forceinline__ int position(int i) const {
-        return (begin + (static_cast<int>(threadIdx.x >> 6) * steps + i) * 64 + static_cast<int>(threadIdx.x & 63)) * kVec<T>;
+        return (begin + (wave * steps + i) * 64 + static_cast<int>(threadIdx.x & 63)) * kVec<T>;
     }
     // What lies before the row or past its end is -inf.
     __device__ __forceinline__ Raw<T, kVec<T>> vector(int p) const {
@@ -207,15 +217,9 @@ struct Bins {
 };
 __device__ __forceinline__ u64 code_of(uint32_t i, float x) { return static_cast<u64>(place_of(x)) << 32 | i; }
 
-// Fills the bins with the tokens' weights (or 1 each) and finds the first at which their
-// running sum from `base` reaches the target: s.found (kBins: none), s.base the sum
-// before it, s.inside its own.  With share >= 0 the target is that share of the sum.
+// Adds the tokens' weights (or 1 each) to their bins.
 template <class T, int NT>
-__device__ __forceinline__ void fill(Shared<NT, true>& s, const Row<T, NT>& row, int vocab, const Weights& k, const Bins& bins, bool mass, u64 base,
-                     u64& target, double share) {
-    for (int b = threadIdx.x; b < kBins; b += NT) s.bins[b] = 0;
-    if (threadIdx.x == 0) s.found = kBins, s.listed = 0, s.low = kAll, s.high = 0;
-    __syncthreads();
+__device__ __forceinline__ void fill(u64* to, const Row<T, NT>& row, int vocab, const Weights& k, const Bins& bins, bool mass) {
     u64 rest = 0;                                         // the last bin's, which may have most of a row (what is barred)
     row.tokens(vocab, [&](uint32_t i, float x) {
         const int b = bins.of(code_of(i, x), x);
@@ -223,38 +227,53 @@ __device__ __forceinline__ void fill(Shared<NT, true>& s, const Row<T, NT>& row,
         if (mass) {
             const u64 w = weight_of(k, x);
             if (b == kBins - 1) rest += w;
-            else atomicAdd(&s.bins[b], w);
+            else atomicAdd(&to[b], w);
         } else {
             if (b == kBins - 1) ++rest;
-            else atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[b]), 1u);
+            else atomicAdd(reinterpret_cast<uint32_t*>(&to[b]), 1u);
         }
     });
     rest = wave_sum(rest);
-    if ((threadIdx.x & 63) == 0 && rest) atomicAdd(&s.bins[kBins - 1], rest);
-    __syncthreads();
+    if ((threadIdx.x & 63) == 0 && rest) atomicAdd(&to[kBins - 1], rest);
+}
+__device__ __forceinline__ u64 share_of(double share, u64 all) {
+    const double want = ceil(share * static_cast<double>(all));
+    const u64 target = want < 1.0 ? 1 : static_cast<u64>(want);
+    return target < all ? target : all;
+}
+// The first bin at which the running sum from `base` reaches the target: s.found (kBins:
+// none), s.base the sum before it, s.inside its own.  With share >= 0 the target is that
+// share of the sum.
+template <int NT>
+__device__ __forceinline__ void locate(Shared<NT, true>& s, const u64* bins, u64 base, u64& target, double share) {
     constexpr int Each = kBins / NT;
-    u64 own = 0, all;
+    u64 v[Each], own = 0, all;
 #pragma unroll
-    for (int b = 0; b < Each; ++b) own += s.bins[threadIdx.x * Each + b];
+    for (int b = 0; b < Each; ++b) own += v[b] = bins[threadIdx.x * Each + b];
     u64 before = block_before(s, own, all) + base;
-    if (share >= 0.0) {
-        const double want = ceil(share * static_cast<double>(all));
-        target = want < 1.0 ? 1 : static_cast<u64>(want);
-        if (target > all) target = all;
-    }
+    if (share >= 0.0) target = share_of(share, all);
     if (before < target && before + own >= target) {
 #pragma unroll
         for (int b = 0; b < Each; ++b) {
-            const u64 v = s.bins[threadIdx.x * Each + b];
-            if (before < target && before + v >= target) {
+            if (before < target && before + v[b] >= target) {
                 s.found = threadIdx.x * Each + b;
                 s.base = before;
-                s.inside = v;
+                s.inside = v[b];
             }
-            before += v;
+            before += v[b];
         }
     }
     __syncthreads();
+}
+template <class T, int NT>
+__device__ __forceinline__ void search(Shared<NT, true>& s, const Row<T, NT>& row, int vocab, const Weights& k, const Bins& bins, bool mass, u64 base,
+                                       u64& target, double share) {
+    for (int b = threadIdx.x; b < kBins; b += NT) s.bins[b] = 0;
+    if (threadIdx.x == 0) s.found = kBins, s.listed = 0, s.low = kAll, s.high = 0;
+    __syncthreads();
+    fill(s.bins, row, vocab, k, bins, mass);
+    __syncthreads();
+    locate(s, s.bins, base, target, share);
 }
 
 // The list's first n entries in ascending order of their codes (their low 32 bits alone:
@@ -304,7 +323,7 @@ __device__ __forceinline__ u64 last_of(Shared<NT, true>& s, const Row<T, NT>& ro
     Bins bins{0, limit, k.top, k.octaves, -1};
     u64 base = 0;
     for (;;) {
-        fill(s, row, vocab, k, bins, mass, base, target, share);
+        search(s, row, vocab, k, bins, mass, base, target, share);
         share = -1.0;
         const int found = s.found;
         if (found >= kBins) return limit;                // less than the target in all: everything is kept
@@ -359,9 +378,55 @@ __device__ __forceinline__ u64 aim(double u, u64 all) {
 
 // What a row asks for.
 struct Asked {
-    double u, share;           // share: top_p, or -1 where it keeps everything
+    double heat, u, share;     // share: top_p, or -1 where it keeps everything
     u64 count, least;          // count: top_k, or kAll; least: the least weight that min_p keeps
+    __device__ __forceinline__ bool every() const { return count == kAll && share < 0.0 && least == 0; }
 };
+template <class T>
+__device__ __forceinline__ Asked asked(const SampleArgs<T>& a, int64_t n) {
+    Asked q;
+    q.heat = a.temperature ? static_cast<double>(a.temperature[n]) : a.temperature_all;
+    q.u = a.u64bits ? static_cast<const double*>(a.u)[n] : static_cast<double>(static_cast<const float*>(a.u)[n]);
+    const double top_p = a.top_p ? static_cast<double>(a.top_p[n]) : a.top_p_all;
+    const double min_p = a.min_p ? static_cast<double>(a.min_p[n]) : a.min_p_all;
+    // no weight is above 1: a larger min_p leaves the highest alone
+    const int64_t top_k = min_p > 1.0 ? 1 : a.top_k ? static_cast<int64_t>(a.top_k[n]) : a.top_k_all;
+    q.share = top_p < 1.0 ? fmax(top_p, 0.0) : -1.0;
+    q.count = top_k > 0 && top_k < a.vocab ? static_cast<u64>(top_k) : kAll;
+    q.least = min_p > 0.0 && min_p <= 1.0 ? static_cast<u64>(ceil(scaled(min_p, a.shift))) : 0;
+    return q;
+}
+// A row's highest logit, NaN where one is: whether it has a token to draw, by its weights.
+__device__ __forceinline__ bool drawn(const Asked& q, float top) { return q.heat > 0.0 && q.u == q.u && top > -INFINITY; }
+__device__ __forceinline__ Weights weights_of(const Asked& q, float top, const double* table) {
+    return Weights{static_cast<double>(top), fmin(1.4426950408889634074 / q.heat, 1e300), table};
+}
+template <class T>
+__device__ __forceinline__ void answer(const SampleArgs<T>& a, int64_t n, int64_t token, float logp) {
+    if (a.token) {
+        if (a.token64) static_cast<int64_t*>(a.token)[n] = token;
+        else static_cast<int32_t*>(a.token)[n] = static_cast<int32_t>(token);
+    }
+    if (a.logp) a.logp[n] = logp;
+}
+// The answer of a row that is not drawn by its weights; `first` its highest logit's first token.
+template <class T>
+__device__ __forceinline__ void answer_plain(const SampleArgs<T>& a, int64_t n, const Asked& q, float top, int64_t first) {
+    const bool none = !(q.heat >= 0.0) || !(q.u == q.u) || !(top == top);
+    if (none || top == -INFINITY) answer(a, n, -1, none ? NAN : -INFINITY);
+    else answer(a, n, first, 0.0f);
+}
+template <class T>
+__device__ __forceinline__ void answer_drawn(const SampleArgs<T>& a, int64_t n, const Asked& q, float top, u64 at, u64 all) {
+    const int64_t token = at < static_cast<u64>(a.vocab) ? static_cast<int64_t>(at) : a.vocab - 1;
+    const double x = static_cast<double>(static_cast<float>(a.logits[n * a.row_stride + token]));
+    answer(a, n, token, static_cast<float>((top == INFINITY ? 0.0 : (x - top) / q.heat) - log(scaled(static_cast<double>(all), top == INFINITY ? 0 : -a.shift))));
+}
+// Of a row's infinities, which share the whole, how many are kept.
+__device__ __forceinline__ u64 infinities(const Asked& q, u64 count) {
+    const u64 some = q.count < count ? q.count : count;
+    return q.share < 0.0 ? some : share_of(q.share, some);
+}
 
 // Every token that may be kept is in the list, n of them: the filters, and the one drawn.
 // Few are ranked by counting those before each, which waits for nothing; more are sorted.
@@ -394,10 +459,7 @@ __device__ __forceinline__ u64 from_list(Shared<NT, true>& s, int n, const Asked
         }
         block_before(s, own, all);
     }
-    if (q.share >= 0.0) {
-        const double want = ceil(q.share * static_cast<double>(all));
-        target = want < 1.0 ? 1 : static_cast<u64>(want);
-    }
+    if (q.share >= 0.0) target = share_of(q.share, all);
     if (!few) {
 #pragma unroll
         for (int e = 0; e < Mine; ++e) {
@@ -443,28 +505,62 @@ __device__ __forceinline__ u64 from_list(Shared<NT, true>& s, int n, const Asked
     return s.low;
 }
 
-// The token drawn from those that `kept` (of an index and a number) gives a weight: the
-// waves' runs are summed, and the wave that has the one that is aimed at goes along it.
-// `some` says of the sum of all how much of it, from the first index on, there is to draw.
-template <class T, int NT, class F, class G>
-__device__ __forceinline__ u64 from_row(Sums<NT>& s, const Row<T, NT>& row, double u, F&& weight, G&& some, u64& all) {
+// The sums of a wave's runs, kCells at most, of what `weight` (of an index and a number)
+// gives; their sum.
+template <class T, int NT, class F>
+__device__ __forceinline__ u64 sum_runs(u64* cells, const Row<T, NT>& row, F&& weight) {
     constexpr int V = kVec<T>;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, run = (row.steps + kCells - 1) / kCells;
-    auto kept = [&](int first, const Raw<T, V>& v, int j) -> u64 { return weight(static_cast<uint32_t>(first + j), widen<T, V>(v, j)); };
+    const int run = (row.steps + kCells - 1) / kCells;
     u64 total = 0;
 #pragma unroll 1
-    for (int c = 0, i = 0; i < row.steps; ++c) {
-        const int end = i + run < row.steps ? i + run : row.steps;
+    for (int c = 0; c < kCells; ++c) {
+        const int from = c * run, end = from + run < row.steps ? from + run : row.steps;
         u64 sum = 0;
-        row.each(i, end, [&](int first, const Raw<T, V>& v) {
+        if (from < end) {
+            row.each(from, end, [&](int first, const Raw<T, V>& v) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum += kept(first, v, j);
-        });
-        sum = wave_sum(sum);
-        if (lane == 0) s.cells[wave * kCells + c] = sum;
+                for (int j = 0; j < V; ++j) sum += weight(static_cast<uint32_t>(first + j), widen<T, V>(v, j));
+            });
+            sum = wave_sum(sum);
+        }
+        if ((threadIdx.x & 63) == 0) cells[c] = sum;
         total += sum;
-        i = end;
     }
+    return total;
+}
+// A wave goes along its run c, before which `before` has passed: the token at which the
+// target is reached is put into `low`.
+template <class T, int NT, class F>
+__device__ __forceinline__ void go_along(u64& low, const Row<T, NT>& row, int c, u64 before, u64 target, F&& weight) {
+    constexpr int V = kVec<T>;
+    const int run = (row.steps + kCells - 1) / kCells, end = (c + 1) * run < row.steps ? (c + 1) * run : row.steps;
+#pragma unroll 1
+    for (int i = c * run; i < end; ++i) {
+        const int p = row.position(i), first = p - row.low;
+        const Raw<T, V> v = row.vector(p);
+        u64 w[V], own = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) own += w[j] = weight(static_cast<uint32_t>(first + j), widen<T, V>(v, j));
+        const u64 step = wave_sum(own);
+        if (before + step >= target) {
+            u64 upto = before + wave_before(own);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (upto < target && upto + w[j] >= target) low = static_cast<u64>(first + j);
+                upto += w[j];
+            }
+            return;
+        }
+        before += step;
+    }
+}
+// The token drawn from those that `weight` gives one: the waves' runs are summed, and the
+// wave that has the one that is aimed at goes along it.  `some` says how much of the sum
+// of all there is to draw from.
+template <class T, int NT, class F, class G>
+__device__ __forceinline__ u64 from_row(Sums<NT>& s, const Row<T, NT>& row, double u, F&& weight, G&& some, u64& all) {
+    const int lane = threadIdx.x & 63, wave = row.wave;
+    const u64 total = sum_runs(s.cells + wave * kCells, row, weight);
     if (lane == 0) s.waves[wave] = total;
     __syncthreads();
     all = 0;
@@ -479,159 +575,379 @@ __device__ __forceinline__ u64 from_row(Sums<NT>& s, const Row<T, NT>& row, doub
     if (before < target && before + total >= target) {
         int c = 0;
         while (before + s.cells[wave * kCells + c] < target) before += s.cells[wave * kCells + c++];
-        const int end = (c + 1) * run < row.steps ? (c + 1) * run : row.steps;
-#pragma unroll 1
-        for (int i = c * run; i < end; ++i) {
-            const Raw<T, V> v = row.vector(row.position(i));
-            const int first = row.position(i) - row.low;
-            u64 w[V], own = 0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) own += w[j] = kept(first, v, j);
-            const u64 step = wave_sum(own);
-            if (before + step >= target) {
-                u64 upto = before + wave_before(own);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (upto < target && upto + w[j] >= target) s.low = static_cast<u64>(first + j);
-                    upto += w[j];
-                }
-                break;
-            }
-            before += step;
-        }
+        go_along(s.low, row, c, before, target, weight);
     }
     __syncthreads();
     return s.low;
 }
 
-// Filtered: a row may have filters.  Listed: every row fits the list.
+// The highest of the threads' numbers, NaN where one is.
+template <class T, int NT>
+__device__ __forceinline__ float top_of(Sums<NT>& s, const Row<T, NT>& row) {
+    constexpr int V = kVec<T>;
+    float m = -INFINITY;
+    bool bad = false;
+    row.each(0, row.steps, [&](int, const Raw<T, V>& v) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float x = widen<T, V>(v, j);
+            m = fmaxf(m, x);
+            bad |= !(x == x);
+        }
+    });
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (threadIdx.x == 0) s.bad = 0;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.tops[threadIdx.x >> 6] = m;
+    if (bad) s.bad = 1;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, s.tops[w]);
+    return s.bad ? NAN : m;
+}
+// The first token of the highest logit (kAll: not here), in s.low.
+template <class T, int NT>
+__device__ __forceinline__ void first_of(Sums<NT>& s, const Row<T, NT>& row, int vocab, float top) {
+    if (threadIdx.x == 0) s.low = kAll;
+    __syncthreads();
+    u64 first = kAll;
+    row.tokens(vocab, [&](uint32_t i, float x) { if (x == top && i < first) first = i; });
+    if (first != kAll) atomicMin(&s.low, first);
+    __syncthreads();
+}
+template <int NT>
+__device__ __forceinline__ void make_table(Sums<NT>& s, int shift) {
+    for (int j = threadIdx.x; j < kTable; j += NT) s.table[j] = scaled(exp2(static_cast<double>(j) / kTable), shift);
+}
+
+// A row of NT threads.  Filtered: it may have filters.  Listed: it fits the list.
+template <bool Filtered, bool Listed, class T, int NT>
+__device__ __forceinline__ u64 from_whole(Shared<NT, Filtered>& s, const Row<T, NT>& row, int vocab, const Asked& q, float top, u64& all) {
+    const Weights k = weights_of(q, top, s.table);
+    auto whole = [](u64 sum) { return sum; };
+    if (top == INFINITY)
+        return from_row(s, row, q.u, [](uint32_t, float x) -> u64 { return x == INFINITY; }, [&](u64 count) { return infinities(q, count); }, all);
+    if (!Filtered || q.every()) return from_row(s, row, q.u, [&](uint32_t, float x) { return weight_of(k, x); }, whole, all);
+    if constexpr (Filtered) {
+        bool listed = Listed;
+        if (Listed) {
+            row.tokens(vocab, [&](uint32_t i, float x) {
+                s.code[i] = code_of(i, x);
+                s.value[i] = weight_of(k, x);
+            });
+            if (threadIdx.x == 0) s.listed = vocab;
+        } else if (q.count <= kList) {
+            // the tokens down to the bin that has the last of the top_k
+            u64 target = q.count;
+            const Bins bins{0, kAll, k.top, k.octaves, -1};
+            search(s, row, vocab, k, bins, false, 0, target, -1.0);
+            if (s.base + s.inside <= kList) {
+                const int found = s.found;
+                row.tokens(vocab, [&](uint32_t i, float x) {
+                    const u64 code = code_of(i, x);
+                    if (bins.of(code, x) > found) return;
+                    const int to = atomicAdd(&s.listed, 1);
+                    s.code[to] = code;
+                    s.value[to] = weight_of(k, x);
+                });
+                listed = true;
+            }
+        }
+        __syncthreads();
+        if (listed) return from_list(s, s.listed, q, all);
+        u64 cut = kAll;
+        for (int f = 0; f < 2; ++f) {                    // top_k, then top_p of what it keeps
+            if (f == 0 ? q.count == kAll : q.share < 0.0) continue;
+            cut = last_of(s, row, vocab, k, cut, f == 1, q.count, f == 0 ? -1.0 : q.share);
+        }
+        return from_row(s, row, q.u, [&](uint32_t i, float x) -> u64 {
+            if (code_of(i, x) > cut) return 0;
+            const u64 w = weight_of(k, x);
+            return w >= q.least ? w : 0;
+        }, whole, all);
+    }
+    return 0;
+}
+
+// Rows of a workgroup each.
 template <class T, int NT, bool Filtered, bool Listed>
 __global__ void __launch_bounds__(NT, 4) hawk_sample(const SampleArgs<T> a) {
-    constexpr int V = kVec<T>, Waves = NT / 64;
     __shared__ Shared<NT, Filtered> s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, vocab = static_cast<int>(a.vocab);
-    for (int j = tid; j < kTable; j += NT) s.table[j] = scaled(exp2(static_cast<double>(j) / kTable), a.shift);
+    const int vocab = static_cast<int>(a.vocab);
+    make_table(s, a.shift);
     for (int64_t n = blockIdx.x; n < a.rows; n += gridDim.x) {
         __syncthreads();
-        const T* from = a.logits + n * a.row_stride;
-        Row<T, NT> row;
-        row.low = static_cast<int>(reinterpret_cast<uintptr_t>(from) % 16 / sizeof(T));
-        row.at = from - row.low;
-        row.high = row.low + vocab;
-        row.begin = 0;
-        row.steps = static_cast<int>((row.high + V * NT - 1) / (V * NT));
-        const double heat = a.temperature ? static_cast<double>(a.temperature[n]) : a.temperature_all;
-        const double u = a.u64bits ? static_cast<const double*>(a.u)[n] : static_cast<double>(static_cast<const float*>(a.u)[n]);
-
-        // the highest logit, and whether one is a NaN
-        float m = -INFINITY;
-        bool bad = false;
-        row.each(0, row.steps, [&](int, const Raw<T, V>& v) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float x = widen<T, V>(v, j);
-                m = fmaxf(m, x);
-                bad |= !(x == x);
-            }
-        });
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-        if (tid == 0) s.bad = 0, s.low = vocab > 0 ? vocab - 1 : 0;
-        __syncthreads();
-        if (lane == 0) s.tops[wave] = m;
-        if (bad) s.bad = 1;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < Waves; ++w) m = fmaxf(m, s.tops[w]);
-        int64_t token = -1;
-        float logp = 0.0f;
-        if (s.bad || !(heat >= 0.0) || !(u == u)) {
-            logp = NAN;
-        } else if (m == -INFINITY) {
-            logp = -INFINITY;
-        } else if (heat == 0.0) {
-            u64 first = kAll;
-            row.tokens(vocab, [&](uint32_t i, float x) { if (x == m && i < first) first = i; });
-            if (first != kAll) atomicMin(&s.low, first);
-            __syncthreads();
-            token = static_cast<int64_t>(s.low);
+        Row<T, NT> row(a, n, 0, 0, threadIdx.x >> 6);
+        row.steps = (row.high + kVec<T> * NT - 1) / (kVec<T> * NT);
+        const Asked q = asked(a, n);
+        const float top = top_of(s, row);
+        if (drawn(q, top)) {
+            u64 all;
+            const u64 at = from_whole<Filtered, Listed>(s, row, vocab, q, top, all);
+            if (threadIdx.x == 0) answer_drawn(a, n, q, top, at, all);
         } else {
-            const bool infinite = m == INFINITY;
-            const Weights k{static_cast<double>(m), fmin(1.4426950408889634074 / heat, 1e300), s.table};
-            const double top_p = a.top_p ? static_cast<double>(a.top_p[n]) : a.top_p_all;
-            const double low_p = a.min_p ? static_cast<double>(a.min_p[n]) : a.min_p_all;
-            // no weight is above 1: a larger min_p leaves the highest alone
-            const int64_t top_k = low_p > 1.0 ? 1 : a.top_k ? static_cast<int64_t>(a.top_k[n]) : a.top_k_all;
-            Asked q;
-            q.u = u;
-            q.share = top_p < 1.0 ? fmax(top_p, 0.0) : -1.0;
-            q.count = top_k > 0 && top_k < a.vocab ? static_cast<u64>(top_k) : kAll;
-            q.least = low_p > 0.0 && low_p <= 1.0 ? static_cast<u64>(ceil(scaled(low_p, a.shift))) : 0;
-            u64 cut = kAll, all, at;
-            const bool every = q.count == kAll && q.share < 0.0 && q.least == 0;
-            auto whole = [](u64 sum) { return sum; };
-            if (infinite) {                              // the infinities share the whole, the first of them what is kept
-                at = from_row(s, row, q.u, [](uint32_t, float x) -> u64 { return x == INFINITY; }, [&](u64 sum) {
-                    const u64 some = q.count < sum ? q.count : sum;
-                    const double part = q.share < 0.0 ? 1e300 : ceil(q.share * static_cast<double>(some));
-                    return part < 1.0 ? 1 : part < static_cast<double>(some) ? static_cast<u64>(part) : some;
-                }, all);
-                all <<= a.shift;
-            } else if (!Filtered || every) {
-                at = from_row(s, row, q.u, [&](uint32_t, float x) { return weight_of(k, x); }, whole, all);
-            } else if constexpr (Filtered) {
-                bool listed = Listed;
-                if (Listed) {
-                    row.tokens(vocab, [&](uint32_t i, float x) {
-                        s.code[i] = code_of(i, x);
-                        s.value[i] = weight_of(k, x);
-                    });
-                    if (tid == 0) s.listed = vocab;
-                } else if (q.count <= kList) {
-                    // the tokens down to the bin that has the last of the top_k
-                    u64 target = q.count;
-                    const Bins bins{0, kAll, k.top, k.octaves, -1};
-                    fill(s, row, vocab, k, bins, false, 0, target, -1.0);
-                    if (s.base + s.inside <= kList) {
-                        const int found = s.found;
-                        row.tokens(vocab, [&](uint32_t i, float x) {
-                            const u64 code = code_of(i, x);
-                            if (bins.of(code, x) > found) return;
-                            const int to = atomicAdd(&s.listed, 1);
-                            s.code[to] = code;
-                            s.value[to] = weight_of(k, x);
-                        });
-                        listed = true;
-                    }
-                }
-                __syncthreads();
-                if (listed) {
-                    at = from_list(s, s.listed, q, all);
-                } else {
-                    for (int f = 0; f < 2; ++f) {        // top_k, then top_p of what it keeps
-                        if (f == 0 ? q.count == kAll : q.share < 0.0) continue;
-                        cut = last_of(s, row, vocab, k, cut, f == 1, q.count, f == 0 ? -1.0 : q.share);
-                    }
-                    at = from_row(s, row, q.u, [&](uint32_t i, float x) -> u64 {
-                        if (code_of(i, x) > cut) return 0;
-                        const u64 w = weight_of(k, x);
-                        return w >= q.least ? w : 0;
-                    }, whole, all);
-                }
-            }
-            token = at < a.vocab ? static_cast<int64_t>(at) : a.vocab - 1;
-            const float x = static_cast<float>(from[token]);
-            logp = static_cast<float>((infinite ? 0.0 : (static_cast<double>(x) - k.top) / heat) - log(scaled(static_cast<double>(all), -a.shift)));
-        }
-        if (tid == 0) {
-            if (a.token) {
-                if (a.token64) static_cast<int64_t*>(a.token)[n] = token;
-                else static_cast<int32_t*>(a.token)[n] = static_cast<int32_t>(token);
-            }
-            if (a.logp) a.logp[n] = logp;
+            if (q.heat == 0.0 && top > -INFINITY) first_of(s, row, vocab, top);
+            if (threadIdx.x == 0) answer_plain(a, n, q, top, static_cast<int64_t>(s.low));
         }
     }
 }
+
+// ---- few long rows: several workgroups a row, four launches --------------------------------
+//
+// Each workgroup has a part of a row.  The first launch finds the parts' highest logits,
+// the second sums the parts' runs or, where a filter needs the order, fills the row's
+// bins; the third sums what is above the bin that the filter ends in and lists that bin's
+// tokens; the fourth, a workgroup a row, ranks the list and draws.  Sums of whole numbers
+// are the same in any order.  A row whose list is too long, or whose top_k is, is taken
+// whole by the fourth.
+
+constexpr int kPart = 256, kMostParts = 64, kDraw = 1024;
+struct Parts {
+    float* tops;               // [row][part]
+    u64* firsts;               // [row][part]: the first token of the part's highest logit, of rows at temperature 0
+    u64 *bins, *cells;         // [row][kBins], [row][part][wave][kCells]
+    u64 *code, *value;         // [row][kList]
+    int* listed;               // [row]
+    int parts, steps;
+};
+// What a row's parts do: nothing (its answer needs no sums, or the last launch takes it
+// whole), sums of runs, bins of counts or of weights.
+enum Way { kNothing, kRuns, kCounts, kMasses };
+__device__ __forceinline__ Way way_of(const Asked& q, float top) {
+    if (!drawn(q, top)) return kNothing;
+    if (top == INFINITY || (q.count == kAll && q.share < 0.0)) return kRuns;
+    return q.count == kAll ? kMasses : q.count <= kList ? kCounts : kNothing;
+}
+// The row's highest logit of its parts', NaN where one is.
+__device__ __forceinline__ float joined_top(const Parts& p, int64_t n) {
+    const int lane = threadIdx.x & 63;
+    float m = lane < p.parts ? p.tops[n * p.parts + lane] : -INFINITY;
+    const bool bad = __any(!(m == m));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    return bad ? NAN : m;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kPart) hawk_sample_tops(const SampleArgs<T> a, const Parts p) {
+    __shared__ Sums<kPart> s;
+    const int part = blockIdx.x;
+    const int64_t n = blockIdx.y;
+    const Row<T, kPart> row(a, n, part, p.steps, threadIdx.x >> 6);
+    for (int b = part * kPart + threadIdx.x; b < kBins; b += p.parts * kPart) p.bins[n * kBins + b] = 0;
+    if (part == 0 && threadIdx.x == 0) p.listed[n] = 0;
+    const float top = top_of(s, row);
+    if (threadIdx.x == 0) p.tops[n * p.parts + part] = top;
+    if (asked(a, n).heat != 0.0) return;
+    first_of(s, row, static_cast<int>(a.vocab), top);
+    if (threadIdx.x == 0) p.firsts[n * p.parts + part] = s.low;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kPart, 4) hawk_sample_bins(const SampleArgs<T> a, const Parts p) {
+    __shared__ Shared<kPart, true> s;
+    const int part = blockIdx.x, vocab = static_cast<int>(a.vocab);
+    const int64_t n = blockIdx.y;
+    const Asked q = asked(a, n);
+    const float top = joined_top(p, n);
+    const Way way = way_of(q, top);
+    if (way == kNothing) return;
+    make_table(s, a.shift);
+    for (int b = threadIdx.x; b < kBins; b += kPart) s.bins[b] = 0;
+    __syncthreads();
+    const Row<T, kPart> row(a, n, part, p.steps, threadIdx.x >> 6);
+    const Weights k = weights_of(q, top, s.table);
+    if (way == kRuns) {
+        u64* cells = p.cells + ((n * p.parts + part) * (kPart / 64) + row.wave) * kCells;
+        if (top == INFINITY) sum_runs(cells, row, [](uint32_t, float x) -> u64 { return x == INFINITY; });
+        else sum_runs(cells, row, [&](uint32_t, float x) -> u64 { const u64 w = weight_of(k, x); return w >= q.least ? w : 0; });
+        return;
+    }
+    fill(s.bins, row, vocab, k, Bins{0, kAll, k.top, k.octaves, -1}, way == kMasses);
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kPart)
+        if (s.bins[b]) atomicAdd(&p.bins[n * kBins + b], s.bins[b]);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kPart, 4) hawk_sample_keep(const SampleArgs<T> a, const Parts p) {
+    __shared__ Shared<kPart, true> s;
+    const int part = blockIdx.x, vocab = static_cast<int>(a.vocab);
+    const int64_t n = blockIdx.y;
+    const Asked q = asked(a, n);
+    const float top = joined_top(p, n);
+    const Way way = way_of(q, top);
+    if (way != kCounts && way != kMasses) return;
+    make_table(s, a.shift);
+    if (threadIdx.x == 0) s.found = kBins;
+    __syncthreads();
+    u64 target = q.count;
+    locate(s, p.bins + n * kBins, 0, target, way == kMasses ? q.share : -1.0);
+    const int found = s.found;
+    const Row<T, kPart> row(a, n, part, p.steps, threadIdx.x >> 6);
+    const Weights k = weights_of(q, top, s.table);
+    const Bins bins{0, kAll, k.top, k.octaves, -1};
+    if (way == kCounts && s.base + s.inside > kList) return;
+    // a part's tokens are listed here first, and take their places in the row's list at once
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    auto list = [&](u64 code, u64 w) {
+        const int to = atomicAdd(&s.listed, 1);
+        if (to < kList) {
+            s.code[to] = code;
+            s.value[to] = w;
+        }
+    };
+    if (way == kCounts) {
+        row.tokens(vocab, [&](uint32_t i, float x) {
+            const u64 code = code_of(i, x);
+            if (bins.of(code, x) <= found) list(code, weight_of(k, x));
+        });
+    } else {
+        sum_runs(p.cells + ((n * p.parts + part) * (kPart / 64) + row.wave) * kCells, row, [&](uint32_t i, float x) -> u64 {
+            if (i >= static_cast<uint32_t>(vocab)) return 0; // (beside the row)
+            const u64 code = code_of(i, x);
+            const int b = bins.of(code, x);
+            if (b > found) return 0;
+            const u64 w = weight_of(k, x);
+            if (b == found) list(code, w);
+            return b < found && w >= q.least ? w : 0;
+        });
+    }
+    __syncthreads();
+    const int own = s.listed;
+    if (threadIdx.x == 0) s.found = atomicAdd(&p.listed[n], own);
+    __syncthreads();
+    const int to = s.found;
+    if (own > kList || to > kList - own) return;         // too long: the row is taken whole
+    for (int i = threadIdx.x; i < own; i += kPart) {
+        p.code[n * kList + to + i] = s.code[i];
+        p.value[n * kList + to + i] = s.value[i];
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kDraw, 4) hawk_sample_draw(const SampleArgs<T> a, const Parts p) {
+    constexpr int Waves = kPart / 64, Most = kMostParts * Waves * kCells, Each = Most / kDraw;
+    __shared__ Shared<kDraw, true> s;
+    __shared__ u64 cells[Most];
+    const int tid = threadIdx.x, vocab = static_cast<int>(a.vocab), count = p.parts * Waves * kCells;
+    const int64_t n = blockIdx.x;
+    const Asked q = asked(a, n);
+    const float top = joined_top(p, n);
+    if (!drawn(q, top)) {
+        u64 first = kAll;
+        if (q.heat == 0.0 && top > -INFINITY)
+            for (int i = p.parts - 1; i >= 0; --i)
+                if (p.tops[n * p.parts + i] == top) first = p.firsts[n * p.parts + i];
+        if (tid == 0) answer_plain(a, n, q, top, static_cast<int64_t>(first));
+        return;
+    }
+    const Way way = way_of(q, top);
+    make_table(s, a.shift);
+    if (tid == 0) s.low = 0, s.found = kBins;
+    __syncthreads();
+    const Weights k = weights_of(q, top, s.table);
+    u64 all, target = q.count, cut = kAll;
+    bool whole = way == kNothing;
+    if (way == kCounts || way == kMasses) {
+        locate(s, p.bins + n * kBins, 0, target, way == kMasses ? q.share : -1.0);
+        const int listed = p.listed[n];
+        whole = way == kCounts ? s.base + s.inside > kList : listed > kList;
+        if (!whole) {
+            for (int i = tid; i < listed; i += kDraw) {
+                s.code[i] = p.code[n * kList + i];
+                s.value[i] = p.value[n * kList + i];
+            }
+            __syncthreads();
+            if (way == kCounts) {
+                const u64 at = from_list(s, listed, q, all);
+                if (tid == 0) answer_drawn(a, n, q, top, at, all);
+                return;
+            }
+        }
+    }
+    if (whole) {
+        Row<T, kDraw> row(a, n, 0, 0, tid >> 6);
+        row.steps = (row.high + kVec<T> * kDraw - 1) / (kVec<T> * kDraw);
+        const u64 at = from_whole<true, false>(s, row, vocab, q, top, all);
+        if (tid == 0) answer_drawn(a, n, q, top, at, all);
+        return;
+    }
+    for (int c = tid; c < count; c += kDraw) cells[c] = p.cells[n * count + c];
+    __syncthreads();
+    const Row<T, kPart> first(a, n, 0, p.steps, 0);
+    const int run = (p.steps + kCells - 1) / kCells, span = p.steps * 64 * kVec<T>;      // the tokens of a wave's share
+    if (way == kMasses) {
+        // the list's tokens up to the one that reaches the target join the runs that they are of
+        const int listed = p.listed[n];
+        u64 before = s.base;
+        int rank = tid;
+        if (listed <= kFew) {
+            if (tid < listed) {
+                rank = 0;
+                for (int o = 0; o < listed; ++o) {
+                    const bool ahead = s.code[o] < s.code[tid];
+                    rank += ahead;
+                    before += ahead ? s.value[o] : 0;
+                }
+            }
+        } else {
+            u64 sum;
+            sort<kDraw, false>(s, listed);
+            before += list_before(s, listed, sum);
+        }
+        if (tid < listed) {
+            const u64 w = s.value[tid], code = s.code[tid];
+            if (before < target) {
+                if (before + w >= target || rank + 1 == listed) s.high = code;
+                if (w >= q.least) {
+                    const int at = static_cast<int>(static_cast<uint32_t>(code)) + first.low;
+                    const int wave = at / span;
+                    atomicAdd(&cells[wave * kCells + (at - wave * span) / (64 * kVec<T>) / run], w);
+                }
+            }
+        }
+        __syncthreads();
+        cut = s.high;
+    }
+    u64 own = 0;
+#pragma unroll
+    for (int e = 0; e < Each; ++e) own += tid * Each + e < count ? cells[tid * Each + e] : 0;
+    u64 before = block_before(s, own, all);
+    if (top == INFINITY) all = infinities(q, all);
+    const u64 aimed = aim(q.u, all);
+    if (before < aimed && before + own >= aimed) {
+#pragma unroll
+        for (int e = 0; e < Each; ++e) {
+            const u64 v = tid * Each + e < count ? cells[tid * Each + e] : 0;
+            if (before < aimed && before + v >= aimed) {
+                s.found = tid * Each + e;
+                s.base = before;
+            }
+            before += v;
+        }
+    }
+    __syncthreads();
+    if (tid < 64) {
+        const int found = s.found / kCells;
+        const Row<T, kPart> row(a, n, found / Waves, p.steps, found % Waves);
+        if (top == INFINITY) {
+            go_along(s.low, row, s.found % kCells, s.base, aimed, [](uint32_t, float x) -> u64 { return x == INFINITY; });
+        } else {
+            go_along(s.low, row, s.found % kCells, s.base, aimed, [&](uint32_t i, float x) -> u64 {
+                if (code_of(i, x) > cut) return 0;
+                const u64 w = weight_of(k, x);
+                return w >= q.least ? w : 0;
+            });
+        }
+    }
+    __syncthreads();
+    if (tid == 0) answer_drawn(a, n, q, top, s.low, all);
+}
+
+// ---- host ----------------------------------------------------------------------------
 
 // A lane has eight vectors of a row or fewer where the threads allow it; of many rows, a
 // unit has several at a time.
@@ -641,12 +957,27 @@ void launch(const SampleArgs<T>& a, dim3 grid, hipStream_t stream) {
     if (a.vocab <= 128) hipLaunchKernelGGL((hawk_sample<T, 64, Filtered, true>), grid, dim3(64), 0, stream, a);
     else if (a.vocab <= kList) hipLaunchKernelGGL((hawk_sample<T, 256, Filtered, true>), grid, dim3(256), 0, stream, a);
     else if (vectors <= 256 * 8) hipLaunchKernelGGL((hawk_sample<T, 256, Filtered, false>), grid, dim3(256), 0, stream, a);
-    else if (a.rows > 2 * 256) hipLaunchKernelGGL((hawk_sample<T, 512, Filtered, false>), grid, dim3(512), 0, stream, a);
+    else if (a.rows > 2 * kUnits) hipLaunchKernelGGL((hawk_sample<T, 512, Filtered, false>), grid, dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((hawk_sample<T, 1024, Filtered, false>), grid, dim3(1024), 0, stream, a);
 }
 
+// The parts of a row: with fewer rows than half the units, and rows of more than eight
+// vectors a lane of a workgroup, as many as give the units four workgroups each, but no
+// part below four vectors a lane.
+int parts_of(int64_t rows, int64_t vocab, int esize) {
+    const int64_t each = 16 / esize, vectors = (vocab + 2 * each - 2) / each;
+    if (rows >= kUnits / 2 || vectors <= 256 * 8) return 1;
+    int64_t parts = 4 * kUnits / rows;
+    parts = parts < kMostParts ? parts : kMostParts;
+    return static_cast<int>(parts < vectors / (4 * kPart) ? parts : vectors / (4 * kPart));
+}
+int size_of(int dtype) { return dtype == HK_F32 ? 4 : 2; }
+size_t row_bytes(int parts) {
+    return static_cast<size_t>(parts) * (16 + kPart / 64 * kCells * 8) + kBins * 8 + kList * 16 + 16;
+}
+
 template <class T>
-int sample(const hk_sample_job& j, hipStream_t stream) {
+int sample(const hk_sample_job& j, void* scratch, hipStream_t stream) {
     SampleArgs<T> a;
     a.logits = static_cast<const T*>(j.logits);
     a.u = j.u;
@@ -667,21 +998,47 @@ int sample(const hk_sample_job& j, hipStream_t stream) {
     a.token64 = j.token64;
     a.shift = 62;
     while (a.shift > 51 || (j.vocab >> (62 - a.shift)) > 1) --a.shift;
-    const int64_t most = 1 << 20;
-    const dim3 grid(static_cast<unsigned>(j.rows < most ? j.rows : most));
     const bool filtered = j.row_temperature || j.row_top_p || j.row_min_p || j.row_top_k || j.top_k > 0 || j.top_p < 1.0 || j.min_p > 0.0;
-    filtered ? launch<T, true>(a, grid, stream) : launch<T, false>(a, grid, stream);
+    const int parts = parts_of(j.rows, j.vocab, sizeof(T));
+    if (parts > 1) {
+        const int64_t vectors = (j.vocab + 2 * kVec<T> - 2) / kVec<T>;
+        Parts p;
+        p.parts = parts;
+        p.steps = static_cast<int>((vectors + parts * kPart - 1) / (parts * kPart));
+        char* room = static_cast<char*>(scratch);
+        auto take = [&](int64_t each) { char* at = room; room += each * j.rows; return at; };
+        p.bins = reinterpret_cast<u64*>(take(kBins * 8));
+        p.cells = reinterpret_cast<u64*>(take(int64_t{parts} * (kPart / 64) * kCells * 8));
+        p.code = reinterpret_cast<u64*>(take(kList * 8));
+        p.value = reinterpret_cast<u64*>(take(kList * 8));
+        p.firsts = reinterpret_cast<u64*>(take(int64_t{parts} * 8));
+        p.tops = reinterpret_cast<float*>(take(int64_t{parts} * 8));
+        p.listed = reinterpret_cast<int*>(take(16));
+        const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(j.rows));
+        hipLaunchKernelGGL((hawk_sample_tops<T>), grid, dim3(kPart), 0, stream, a, p);
+        hipLaunchKernelGGL((hawk_sample_bins<T>), grid, dim3(kPart), 0, stream, a, p);
+        if (filtered) hipLaunchKernelGGL((hawk_sample_keep<T>), grid, dim3(kPart), 0, stream, a, p);
+        hipLaunchKernelGGL((hawk_sample_draw<T>), dim3(static_cast<unsigned>(j.rows)), dim3(kDraw), 0, stream, a, p);
+    } else {
+        const int64_t most = 1 << 20;
+        const dim3 grid(static_cast<unsigned>(j.rows < most ? j.rows : most));
+        filtered ? launch<T, true>(a, grid, stream) : launch<T, false>(a, grid, stream);
+    }
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? HK_OK : hawk_internal::set_hip_error("hawk_sample launch", err);
 }
 
 }  // namespace
 
-extern "C" size_t hk_sample_scratch_bytes(const hk_sample_job*) { return 0; }
+extern "C" size_t hk_sample_scratch_bytes(const hk_sample_job* job) {
+    if (!job || job->rows <= 0 || job->vocab <= 0 || job->vocab > kMostVocab) return 0;
+    if (job->dtype != HK_F32 && job->dtype != HK_BF16 && job->dtype != HK_F16) return 0;
+    const int parts = parts_of(job->rows, job->vocab, size_of(job->dtype));
+    return parts > 1 ? static_cast<size_t>(job->rows) * row_bytes(parts) : 0;
+}
 
 extern "C" int hk_sample(const hk_sample_job* job, void* scratch, void* stream) {
     using hawk_internal::set_error;
-    (void)scratch;
     if (!job) return set_error(HK_EVALUE, "hk_sample: a job is required");
     if (job->rows < 0 || job->vocab < 0) return set_error(HK_EVALUE, "hk_sample: sizes must be >= 0");
     if (job->vocab > kMostVocab) return set_error(HK_EVALUE, "hk_sample: the vocabulary has at most 2^22 tokens");
@@ -689,7 +1046,8 @@ extern "C" int hk_sample(const hk_sample_job* job, void* scratch, void* stream) 
         return set_error(HK_EVALUE, "hk_sample: the logits' element type is 32-bit or 16-bit");
     if (job->rows == 0) return HK_OK;
     if ((job->vocab > 0 && !job->logits) || !job->u) return set_error(HK_EVALUE, "hk_sample: logits and u are required");
+    if (hk_sample_scratch_bytes(job) && !scratch) return set_error(HK_EVALUE, "hk_sample: scratch is required for few long rows");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (job->dtype == HK_F32) return sample<float>(*job, s);
-    return job->dtype == HK_BF16 ? sample<bf16>(*job, s) : sample<f16>(*job, s);
+    if (job->dtype == HK_F32) return sample<float>(*job, scratch, s);
+    return job->dtype == HK_BF16 ? sample<bf16>(*job, scratch, s) : sample<f16>(*job, scratch, s);
 }
