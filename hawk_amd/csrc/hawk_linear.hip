@@ -624,14 +624,17 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             }
 }
 
-// Each segment's own state becomes the one that enters it.
+// Each segment's own state becomes the one that enters it: kAhead segments are read at a
+// time, before what waits for the one before.
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> walks) {
+    constexpr int kAhead = 8;
     const LinearArgs<T>& a = walks.walk[blockIdx.y];
-    const int64_t plane = static_cast<int64_t>(a.width) * a.columns, blocks = (plane + kJoinThreads - 1) / kJoinThreads;
+    const int plane = a.width * a.columns, blocks = (plane + kJoinThreads - 1) / kJoinThreads;
     const int64_t total = a.seqs * a.heads * blocks;
     for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
-        const int64_t pair = id / blocks, i = (id - pair * blocks) * kJoinThreads + threadIdx.x;
+        const int64_t pair = id / blocks;
+        const int i = static_cast<int>(id - pair * blocks) * kJoinThreads + static_cast<int>(threadIdx.x);
         if (i >= plane) continue;
         const int64_t seq = pair / a.heads, head = pair - seq * a.heads;
         int64_t length = a.steps, slot = seq * a.segments;
@@ -640,18 +643,109 @@ __global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> 
             length = bound_of(a, seq + 1) - first;
             slot = first / a.segment + seq;
         }
+        int64_t segments = length > 0 ? (length + a.segment - 1) / a.segment : 1;
+        if (segments > a.slots - slot) segments = a.slots - slot;            // offsets that do not ascend
         const double octaves = octaves_of(a.decay[head]);
         const float keep = power(octaves, a.segment);
-        const int64_t d = i / a.columns, e = i - d * a.columns;
+        const int d = i / a.columns, e = i - d * a.columns;
         float x = 0.0f;
         if (a.start) x = a.start[pair * plane + d * a.state_d + e * a.state_e] * (a.reverse ? 1.0f : power(octaves, 1));
-        for (int64_t t = 0; t == 0 || t < length; t += a.segment, ++slot) {
-            if (slot >= a.slots) break;                    // offsets that do not ascend
-            float* at = a.cuts + (slot * a.heads + head) * plane + i;
-            const float own = t + a.segment < length ? *at : 0.0f;
-            *at = x;
-            x = fused(keep, x, own);
+        const int64_t step = a.heads * plane;
+        float* at = a.cuts + (slot * a.heads + head) * plane + i;
+        for (int64_t t = 0; t < segments; t += kAhead, at += kAhead * step) {
+            float own[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) own[k] = t + k + 1 < segments ? at[k * step] : 0.0f;   // (the last leaves nothing here)
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (t + k >= segments) break;
+                at[k * step] = x;
+                x = fused(keep, x, own[k]);
+            }
         }
+    }
+}
+
+// ---- few tokens ------------------------------------------------------------------------
+//
+// S_t = g S_(t-1) + k_t v_t^T and o_t = scale q_t S_t as they stand: the states' traffic is
+// the work.  A workgroup has 64 columns of a head's state in registers, 16 groups of 16
+// lanes, each every 16th row, a lane four columns of it.
+
+constexpr int kFewTokens = 8, kStepThreads = 256, kStepColumns = 64, kGroups = 16;
+// The four numbers at column c of a row of `columns`, and the same written.
+__device__ __forceinline__ F4 four(const float* row, int c, int columns) {
+    F4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c + 4 <= columns) {
+        x = load_raw<float, 4>(row + c);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (c + j < columns) x[j] = row[c + j];
+    }
+    return x;
+}
+__device__ __forceinline__ void put_four(float* row, int c, int columns, const F4& x) {
+    if (c + 4 <= columns) {
+        store_raw<float, 4>(row + c, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (c + j < columns) row[c + j] = x[j];
+    }
+}
+template <class T, int Rows>
+__global__ void __launch_bounds__(kStepThreads) hawk_linear_steps(const LinearArgs<T> a, const int64_t before) {
+    __shared__ float q[kMostWidth], k[kMostWidth], v[kStepColumns];
+    __shared__ F4 sums[kGroups][kStepColumns / 4];
+    const int tid = threadIdx.x, lane = tid % 16, group = tid / 16;
+    const int64_t id = before + blockIdx.x, pair = id / a.slices, seq = pair / a.heads, head = pair - seq * a.heads;
+    const int e0 = static_cast<int>(id - pair * a.slices) * kStepColumns, c = e0 + lane * 4;
+    const int64_t state = pair * (static_cast<int64_t>(a.width) * a.columns);
+    const float given = a.decay[head], g = given >= 0.0f && given <= 1.0f ? given : NAN;
+    F4 S[Rows];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        const int d = group + r * kGroups;
+        S[r] = F4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.start && d < a.width) S[r] = four(a.start + state + d * a.columns, c, a.columns);
+    }
+    for (int64_t t = 0; t < a.steps; ++t) {
+        __syncthreads();
+        if (tid < a.width) {
+            q[tid] = static_cast<float>(a.a.at[seq * a.a.seq + t * a.a.step + head * a.a.head + tid]);
+            k[tid] = static_cast<float>(a.b.at[seq * a.b.seq + t * a.b.step + head * a.b.head + tid]);
+        }
+        if (tid < kStepColumns) v[tid] = e0 + tid < a.columns ? static_cast<float>(a.c.at[seq * a.c.seq + t * a.c.step + head * a.c.head + e0 + tid]) : 0.0f;
+        __syncthreads();
+        const F4 x = *reinterpret_cast<const F4*>(&v[lane * 4]);
+        F4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < Rows; ++r) {
+            const int d = group + r * kGroups;
+            if (d >= a.width) continue;
+            const float kd = k[d], qd = q[d];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                S[r][j] = fused(g, S[r][j], kd * x[j]);
+                sum[j] = fused(qd, S[r][j], sum[j]);
+            }
+        }
+        if (!a.out.at) continue;
+        sums[group][lane] = sum;
+        __syncthreads();
+        if (tid < kStepColumns && e0 + tid < a.columns) {
+            float o = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kGroups; ++r) o += reinterpret_cast<const float*>(sums[r])[tid];
+            a.out.at[seq * a.out.seq + t * a.out.step + head * a.out.head + e0 + tid] = static_cast<T>(o * a.outer);
+        }
+    }
+    if (!a.end) return;
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        const int d = group + r * kGroups;
+        if (d < a.width) put_four(a.end + state + d * a.columns, c, a.columns, S[r]);
     }
 }
 
@@ -685,14 +779,15 @@ int bucket_of(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : width <=
 
 // The tokens of a segment.  Walks that are enough for most of the units go whole: what
 // cutting costs, the segments' own states first, is about half a walk.  Otherwise, and
-// where sequences are of any length, as many as give the units two workgroups each, 256
-// at least.
+// where sequences are of any length, as many as give the units two workgroups each, two
+// chunks at least.
 struct Cut { int64_t segment, segments, slots; };
 Cut cut_of(const hk_linear_attention_job& j, int columns, int walks) {
     const int64_t slices = (columns + slice_of(columns) - 1) / slice_of(columns), most = j.steps > 1 ? j.steps : 1;
     const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps, beside = j.heads * slices * walks;
     int64_t each = tokens / (2 * kUnits) * beside + 1;
-    each = each < 256 ? 256 : (each + 63) / 64 * 64;
+    const int64_t least = j.dtype == HK_BF16 ? 128 : 64;
+    each = each < least ? least : (each + 63) / 64 * 64;
     if (!j.offsets && j.seqs * beside >= kUnits * 3 / 4) each = most;
     if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1} : Cut{most, 1, j.seqs};
     if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs};
@@ -781,11 +876,30 @@ LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w, int walks
     return a;
 }
 
+// Dense sequences of up to kFewTokens tokens, forward: as they stand.  
+template <class T>
+int steps(const hk_linear_attention_job& j, const Walk& w, hipStream_t stream) {
+    LinearArgs<T> a = args_of<T>(j, w, 1);
+    a.slices = (w.columns + kStepColumns - 1) / kStepColumns;
+    const int64_t total = j.seqs * j.heads * a.slices, most = 1 << 22;
+    auto each = [&](auto kernel) {
+        for (int64_t before = 0; before < total; before += most) {
+            const int64_t left = total - before;
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(left < most ? left : most)), dim3(kStepThreads), 0, stream, a, before);
+        }
+    };
+    if (w.width <= 4 * kGroups) each(hawk_linear_steps<T, 4>);
+    else if (w.width <= 8 * kGroups) each(hawk_linear_steps<T, 8>);
+    else each(hawk_linear_steps<T, 16>);
+    return launched("hawk_linear_steps launch");
+}
+
 // Walks of one form are one launch.
 template <class T>
 int all(const hk_linear_attention_job& j, int vjp, void* scratch, hipStream_t stream) {
     Walk w[kMostWalks];
     const int n = walks_of(j, vjp, w);
+    if (!vjp && !j.offsets && j.steps <= kFewTokens) return steps<T>(j, w[0], stream);
     char* room = static_cast<char*>(scratch);
     bool done[kMostWalks] = {};
     for (int i = 0; i < n; ++i) {
