@@ -673,31 +673,28 @@ __global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> 
 // lanes, each every 16th row, a lane four columns of it.
 
 constexpr int kFewTokens = 8, kStepThreads = 256, kStepColumns = 64, kGroups = 16;
-// The four numbers at column c of a row of `columns` (Fours: a multiple of four), and the
-// same written.
-template <bool Fours>
+// The four numbers at column c of a row of `columns`, and the same written.
 __device__ __forceinline__ F4 four(const float* row, int c, int columns) {
     F4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (Fours ? c < columns : c + 4 <= columns) {
+    if (c + 4 <= columns) {
         x = load_raw<float, 4>(row + c);
-    } else if (!Fours) {
+    } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
             if (c + j < columns) x[j] = row[c + j];
     }
     return x;
 }
-template <bool Fours>
 __device__ __forceinline__ void put_four(float* row, int c, int columns, const F4& x) {
-    if (Fours ? c < columns : c + 4 <= columns) {
+    if (c + 4 <= columns) {
         store_raw<float, 4>(row + c, x);
-    } else if (!Fours) {
+    } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
             if (c + j < columns) row[c + j] = x[j];
     }
 }
-template <class T, int Rows, bool Fours>
+template <class T, int Rows>
 __global__ void __launch_bounds__(kStepThreads, Rows <= 8 ? 6 : 4) hawk_linear_steps(const LinearArgs<T> a, const int64_t before) {
     __shared__ float q[kMostWidth], k[kMostWidth], v[kStepColumns];
     __shared__ F4 sums[kGroups][kStepColumns / 4];
@@ -711,7 +708,7 @@ __global__ void __launch_bounds__(kStepThreads, Rows <= 8 ? 6 : 4) hawk_linear_s
     for (int r = 0; r < Rows; ++r) {
         const int d = group + r * kGroups;
         S[r] = F4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (a.start && d < a.width) S[r] = four<Fours>(a.start + state + d * a.columns, c, a.columns);
+        if (a.start && d < a.width) S[r] = four(a.start + state + d * a.columns, c, a.columns);
     }
     for (int64_t t = 0; t < a.steps; ++t) {
         __syncthreads();
@@ -748,7 +745,7 @@ __global__ void __launch_bounds__(kStepThreads, Rows <= 8 ? 6 : 4) hawk_linear_s
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {
         const int d = group + r * kGroups;
-        if (d < a.width) put_four<Fours>(a.end + state + d * a.columns, c, a.columns, S[r]);
+        if (d < a.width) put_four(a.end + state + d * a.columns, c, a.columns, S[r]);
     }
 }
 
@@ -891,14 +888,9 @@ int steps(const hk_linear_attention_job& j, const Walk& w, hipStream_t stream) {
             hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(left < most ? left : most)), dim3(kStepThreads), 0, stream, a, before);
         }
     };
-    auto rows = [&](auto fours) {
-        constexpr bool Fours = decltype(fours)::value;
-        if (w.width <= 4 * kGroups) each(hawk_linear_steps<T, 4, Fours>);
-        else if (w.width <= 8 * kGroups) each(hawk_linear_steps<T, 8, Fours>);
-        else each(hawk_linear_steps<T, 16, Fours>);
-    };
-    if (w.columns % 4 == 0) rows(std::true_type());
-    else rows(std::false_type());
+    if (w.width <= 4 * kGroups) each(hawk_linear_steps<T, 4>);
+    else if (w.width <= 8 * kGroups) each(hawk_linear_steps<T, 8>);
+    else each(hawk_linear_steps<T, 16>);
     return launched("hawk_linear_steps launch");
 }
 
