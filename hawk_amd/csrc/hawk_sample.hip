@@ -88,24 +88,33 @@ __device__ __forceinline__ float placed(uint32_t at) {
     return __builtin_bit_cast(float, at & 0x80000000u ? at : ~at & 0x7fffffffu);
 }
 
-// The sum of a wave's numbers, in every lane, and of the lanes before this one.
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+// Running sums over a wave's lanes, by moves between lanes that need no memory: within
+// rows of 16 lanes by 1, 2, 4 and 8, then a row's last lane into the rows after it.
+template <int Control, int Rows>
+__device__ __forceinline__ u64 moved(u64 v) {
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), Control, Rows, 0xf, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), Control, Rows, 0xf, false);
+    return static_cast<u64>(high) << 32 | low;
+}
+__device__ __forceinline__ u64 wave_upto(u64 v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ u64 wave_before(u64 v) {
-    u64 sum = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 t = __shfl_up(sum, d);
-        if (static_cast<int>(threadIdx.x & 63) >= d) sum += t;
-    }
-    return sum - v;
+__device__ __forceinline__ u64 last_lane(u64 v) {
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(v), 63), high = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
+    return static_cast<u64>(high) << 32 | low;
 }
+// The sum of a wave's numbers, and of the lanes before this one.
+__device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_upto(v)); }
+__device__ __forceinline__ u64 wave_before(u64 v) { return wave_upto(v) - v; }
 
 constexpr int kFew = 256;                  // candidates that are ranked by counting
-constexpr int kCells = 16;                 // of a wave: runs of its part of a row
+constexpr int kCells = 4;                  // of a wave: runs of its part of a row
 template <int NT>
 struct Sums {
     double table[kTable];
@@ -832,6 +841,7 @@ __global__ void __launch_bounds__(kDraw, 4) hawk_sample_draw(const SampleArgs<T>
     constexpr int Waves = kPart / 64, Most = kMostParts * Waves * kCells, Each = Most / kDraw;
     __shared__ Shared<kDraw, true> s;
     __shared__ u64 cells[Most];
+    static_assert(Most % kDraw == 0, "whole cells a thread");
     const int tid = threadIdx.x, vocab = static_cast<int>(a.vocab), count = p.parts * Waves * kCells;
     const int64_t n = blockIdx.x;
     const Asked q = asked(a, n);
