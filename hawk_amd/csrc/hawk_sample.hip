@@ -681,7 +681,7 @@ __device__ __forceinline__ u64 from_whole(Shared<NT, Filtered>& s, const Row<T, 
 
 // Rows of a workgroup each.
 template <class T, int NT, bool Filtered, bool Listed>
-__global__ void __launch_bounds__(NT, 4) hawk_sample(const SampleArgs<T> a) {
+__global__ void __launch_bounds__(NT, Filtered ? 4 : 6) hawk_sample(const SampleArgs<T> a) {
     __shared__ Shared<NT, Filtered> s;
     const int vocab = static_cast<int>(a.vocab);
     make_table(s, a.shift);
