@@ -180,7 +180,7 @@ struct Row {
     // f(first index, vector) of every step from `from` up to `end`, kAhead loads at a time;
     // a wave whose vectors are all in the row asks that once.
     template <class F> __device__ __forceinline__ void each(int from, int end, F&& f) const {
-        constexpr int V = kVec<T>, kAhead = 4;
+        constexpr int V = kVec<T>, kAhead = 2;
         for (int i = from; i < end; i += kAhead) {
             Raw<T, V> x[kAhead];
             const int p = position(i), first = __builtin_amdgcn_readfirstlane(p);
@@ -967,7 +967,7 @@ void launch(const SampleArgs<T>& a, dim3 grid, hipStream_t stream) {
     if (a.vocab <= 128) hipLaunchKernelGGL((hawk_sample<T, 64, Filtered, true>), grid, dim3(64), 0, stream, a);
     else if (a.vocab <= kList) hipLaunchKernelGGL((hawk_sample<T, 256, Filtered, true>), grid, dim3(256), 0, stream, a);
     else if (vectors <= 256 * 8) hipLaunchKernelGGL((hawk_sample<T, 256, Filtered, false>), grid, dim3(256), 0, stream, a);
-    else if (a.rows > 2 * kUnits) hipLaunchKernelGGL((hawk_sample<T, 512, Filtered, false>), grid, dim3(512), 0, stream, a);
+    else if (a.rows > kUnits) hipLaunchKernelGGL((hawk_sample<T, 512, Filtered, false>), grid, dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((hawk_sample<T, 1024, Filtered, false>), grid, dim3(1024), 0, stream, a);
 }
 
