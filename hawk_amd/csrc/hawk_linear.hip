@@ -113,7 +113,7 @@ struct LinearArgs {
     const float* decay;
     const float* start;        // the state that enters, element (d, e) at d*state_d + e*state_e of a head's; or NULL
     float* end;                // the state that leaves, or NULL
-    float* cuts;               // the segments' states, [slot][head][width][columns], or NULL
+    float* cuts;               // the states of sequences of several segments, [cut][head][width][columns], or NULL
     const void* offsets;
     int64_t seqs, steps, heads, slots, segment, segments;    // segments: of a dense sequence
     int state_d, state_e, width, columns, slices;
@@ -123,7 +123,8 @@ struct LinearArgs {
 
 struct Span {
     int64_t seq, first, length, begin, end;    // tokens [begin, end) of a sequence that starts at row `first`
-    bool real, last;
+    int64_t cut;                               // where its states are kept
+    bool real, last, whole;                    // whole: the sequence is one segment, which needs none
 };
 template <class T>
 __device__ __forceinline__ int64_t bound_of(const LinearArgs<T>& a, int64_t k) {
@@ -132,6 +133,12 @@ __device__ __forceinline__ int64_t bound_of(const LinearArgs<T>& a, int64_t k) {
 }
 // Sequence s's segments have the slots from bound(s) / segment + s on: more than it needs
 // by one at most, and none of two sequences.
+// Of packed sequences, at most one of several segments begins in each `segment` rows, and at
+// most one has a later segment that does: two states for each of those runs of rows.
+template <class T>
+__device__ __forceinline__ int64_t cut_at(const LinearArgs<T>& a, int64_t seq, int64_t first, int64_t segment) {
+    return a.offsets ? 2 * (first / a.segment + segment) + (segment == 0) : seq * a.segments + segment;
+}
 template <class T>
 __device__ __forceinline__ Span span_of(const LinearArgs<T>& a, int64_t slot) {
     Span s;
@@ -158,6 +165,8 @@ __device__ __forceinline__ Span span_of(const LinearArgs<T>& a, int64_t slot) {
     s.real = segment >= 0 && (segment == 0 || s.begin < s.length);
     s.end = s.begin + a.segment < s.length ? s.begin + a.segment : s.length;
     s.last = s.end == s.length;
+    s.whole = s.length <= a.segment;
+    s.cut = cut_at(a, s.seq, s.first, segment);
     return s;
 }
 
@@ -361,7 +370,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
     const double octaves = octaves_of(a.decay[head]);
     const int e0 = slice * Slice, columns = a.columns - e0;
     const int64_t plane = static_cast<int64_t>(a.width) * a.columns;
-    const int64_t state = (span.seq * a.heads + head) * plane, mark = pair * plane;
+    const int64_t state = (span.seq * a.heads + head) * plane, mark = (span.cut * a.heads + head) * plane;
     const int way = a.reverse ? -1 : 1;
     const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
     for (int n = tid; n <= C; n += Threads) {
@@ -372,8 +381,8 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
     // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
     F4 X[DP / 16];
     const int e = e0 + wave * 16 + col;
-    const float* enters = Whole ? a.cuts && span.length > 0 ? a.cuts + mark : a.start ? a.start + state : nullptr : nullptr;
-    const bool joined = enters && a.cuts && span.length > 0;
+    const bool joined = Whole && !span.whole;              // (such a call has cuts)
+    const float* enters = joined ? a.cuts + mark : Whole && a.start ? a.start + state : nullptr;
     const int enters_d = joined ? a.columns : a.state_d, enters_e = joined ? 1 : a.state_e;
     const float once = joined || a.reverse || span.length == 0 ? 1.0f : power(octaves, 1);
 #pragma unroll
@@ -637,22 +646,21 @@ __global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> 
         const int i = static_cast<int>(id - pair * blocks) * kJoinThreads + static_cast<int>(threadIdx.x);
         if (i >= plane) continue;
         const int64_t seq = pair / a.heads, head = pair - seq * a.heads;
-        int64_t length = a.steps, slot = seq * a.segments;
-        if (a.offsets) {
-            const int64_t first = bound_of(a, seq);
-            length = bound_of(a, seq + 1) - first;
-            slot = first / a.segment + seq;
-        }
-        int64_t segments = length > 0 ? (length + a.segment - 1) / a.segment : 1;
-        if (segments > a.slots - slot) segments = a.slots - slot;            // offsets that do not ascend
+        const int64_t first = a.offsets ? bound_of(a, seq) : 0, length = (a.offsets ? bound_of(a, seq + 1) : a.steps) - first;
+        if (length <= a.segment) continue;
+        const int64_t segments = (length + a.segment - 1) / a.segment;
         const double octaves = octaves_of(a.decay[head]);
         const float keep = power(octaves, a.segment);
         const int d = i / a.columns, e = i - d * a.columns;
         float x = 0.0f;
         if (a.start) x = a.start[pair * plane + d * a.state_d + e * a.state_e] * (a.reverse ? 1.0f : power(octaves, 1));
-        const int64_t step = a.heads * plane;
-        float* at = a.cuts + (slot * a.heads + head) * plane + i;
-        for (int64_t t = 0; t < segments; t += kAhead, at += kAhead * step) {
+        float* at = a.cuts + (cut_at(a, seq, first, 0) * a.heads + head) * plane + i;
+        const float leaves = *at;
+        *at = x;
+        x = fused(keep, x, leaves);
+        at = a.cuts + (cut_at(a, seq, first, 1) * a.heads + head) * plane + i;
+        const int64_t step = (a.offsets ? 2 : 1) * a.heads * plane;
+        for (int64_t t = 1; t < segments; t += kAhead, at += kAhead * step) {
             float own[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) own[k] = t + k + 1 < segments ? at[k * step] : 0.0f;   // (the last leaves nothing here)
@@ -779,25 +787,24 @@ int bucket_of(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : width <=
 
 // The tokens of a segment.  Walks that are enough for most of the units go whole: what
 // cutting costs, the segments' own states first, is about half a walk.  Otherwise, and
-// where sequences are of any length, as many as give the units two workgroups each, two
-// chunks at least.
-struct Cut { int64_t segment, segments, slots; };
+// where sequences are of any length (up to 16 workgroups a unit of them), as many as give
+// the units two workgroups each, two chunks at least.
+struct Cut { int64_t segment, segments, slots, cuts; };
 Cut cut_of(const hk_linear_attention_job& j, int columns, int walks) {
     const int64_t slices = (columns + slice_of(columns) - 1) / slice_of(columns), most = j.steps > 1 ? j.steps : 1;
     const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps, beside = j.heads * slices * walks;
     int64_t each = tokens / (2 * kUnits) * beside + 1;
     const int64_t least = j.dtype == HK_BF16 ? 128 : 64;
     each = each < least ? least : (each + 63) / 64 * 64;
-    if (!j.offsets && j.seqs * beside >= kUnits * 3 / 4) each = most;
-    if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1} : Cut{most, 1, j.seqs};
-    if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs};
+    if (j.seqs * beside >= (j.offsets ? 16 * kUnits : kUnits * 3 / 4)) each = most;
+    if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1, 0} : Cut{most, 1, j.seqs, 0};
+    if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs, 2 * (j.steps / each + 1)};
     const int64_t n = (j.steps + each - 1) / each;
-    return Cut{each, n, n * j.seqs};
+    return Cut{each, n, n * j.seqs, n * j.seqs};
 }
 size_t cuts_bytes(const hk_linear_attention_job& j, const Walk& w, int walks) {
     const Cut c = cut_of(j, w.columns, walks);
-    if (c.segment >= j.steps) return 0;
-    return static_cast<size_t>(c.slots) * static_cast<size_t>(j.heads) * w.width * w.columns * sizeof(float);
+    return static_cast<size_t>(c.cuts) * static_cast<size_t>(j.heads) * w.width * w.columns * sizeof(float);
 }
 
 template <class T>
@@ -811,14 +818,13 @@ int launched(const char* what) {
 template <class T, int DP, int C, int W>
 void launch(const Walks<T>& walks, int n, hipStream_t stream) {
     int64_t total = 0, joins = 0;
-    bool cuts = false;
+    const bool cuts = walks.walk[0].cuts;                  // walks of one form have their sequences cut alike
     for (int i = 0; i < n; ++i) {
         const LinearArgs<T>& a = walks.walk[i];
         const int64_t each = (a.slots * a.heads + kDies - 1) / kDies * kDies * a.slices;
         const int64_t plane = static_cast<int64_t>(a.width) * a.columns, parts = a.seqs * a.heads * ((plane + kJoinThreads - 1) / kJoinThreads);
         total = each > total ? each : total;
         joins = parts > joins ? parts : joins;
-        cuts = cuts || a.cuts;
     }
     const int64_t most = 1 << 20;
     auto each = [&](auto kernel) {                         // launches stay below 2^32 threads

@@ -321,7 +321,8 @@ def test_linear_attention_and_its_derivative_are_the_loop(gpu, shape, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape,packed", [((1, 1500, 2, 48, 80), False), ((3, 700, 1, 130, 24), False), ((1, 2049, 1, 16, 16), True),
-                                          ((7, 3000, 1, 64, 32), True)], ids=str)
+                                          ((7, 3000, 1, 64, 32), True), ((700, 1500, 8, 9, 12), True), ((300, 2600, 2, 20, 33), True)],
+                         ids=str)
 def test_a_long_sequence_is_cut_and_joined(gpu, shape, packed, dtype):
     check_attention(gpu, *shape, dtype, "steps", True, packed, 1)
 
