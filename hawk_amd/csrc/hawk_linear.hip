@@ -785,18 +785,27 @@ int walks_of(const hk_linear_attention_job& j, int vjp, Walk (&w)[kMostWalks]) {
 int slice_of(int columns) { return columns > 64 ? 128 : 64; }
 int bucket_of(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : width <= 128 ? 128 : 256; }
 
-// The tokens of a segment.  Walks that are enough for most of the units go whole: what
-// cutting costs, the segments' own states first, is about half a walk.  Otherwise, and
-// where sequences are of any length (up to 16 workgroups a unit of them), as many as give
-// the units two workgroups each, two chunks at least.
+// Walks of one form are one launch: those like w[i] of the n.
+bool alike(const Walk& a, const Walk& b) { return bucket_of(a.width) == bucket_of(b.width) && slice_of(a.columns) == slice_of(b.columns); }
+int beside_of(const Walk* w, int n, int i) {
+    int count = 0;
+    for (int k = 0; k < n; ++k) count += alike(w[i], w[k]);
+    return count;
+}
+
+// The tokens of a segment.  A launch whose whole walks are enough for most of the units
+// goes uncut: what cutting costs, the segments' own states first, is about half a walk.
+// Otherwise, and where sequences are of any length (up to eight times as many workgroups of
+// them), as many segments as give each unit two workgroups of eight waves, or four of four,
+// of two chunks at least.
 struct Cut { int64_t segment, segments, slots, cuts; };
 Cut cut_of(const hk_linear_attention_job& j, int columns, int walks) {
     const int64_t slices = (columns + slice_of(columns) - 1) / slice_of(columns), most = j.steps > 1 ? j.steps : 1;
     const int64_t tokens = j.offsets ? j.steps : j.seqs * j.steps, beside = j.heads * slices * walks;
-    int64_t each = tokens / (2 * kUnits) * beside + 1;
-    const int64_t least = j.dtype == HK_BF16 ? 128 : 64;
+    const int64_t full = (slice_of(columns) == 64 ? 4 : 2) * kUnits, least = j.dtype == HK_BF16 ? 128 : 64;
+    int64_t each = tokens / full * beside + 1;
     each = each < least ? least : (each + 63) / 64 * 64;
-    if (j.seqs * beside >= (j.offsets ? 16 * kUnits : kUnits * 3 / 4)) each = most;
+    if (j.seqs * beside >= (j.offsets ? 8 * full : full * 3 / 8)) each = most;
     if (each >= most) return j.offsets ? Cut{most, 1, j.seqs + 1, 0} : Cut{most, 1, j.seqs, 0};
     if (j.offsets) return Cut{each, 0, j.steps / each + j.seqs, 2 * (j.steps / each + 1)};
     const int64_t n = (j.steps + each - 1) / each;
@@ -900,7 +909,7 @@ int steps(const hk_linear_attention_job& j, const Walk& w, hipStream_t stream) {
     return launched("hawk_linear_steps launch");
 }
 
-// Walks of one form are one launch.
+// Every walk, those of one form in one launch.
 template <class T>
 int all(const hk_linear_attention_job& j, int vjp, void* scratch, hipStream_t stream) {
     Walk w[kMostWalks];
@@ -912,17 +921,18 @@ int all(const hk_linear_attention_job& j, int vjp, void* scratch, hipStream_t st
         if (done[i]) continue;
         Walks<T> walks = {};
         int count = 0;
-        const int bucket = bucket_of(w[i].width), slice = slice_of(w[i].columns);
+        const int beside = beside_of(w, n, i);
         for (int k = i; k < n; ++k) {
-            if (done[k] || bucket_of(w[k].width) != bucket || slice_of(w[k].columns) != slice) continue;
+            if (done[k] || !alike(w[i], w[k])) continue;
             done[k] = true;
-            walks.walk[count] = args_of<T>(j, w[k], n);
-            const size_t bytes = cuts_bytes(j, w[k], n);
+            walks.walk[count] = args_of<T>(j, w[k], beside);
+            const size_t bytes = cuts_bytes(j, w[k], beside);
             if (bytes) walks.walk[count].cuts = reinterpret_cast<float*>(room);
             room += bytes;
             ++count;
         }
-        if (slice == 64) launch<T, 4>(walks, count, bucket, stream);
+        const int bucket = bucket_of(w[i].width);
+        if (slice_of(w[i].columns) == 64) launch<T, 4>(walks, count, bucket, stream);
         else launch<T, 8>(walks, count, bucket, stream);
         const int rc = launched("hawk_linear launch");
         if (rc != HK_OK) return rc;
@@ -960,7 +970,7 @@ extern "C" size_t hk_linear_attention_scratch_bytes(const hk_linear_attention_jo
     Walk w[kMostWalks];
     const int n = walks_of(*job, vjp, w);
     size_t bytes = 0;
-    for (int i = 0; i < n; ++i) bytes += cuts_bytes(*job, w[i], n);
+    for (int i = 0; i < n; ++i) bytes += cuts_bytes(*job, w[i], beside_of(w, n, i));
     return bytes;
 }
 
