@@ -19,7 +19,16 @@
 // The numbers.  X and every sum are held in 32 bits.  The matrix cores multiply bf16;
 // a number of more digits is a sum of bf16 parts (three make 24 bits), and a product is
 // the sum of the parts' products down to 2^-17 of it where the result is rounded to 16
-// bits, 2^-25 otherwise, and always 2^-25 in X.
+// bits, 2^-25 otherwise, and always 2^-25 in X where it leaves.
+//
+// What bounds it.  The eight waves of a workgroup share a chunk, in phases between four
+// barriers; registers and LDS hold two workgroups a unit.  In the walk of 16 heads of 128
+// bfloat16 columns LDS is busy half of the time, the vector units half and
+// the matrix cores a quarter.  One sequence of 32768 such tokens takes 265 us (states of
+// its segments 81, their join 14, the walk 180; the bytes' time is 81); the derivative of
+// 8 x 4096 tokens, whose 8 * 16 * 3 walks fill the chip uncut, 525 in one launch, where
+// cut sequences took 750.  Waves of two column tiles, four to a workgroup, took 566 and
+// 292; products of two tiles in turn, no less.
 
 #include "hawk_core.h"
 #include "hawk_internal.h"
@@ -891,7 +900,8 @@ LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w, int walks
     return a;
 }
 
-// Dense sequences of up to kFewTokens tokens, forward: as they stand.
+// Dense sequences of up to kFewTokens tokens, forward: as they stand, by vector arithmetic
+// (64 x 16 heads of 128 x 128, one token: 29.7 us, 41.9 by chunks; its states take 20.7).
 template <class T>
 int steps(const hk_linear_attention_job& j, const Walk& w, hipStream_t stream) {
     LinearArgs<T> a = args_of<T>(j, w, 1);
