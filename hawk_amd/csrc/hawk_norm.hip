@@ -566,14 +566,14 @@ int norm_vjp(const hk_layer_norm_job& j, float* scratch, hipStream_t stream) {
     if (j.rows) {
         const Shape s = shape_of(j.cols, sizeof(T));
         if (s.lanes == 0) {
-            if (a.bar_x) {
-                const dim3 grid(static_cast<unsigned>(j.rows < 4 * kUnits ? j.rows : 4 * kUnits)), block(kMost);
-                hipLaunchKernelGGL((hawk_norm_vjp_long<T>), grid, block, 0, stream, a);
-            }
-            if (sums) {
+            if (sums) {                                    // first: bar_x may be x or bar_y
                 const int64_t tile = kThreads * kVec<T>;
                 const dim3 grid(static_cast<unsigned>((j.cols + tile - 1) / tile), static_cast<unsigned>(parts)), block(kThreads);
                 hipLaunchKernelGGL((hawk_norm_columns<T>), grid, block, 0, stream, a);
+            }
+            if (a.bar_x) {
+                const dim3 grid(static_cast<unsigned>(j.rows < 4 * kUnits ? j.rows : 4 * kUnits)), block(kMost);
+                hipLaunchKernelGGL((hawk_norm_vjp_long<T>), grid, block, 0, stream, a);
             }
         } else if (s.lanes == 16) launch_vjp<T, 16, 1>(a, parts, stream);
         else if (s.lanes == 64) s.vectors == 1 ? launch_vjp<T, 64, 1>(a, parts, stream) : s.vectors == 2 ? launch_vjp<T, 64, 2>(a, parts, stream) : wave_of_four<T>([&](auto four) { launch_vjp<T, 64, decltype(four)::value>(a, parts, stream); });

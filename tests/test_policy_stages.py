@@ -183,6 +183,28 @@ def test_layer_norm_in_place_and_a_row_that_is_no_number(gpu, C):
     assert torch.equal(x[[0, 2, 4]], y[[0, 2, 4]])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,C", [("float32", 50), ("bfloat16", 2049), ("float16", 16383), ("bfloat16", 16400), ("float32", 8200)])
+def test_layer_norms_derivative_written_over_its_inputs(gpu, dtype, C):
+    """``bar_x`` over ``x`` or ``bar_y``: the bits of the call that writes another plane."""
+    import torch
+    g, N = torch.Generator().manual_seed(C), 700
+    x, by = (torch.randn(N, C, generator=g).to(gpu, getattr(torch, dtype)) for _ in range(2))
+    w, y, mean, rstd = torch.randn(C, generator=g).to(gpu), torch.empty_like(x), torch.empty(N, device=gpu), torch.empty(N, device=gpu)
+    stage = hawk.stages.layer_norm()
+    hawk.run(stage, x=x, weight=w, y=y, mean=mean, rstd=rstd)
+
+    def derivative(x, by, bx):
+        bw, bb = torch.full((2, C), 7.0, device=gpu)
+        hawk.run(stage.vjp, x=x, weight=w, mean=mean, rstd=rstd, bar_y=by, bar_x=bx, bar_weight=bw, bar_bias=bb)
+        return bx, bw, bb
+
+    want = derivative(x, by, torch.empty_like(x))
+    a, b = x.clone(), by.clone()
+    for got in (derivative(a, by, a), derivative(x, b, b)):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 # -- linear attention --------------------------------------------------------------------------
 
 def spans(S, T, offsets):
