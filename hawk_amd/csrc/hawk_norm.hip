@@ -163,7 +163,7 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_norm(const
         const T* row = a.x + n * a.x_stride;
         Raw<T, V> x[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] = fetch<T, Whole, kOnce<T>>(row, begin_of<T, Whole>((i * L + lane) * V, cols), cols);
+        for (int i = 0; i < NV; ++i) x[i] = fetch<T, Whole, kOnce<T> && Whole>(row, begin_of<T, Whole>((i * L + lane) * V, cols), cols);
         float s[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_norm(const
             factors<T, Whole>(a.bias, a.wide, c, cols, 0.0f, b);
 #pragma unroll
             for (int j = 0; j < V; ++j) y[j] = fused((widen<T, V>(x[i], j) - mean) * rstd, w[j], b[j]);
-            leave<T, Whole, kOnce<T>>(out, c, cols, y);
+            leave<T, Whole, kOnce<T> && Whole>(out, c, cols, y);
         }
     }
 }
@@ -279,8 +279,8 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_norm_vjp(c
         next_rstd = a.rstd[row];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            nx[i] = order<T, Whole, kOnce<T>>(a.x + row * a.x_stride, (i * L + lane) * V, cols);
-            nb[i] = order<T, Whole, kOnce<T>>(a.bar_y + row * a.bar_y_stride, (i * L + lane) * V, cols);
+            nx[i] = order<T, Whole, kOnce<T> && Whole>(a.x + row * a.x_stride, (i * L + lane) * V, cols);
+            nb[i] = order<T, Whole, kOnce<T> && Whole>(a.bar_y + row * a.bar_y_stride, (i * L + lane) * V, cols);
         }
     };
     ask(n);
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__((L > kThreads ? L : kThreads)) hawk_norm_vjp(c
                 const float xh = (widen<T, V>(x[i], j) - mean) * rstd;
                 out[j] = rstd * (fused(widen<T, V>(b[i], j), w[i][j], -one) - xh * two);
             }
-            leave<T, Whole, kOnce<T>>(a.bar_x + n * a.bar_x_stride, (i * L + lane) * V, cols, out);
+            leave<T, Whole, kOnce<T> && Whole>(a.bar_x + n * a.bar_x_stride, (i * L + lane) * V, cols, out);
         }
     }
     if (!a.parts) return;
