@@ -30,7 +30,7 @@ namespace {
 using namespace hawk_vec;
 
 constexpr int kThreads = 256;
-constexpr int kMost = 1024;                // lanes that a row is spread over at most
+constexpr int kMost = 1024;                // lanes of a row that is not held in registers
 constexpr int64_t kUnits = 256;            // compute units
 
 template <class T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -54,7 +54,7 @@ struct NormArgs {
 // where they are that lane's and are written by both, the same; in the derivative, which
 // keeps sums of the columns, the vector is ordered ahead and settled, moved into place, when
 // it is used.  (144416 rows of 347 bfloat16 columns, element by element: 100 and 257 us;
-// this way 96 and 180.  Of floats there are three at most, and element by element is as good.)
+// this way 81 and 180.  Of floats there are three at most, and element by element is as good.)
 template <class T, bool Whole>
 __device__ __forceinline__ bool shared_end(int c, int cols) {
     constexpr int V = kVec<T>;
@@ -460,22 +460,26 @@ int size_of(int dtype) { return dtype == HK_F32 ? 4 : 2; }
 // How a row is held: `lanes` lanes of `vectors` vectors, or lanes = 0 for one that is
 // not.  A row takes the fewest lanes that hold it in two vectors each; a wave four of them
 // where those are 16 numbers, as it waits for no other wave (the derivative of 3001 rows of
-// 777 floats with the sums: 14.9 us, 16.9 by four waves a row).
+// 777 floats with the sums: 14.9 us, 16.9 by four waves a row).  The wider the workgroup of a
+// row is, the fewer rows are under way beside one that waits at its barrier, so long rows
+// take few waves: 16384 x 8192 bfloat16 forward 122 us by 256 lanes of four, 165 by 1024 of
+// one, its derivative 146 by 512 of two, 182 by 1024 of one; 4096 x 16384 forward 61 by 512 of four, 78 by
+// 1024 of two.  The derivative's sums leave no registers for more vectors a lane.
 struct Shape { int lanes, vectors; };
-Shape shape_of(int64_t cols, int esize) {
+Shape shape_of(int64_t cols, int esize, bool vjp) {
     const int64_t vectors = (cols + 16 / esize - 1) / (16 / esize);
     if (vectors <= 16) return {16, 1};
     if (vectors <= 64) return {64, 1};
     if (vectors <= 128) return {64, 2};
     if (vectors <= 256) return esize == 4 ? Shape{64, 4} : Shape{256, 1};
     if (vectors <= 512) return {256, 2};
-    if (vectors <= 1024) return {1024, 1};
-    if (vectors <= 2048) return {1024, 2};
+    if (vectors <= 1024) return vjp ? Shape{512, 2} : Shape{256, 4};
+    if (vectors <= 2048) return vjp ? Shape{1024, 2} : Shape{512, 4};
     return {0, 0};
 }
 // The derivative's workgroups, each with a partial sum a column.
 int64_t parts_of(int64_t rows, int64_t cols, int esize) {
-    const Shape s = shape_of(cols, esize);
+    const Shape s = shape_of(cols, esize, true);
     if (s.lanes == 0) return rows < kUnits / 4 ? rows : kUnits / 4;
     const int64_t at_once = s.lanes > kThreads ? 1 : kThreads / s.lanes;
     const int64_t need = (rows + at_once - 1) / at_once, most = s.lanes > kThreads ? kUnits : 2 * kUnits;
@@ -528,14 +532,14 @@ void launch_norm(const NormArgs<T>& a, hipStream_t stream) {
 template <class T>
 int norm(const hk_layer_norm_job& j, hipStream_t stream) {
     const NormArgs<T> a = args_of<T>(j);
-    const Shape s = shape_of(j.cols, sizeof(T));
+    const Shape s = shape_of(j.cols, sizeof(T), false);
     if (s.lanes == 0) {
         const dim3 grid(static_cast<unsigned>(j.rows < 4 * kUnits ? j.rows : 4 * kUnits)), block(kMost);
         hipLaunchKernelGGL((hawk_norm_long<T>), grid, block, 0, stream, a);
     } else if (s.lanes == 16) launch_norm<T, 16, 1>(a, stream);
     else if (s.lanes == 64) s.vectors == 1 ? launch_norm<T, 64, 1>(a, stream) : s.vectors == 2 ? launch_norm<T, 64, 2>(a, stream) : wave_of_four<T>([&](auto four) { launch_norm<T, 64, decltype(four)::value>(a, stream); });
-    else if (s.lanes == 256) s.vectors == 1 ? launch_norm<T, 256, 1>(a, stream) : launch_norm<T, 256, 2>(a, stream);
-    else s.vectors == 1 ? launch_norm<T, 1024, 1>(a, stream) : launch_norm<T, 1024, 2>(a, stream);
+    else if (s.lanes == 256) s.vectors == 1 ? launch_norm<T, 256, 1>(a, stream) : s.vectors == 2 ? launch_norm<T, 256, 2>(a, stream) : launch_norm<T, 256, 4>(a, stream);
+    else launch_norm<T, 512, 4>(a, stream);
     return launched("hawk_norm launch");
 }
 
@@ -564,7 +568,7 @@ int norm_vjp(const hk_layer_norm_job& j, float* scratch, hipStream_t stream) {
     const int64_t parts = j.rows ? parts_of(j.rows, j.cols, sizeof(T)) : 0;
     if (sums) a.parts = scratch;
     if (j.rows) {
-        const Shape s = shape_of(j.cols, sizeof(T));
+        const Shape s = shape_of(j.cols, sizeof(T), true);
         if (s.lanes == 0) {
             if (sums) {                                    // first: bar_x may be x or bar_y
                 const int64_t tile = kThreads * kVec<T>;
@@ -578,7 +582,8 @@ int norm_vjp(const hk_layer_norm_job& j, float* scratch, hipStream_t stream) {
         } else if (s.lanes == 16) launch_vjp<T, 16, 1>(a, parts, stream);
         else if (s.lanes == 64) s.vectors == 1 ? launch_vjp<T, 64, 1>(a, parts, stream) : s.vectors == 2 ? launch_vjp<T, 64, 2>(a, parts, stream) : wave_of_four<T>([&](auto four) { launch_vjp<T, 64, decltype(four)::value>(a, parts, stream); });
         else if (s.lanes == 256) s.vectors == 1 ? launch_vjp<T, 256, 1>(a, parts, stream) : launch_vjp<T, 256, 2>(a, parts, stream);
-        else s.vectors == 1 ? launch_vjp<T, 1024, 1>(a, parts, stream) : launch_vjp<T, 1024, 2>(a, parts, stream);
+        else if (s.lanes == 512) launch_vjp<T, 512, 2>(a, parts, stream);
+        else launch_vjp<T, 1024, 2>(a, parts, stream);
         const int rc = launched("hawk_norm_vjp launch");
         if (rc != HK_OK) return rc;
     }
