@@ -18,8 +18,11 @@
 //
 // The numbers.  X and every sum are held in 32 bits.  The matrix cores multiply bf16;
 // a number of more digits is a sum of bf16 parts (three make 24 bits), and a product is
-// the sum of the parts' products down to 2^-17 of it where the result is rounded to 16
-// bits, 2^-25 otherwise, and always 2^-25 in X where it leaves.
+// the sum of the parts' products down to 2^-25 of it wherever X is made or read.  Inside a
+// chunk (a_i . b_j, and that times c_j) it is so for 32-bit planes; where the result is
+// rounded to 16 bits, a_i . b_j is held as two parts, 2^-18 of it, which leaves 6e-5 of a
+// bfloat16 result's norm in places that round the other way (three parts: 4e-5, and 345
+// and 824 us where the two below take 289 and 604).
 //
 // What bounds it.  The eight waves of a workgroup share a chunk, in phases between four
 // barriers; registers and LDS hold two workgroups a unit.  In the walk of 16 heads of 128
@@ -91,12 +94,12 @@ __device__ __forceinline__ void parts_of(T x, uint16_t (&out)[N]) {
 }
 __device__ __forceinline__ float part(uint16_t h) { return __builtin_bit_cast(float, static_cast<uint32_t>(h) << 16); }
 
-// The parts of a type's elements, and of what is computed from them.
+// The parts of a type's elements, and of what a chunk computes from them.
 template <class T> struct Parts;
 template <> struct Parts<bf16> { static constexpr int in = 1, made = 2, reach = 2; };
 template <> struct Parts<f16> { static constexpr int in = 2, made = 2, reach = 2; };
 template <> struct Parts<float> { static constexpr int in = 3, made = 3, reach = 3; };
-constexpr int kExact = 3;                  // X is kept to 24 bits
+constexpr int kExact = 3;                  // X is kept, made and read to 24 bits
 
 // sum over pairs of parts (p, q) with p + q < Reach
 template <int Reach, int N, int M>
@@ -507,19 +510,19 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             for (int t = 0; t < C / 16; ++t) o[t] = F4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int d = 0; d < DP; d += 32) {
-                H8 fx[M];
+                H8 fx[kExact];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    uint16_t q[M];
-                    cut<M>(X[d / 16 + k / 4][k & 3], q);
+                    uint16_t q[kExact];
+                    cut<kExact>(X[d / 16 + k / 4][k & 3], q);
 #pragma unroll
-                    for (int n = 0; n < M; ++n) fx[n][k] = q[n];
+                    for (int n = 0; n < kExact; ++n) fx[n][k] = q[n];
                 }
 #pragma unroll
                 for (int t = 0; t < C / 16; ++t) {
                     H8 fa[N];
                     take(fa, s.a, t * 16 + col, d + quad * 8);
-                    o[t] = product<Reach>(fx, fa, o[t]);
+                    o[t] = product<kExact>(fx, fa, o[t]);
                 }
                 in_order();
             }
@@ -608,24 +611,12 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
 #pragma unroll
                 for (int p = 0; p < kExact; ++p) fw[p][k] = q[p];
             }
-            // X's last digits show in the state that leaves, not in results of 16 bits
-            if (Reach < kExact && a.end) {
-                in_order();
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    H8 fb[N];
-                    take(fb, s.turned, i * 16 + col, unit(i * 16 + col, j / 8 + quad));
-#pragma unroll
-                    for (int p = 0; p < N; ++p) X[i] = product(fb[p], fw[kExact - 1 - p], X[i]);
-                    if (i & 1) in_order();
-                }
-            }
             in_order();
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 H8 fb[N];
                 take(fb, s.turned, i * 16 + col, unit(i * 16 + col, j / 8 + quad));
-                X[i] = product<Reach>(fb, fw, X[i]);
+                X[i] = product<kExact>(fb, fw, X[i]);
                 if (i & 1) in_order();
             }
         }

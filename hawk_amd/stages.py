@@ -868,8 +868,9 @@ def linear_attention(scale: float = 1.0) -> Stage:
     are ``(sequences, heads, keys, values)`` in float32.  One token of running
     sequences is the same call with one step, ``h0`` and ``last``.
 
-    States and sums are held in 32 bits; products are taken to 2^-24 in the states and
-    for float32 planes, to 2^-16 of each where ``o`` is rounded to 16 bits.  A token
+    States and sums are held in 32 bits; products are taken to 2^-24 where states are made
+    and read and for float32 planes; with 16-bit planes those of a token with the last 63
+    before it are taken to 2^-16 of each.  A token
     with an infinity or a NaN makes what it reaches no number (an infinity may come
     out as a NaN) and leaves earlier tokens as they are.
 

@@ -1,0 +1,53 @@
+"""Linear attention, layer norm and sampling (``hawk.stages``) where their digits, their
+planes' layouts and their launches end, against plain sums in 64 bits.
+
+``u`` = 2^-24 is the most that one rounding to 24 bits is off, relative to the value.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import hawk_amd as hawk
+
+U = 2.0 ** -24
+
+
+def back(x):
+    return x.double().cpu().numpy()
+
+
+# -- linear attention --------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 13], ids=["cut", "whole"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_the_state_is_made_and_read_to_24_bits(gpu, dtype, S):
+    """Two channels of the state that cancel: one made of the first token, one that entered.  From the
+    second chunk on a result is their difference alone, whose error is that of the states' digits.
+
+    Each channel has at most half of the magnitudes' sum M.  Its roundings: the token's factor, its product
+    and that one's parts and sum (4), two a chunk for each of five chunks, two where segments are joined, the
+    parts as it is read (1), six products added: 23.  A float16 result is a multiple of 2^-24."""
+    import torch
+    T, H, V = 130, 32, 16
+    g = np.random.default_rng([S, len(dtype)])
+    kind = getattr(torch, dtype)
+    decay = np.float32(1 - 2.0 ** -8 * g.random(H))
+    v = torch.zeros(S, T, H, V, dtype=kind)
+    v[:, 0] = torch.from_numpy(g.uniform(0.5, 2, (S, H, V))).to(kind)
+    first = back(v[:, 0])
+    h0 = np.zeros((S, H, 2, V), np.float32)
+    h0[:, :, 1] = first / decay.astype(np.float64)[:, None]
+    q, k = torch.empty(S, T, H, 2, dtype=kind), torch.zeros(S, T, H, 2, dtype=kind)
+    q[..., 0], q[..., 1], k[:, 0, :, 0] = 1, -1, 1
+    q, k, v = q.to(gpu), k.to(gpu), v.to(gpu)
+    o = torch.empty_like(v)
+    hawk.run(hawk.stages.linear_attention(), q=q, k=k, v=v, decay=torch.from_numpy(decay).to(gpu),
+             h0=torch.from_numpy(h0).to(gpu), o=o)
+    power = decay.astype(np.float64)[None, :] ** np.arange(T + 1)[:, None]           # (T + 1, H)
+    made = power[None, :T, :, None] * first[:, None]
+    entered = power[None, 1:, :, None] * h0[:, None, :, 1].astype(np.float64)
+    off = np.abs(back(o) - (made - entered)) - (24 * U * (made + np.abs(entered)) + 2.0 ** -25)
+    assert (off[:, 64:] <= 0).all(), off[:, 64:].max()
