@@ -182,11 +182,13 @@ __device__ __forceinline__ Span span_of(const LinearArgs<T>& a, int64_t slot) {
     return s;
 }
 
-__device__ __forceinline__ double octaves_of(float g) {
-    if (!(g >= 0.0f && g <= 1.0f)) return NAN;
-    return g == 0.0f ? -1e30 : log2(static_cast<double>(g));
-}
-__device__ __forceinline__ float power(double octaves, int64_t n) { return exp2f(static_cast<float>(octaves * static_cast<double>(n))); }
+__device__ __forceinline__ float decay_of(float given) { return given >= 0.0f && given <= 1.0f ? given : NAN; }
+// g^n in 64 bits.  A factor of the state that is applied chunk after chunk is held as a
+// float and a rest: rounded alone, it would be off the same way every time, and a state that
+// remembers n chunks by n roundings.
+__device__ __forceinline__ double octaves_of(float g) { return g == 0.0f ? -1e30 : log2(static_cast<double>(g)); }
+__device__ __forceinline__ double power(double octaves, int64_t n) { return exp2(octaves * static_cast<double>(n)); }
+__device__ __forceinline__ float rest_of(double x) { return static_cast<float>(x - static_cast<double>(static_cast<float>(x))); }
 
 // Where column d of a is staged: the order in which X's rows lie in the lanes, two
 // tiles of 16 after each other.
@@ -282,6 +284,7 @@ struct Tiles {
     uint16_t c[N][16 * W][Long];
     uint16_t inside[M][C][Long];                           // g^(i-j) a_i . b_j
     float power[C + 1];                                    // g^n
+    float rest;                                            // what g^C has below its 24 bits
     float scaled[C];                                       // the same, times what inside is scaled by
     alignas(16) float weight[C];                           // what a token of the chunk has in X'
     int odd;                                               // c holds what is no number
@@ -379,15 +382,18 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
     const int64_t slot = pair / a.heads, head = pair - slot * a.heads;
     const Span span = span_of(a, slot);
     if (!span.real || (!Whole && span.last)) return;
-    const double octaves = octaves_of(a.decay[head]);
+    const float g = decay_of(a.decay[head]);
+    const double octaves = octaves_of(g);
     const int e0 = slice * Slice, columns = a.columns - e0;
     const int64_t plane = static_cast<int64_t>(a.width) * a.columns;
     const int64_t state = (span.seq * a.heads + head) * plane, mark = (span.cut * a.heads + head) * plane;
     const int way = a.reverse ? -1 : 1;
     const int64_t row0 = a.reverse ? span.first + span.length - 1 : span.first;
     for (int n = tid; n <= C; n += Threads) {
-        s.power[n] = power(octaves, n);
+        const double p = power(octaves, n);
+        s.power[n] = static_cast<float>(p);
         if (n < C) s.scaled[n] = s.power[n] * (a.inner * a.outer);
+        else s.rest = rest_of(p);
     }
 
     // X: tile i holds rows 16 i + 4 quad .. + 3 of column e
@@ -396,7 +402,7 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
     const bool joined = Whole && !span.whole;              // (such a call has cuts)
     const float* enters = joined ? a.cuts + mark : Whole && a.start ? a.start + state : nullptr;
     const int enters_d = joined ? a.columns : a.state_d, enters_e = joined ? 1 : a.state_e;
-    const float once = joined || a.reverse || span.length == 0 ? 1.0f : power(octaves, 1);
+    const float once = joined || a.reverse || span.length == 0 ? 1.0f : g;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) X[i] = F4{0.0f, 0.0f, 0.0f, 0.0f};
     if (enters)
@@ -589,11 +595,11 @@ __global__ void __launch_bounds__(64 * W, (DP < 256 && sizeof(T) == 2 && W == 8 
             __syncthreads();
         }
         // X' = g^n X + sum_j g^(n-j) b_j c_j
-        const float keep = s.power[n];
+        const float keep = s.power[n], rest = n == C ? s.rest : 0.0f;
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) X[i][k] *= keep;
+            for (int k = 0; k < 4; ++k) X[i][k] = fused(keep, X[i][k], rest * X[i][k]);
 #pragma unroll
         for (int j = 0; j < C; j += 32) {
             H8 fc[N], fw[kExact];
@@ -649,15 +655,17 @@ __global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> 
         const int64_t first = a.offsets ? bound_of(a, seq) : 0, length = (a.offsets ? bound_of(a, seq + 1) : a.steps) - first;
         if (length <= a.segment) continue;
         const int64_t segments = (length + a.segment - 1) / a.segment;
-        const double octaves = octaves_of(a.decay[head]);
-        const float keep = power(octaves, a.segment);
+        const float g = decay_of(a.decay[head]);
+        const double whole = power(octaves_of(g), a.segment);
+        const float keep = static_cast<float>(whole), rest = rest_of(whole);
+        auto joined = [&](float x, float own) { return fused(keep, x, fused(rest, x, own)); };
         const int d = i / a.columns, e = i - d * a.columns;
         float x = 0.0f;
-        if (a.start) x = a.start[pair * plane + d * a.state_d + e * a.state_e] * (a.reverse ? 1.0f : power(octaves, 1));
+        if (a.start) x = a.start[pair * plane + d * a.state_d + e * a.state_e] * (a.reverse ? 1.0f : g);
         float* at = a.cuts + (cut_at(a, seq, first, 0) * a.heads + head) * plane + i;
         const float leaves = *at;
         *at = x;
-        x = fused(keep, x, leaves);
+        x = joined(x, leaves);
         at = a.cuts + (cut_at(a, seq, first, 1) * a.heads + head) * plane + i;
         const int64_t step = (a.offsets ? 2 : 1) * a.heads * plane;
         for (int64_t t = 1; t < segments; t += kAhead, at += kAhead * step) {
@@ -668,7 +676,7 @@ __global__ void __launch_bounds__(kJoinThreads) hawk_linear_join(const Walks<T> 
             for (int k = 0; k < kAhead; ++k) {
                 if (t + k >= segments) break;
                 at[k * step] = x;
-                x = fused(keep, x, own[k]);
+                x = joined(x, own[k]);
             }
         }
     }
@@ -710,7 +718,7 @@ __global__ void __launch_bounds__(kStepThreads, Rows <= 8 ? 6 : 4) hawk_linear_s
     const int64_t id = before + blockIdx.x, pair = id / a.slices, seq = pair / a.heads, head = pair - seq * a.heads;
     const int e0 = static_cast<int>(id - pair * a.slices) * kStepColumns, c = e0 + lane * 4;
     const int64_t state = pair * (static_cast<int64_t>(a.width) * a.columns);
-    const float given = a.decay[head], g = given >= 0.0f && given <= 1.0f ? given : NAN;
+    const float g = decay_of(a.decay[head]);
     F4 S[Rows];
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {

@@ -51,3 +51,27 @@ def test_the_state_is_made_and_read_to_24_bits(gpu, dtype, S):
     entered = power[None, 1:, :, None] * h0[:, None, :, 1].astype(np.float64)
     off = np.abs(back(o) - (made - entered)) - (24 * U * (made + np.abs(entered)) + 2.0 ** -25)
     assert (off[:, 64:] <= 0).all(), off[:, 64:].max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,T,K", [(100, 8192, 16), (1, 65536, 64)], ids=["whole", "cut"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_state_that_fades_slowly_is_off_by_roundings_of_either_sign(gpu, dtype, S, T, K):
+    """Tokens of zeros: the state only decays, a factor a chunk (of 32 tokens at least) or a segment.  Each
+    rounds every number, by u / sqrt(3) in the mean square, so the mean over a head's numbers errs by
+    sqrt(n / (3 numbers)) u; six times that, and u for the factor of the last tokens, which are no whole chunk.
+    A factor that is itself rounded moves all numbers the same way, by up to u for each of the n."""
+    import torch
+    decay = np.float32([1 - 2.0 ** -10, 1 - 2.0 ** -11, 1 - 2.0 ** -13, 1 - 2.0 ** -16])
+    H = len(decay)
+    plane = torch.zeros(K, dtype=getattr(torch, dtype), device=gpu).expand(S, T, H, K)
+    g = np.random.default_rng(S)
+    h0 = torch.from_numpy(g.uniform(1, 2, (S, H, K, K)).astype(np.float32)).to(gpu)
+    for stage, planes in ((hawk.stages.linear_attention(), dict(h0=h0, last=torch.empty_like(h0))),
+                          (hawk.stages.linear_attention().vjp, dict(bar_o=plane, bar_last=h0, bar_h0=torch.empty_like(h0)))):
+        hawk.run(stage, q=plane, k=plane, v=plane, decay=torch.from_numpy(decay).to(gpu), **planes)
+        left = back(planes.get("last", planes.get("bar_h0")))
+        want = back(h0) * (decay.astype(np.float64) ** T)[None, :, None, None]
+        off = (left / want - 1).mean((0, 2, 3))
+        allowed = U * (1 + 6 * np.sqrt(T / 32 / (3 * S * K * K)))
+        assert (np.abs(off) <= allowed).all(), (off / U, allowed / U)
