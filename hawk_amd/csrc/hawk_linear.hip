@@ -875,6 +875,7 @@ LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w, int walks
     a.b = in<T>(*w.b);
     a.c = in<T>(*w.c);
     a.out = Plane<T>{static_cast<T*>(w.out->data), w.out->seq, w.out->step, w.out->head};
+    if (j.offsets) a.a.seq = a.b.seq = a.c.seq = a.out.seq = 0;    // packed planes have no such axis, whatever the job says
     a.decay = j.decay;
     a.start = w.start;
     a.end = w.end;

@@ -6,10 +6,13 @@ planes' layouts and their launches end, against plain sums in 64 bits.
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
 import hawk_amd as hawk
+from hawk_amd import _core
 
 U = 2.0 ** -24
 
@@ -75,3 +78,42 @@ def test_a_state_that_fades_slowly_is_off_by_roundings_of_either_sign(gpu, dtype
         off = (left / want - 1).mean((0, 2, 3))
         allowed = U * (1 + 6 * np.sqrt(T / 32 / (3 * S * K * K)))
         assert (np.abs(off) <= allowed).all(), (off / U, allowed / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bounds", [(0, 5, 5, 40), (0, 300, 1700, 2000)], ids=str)
+def test_packed_planes_have_no_sequence_stride(gpu, bounds):
+    """The C entries' ``seq`` of a packed plane is not looked at: the bits of a job that has 0 there, and
+    nothing is written where the strides would lead."""
+    import torch
+    S, T, H, K, V = len(bounds) - 1, bounds[-1], 2, 8, 12
+    g = torch.Generator(device=gpu).manual_seed(T)
+    stray = T * H * V                                           # S times this is allocated behind each plane
+    width = {"q": K, "k": K, "v": V, "o": V, "bar_o": V, "bar_q": K, "bar_k": K, "bar_v": V}
+    L, got = _core.lib(), []
+    values = {n: torch.randn(T * H * width[n], generator=g, device=gpu) for n in ("q", "k", "v", "bar_o")}
+    states = {n: torch.randn(S, H, K, V, generator=g, device=gpu) for n in ("h0", "bar_last")}
+    for seq in (0, stray):
+        job = _core.LinearAttentionJob()
+        planes = {n: torch.full((T * H * w + S * stray,), 7.0, device=gpu) for n, w in width.items()}
+        held = {**states, **{n: torch.zeros(S, H, K, V, device=gpu) for n in ("last", "bar_h0")},
+                "decay": torch.tensor([0.9, 0.999], device=gpu), "offsets": torch.tensor(bounds, device=gpu)}
+        for n, x in values.items():
+            planes[n][:len(x)] = x
+        for n, x in planes.items():
+            at = getattr(job, n)
+            at.data, at.seq, at.step, at.head = x.data_ptr(), seq, H * width[n], width[n]
+        for n, x in held.items():
+            setattr(job, n, x.data_ptr())
+        job.seqs, job.steps, job.heads, job.keys, job.values = S, T, H, K, V
+        job.scale, job.dtype, job.offsets64 = 0.5, 0, 1
+        ref = ctypes.byref(job)
+        for vjp, entry in ((0, L.hk_linear_attention), (1, L.hk_linear_attention_vjp)):
+            room = torch.empty(max(1, L.hk_linear_attention_scratch_bytes(ref, vjp)), dtype=torch.uint8, device=gpu)
+            assert entry(ref, room.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+            torch.cuda.synchronize()
+        got.append({**planes, **held})
+    for n, w in width.items():
+        assert torch.equal(got[0][n], got[1][n]) and (got[1][n][T * H * w:] == 7).all(), n
+    assert all(torch.equal(got[0][n], got[1][n]) for n in ("last", "bar_h0"))
+    assert torch.isfinite(got[1]["o"]).all() and (got[1]["o"][:T * H * V] != 7).any()
