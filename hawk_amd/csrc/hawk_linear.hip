@@ -20,7 +20,7 @@
 // a number of more digits is a sum of bf16 parts (three make 24 bits), and a product is
 // the sum of the parts' products down to 2^-25 of it wherever X is made or read.  Inside a
 // chunk (a_i . b_j, and that times c_j) it is so for 32-bit planes; where the result is
-// rounded to 16 bits, a_i . b_j is held as two parts, 2^-18 of it, which leaves 6e-5 of a
+// rounded to 16 bits, a_i . b_j is held as two parts, 2^-17 of it, which leaves 6e-5 of a
 // bfloat16 result's norm in places that round the other way (three parts: 4e-5, and 345
 // and 824 us where the two below take 289 and 604).
 //
@@ -64,33 +64,22 @@ __device__ __forceinline__ F4 product(const H8& a, const H8& b, const F4& c) {
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // The N bf16 parts of a number, each the nearest to what the ones before leave: two are
-// within 2^-18 of it, three are a number of 24 bits.
-template <int N>
+// within 2^-17 of it, three are a number of 24 bits.  The first is no infinity where the
+// number is none (Large: it may be above bf16's largest, and the nearest would be one).
+constexpr float kMostPart = 0x1.fep127f;
+template <int N, bool Large = true>
 __device__ __forceinline__ void cut(float x, uint16_t (&out)[N]) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-        const bf16 h = static_cast<bf16>(x);
+        const bf16 h = static_cast<bf16>(Large && p == 0 && N > 1 ? __builtin_amdgcn_fmed3f(x, -kMostPart, kMostPart) : x);
         out[p] = __builtin_bit_cast(uint16_t, h);
         if (p + 1 < N) x -= static_cast<float>(h);
     }
 }
 template <class T, int N>
 __device__ __forceinline__ void parts_of(T x, uint16_t (&out)[N]) {
-    if constexpr (N == 1) {
-        out[0] = __builtin_bit_cast(uint16_t, x);
-    } else if constexpr (sizeof(T) == 2) {
-        cut<N>(static_cast<float>(x), out);
-    } else {
-        // above bf16's largest number the nearest one is an infinity: the next below is taken
-        const uint32_t bits = __builtin_bit_cast(uint32_t, x);
-        const bf16 near = static_cast<bf16>(x);
-        const uint16_t h = fabsf(static_cast<float>(near)) < INFINITY ? __builtin_bit_cast(uint16_t, near) : static_cast<uint16_t>(bits >> 16);
-        uint16_t rest[N - 1];
-        cut<N - 1>(x - __builtin_bit_cast(float, static_cast<uint32_t>(h) << 16), rest);
-        out[0] = h;
-#pragma unroll
-        for (int p = 1; p < N; ++p) out[p] = rest[p - 1];
-    }
+    if constexpr (N == 1) out[0] = __builtin_bit_cast(uint16_t, x);
+    else cut<N, sizeof(T) == 4>(static_cast<float>(x), out);
 }
 __device__ __forceinline__ float part(uint16_t h) { return __builtin_bit_cast(float, static_cast<uint32_t>(h) << 16); }
 

@@ -117,3 +117,41 @@ def test_packed_planes_have_no_sequence_stride(gpu, bounds):
         assert torch.equal(got[0][n], got[1][n]) and (got[1][n][T * H * w:] == 7).all(), n
     assert all(torch.equal(got[0][n], got[1][n]) for n in ("last", "bar_h0"))
     assert torch.isfinite(got[1]["o"]).all() and (got[1]["o"][:T * H * V] != 7).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_numbers_up_to_the_types_largest_are_numbers(gpu, dtype):
+    """A state, a token's share of one and a product q . k above the largest bfloat16, read with small factors:
+    results of some 1e35, in three of four cases of one term, within 8 roundings to 24 bits or 2^-16."""
+    import torch
+    T, V, kind = 70, 16, getattr(torch, dtype)
+    most = (2 - 2.0 ** -8) * 2.0 ** 127                         # halfway from there to 2^128
+    small = 2.0 ** -10
+    z = lambda w: torch.zeros(1, T, 1, w, dtype=torch.float64)  # noqa: E731
+    stage, one = hawk.stages.linear_attention(), torch.ones(1, device=gpu)
+
+    def results(q, k, v, **planes):
+        o = torch.empty(1, T, 1, V, dtype=kind, device=gpu)
+        hawk.run(stage, q=q.to(gpu, kind), k=k.to(gpu, kind), v=v.to(gpu, kind), decay=one, o=o, **planes)
+        return back(o)[0, :, 0]
+
+    r = {"float32": 8 * U, "bfloat16": 2.0 ** -8 + 2.0 ** -16}[dtype]
+    q, k, v = z(2), z(2), z(V)
+    q[..., 0] = small
+    for x in (most, -(2 - 2.0 ** -23) * 2.0 ** 127):
+        h0 = torch.zeros(1, 1, 2, V, device=gpu)
+        h0[..., 0, :] = x
+        got = results(q, k, v, h0=h0)
+        assert (np.abs(got - x * small) <= r * abs(x) * small).all()
+    # q . k, of two numbers that bfloat16 has, of which the product is above its largest
+    q, k, v = z(2), z(2), z(V)
+    big = 1.453125 * 2.0 ** 127
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = 1.375, big, small
+    got, want = results(q, k, v), 1.375 * big * small
+    assert most < 1.375 * big < 2.0 ** 128 and (np.abs(got - want) <= r * want).all()
+    # a token's v, and its sum with what entered
+    if dtype == "float32":
+        q, k, v = z(2), z(2), z(V)
+        q[..., 0], k[:, 0, :, 0], v[:, 0] = 1, small, most
+        assert (np.abs(results(q, k, v) - most * small) <= r * most * small).all()
