@@ -455,6 +455,14 @@ __global__ void __launch_bounds__(kThreads) hawk_norm_none(int64_t cols, G* weig
     if (bias) bias[c] = static_cast<G>(0.0f);
 }
 
+// Rows without columns: the mean of no numbers.
+__global__ void __launch_bounds__(kThreads) hawk_norm_empty(int64_t rows, float* mean, float* rstd) {
+    for (int64_t n = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; n < rows; n += static_cast<int64_t>(gridDim.x) * kThreads) {
+        if (mean) mean[n] = NAN;
+        if (rstd) rstd[n] = NAN;
+    }
+}
+
 int size_of(int dtype) { return dtype == HK_F32 ? 4 : 2; }
 
 // How a row is held: `lanes` lanes of `vectors` vectors, or lanes = 0 for one that is
@@ -617,9 +625,16 @@ extern "C" int hk_layer_norm(const hk_layer_norm_job* job, void* scratch, void* 
     (void)scratch;
     const int rc = refuse(job);
     if (rc != HK_OK) return rc;
-    if (job->rows == 0 || job->cols == 0) return HK_OK;
-    if (!job->x) return hawk_internal::set_error(HK_EVALUE, "hk_layer_norm: x is required");
+    if (job->rows == 0) return HK_OK;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (job->cols == 0) {
+        if (!job->mean && !job->rstd) return HK_OK;
+        const int64_t need = (job->rows + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(hawk_norm_empty, dim3(static_cast<unsigned>(need < 4 * kUnits ? need : 4 * kUnits)), dim3(kThreads), 0, s, job->rows,
+                           job->mean, job->rstd);
+        return launched("hawk_norm_empty launch");
+    }
+    if (!job->x) return hawk_internal::set_error(HK_EVALUE, "hk_layer_norm: x is required");
     if (job->dtype == HK_F32) return norm<float>(*job, s);
     return job->dtype == HK_BF16 ? norm<bf16>(*job, s) : norm<f16>(*job, s);
 }

@@ -727,7 +727,7 @@ class _LayerNorm(_Stage):
         if x.dim() < 1:
             self._refuse("x has rows of at least one axis")
         job.cols = x.shape[-1]
-        job.rows = x.numel() // job.cols if job.cols else 0
+        job.rows = x.shape[:-1].numel()
         for n in ("x", "y", "bar_y", "bar_x"):
             if n not in t:
                 continue
@@ -769,7 +769,7 @@ def layer_norm(eps: float = 1e-5) -> Stage:
     bfloat16, float16), rows contiguous and evenly apart; ``weight`` and ``bias``
     (1 and 0 if not given) of one number a column, in float32 or the planes' type;
     ``mean`` and ``rstd`` float32, one a row, as a contiguous 1-D tensor, written
-    where given.
+    where given (NaN where a row has no columns).
 
     ``.vjp`` reads ``x``, ``weight``, ``mean``, ``rstd``, ``bar_y`` and writes those
     given of ``bar_x`` (it may be ``x`` or ``bar_y``), ``bar_weight`` and

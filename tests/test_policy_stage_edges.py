@@ -155,3 +155,22 @@ def test_numbers_up_to_the_types_largest_are_numbers(gpu, dtype):
         q, k, v = z(2), z(2), z(V)
         q[..., 0], k[:, 0, :, 0], v[:, 0] = 1, small, most
         assert (np.abs(results(q, k, v) - most * small) <= r * most * small).all()
+
+
+# -- layer norm ------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(12,), (2, 3), (300000,), ()], ids=str)
+def test_rows_without_columns_have_no_mean(gpu, lead):
+    import torch
+    stage, N = hawk.stages.layer_norm(), int(np.prod(lead))
+    x = torch.empty(*lead, 0, device=gpu)
+    mean, rstd = torch.full((2, N), 7.0, device=gpu)
+    hawk.run(stage, x=x, y=torch.empty_like(x), mean=mean, rstd=rstd)
+    assert torch.isnan(mean).all() and torch.isnan(rstd).all()
+    mean.fill_(7)
+    hawk.run(stage, x=x, mean=mean)
+    assert torch.isnan(mean).all()
+    hawk.run(stage, x=x, y=torch.empty_like(x))
+    none = torch.empty(0, device=gpu)
+    hawk.run(stage.vjp, x=x, mean=mean, rstd=rstd, bar_y=x, bar_x=torch.empty_like(x), bar_weight=none, bar_bias=torch.empty(0, device=gpu))
