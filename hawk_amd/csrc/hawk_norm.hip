@@ -424,28 +424,33 @@ __global__ void __launch_bounds__(kThreads) hawk_norm_columns(const NormArgs<T> 
 }
 
 // The workgroups' sums of kTile columns added in a fixed order, in 64 bits: 64 streams
-// of parts by 16 columns, so a wave reads whole 64-byte lines.
+// of parts by 16 columns, so a wave reads whole 64-byte lines.  A launch stays below 2^32
+// threads: past kMostTiles * kTile columns a workgroup has several tiles.
 constexpr int kTile = 16, kStreams = 64;
+constexpr int64_t kMostTiles = 1 << 20;
 template <class G>
 __global__ void __launch_bounds__(kTile* kStreams) hawk_norm_total(const float* parts, int64_t count, int64_t cols, G* weight, G* bias) {
     __shared__ double lds[kStreams][kTile + 1];
     G* out = blockIdx.y ? bias : weight;
     if (!out) return;
     const int lane = threadIdx.x % kTile, stream = threadIdx.x / kTile;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * kTile + lane;
-    double t = 0.0;
-    if (c < cols) {
-        const float* at = parts + blockIdx.y * count * cols + c;
+    for (int64_t tile = blockIdx.x; tile * kTile < cols; tile += gridDim.x) {
+        const int64_t c = tile * kTile + lane;
+        double t = 0.0;
+        if (c < cols) {
+            const float* at = parts + blockIdx.y * count * cols + c;
 #pragma unroll 4
-        for (int64_t p = stream; p < count; p += kStreams) t += static_cast<double>(at[p * cols]);
-    }
-    lds[stream][lane] = t;
-    __syncthreads();
-    for (int d = kStreams / 2; d > 0; d >>= 1) {
-        if (stream < d) lds[stream][lane] += lds[stream + d][lane];
+            for (int64_t p = stream; p < count; p += kStreams) t += static_cast<double>(at[p * cols]);
+        }
+        lds[stream][lane] = t;
         __syncthreads();
+        for (int d = kStreams / 2; d > 0; d >>= 1) {
+            if (stream < d) lds[stream][lane] += lds[stream + d][lane];
+            __syncthreads();
+        }
+        if (stream == 0 && c < cols) out[c] = static_cast<G>(static_cast<float>(lds[0][lane]));
+        // (row 0 is written anew by the threads that read it here, the others' were read before the last barrier)
     }
-    if (stream == 0 && c < cols) out[c] = static_cast<G>(static_cast<float>(lds[0][lane]));
 }
 template <class G>
 __global__ void __launch_bounds__(kThreads) hawk_norm_none(int64_t cols, G* weight, G* bias) {
@@ -564,7 +569,8 @@ int totals(const hk_layer_norm_job& j, const float* parts, int64_t count, hipStr
         const dim3 grid(static_cast<unsigned>((j.cols + kThreads - 1) / kThreads)), block(kThreads);
         hipLaunchKernelGGL((hawk_norm_none<G>), grid, block, 0, stream, j.cols, weight, bias);
     } else {
-        const dim3 grid(static_cast<unsigned>((j.cols + kTile - 1) / kTile), 2), block(kTile * kStreams);
+        const int64_t tiles = (j.cols + kTile - 1) / kTile;
+        const dim3 grid(static_cast<unsigned>(tiles < kMostTiles ? tiles : kMostTiles), 2), block(kTile * kStreams);
         hipLaunchKernelGGL((hawk_norm_total<G>), grid, block, 0, stream, parts, count, j.cols, weight, bias);
     }
     return launched("hawk_norm_total launch");

@@ -174,3 +174,16 @@ def test_rows_without_columns_have_no_mean(gpu, lead):
     hawk.run(stage, x=x, y=torch.empty_like(x))
     none = torch.empty(0, device=gpu)
     hawk.run(stage.vjp, x=x, mean=mean, rstd=rstd, bar_y=x, bar_x=torch.empty_like(x), bar_weight=none, bar_bias=torch.empty(0, device=gpu))
+
+
+@pytest.mark.gpu
+def test_the_sums_over_rows_of_more_columns_than_a_launch_has_threads_for(gpu):
+    """One row at mean 0 and rstd 1: bar_bias is bar_y, bar_weight its product with x, which float32 holds whole."""
+    import torch
+    C = (1 << 26) + 53
+    g = torch.Generator(device=gpu).manual_seed(3)
+    x, bar = (torch.randn(1, C, generator=g, device=gpu, dtype=torch.bfloat16) for _ in range(2))
+    mean, rstd = torch.zeros(1, device=gpu), torch.ones(1, device=gpu)
+    bw, bb = torch.full((2, C), 7.0, device=gpu)
+    hawk.run(hawk.stages.layer_norm().vjp, x=x, mean=mean, rstd=rstd, bar_y=bar, bar_weight=bw, bar_bias=bb)
+    assert torch.equal(bb, bar[0].float()) and torch.equal(bw, bar[0].float() * x[0].float())
