@@ -615,6 +615,12 @@ int refuse(const hk_layer_norm_job* j) {
         return set_error(HK_EVALUE, "hk_layer_norm: the weights' element type is 32-bit or the planes'");
     if (j->cols > INT32_MAX / 2 || (j->cols > 0 && j->rows > INT64_MAX / 16 / j->cols))
         return set_error(HK_EVALUE, "hk_layer_norm: the planes exceed the grid limit");
+    auto crosses = [&](const void* out, int64_t out_stride, const void* in, int64_t in_stride) {
+        return j->rows > 1 && j->cols > 0 && out && out == in && out_stride != in_stride;
+    };
+    if (crosses(j->y, j->y_stride, j->x, j->x_stride) || crosses(j->bar_x, j->bar_x_stride, j->x, j->x_stride) ||
+        crosses(j->bar_x, j->bar_x_stride, j->bar_y, j->bar_y_stride))
+        return set_error(HK_EVALUE, "hk_layer_norm: an output over an input has its row distance");
     if (!(j->eps >= 0.0f)) return set_error(HK_EVALUE, "hk_layer_norm: eps must be >= 0");
     return HK_OK;
 }

@@ -23,7 +23,8 @@ a stage whose planes are the primal's with ``bar_`` names for adjoints::
 A stage is no traced kernel: it has no ``hawk.diff.jvp`` and is no member of a
 ``hawk.chain`` or ``hawk.steps``; it takes the planes that kernels write and read.
 
-Planes are PyTorch-ROCm tensors, bound by address.  Scratch belongs to a stream,
+Planes are PyTorch-ROCm tensors, bound by address.  An output that may be an input is
+that tensor: one address with other strides is refused.  Scratch belongs to a stream,
 or to the graph a call is captured in: calls on several streams and replays of
 several graphs may run at once (a launcher's own run one after another).  Nothing
 synchronises.
@@ -191,11 +192,21 @@ class _Stage(Stage):
                 self._refuse(f"the output {n!r} repeats memory (strides {tuple(x.stride())})")
         return tensors
 
+    def _crossed(self, tensors: dict) -> tuple:
+        """The pairs of an output and another plane that lie differently: at one address
+        an element of the one would be written over others of the other."""
+        def lies(x):
+            return [(d, st) for d, st in zip(x.shape, x.stride()) if d > 1]
+        return tuple((out, n) for out in self.writes if out in tensors for n, x in tensors.items()
+                     if n != out and x.shape == tensors[out].shape and lies(x) != lies(tensors[out]))
+
     def _plan(self, key, arrays: dict, device: int) -> _Plan:
         """A plan of ``key``, made, checked and bound before another thread may
         find it."""
         self._names(arrays)
-        plan = self._make(self._placed(arrays))
+        tensors = self._placed(arrays)
+        plan = self._make(tensors)
+        plan.apart += self._crossed(tensors)
         if key is None:
             self._refuse("a plane is no dense tensor")
         plan.bind(arrays, self.values, device)
@@ -237,7 +248,8 @@ class _Stage(Stage):
         for one, two in plan.apart:
             a, b = arrays.get(one), arrays.get(two)
             if a is not None and b is not None and a.data_ptr() == b.data_ptr() and a.numel():
-                self._refuse(f"the output {one!r} and {two!r} are one tensor")
+                other = a.shape == b.shape and a.stride() != b.stride()
+                self._refuse(f"the output {one!r} and {two!r} are one tensor" + other * ", which lies in two ways")
         for name, word in plan.cells:
             bound.append((word, self._value(name, arrays.get(name))))
         return plan, bound, device

@@ -503,7 +503,8 @@ int hk_dropout(const hk_dropout_job* job, void* stream);
  * HK_F16; weight, bias and their gradients are of weight_dtype, HK_F32 or the
  * planes' own; mean and rstd are float, one a row.
  * hk_layer_norm reads x, weight, bias and writes y, mean, rstd (each may be NULL;
- * y may be x; mean and rstd of rows without columns are NaN).
+ * y may be x; mean and rstd of rows without columns are NaN).  An output over an
+ * input has its row distance.
  * hk_layer_norm_vjp reads x, weight, mean, rstd, bar_y and writes, each may be NULL,
  *   bar_x = rstd (g - mean(g) - xh mean(g xh)), g = bar_y weight  (it may be x or bar_y),
  *   bar_weight = sum over rows of bar_y xh, bar_bias = sum over rows of bar_y

@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 
 import hawk_amd as hawk
-from hawk_amd import _core
+from hawk_amd import HawkError, _core
 
 U = 2.0 ** -24
 
@@ -187,3 +187,48 @@ def test_the_sums_over_rows_of_more_columns_than_a_launch_has_threads_for(gpu):
     bw, bb = torch.full((2, C), 7.0, device=gpu)
     hawk.run(hawk.stages.layer_norm().vjp, x=x, mean=mean, rstd=rstd, bar_y=bar, bar_weight=bw, bar_bias=bb)
     assert torch.equal(bb, bar[0].float()) and torch.equal(bw, bar[0].float() * x[0].float())
+
+
+def test_the_layer_norm_entries_refuse_rows_that_lie_in_two_ways():
+    L, n = _core.lib(), _core.LayerNormJob()
+    ref = ctypes.byref(n)
+    n.x = n.y = n.bar_y = n.bar_x = n.mean = n.rstd = 1 << 20
+    n.rows, n.cols, n.x_stride, n.y_stride, n.bar_y_stride, n.bar_x_stride = 3, 8, 8, 9, 8, 8
+    for entry in (L.hk_layer_norm, L.hk_layer_norm_vjp):
+        assert entry(ref, None, None) == 1 and b"row distance" in L.hk_last_error()
+    n.y = None
+    for x, bar_y in ((8, 9), (9, 8)):
+        n.x_stride, n.bar_y_stride = x, bar_y
+        assert L.hk_layer_norm_vjp(ref, None, None) == 1 and b"row distance" in L.hk_last_error()
+
+
+@pytest.mark.gpu
+def test_an_output_over_an_input_lies_as_it_does(gpu):
+    """At one address with other strides a call would write over what it has not read yet."""
+    import torch
+    room = torch.zeros(400, device=gpu)
+    near, far = room.as_strided((5, 8), (8, 1)), room.as_strided((5, 8), (9, 1))
+    block = torch.zeros(2, 4, 8, device=gpu)
+    turned = block, block.as_strided((2, 4, 8), (32, 1, 4))
+    other, m = torch.zeros(5, 8, device=gpu), torch.ones(5, device=gpu)
+    target, s = torch.zeros(5, dtype=torch.int64, device=gpu), hawk.stages
+    gate = torch.zeros(2, 4, 8, device=gpu)
+    norm, logp, drop, scan = s.layer_norm(), s.token_logp(), s.dropout(0.5), s.recurrence()
+    calls = [(norm, lambda a, b: dict(x=a, y=b)),
+             (norm.vjp, lambda a, b: dict(x=a, bar_y=other, bar_x=b, mean=m, rstd=m)),
+             (norm.vjp, lambda a, b: dict(x=other, bar_y=a, bar_x=b, mean=m, rstd=m)),
+             (logp.vjp, lambda a, b: dict(logits=a, target=target, lse=m, bar_logp=m, bar_logits=b)),
+             (drop, lambda a, b: dict(x=a, y=b, seed=1)),
+             (drop, lambda a, b: dict(x=other, residual=a, y=b, seed=1)),
+             (scan, lambda a, b: dict(gate=gate, x=a, h=b)),
+             (scan, lambda a, b: dict(gate=a, x=gate, h=b)),
+             (scan.vjp, lambda a, b: dict(gate=gate, h=gate, bar_h=a, bar_gate=b))]
+    for stage, planes in calls:
+        a, b = turned if "gate" in stage.planes else (near, far)
+        for one, two in ((a, b), (b, a)):
+            with pytest.raises(HawkError, match="lies in two ways"):
+                hawk.run(stage, **planes(one, two))
+            with pytest.raises(HawkError, match="lies in two ways"):
+                stage.prepare(**planes(one, two))
+            hawk.run(stage, **planes(one, one))                 # over the input itself, as before
+    hawk.run(norm, x=near[:1], y=far[:1])                       # one row has no distance
