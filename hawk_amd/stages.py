@@ -767,8 +767,12 @@ class _LayerNorm(_Stage):
             setattr(job, n, 16)             # any address: which planes there are decides what a call works in
         L = _core.lib()
         fn = L.hk_layer_norm_vjp if self.derivative else L.hk_layer_norm
-        apart = tuple((out, n) for out in ("y", "mean", "rstd") for n in ("weight", "bias")) if not self.derivative else \
-            (("bar_weight", "weight"), ("bar_weight", "bar_bias"), ("bar_bias", "weight"), ("bar_x", "weight"))
+        if self.derivative:
+            apart = (("bar_weight", "weight"), ("bar_weight", "bar_bias"), ("bar_bias", "weight"), ("bar_x", "weight"),
+                     ("bar_x", "mean"), ("bar_x", "rstd"), ("bar_x", "bar_weight"), ("bar_x", "bar_bias"))
+        else:
+            apart = (*((out, n) for out in self.writes for n in self.may_read), ("mean", "x"), ("rstd", "x"), ("y", "mean"),
+                     ("y", "rstd"), ("mean", "rstd"))
         return _Plan(job, slots, fn, int(L.hk_layer_norm_scratch_bytes(ctypes.byref(job), int(self.derivative))),
                      apart=apart)
 
@@ -781,7 +785,7 @@ def layer_norm(eps: float = 1e-5) -> Stage:
     bfloat16, float16), rows contiguous and evenly apart; ``weight`` and ``bias``
     (1 and 0 if not given) of one number a column, in float32 or the planes' type;
     ``mean`` and ``rstd`` float32, one a row, as a contiguous 1-D tensor, written
-    where given (NaN where a row has no columns).
+    where given (NaN where a row has no columns).  Each output is a tensor of its own.
 
     ``.vjp`` reads ``x``, ``weight``, ``mean``, ``rstd``, ``bar_y`` and writes those
     given of ``bar_x`` (it may be ``x`` or ``bar_y``), ``bar_weight`` and

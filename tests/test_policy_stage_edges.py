@@ -232,3 +232,19 @@ def test_an_output_over_an_input_lies_as_it_does(gpu):
                 stage.prepare(**planes(one, two))
             hawk.run(stage, **planes(one, one))                 # over the input itself, as before
     hawk.run(norm, x=near[:1], y=far[:1])                       # one row has no distance
+
+
+@pytest.mark.gpu
+def test_layer_norms_outputs_are_tensors_of_their_own(gpu):
+    import torch
+    stage = hawk.stages.layer_norm()
+    x, y, m, r, w = torch.ones(5, 1, device=gpu), *(torch.ones(5, 1, device=gpu), *torch.ones(2, 5, device=gpu)), torch.ones(1, device=gpu)
+    for planes in (dict(x=x, mean=m, rstd=m), dict(x=x, y=y, mean=y[:, 0]), dict(x=x, y=y, rstd=y[:, 0]), dict(x=x, mean=x[:, 0]),
+                   dict(x=x, rstd=x[:, 0])):
+        with pytest.raises(HawkError, match="one tensor"):
+            hawk.run(stage, **planes)
+    for bars in (dict(bar_x=m[:, None]), dict(bar_x=r[:, None]), dict(bar_x=y, bar_weight=y[0]), dict(bar_x=y, bar_bias=y[0])):
+        with pytest.raises(HawkError, match="one tensor"):
+            hawk.run(stage.vjp, x=x, mean=m, rstd=r, bar_y=x, **bars)
+    hawk.run(stage, x=x, y=x, mean=m, rstd=r)
+    hawk.run(stage.vjp, x=x, mean=m, rstd=r, bar_y=y, bar_x=x, bar_weight=w)
