@@ -157,6 +157,48 @@ def test_numbers_up_to_the_types_largest_are_numbers(gpu, dtype):
         assert (np.abs(results(q, k, v) - most * small) <= r * most * small).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("shape", [(3, 1, 2, 128, 128), (2, 3, 2, 72, 100), (1, 8, 1, 256, 256), (2, 2, 3, 129, 65), (5, 1, 4, 65, 256),
+                                   (1, 8, 2, 64, 64), (1, 9, 1, 256, 256), (2, 9, 3, 129, 65)], ids=str)
+def test_a_few_tokens_of_wide_heads(gpu, shape, dtype):
+    """Up to 8 tokens as they stand: a state takes two roundings a token, a result K / 16 + 16 sums and three
+    roundings more.  Nine go by way of chunks, whose products are taken to 2^-16 (16-bit planes) or 2^-23."""
+    import torch
+    S, T, H, K, V = shape
+    g, kind = np.random.default_rng(shape), getattr(torch, dtype)
+    q, k, v = (torch.from_numpy(g.normal(size=(S, T, H, w))).to(kind) for w in (K, K, V))
+    h0 = torch.from_numpy(g.normal(size=(S, H, K, V))).float()
+    decay = np.float32([0.9, 1.0, 0.0, 0.97])[:H]
+    gain, scale = decay.astype(np.float64)[None, :, None, None], 0.37
+    state = back(h0)
+    mass, want, size = np.abs(state), [], []
+    for t in range(T):
+        kv = back(k[:, t])[..., :, None] * back(v[:, t])[..., None, :]
+        state, mass = gain * state + kv, gain * mass + np.abs(kv)
+        want.append(scale * np.einsum("shk,shkv->shv", back(q[:, t]), state))
+        size.append(scale * np.einsum("shk,shkv->shv", np.abs(back(q[:, t])), mass))
+    want, size = np.stack(want, 1), np.stack(size, 1)
+    r = {"float32": U, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}[dtype]
+    if T <= 8:
+        p_state = (2 * T + 2) * U
+        p = p_state + (K / 16 + 19) * U
+    else:
+        p_state = 2.0 ** -23 + ((max(K, V) + 64) / 4 + 65) * U
+        p = p_state + (0 if dtype == "float32" else 2.0 ** -16)
+    q, k, v = q.to(gpu), k.to(gpu), v.to(gpu)
+    stage, decay = hawk.stages.linear_attention(scale=scale), torch.from_numpy(decay).to(gpu)
+    for held in (False, True):                                  # the state beside what entered, or over it
+        o, h = torch.empty_like(v), h0.to(gpu)
+        last = h if held else torch.full_like(h, 7.0)
+        hawk.run(stage, q=q, k=k, v=v, decay=decay, o=o, h0=h, last=last)
+        assert (np.abs(back(o) - want) <= p * size * (1 + r) + r * np.abs(want) + 2.0 ** -25).all()
+        assert (np.abs(back(last) - state) <= p_state * mass).all()
+        h = h0.to(gpu)
+        hawk.run(stage, q=q, k=k, v=v, decay=decay, h0=h, last=h)
+        assert torch.equal(h, last)                             # without results
+
+
 # -- layer norm ------------------------------------------------------------------------------
 
 @pytest.mark.gpu
