@@ -12,13 +12,16 @@
 // another token.  The weights are taken in 64 bits and held as whole numbers of
 // 2^-shift, shift = 62 - log2(vocabulary) (51 at most): their sums stay below 2^63 and
 // are exact, so neither the order in which atomics add them nor the way a row is cut
-// changes a bit.
+// changes a bit.  A weight is off by half a unit, so a row's sum by up to vocabulary *
+// 2^-(shift + 1) of the highest weight: 2^-29 of it at 2^17 tokens, 2^-19 at 2^22.  A
+// token below half a unit weighs nothing.
 //
-// What bounds it: the weights' 64-bit arithmetic, some thirty instructions a token, in a
-// pass that sums and one that finds (4096 rows of 50001 float16 logits: 218 us, where their
-// bytes take 62), and, where rows are few, four launches that wait for one another (64
-// rows of 131072 bfloat16 with a top-p: 69.5 us, of which the largest kernels take 23
-// each; a workgroup a row took 156).
+// What bounds it: the weights' 64-bit arithmetic, some thirty instructions a token, in the
+// pass that sums them (one before it finds the highest logit; the token is looked for along
+// one run of one wave): 4096 rows of 50001 float16 logits take 218 us, their bytes 62.  And,
+// where rows are few, four launches that wait for one another (64 rows of 131072 bfloat16
+// with a top-p: 69.5 us, of which the largest kernels take 23 each; a workgroup a row took
+// 156).
 
 #include "hawk_core.h"
 #include "hawk_internal.h"
@@ -89,9 +92,6 @@ __device__ __forceinline__ u64 weight_of(const Weights& k, float x) {
 __device__ __forceinline__ uint32_t place_of(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
     return b & 0x80000000u ? b : ~b & 0x7fffffffu;
-}
-__device__ __forceinline__ float placed(uint32_t at) {
-    return __builtin_bit_cast(float, at & 0x80000000u ? at : ~at & 0x7fffffffu);
 }
 
 // Running sums over a wave's lanes, by moves between lanes that need no memory: within

@@ -968,8 +968,9 @@ def sample(temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: 
     ``logp`` of 0.  A row that holds a NaN, or whose ``u`` is one or whose
     temperature is below 0 or one, gives token -1 and a NaN; a row of -inf alone
     (nothing is allowed) token -1 and -inf; logits of +inf share the whole.  Weights
-    are summed exactly, as whole numbers of 2^-40 of the highest or less, so a call
-    repeats bit for bit.  There is no derivative: the loss reads the token's
+    are whole numbers of 2^-40 of the highest (2^22 tokens; 2^-45 for 2^17) and summed
+    exactly, so a call repeats bit for bit and a border is off by half of one for each
+    token at most.  There is no derivative: the loss reads the token's
     ``token_logp``."""
     def number(x):
         return isinstance(x, (int, float)) and not isinstance(x, bool) and x == x

@@ -290,3 +290,34 @@ def test_layer_norms_outputs_are_tensors_of_their_own(gpu):
             hawk.run(stage.vjp, x=x, mean=m, rstd=r, bar_y=x, **bars)
     hawk.run(stage, x=x, y=x, mean=m, rstd=r)
     hawk.run(stage.vjp, x=x, mean=m, rstd=r, bar_y=y, bar_x=x, bar_weight=w)
+
+
+# -- sampling ----------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [131072, 1000003, 1 << 20, 1 << 22])
+@pytest.mark.parametrize("low", [25.0, 28.5, 30.5])
+def test_a_flat_tail_far_below_the_highest_logit(gpu, V, low):
+    """One token above V - 1 equal ones.  A weight is a whole number of units of 2^-shift, so many that V of them
+    stay below 2^63, and half a unit off: sums by E = V 2^-(shift + 1) of the highest weight, shares of the whole
+    by 2 E, its logarithm by E.  The weights' polynomial adds 2^-48."""
+    import torch
+    shift = min(51, 63 - V.bit_length())
+    E = V * 2.0 ** -(shift + 1) + 2.0 ** -48
+    at, w = V // 3, float(np.exp(-np.float64(np.float32(low))))
+    x = torch.full((1, V), -low, device=gpu)
+    x[0, at] = 0
+    whole = 1 + w * (V - 1)
+    tail = w * (V - 1) / whole
+    u = torch.from_numpy(np.array([0.0, tail / 5, tail / 3 + 2.5 * E, 0.5, 1 - 2 * tail / 3 - 2.5 * E, 1 - tail / 3, 1 - 2.0 ** -50])).to(gpu)
+    N = len(u)
+    for filters in ({}, dict(min_p=1e-30), dict(top_k=V - 1)):
+        token, logp = torch.empty(N, dtype=torch.int64, device=gpu), torch.empty(N, device=gpu)
+        hawk.run(hawk.stages.sample(**filters), logits=x.expand(N, V), u=u, token=token, logp=logp)
+        got = token.cpu().numpy()
+        upto = (w * (got + 1) + (got >= at) * (1 - w)) / whole  # the whole's share up to the token, and before it
+        before = upto - np.where(got == at, 1, w) / whole
+        assert (before <= back(u) + 2 * E).all() and (upto >= back(u) - 2 * E).all(), (got, back(u))
+        want = np.where(got == at, 0, -np.float64(np.float32(low))) - np.log(whole)
+        assert (np.abs(back(logp) - want) <= E + U * np.abs(want)).all()
+        assert got[3] == at
