@@ -21,17 +21,17 @@
 // the sum of the parts' products down to 2^-25 of it wherever X is made or read.  Inside a
 // chunk (a_i . b_j, and that times c_j) it is so for 32-bit planes; where the result is
 // rounded to 16 bits, a_i . b_j is held as two parts, 2^-17 of it, which leaves 6e-5 of a
-// bfloat16 result's norm in places that round the other way (three parts: 4e-5, and 345
-// and 824 us where the two below take 289 and 604).
+// bfloat16 result's norm in places that round the other way (three parts: 4e-5, and 340
+// and 785 us where the two calls below take 270 and 566).
 //
 // What bounds it.  The eight waves of a workgroup share a chunk, in phases between four
 // barriers; registers and LDS hold two workgroups a unit.  In the walk of 16 heads of 128
-// bfloat16 columns LDS is busy half of the time, the vector units half and
-// the matrix cores a quarter.  One sequence of 32768 such tokens takes 265 us (states of
-// its segments 81, their join 14, the walk 180; the bytes' time is 81); the derivative of
-// 8 x 4096 tokens, whose 8 * 16 * 3 walks fill the chip uncut, 525 in one launch, where
-// cut sequences took 750.  Waves of two column tiles, four to a workgroup, took 566 and
-// 292; products of two tiles in turn, no less.
+// bfloat16 columns LDS is active in 47 % of the units' busy cycles (44 % of those are bank
+// conflicts), the vector units in 57 %, the matrix cores in 34 %.  One sequence of 32768 such
+// tokens takes 270 us (states of its segments 76, their join 14, the walk 178; the bytes'
+// time is 81); the derivative of 8 x 4096 tokens, whose 8 * 16 * 3 walks fill the chip
+// uncut, 566 in one launch.  Waves of two column tiles, four to a workgroup, took a tenth
+// longer; products of two tiles in turn were no faster.
 
 #include "hawk_core.h"
 #include "hawk_internal.h"
@@ -149,14 +149,14 @@ __device__ __forceinline__ int64_t bound_of(const LinearArgs<T>& a, int64_t k) {
     const int64_t v = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[k] : static_cast<const int32_t*>(a.offsets)[k];
     return v < 0 ? 0 : v > a.steps ? a.steps : v;
 }
-// Sequence s's segments have the slots from bound(s) / segment + s on: more than it needs
-// by one at most, and none of two sequences.
-// Of packed sequences, at most one of several segments begins in each `segment` rows, and at
+// Where a segment's states are kept.  Of packed sequences, at most one of several segments begins in each `segment` rows, and at
 // most one has a later segment that does: two states for each of those runs of rows.
 template <class T>
 __device__ __forceinline__ int64_t cut_at(const LinearArgs<T>& a, int64_t seq, int64_t first, int64_t segment) {
     return a.offsets ? 2 * (first / a.segment + segment) + (segment == 0) : seq * a.segments + segment;
 }
+// A workgroup's segment, from its slot.  Packed sequence s's segments have the slots from
+// bound(s) / segment + s on: more than it needs by one at most, and none of two sequences.
 template <class T>
 __device__ __forceinline__ Span span_of(const LinearArgs<T>& a, int64_t slot) {
     Span s;
@@ -322,8 +322,8 @@ struct Shares {
     }
 };
 
-// Where eight tokens' unit of a row of channels lies: eight lanes that read neighbouring
-// rows, or write every fourth one, meet the banks once each.
+// Where eight tokens' unit of a row of channels lies: so that eight lanes that read
+// neighbouring rows, or write every fourth one, meet the banks once each.
 __device__ __forceinline__ int unit(int d, int eight) { return (eight ^ (d >> 4 & 1)) * 8; }
 
 template <class T, int DP, int C>
@@ -808,7 +808,9 @@ int beside_of(const Walk* w, int n, int i) {
 }
 
 // The tokens of a segment.  A launch whose whole walks are enough for most of the units
-// goes uncut: what cutting costs, the segments' own states first, is about half a walk.
+// goes uncut: what cutting costs, the segments' own states first, is about half a walk
+// (4096 tokens of 128 bfloat16 channels: 192 walks whole 378 us, cut 436; 144: 376 and 420;
+// 96: 373 and 213).
 // Otherwise, and where sequences are of any length (up to eight times as many workgroups of
 // them), as many segments as give each unit two workgroups of eight waves, or four of four,
 // of two chunks at least.
@@ -907,7 +909,7 @@ LinearArgs<T> args_of(const hk_linear_attention_job& j, const Walk& w, int walks
 }
 
 // Dense sequences of up to kFewTokens tokens, forward: as they stand, by vector arithmetic
-// (64 x 16 heads of 128 x 128, one token: 29.7 us, 41.9 by chunks; its states take 20.7).
+// (64 x 16 heads of 128 x 128, one token: 29.7 us, 42.3 by chunks; its states take 20.7).
 template <class T>
 int steps(const hk_linear_attention_job& j, const Walk& w, hipStream_t stream) {
     LinearArgs<T> a = args_of<T>(j, w, 1);
