@@ -720,6 +720,14 @@ def dropout(p: float) -> Stage:
 
 # -- layer norm ----------------------------------------------------------------------------
 
+def _float32(x) -> float:
+    """A number as the kernels hold it: one past float32's range is an infinity."""
+    try:
+        return ctypes.c_float(x).value
+    except OverflowError:                   # an int past float64's
+        return math.inf
+
+
 class _LayerNorm(_Stage):
     def __init__(self, eps: float, derivative: bool):
         super().__init__()
@@ -791,8 +799,8 @@ def layer_norm(eps: float = 1e-5) -> Stage:
     given of ``bar_x`` (it may be ``x`` or ``bar_y``), ``bar_weight`` and
     ``bar_bias`` (of the weight's type).  The sums over rows are taken in a fixed
     order, 0 where there are no rows."""
-    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 0 <= eps < math.inf:
-        raise HawkError(f"layer_norm: eps= is a finite number from 0, got {eps!r}")
+    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not (eps >= 0 and _float32(eps) < math.inf):
+        raise HawkError(f"layer_norm: eps= is a finite float32 from 0, got {eps!r}")
     return _LayerNorm(float(eps), False)
 
 
@@ -895,8 +903,8 @@ def linear_attention(scale: float = 1.0) -> Stage:
     ``bar_h0``.  A plane that was expanded along an axis (heads that share keys and
     values) gets its full gradient; its own is the sum along that axis.  No output
     may be an input or another output."""
-    if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not math.isfinite(scale):
-        raise HawkError(f"linear_attention: scale= is a finite number, got {scale!r}")
+    if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not math.isfinite(_float32(scale)):
+        raise HawkError(f"linear_attention: scale= is a finite float32, got {scale!r}")
     return _LinearAttention(float(scale), False)
 
 

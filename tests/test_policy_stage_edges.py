@@ -321,3 +321,14 @@ def test_a_flat_tail_far_below_the_highest_logit(gpu, V, low):
         want = np.where(got == at, 0, -np.float64(np.float32(low))) - np.log(whole)
         assert (np.abs(back(logp) - want) <= E + U * np.abs(want)).all()
         assert got[3] == at
+
+
+# -- options -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("big", [3.5e38, 1e300, 1 << 200, 1 << 2000])
+def test_numbers_past_float32_are_refused(big):
+    with pytest.raises(HawkError, match="scale="):
+        hawk.stages.linear_attention(scale=-big)
+    with pytest.raises(HawkError, match="eps="):
+        hawk.stages.layer_norm(eps=big)
+    hawk.stages.linear_attention(scale=-3.4e38), hawk.stages.layer_norm(eps=3.4e38), hawk.stages.layer_norm(eps=0)
